@@ -14,8 +14,8 @@ A case is a dict; "kind" names the operator:
 
 Q8_0 page of `block` tokens: block x kv_dim int8 digits, then block x
 kv_dim / 32 half scales; dim i of a token is digit * scale of its block of 32.
-A head's digits are stored as a 16 x (head_dim / 16) matrix: byte
-r * (head_dim / 16) + j holds dim 16 j + r.
+Every 64 dims' digits are stored as a 16 x 4 matrix: byte 4 r + j of the 64
+holds dim 16 j + r.
 """
 from __future__ import annotations
 
@@ -256,9 +256,10 @@ def _values(state, pool, at):
         rows = state[pool].view(torch.float16).unflatten(1, (c["block"], -1))[page, slot]
         return rows.to(torch.float32).unflatten(2, (c["kv_heads"], c["head_dim"]))
     digits, scales = _planes(state, pool)
-    digits = digits[page, slot].unflatten(2, (c["kv_heads"], 16, -1)).transpose(3, 4)
-    scales = scales[page, slot].to(torch.float32).unflatten(2, (c["kv_heads"], -1))
-    return (digits.to(torch.float32).flatten(3).unflatten(3, (-1, 32)) * scales.unsqueeze(4)).flatten(3)
+    digits = digits[page, slot].unflatten(2, (-1, 16, 4)).transpose(3, 4).to(torch.float32)
+    scales = scales[page, slot].to(torch.float32)
+    values = digits.flatten(2).unflatten(2, (-1, 32)) * scales.unsqueeze(3)
+    return values.flatten(2).unflatten(2, (c["kv_heads"], c["head_dim"]))
 
 
 def _half_up(x):
@@ -269,16 +270,14 @@ def _half_up(x):
 
 
 def _append(state, pool, x, at):
-    c = state["case"]
-    x = x.unflatten(2, (c["kv_heads"], -1, 32))
-    scale = _half_up(x.abs().amax(4) / 127)
-    inverse = torch.where(scale > 0, 1 / scale.to(torch.float32), 0)
-    digits = torch.round(x * inverse.unsqueeze(4)).clamp(-127, 127).to(torch.int8)
-    digits = digits.flatten(3).unflatten(3, (-1, 16)).transpose(3, 4).flatten(2)  # [head][16][head_dim / 16]
+    x = x.unflatten(2, (-1, 32))
+    scale = x.abs().amax(3, keepdim=True) / 127
+    steps = torch.where(scale > 0, x / scale, 0).to(torch.float64)  # in 64 bits from here: halves round away from zero
+    digits = (torch.floor(steps.abs() + 0.5) * torch.sign(steps)).to(torch.int8)
     page, slot = _slots(state, at)
     to_digits, to_scales = _planes(state, pool)
-    to_digits[page, slot] = digits
-    to_scales[page, slot] = scale.flatten(2)
+    to_digits[page, slot] = digits.flatten(2).unflatten(2, (-1, 4, 16)).transpose(3, 4).flatten(2)
+    to_scales[page, slot] = _half_up(scale.squeeze(3))
     return _values(state, pool, at).flatten(2)
 
 
@@ -304,15 +303,14 @@ def _attention(state):
 # -------------------------------------------------------------------- exact
 
 def _stored(rows):
-    """Float64 rows [..., kv_dim] after the Q8_0 rounding: blocks of 32, half scales of amax / 127 (float32 quotient,
-    ties upwards), digits of the float32 product with the scale's float32 inverse, ties to even."""
+    """Float64 rows [..., kv_dim] after the Q8_0 rounding: blocks of 32, s = max|x| / 127 and x / s rounded to float32,
+    the scale s to the nearest half (ties upwards), the digit x / s to the nearest integer (halves away from zero)."""
     x = rows.unflatten(-1, (-1, 32))
-    quotient = (x.abs().amax(-1, keepdim=True) / 127).to(torch.float32).to(torch.float64)
-    step = torch.exp2((torch.frexp(quotient)[1] - 11).clamp(min=-24).to(torch.float64))
-    scale = torch.floor(quotient / step + 0.5) * step
-    inverse = torch.where(scale > 0, 1 / scale, 0).to(torch.float32).to(torch.float64)
-    digits = (x * inverse).to(torch.float32).to(torch.float64).round().clamp(-127, 127)
-    return (digits * scale).flatten(-2)
+    s = (x.abs().amax(-1, keepdim=True) / 127).to(torch.float32).to(torch.float64)
+    step = torch.exp2((torch.frexp(s)[1] - 11).clamp(min=-24).to(torch.float64))
+    digits = (x / s).to(torch.float32).to(torch.float64)
+    digits = digits.trunc() + digits.frac().mul(2).trunc()
+    return (digits.nan_to_num() * torch.floor(s / step + 0.5) * step).flatten(-2)
 
 
 def _exact_rows(c, s, pool, j, n):
@@ -322,10 +320,10 @@ def _exact_rows(c, s, pool, j, n):
     if c.get("kv") == "f16":
         return pages.view(torch.float16).to(torch.float64).reshape(-1, kv_heads, d)[:n]
     split = block * kv_heads * d
-    digits = pages[:, :split].contiguous().view(torch.int8).reshape(-1, kv_heads, 16, d // 16)[:n].to(torch.float64)
+    digits = pages[:, :split].contiguous().view(torch.int8).reshape(-1, kv_heads, d // 64, 16, 4)[:n].to(torch.float64)
     scales = pages[:, split:].contiguous().view(torch.float16).reshape(-1, kv_heads, d // 32)[:n].to(torch.float64)
     dim = torch.arange(d, device="cuda")
-    return digits[:, :, dim % 16, dim // 16] * scales[:, :, dim // 32]
+    return digits[:, :, dim // 64, dim % 16, dim % 64 // 16] * scales[:, :, dim // 32]
 
 
 def exact(case, seed):
