@@ -7,6 +7,7 @@
 #include <cstdlib>
 #include <cstring>
 #include <exception>
+#include <memory>
 #include <new>
 
 #include "ops.h"
@@ -215,25 +216,33 @@ static yuuka_status execute(const yuuka_op &op, const ExecCtx &ctx) {
     }
 }
 
-static yuuka_status prepare(yuuka_plan *plan) {
-    if (plan->ws_bytes < plan->ws_need) {
-        if (plan->ws) (void)hipFree(plan->ws);
-        plan->ws = nullptr;
-        plan->ws_bytes = 0;
+static void release(yk_work *w) {
+    if (w->ws) (void)hipFree(w->ws);
+    if (w->tickets) (void)hipFree(w->tickets);
+    *w = yk_work{};
+}
+
+// Grows a workspace to what the plan's ops need.
+static yuuka_status prepare(const yuuka_plan *plan, yk_work *w) {
+    if (w->ws_bytes < plan->ws_need) {
+        if (w->ws) (void)hipFree(w->ws);
+        w->ws = nullptr;
+        w->ws_bytes = 0;
         const uint64_t want = (plan->ws_need + 0xffffull) & ~0xffffull;
-        hipError_t err = hipMalloc(&plan->ws, want);
+        hipError_t err = hipMalloc(&w->ws, want);
         if (err != hipSuccess) return fail(YUUKA_ERR_ALLOCATION, "plan workspace: %s", hip_error(err));
-        plan->ws_bytes = want;
+        w->ws_bytes = want;
     }
     // split-K tickets, then the chained GEMMs' counters in the last words
-    if (plan->tickets_len < plan->ticket_need + 1) {
-        if (plan->tickets) (void)hipFree(plan->tickets);
-        plan->tickets = nullptr;
+    if (w->tickets_len < plan->ticket_need + 1) {
+        if (w->tickets) (void)hipFree(w->tickets);
+        w->tickets = nullptr;
         const uint32_t want = plan->ticket_need + 64;
-        hipError_t err = hipMalloc(reinterpret_cast<void **>(&plan->tickets), (size_t)want * 4);
-        if (err == hipSuccess) err = hipMemset(plan->tickets, 0, (size_t)want * 4);
+        hipError_t err = hipMalloc(reinterpret_cast<void **>(&w->tickets), (size_t)want * 4);
+        if (err == hipSuccess) err = hipMemset(w->tickets, 0, (size_t)want * 4);
+        if (err == hipSuccess) err = hipStreamSynchronize(nullptr);
         if (err != hipSuccess) return fail(YUUKA_ERR_ALLOCATION, "plan tickets: %s", hip_error(err));
-        plan->tickets_len = want;
+        w->tickets_len = want;
     }
     return YUUKA_OK;
 }
@@ -251,10 +260,10 @@ static yuuka_status guard(F &&f) {
     }
 }
 
-static yuuka_status run_ops(yuuka_plan *plan, hipStream_t stream, int32_t token, uint32_t position,
+static yuuka_status run_ops(const yuuka_plan *plan, const yk_work &w, hipStream_t stream, int32_t token, uint32_t position,
                             const int32_t *dyn, int run_tail, uint32_t *codes, uint64_t *times,
                             uint64_t capacity, uint64_t *count) {
-    ExecCtx ctx{stream, token, position, dyn, plan->ws, plan->tickets, plan->ws_bytes};
+    ExecCtx ctx{stream, token, position, dyn, w.ws, w.tickets, w.ws_bytes};
     ctx.part_off = plan->chain_quant ? (plan->chain_quant + 255) & ~255ull : 0;
     uint64_t n = 0;
     hipEvent_t a = nullptr, b = nullptr;
@@ -354,9 +363,9 @@ yuuka_status run_verify_gemm_op(const yuuka_op &op, hipStream_t stream, void *ws
 }
 
 yuuka_status plan_run_dynamic(yuuka_plan *plan, hipStream_t stream, const int32_t *dyn) {
-    yuuka_status st = prepare(plan);
+    yuuka_status st = prepare(plan, &plan->work);
     if (st != YUUKA_OK) return st;
-    return run_ops(plan, stream, 0, 0, dyn, 1, nullptr, nullptr, 0, nullptr);
+    return run_ops(plan, plan->work, stream, 0, 0, dyn, 1, nullptr, nullptr, 0, nullptr);
 }
 }  // namespace yk
 
@@ -375,8 +384,7 @@ yuuka_status yuuka_plan_create(yuuka_device *dev, yuuka_plan **out) {
 void yuuka_plan_destroy(yuuka_plan *plan) {
     if (!plan) return;
     (void)hipDeviceSynchronize();
-    if (plan->ws) (void)hipFree(plan->ws);
-    if (plan->tickets) (void)hipFree(plan->tickets);
+    release(&plan->work);
     delete plan;
 }
 
@@ -403,9 +411,9 @@ yuuka_status yuuka_plan_execute(yuuka_plan *plan, yuuka_stream *stream, int32_t 
                                 uint32_t position, int run_tail, yuuka_event *completion) {
     return guard([&]() -> yuuka_status {
         if (!plan || !stream) return fail(YUUKA_ERR_INVALID_ARGUMENT, "plan or stream is null");
-        yuuka_status st = prepare(plan);
+        yuuka_status st = prepare(plan, &plan->work);
         if (st != YUUKA_OK) return st;
-        st = run_ops(plan, stream->stream, token, position, nullptr, run_tail, nullptr, nullptr, 0, nullptr);
+        st = run_ops(plan, plan->work, stream->stream, token, position, nullptr, run_tail, nullptr, nullptr, 0, nullptr);
         if (st != YUUKA_OK) return st;
         hipError_t err = hipGetLastError();
         if (err != hipSuccess) return fail(YUUKA_ERR_DEVICE, "plan execute: %s", hip_error(err));
@@ -424,9 +432,9 @@ yuuka_status yuuka_plan_execute_profiled(yuuka_plan *plan, yuuka_stream *stream,
     return guard([&]() -> yuuka_status {
         if (!plan || !stream || !op_codes || !op_times_ns || !op_count)
             return fail(YUUKA_ERR_INVALID_ARGUMENT, "null argument");
-        yuuka_status st = prepare(plan);
+        yuuka_status st = prepare(plan, &plan->work);
         if (st != YUUKA_OK) return st;
-        st = run_ops(plan, stream->stream, token, position, nullptr, run_tail, op_codes, op_times_ns,
+        st = run_ops(plan, plan->work, stream->stream, token, position, nullptr, run_tail, op_codes, op_times_ns,
                      capacity, op_count);
         if (st != YUUKA_OK) return st;
         if (completion) {
@@ -448,31 +456,21 @@ yuuka_status yuuka_graph_create(yuuka_plan *plan, yuuka_stream *stream, yuuka_bu
         for (const yuuka_op &op : plan->ops)
             if (op_uses_position(op) && !dynamic)
                 return fail(YUUKA_ERR_UNSUPPORTED, "plan op %u needs a dynamic-parameter buffer", op.code);
-        yuuka_status st = prepare(plan);
+        std::unique_ptr<yuuka_graph, decltype(&yuuka_graph_destroy)> g(new yuuka_graph(), yuuka_graph_destroy);
+        yuuka_status st = prepare(plan, &g->work);
         if (st != YUUKA_OK) return st;
         hipError_t err = hipStreamSynchronize(stream->stream);
         if (err != hipSuccess) return fail(YUUKA_ERR_DEVICE, "pre-capture sync: %s", hip_error(err));
         err = hipStreamBeginCapture(stream->stream, hipStreamCaptureModeThreadLocal);
         if (err != hipSuccess) return fail(YUUKA_ERR_DEVICE, "begin capture: %s", hip_error(err));
         const int32_t *dyn = dynamic ? static_cast<const int32_t *>(dynamic->ptr) : nullptr;
-        st = run_ops(plan, stream->stream, 0, 0, dyn, run_tail, nullptr, nullptr, 0, nullptr);
-        hipGraph_t graph = nullptr;
-        err = hipStreamEndCapture(stream->stream, &graph);
-        if (st != YUUKA_OK) {
-            if (graph) (void)hipGraphDestroy(graph);
-            return st;
-        }
+        st = run_ops(plan, g->work, stream->stream, 0, 0, dyn, run_tail, nullptr, nullptr, 0, nullptr);
+        err = hipStreamEndCapture(stream->stream, &g->graph);
+        if (st != YUUKA_OK) return st;
         if (err != hipSuccess) return fail(YUUKA_ERR_DEVICE, "end capture: %s", hip_error(err));
-        hipGraphExec_t exec = nullptr;
-        err = hipGraphInstantiate(&exec, graph, nullptr, nullptr, 0);
-        if (err != hipSuccess) {
-            (void)hipGraphDestroy(graph);
-            return fail(YUUKA_ERR_DEVICE, "graph instantiate: %s", hip_error(err));
-        }
-        auto *g = new yuuka_graph();
-        g->graph = graph;
-        g->exec = exec;
-        *out = g;
+        err = hipGraphInstantiate(&g->exec, g->graph, nullptr, nullptr, 0);
+        if (err != hipSuccess) return fail(YUUKA_ERR_DEVICE, "graph instantiate: %s", hip_error(err));
+        *out = g.release();
         return YUUKA_OK;
     });
 }
@@ -494,6 +492,7 @@ void yuuka_graph_destroy(yuuka_graph *graph) {
     if (!graph) return;
     if (graph->exec) (void)hipGraphExecDestroy(graph->exec);
     if (graph->graph) (void)hipGraphDestroy(graph->graph);
+    release(&graph->work);  // (hipFree waits for the device)
     delete graph;
 }
 

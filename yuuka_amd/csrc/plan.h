@@ -5,6 +5,14 @@
 
 #include "internal.h"
 
+// Device workspace of a plan's ops.
+struct yk_work {
+    void *ws = nullptr;
+    uint64_t ws_bytes = 0;
+    uint32_t *tickets = nullptr;
+    uint32_t tickets_len = 0;
+};
+
 struct yuuka_plan {
     yuuka_device *dev = nullptr;
     std::vector<yuuka_op> ops;
@@ -12,15 +20,16 @@ struct yuuka_plan {
     uint64_t chain_quant = 0;  // many-row GEMMs: largest quantized-row area
     uint64_t chain_part = 0;   // and largest split partial-sum area (chained layout)
     uint32_t ticket_need = 0;  // split-K tickets (max over ops)
-    void *ws = nullptr;
-    uint64_t ws_bytes = 0;
-    uint32_t *tickets = nullptr;
-    uint32_t tickets_len = 0;
+    yk_work work;              // of yuuka_plan_execute; grows with the plan
 };
 
+// A captured graph holds the addresses of its workspace, so it owns one: the
+// plan may grow (and move its own) or end while the graph lives, and two
+// graphs, of one plan too, may run at once.
 struct yuuka_graph {
     hipGraph_t graph = nullptr;
     hipGraphExec_t exec = nullptr;
+    yk_work work;
 };
 
 namespace yk {
