@@ -439,8 +439,8 @@ YUUKA_API yuuka_status yuuka_verify_accept_noalloc(yuuka_stream * stream,
  *               buf5 FP32 out [rows][heads][head_dim], buf6 int32 block
  *               table, buf7 q_norm [head_dim], buf8 k_norm [head_dim],
  *               buf9 ROPE_TABLE output; n={kv_heads, heads, head_dim, kv_dim,
- *               rows, displacement}; u={block_size, capacity, kv dtype (F32 or
- *               F16), rot_dim | requests << 8 | request_rows << 20};
+ *               rows, displacement}; u={block_size, capacity, kv dtype (F32,
+ *               F16 or Q8_0), rot_dim | requests << 8 | request_rows << 20};
  *               f={scale, eps}. Writes the rows' K/V to the pool at position
  *               + displacement + row. With requests > 1 (and OWN_POS) request
  *               j's rows start request_rows rows after request j-1's, its
@@ -482,6 +482,30 @@ YUUKA_API yuuka_status yuuka_verify_accept_noalloc(yuuka_stream * stream,
  *               uint64 step counter (0 when null); n={rows, experts, seed,
  *               layer}. */
 #define YUUKA_EXT_OP_ROUTER_NORMAL 74u
+/* Paged key/value cache of a batch of requests, F32, F16 or Q8_0 pages (the
+ * direct calls yuuka_kv_append, yuuka_kv_read and yuuka_attn_decode below say
+ * what each computes; the v10 ops KV_WRITE_PAGED, KV_WRITE_BATCH_PAGED,
+ * ATTENTION_PAGED and ATTENTION_PREFILL_PAGED, ATTN_VERIFY and
+ * yuuka_q35_config.kv_dtype take YUUKA_DTYPE_Q8_0 pools of this layout too).
+ * Positions come from the plan's dynamic parameters, or with
+ * YUUKA_EXT_FLAG_OWN_POS from the requests' {token, position} pairs in buf15;
+ * several requests need their own.
+ *   KV_APPEND:  buf0 FP32 k rows, buf1 v rows, buf2 K pool, buf3 V pool, buf4
+ *               int32 block tables, optional buf5 k_norm [head_dim], optional
+ *               buf6 ROPE_TABLE output; n={kv_heads, 0, head_dim, kv_dim, rows,
+ *               displacement}; u={block_size, capacity, dtype, rot_dim |
+ *               requests << 8 | request_rows << 20}; f1 eps.
+ *   KV_READ:    buf0 K pool, buf1 V pool, buf2 FP32 k rows, buf3 v rows (a pool
+ *               and its rows may both be null), buf4 block tables; n and u as
+ *               KV_APPEND without rotation. Without OWN_POS the rows start at
+ *               position `displacement`.
+ *   ATTN_DECODE: buf0 FP32 q rows, buf1 K pool, buf2 V pool, buf3 FP32 out,
+ *               buf4 block tables; n={kv_heads, heads, head_dim, kv_dim, rows,
+ *               displacement}; u={block_size, capacity, dtype, gated |
+ *               requests << 8 | request_rows << 20}; f0 scale. */
+#define YUUKA_EXT_OP_KV_APPEND 75u
+#define YUUKA_EXT_OP_KV_READ 76u
+#define YUUKA_EXT_OP_ATTN_DECODE 77u
 #define YUUKA_EXT_FLAG_DEFER 0x100u
 /* With YUUKA_EXT_FLAG_DEFER: buf10 receives the raw per-head scan outputs;
  * the gated RMSNorm is left to the consumer (GEMM_FUSED gated head norm). */
@@ -517,6 +541,81 @@ YUUKA_API yuuka_status yuuka_verify_accept_noalloc(yuuka_stream * stream,
  * GGUF rows directly). */
 YUUKA_API yuuka_status yuuka_moe_pack_q4k(yuuka_stream * stream, yuuka_buffer * dst, const yuuka_buffer * src,
                         uint64_t rows, uint64_t n_in, yuuka_event * completion);
+
+/* ----------------------------------------------------------------------
+ * Paged key/value cache of a batch of requests (extension; the reference's
+ * Q8_0 cache format is model/qwen35/kv_format.go, its device codec
+ * kernels/hip/kv.cuh).
+ *
+ * A pool is an array of pages of block_size tokens. F32 and F16 pages are
+ * [block_size][kv_dim] (kv_dim = kv_heads * head_dim; F16 rounds half up, as
+ * the v10 KV writes). A Q8_0 page is [block_size][kv_dim] int8 digits followed
+ * by [block_size][kv_dim / 32] F16 scales; a value is digit * scale of its block
+ * of 32 dims. Every 64 dims' digits are stored as a 16 x 4 matrix: byte
+ * 4 r + j of the 64 holds dim 16 j + r. Rounding, in FP32 as the reference's
+ * kv_format.go:93-137: s = max|x| / 127, scale = F16(s), half up; digit = x / s
+ * to the nearest, halves away from zero. A block holding a NaN reads back as
+ * NaN, one past the scale's range (|x| over 8.3e6) as infinities and NaN.
+ *
+ * Request j's block table is the j-th run of ceil(capacity / block_size) int32
+ * page indices. An entry outside the pool (such as -1) is an unmapped page:
+ * writes to it are dropped, it reads back as zeros, and attention leaves its
+ * tokens out. The same holds for positions below 0 and from `capacity` on.
+ * A position that two rows write in one call, through one page in two tables,
+ * holds either row's bytes.
+ *
+ * `positions` holds request j's {token, position} int32 pair at 8 j (the
+ * device state that ADVANCE moves). Row r of request j is at position +
+ * displacement + r; its rows start request_rows rows after request j-1's, and
+ * rows in between are neither read nor written. Every buffer has to be on the
+ * stream's device. Calls on one stream run in order; yuuka_attn_decode keeps its
+ * partial results in the stream's workspace.
+ * ---------------------------------------------------------------------- */
+typedef struct yuuka_kv_params {
+    uint32_t dtype;       /* YUUKA_DTYPE_F32, F16 or Q8_0 */
+    int32_t block_size;   /* tokens per page */
+    int32_t capacity;     /* tokens a request can hold */
+    int32_t requests;     /* 1..65535 */
+    int32_t rows;         /* rows of every request */
+    int32_t request_rows; /* rows between consecutive requests (0: rows) */
+    int32_t heads;        /* query heads, a multiple of kv_heads (attention) */
+    int32_t kv_heads;
+    int32_t head_dim;     /* 64, 128, 192 or 256 */
+    int32_t rope_dim;     /* append: rotated dimensions of a key, <= 128 (0: none) */
+    int32_t gated;        /* attention: query rows hold [q | gate] per head */
+    int32_t displacement;
+    float scale;          /* attention: factor of q . k */
+    float eps;            /* append: of the key norm */
+} yuuka_kv_params;
+
+/* Bytes of one page of one pool; 0 when the parameters are not served. */
+YUUKA_API uint64_t yuuka_kv_page_bytes(const yuuka_kv_params * params);
+
+/* Rounds rows k and v [.][kv_dim] (FP32) into the pools. With k_norm
+ * [head_dim] the keys first take the per-head RMSNorm (forward.go:472-482),
+ * with rope_dim the rotation by `rope`, {cos, sin} [.][rope_dim / 2] of every
+ * row as ROPE_TABLE writes it (forward.go:495-514); null otherwise. */
+YUUKA_API yuuka_status yuuka_kv_append(yuuka_stream * stream, const yuuka_buffer * k, const yuuka_buffer * v,
+                        yuuka_buffer * kpool, yuuka_buffer * vpool, const yuuka_buffer * table,
+                        const yuuka_buffer * positions, const yuuka_buffer * k_norm, const yuuka_buffer * rope,
+                        const yuuka_kv_params * params, yuuka_event * completion);
+
+/* Reads rows back as FP32 [.][kv_dim]. Either side's pool and output may both
+ * be null; positions may be null (0). */
+YUUKA_API yuuka_status yuuka_kv_read(yuuka_stream * stream, yuuka_buffer * k_out, yuuka_buffer * v_out,
+                        const yuuka_buffer * kpool, const yuuka_buffer * vpool, const yuuka_buffer * table,
+                        const yuuka_buffer * positions, const yuuka_kv_params * params, yuuka_event * completion);
+
+/* Attention of the rows' queries over their request's cached keys at positions
+ * up to the row's own (the rows' keys are appended before):
+ *   out[h] = sum_t softmax_t(scale q[h] . k_t) v_t [* sigmoid(gate[h])]
+ * with kv head h / (heads / kv_heads). q is [.][heads][head_dim] FP32, or
+ * [.][heads][2 * head_dim] holding [q | gate]; out [.][heads][head_dim]. F16 and
+ * Q8_0 pools. At most 4096 rows. A row that sees no key is zero. A non-finite
+ * query or visible key or value makes its rows NaN. */
+YUUKA_API yuuka_status yuuka_attn_decode(yuuka_stream * stream, yuuka_buffer * out, const yuuka_buffer * q,
+                        const yuuka_buffer * kpool, const yuuka_buffer * vpool, const yuuka_buffer * table,
+                        const yuuka_buffer * positions, const yuuka_kv_params * params, yuuka_event * completion);
 
 /* Timing events (extension): an event created with timing enabled, recorded
  * on a stream, and the elapsed milliseconds between two recorded events. */
@@ -557,7 +656,7 @@ typedef struct yuuka_q35_config {
     float eps;
     int32_t capacity;    /* tokens of context per request */
     int32_t block_size;  /* paged KV block (16) */
-    uint32_t kv_dtype;   /* YUUKA_DTYPE_F16 (reference default) or F32 */
+    uint32_t kv_dtype;   /* YUUKA_DTYPE_F16 (reference default), F32 or Q8_0 */
     int32_t max_rows;    /* largest row block of one request in one step (<= 32) */
     int32_t batch;       /* concurrent requests (0 means 1) */
     int32_t kv_blocks;   /* blocks of the KV pool the requests share (0: every

@@ -1,0 +1,334 @@
+"""CPU checks of the paged key/value cache: page addressing (kv_addr.h compiled
+for the host) and the refusals of the direct calls and plan ops, which are
+decided before anything is launched."""
+import ctypes as C
+import shutil
+import subprocess
+from pathlib import Path
+
+import pytest
+
+from yuuka_amd import hip
+
+CSRC = Path(__file__).resolve().parent.parent / "yuuka_amd" / "csrc"
+
+PROGRAM = r"""
+#include "kv_addr.h"
+#include <cstdio>
+#include <map>
+#include <random>
+#include <vector>
+
+using namespace yk;
+
+int main() {
+    std::mt19937 rng(5);
+    auto pick = [&](int lo, int hi) { return lo + (int)(rng() % (unsigned)(hi - lo + 1)); };
+    long inside = 0, dropped = 0, bad = 0;
+    for (int trial = 0; trial < 4000; trial++) {
+        KvLayout a;
+        a.fmt = pick(0, 2);
+        a.block_size = pick(1, 40);
+        a.capacity = trial % 7 ? pick(1, 300) : pick(1, 5);
+        a.kv_dim = 64 * pick(1, 16);
+        a.pages = pick(1, 40);
+        const int requests = pick(1, 3), blocks = kv_table_blocks(a);
+        if ((int64_t)blocks * a.block_size < a.capacity || (int64_t)(blocks - 1) * a.block_size >= a.capacity) bad++;
+        // entries inside, on and outside the pool's borders; canaries around the table
+        std::vector<int32_t> table(requests * blocks + 2, 0x7eadbeef);
+        for (int i = 0; i < requests * blocks; i++) {
+            const int edge[] = {-1, a.pages, a.pages - 1, 0, INT32_MIN, INT32_MAX};
+            table[i + 1] = pick(0, 2) ? pick(0, a.pages - 1) : edge[pick(0, 5)];
+        }
+        const int64_t pool = kv_page_bytes(a) * a.pages, row_bytes = a.fmt == kKvQ8 ? a.kv_dim : kv_token_bytes(a.fmt, a.kv_dim);
+        std::map<int64_t, int64_t> taken;  // byte runs by start, of distinct (page, token) pairs
+        for (int j = 0; j < requests; j++)
+            for (int64_t p : {(int64_t)-1, (int64_t)INT32_MIN - 5, (int64_t)0, (int64_t)a.capacity - 1, (int64_t)a.capacity,
+                              (int64_t)INT32_MAX + 9, (int64_t)pick(0, a.capacity - 1)}) {
+                int64_t row = -1, scales = -1;
+                const bool ok = kv_slot(a, table.data() + 1, j, p, &row, &scales);
+                const bool within = p >= 0 && p < a.capacity;
+                const int page = within ? table[1 + j * blocks + (int)(p / a.block_size)] : -1;
+                if (ok != (within && page >= 0 && page < a.pages)) bad++;
+                if (!ok) { dropped++; continue; }
+                inside++;
+                if (row < 0 || row + row_bytes > pool || row % 4) bad++;
+                if (a.fmt == kKvQ8 && (scales < row || scales + a.kv_dim / 16 > pool || scales % 4)) bad++;
+                if (row / kv_page_bytes(a) != page) bad++;
+                if (a.fmt == kKvQ8 && (scales + a.kv_dim / 16 - 1) / kv_page_bytes(a) != page) bad++;
+            }
+    }
+    // a page's rows and scales cover it once
+    for (int fmt = 0; fmt < 3; fmt++) {
+        KvLayout a{fmt, 7, 21, 192, 3};
+        int32_t table[3] = {2, 0, 1};
+        std::vector<int> hits(kv_page_bytes(a) * 3);
+        for (int p = 0; p < 21; p++) {
+            int64_t row, scales;
+            if (!kv_slot(a, table, 0, p, &row, &scales)) bad++;
+            for (int64_t i = 0; i < (fmt == kKvQ8 ? 192 : kv_token_bytes(fmt, 192)); i++) hits[row + i]++;
+            if (fmt == kKvQ8) for (int i = 0; i < 12; i++) hits[scales + i]++;
+        }
+        for (int h : hits) bad += h != 1;
+    }
+    // offsets past 32 bits
+    KvLayout a{kKvQ8, 16, 1 << 24, 1024, 1 << 20};
+    std::vector<int32_t> table(kv_table_blocks(a), (1 << 20) - 1);
+    int64_t row, scales;
+    if (!kv_slot(a, table.data(), 0, (1 << 24) - 1, &row, &scales) || scales + 64 != kv_page_bytes(a) << 20) bad++;
+    printf("%ld %ld %ld\n", inside > 5000, dropped > 5000, bad);
+}
+"""
+
+
+def test_no_table_or_position_leads_outside_the_pool(tmp_path):
+    cxx = shutil.which("g++") or shutil.which("clang++")
+    if not cxx:
+        pytest.skip("no host C++ compiler")
+    src = tmp_path / "addr.cpp"
+    src.write_text(PROGRAM)
+    subprocess.run([cxx, "-O1", "-std=c++17", "-Wall", "-fsanitize=undefined", "-fno-sanitize-recover", f"-I{CSRC}",
+                    str(src), "-o", str(tmp_path / "addr")], check=True)
+    out = subprocess.run([str(tmp_path / "addr")], check=True, capture_output=True, text=True).stdout
+    assert out.split() == ["1", "1", "0"]
+
+
+# Handles as the library lays them out (internal.h), over no device memory: a
+# call that gets past its checks would be refused by the missing device, with
+# another status than the ones asked for here.
+
+class _Handle(C.Structure):
+    _fields_ = [("dev", C.c_void_p), ("ptr", C.c_void_p), ("bytes", C.c_uint64)]
+
+
+class _Stream(C.Structure):
+    _fields_ = [("dev", C.c_void_p), ("stream", C.c_void_p), ("areas", C.c_uint64 * 4)]
+
+
+class _Mem:
+    def __init__(self, nbytes):
+        self.handle = _Handle(None, 4096, nbytes)
+        self.ptr = C.c_void_p(C.addressof(self.handle))
+
+
+GOOD = dict(dtype=hip.Q8_0, block_size=16, capacity=100, kv_heads=2, head_dim=128, rows=3, requests=2)
+KVD, PAGES = 256, 14
+
+
+def _memory(dtype=hip.Q8_0, heads=4, gated=False):
+    token = {hip.F32: 4 * KVD, hip.F16: 2 * KVD, hip.Q8_0: KVD * 34 // 32}[dtype]
+    return dict(k=_Mem(6 * KVD * 4), v=_Mem(6 * KVD * 4), kpool=_Mem(PAGES * 16 * token), vpool=_Mem(PAGES * 16 * token),
+                table=_Mem(2 * 7 * 4), positions=_Mem(16), norm=_Mem(128 * 4), rope=_Mem(6 * 32 * 8),
+                q=_Mem(6 * heads * 128 * 4 * (2 if gated else 1)), out=_Mem(6 * heads * 128 * 4))
+
+
+def _call(name, m, p):
+    """The status of a direct call on a stream without a device."""
+    raw = _Stream()
+    s = C.c_void_p(C.addressof(raw))
+    g = lambda n: m[n].ptr if m.get(n) is not None else None  # noqa: E731
+    L = hip.lib()
+    if name == "append":
+        return L.yuuka_kv_append(s, g("k"), g("v"), g("kpool"), g("vpool"), g("table"), g("positions"), g("norm"),
+                                 g("rope"), C.byref(p), None)
+    if name == "read":
+        return L.yuuka_kv_read(s, g("k"), g("v"), g("kpool"), g("vpool"), g("table"), g("positions"), C.byref(p), None)
+    return L.yuuka_attn_decode(s, g("out"), g("q"), g("kpool"), g("vpool"), g("table"), g("positions"), C.byref(p), None)
+
+
+SHAPES = [
+    (dict(dtype=hip.Q4_K), hip.UNSUPPORTED), (dict(dtype=99), hip.UNSUPPORTED),
+    (dict(head_dim=32), hip.UNSUPPORTED), (dict(head_dim=96), hip.UNSUPPORTED), (dict(head_dim=320), hip.UNSUPPORTED),
+    (dict(head_dim=0), hip.UNSUPPORTED), (dict(head_dim=-64), hip.UNSUPPORTED),
+    (dict(block_size=0), hip.INVALID_ARGUMENT), (dict(block_size=-16), hip.INVALID_ARGUMENT),
+    (dict(capacity=0), hip.INVALID_ARGUMENT), (dict(capacity=-5), hip.INVALID_ARGUMENT),
+    (dict(requests=0), hip.INVALID_ARGUMENT), (dict(requests=65536), hip.INVALID_ARGUMENT),
+    (dict(rows=0), hip.INVALID_ARGUMENT), (dict(rows=-1), hip.INVALID_ARGUMENT),
+    (dict(rows=1 << 29), hip.INVALID_ARGUMENT), (dict(request_rows=-3), hip.INVALID_ARGUMENT),
+    (dict(kv_heads=0), hip.INVALID_ARGUMENT), (dict(kv_heads=5000), hip.INVALID_ARGUMENT),
+    (dict(displacement=-(1 << 31)), hip.INVALID_ARGUMENT), (dict(displacement=(1 << 31) - 1), hip.INVALID_ARGUMENT),
+]
+
+
+@pytest.mark.parametrize("name", ["append", "read", "attn"])
+@pytest.mark.parametrize("change,status", SHAPES)
+def test_direct_calls_refuse_shapes(name, change, status):
+    extra = dict(heads=4) if name == "attn" else {}
+    m = _memory()
+    m.update(norm=None, rope=None)
+    assert _call(name, m, hip.kv_params(**{**GOOD, **extra, **change})) == status
+    assert hip.lib().yuuka_last_error()
+
+
+@pytest.mark.parametrize("change,status", [
+    (dict(dtype=hip.F32), hip.UNSUPPORTED), (dict(heads=0), hip.INVALID_ARGUMENT), (dict(heads=3), hip.INVALID_ARGUMENT),
+    (dict(heads=-4), hip.INVALID_ARGUMENT), (dict(heads=65538), hip.INVALID_ARGUMENT),
+    (dict(rows=4097), hip.INVALID_ARGUMENT)])
+def test_attention_refuses_heads_and_rows(change, status):
+    assert _call("attn", _memory(), hip.kv_params(**{**GOOD, "heads": 4, **change})) == status
+
+
+@pytest.mark.parametrize("name,small", [(n, b) for n, bs in dict(
+    append=("k", "v", "kpool", "vpool", "table", "positions", "norm", "rope"),
+    read=("k", "v", "kpool", "vpool", "table", "positions"),
+    attn=("q", "out", "kpool", "vpool", "table", "positions")).items() for b in bs])
+def test_direct_calls_refuse_missing_and_short_buffers(name, small):
+    p = hip.kv_params(**GOOD, heads=4, rope_dim=64)
+    m = _memory()
+    # a pool may hold fewer pages than the tables could name, but not less than one
+    m[small].handle.bytes = 16 * (KVD * 34 // 32) - 1 if small in ("kpool", "vpool") else m[small].handle.bytes - 1
+    assert _call(name, m, p) == hip.INVALID_ARGUMENT
+    m = _memory()
+    m[small] = None
+    if (name, small) not in (("append", "norm"), ("read", "positions")):
+        assert _call(name, m, p) == hip.INVALID_ARGUMENT
+
+
+def test_a_rotation_needs_its_table_and_its_width():
+    m = _memory()
+    assert _call("append", m, hip.kv_params(**GOOD, rope_dim=0)) == hip.INVALID_ARGUMENT   # a table, no width
+    for width in (-2, 3, 130, 256):
+        assert _call("append", m, hip.kv_params(**GOOD, rope_dim=width)) == hip.INVALID_ARGUMENT
+    m["rope"] = None
+    assert _call("append", m, hip.kv_params(**GOOD, rope_dim=64)) == hip.INVALID_ARGUMENT  # a width, no table
+
+
+def test_the_gate_doubles_the_query_rows():
+    assert _call("attn", _memory(), hip.kv_params(**GOOD, heads=4, gated=True)) == hip.INVALID_ARGUMENT
+
+
+def test_buffers_of_another_device_are_refused():
+    # yuuka_device starts with its index
+    one, two = C.c_int32(0), C.c_int32(1)
+    for name, moved in (("append", "vpool"), ("read", "table"), ("attn", "positions")):
+        m = _memory()
+        m.update(norm=None, rope=None)
+        raw = _Stream(dev=C.addressof(one))
+        for b in m.values():
+            if b is not None:
+                b.handle.dev = C.addressof(one)
+        m[moved].handle.dev = C.addressof(two)
+        s, p = C.c_void_p(C.addressof(raw)), hip.kv_params(**GOOD, heads=4)
+        g = lambda n: m[n].ptr  # noqa: E731
+        L = hip.lib()
+        st = (L.yuuka_kv_append(s, g("k"), g("v"), g("kpool"), g("vpool"), g("table"), g("positions"), None, None,
+                                C.byref(p), None) if name == "append" else
+              L.yuuka_kv_read(s, g("k"), g("v"), g("kpool"), g("vpool"), g("table"), g("positions"), C.byref(p), None)
+              if name == "read" else
+              L.yuuka_attn_decode(s, g("out"), g("q"), g("kpool"), g("vpool"), g("table"), g("positions"), C.byref(p),
+                                  None))
+        assert st == hip.INVALID_ARGUMENT
+        assert b"device 1" in L.yuuka_last_error()
+
+
+@pytest.mark.parametrize("dtype,token", [(hip.F32, 1024), (hip.F16, 512), (hip.Q8_0, 272)])
+def test_page_bytes(dtype, token):
+    assert hip.kv_page_bytes(hip.kv_params(**{**GOOD, "dtype": dtype})) == 16 * token
+    assert hip.kv_page_bytes(hip.kv_params(**{**GOOD, "dtype": dtype, "head_dim": 80})) == 0
+    assert hip.kv_page_bytes(hip.kv_params(**{**GOOD, "dtype": hip.Q6_K})) == 0
+
+
+# ---------------------------------------------------------------- plan ops
+
+class _Plan:
+    """A plan that only records: it is never executed."""
+
+    def __init__(self):
+        p = C.c_void_p()
+        self.dev = C.create_string_buffer(8192)
+        hip.check(hip.lib().yuuka_plan_create(C.addressof(self.dev), C.byref(p)), "plan_create")
+        self.ptr = p
+
+    def add(self, name, bufs, n, u, f=(), offs=(), flags=0):
+        op = hip.yuuka_op()
+        op.code, op.flags = OPS[name], flags
+        for i, b in enumerate(bufs):
+            op.buf[i] = None if b is None else b.ptr.value
+        for i, v in enumerate(offs):
+            op.off[i] = v
+        for i, v in enumerate(n):
+            op.n[i] = v
+        for i, v in enumerate(u):
+            op.u[i] = v
+        for i, v in enumerate(f):
+            op.f[i] = v
+        return hip.lib().yuuka_plan_add(self.ptr, C.byref(op))
+
+
+OPS = dict(hip.OP, KV_WRITE_PAGED=26, ATTENTION_PAGED=27)
+_U = lambda low=0, requests=2, stride=0: low | requests << 8 | stride << 20  # noqa: E731
+
+
+def _ops(m):
+    """The ops over Q8_0 pools, each as it is accepted: (name, buffers, n, u, flags)."""
+    pos = m["positions"]
+
+    def bufs(*b):
+        return list(b) + [None] * (15 - len(b)) + [pos]
+
+    n, au = [2, 4, 128, KVD, 3, 0], [16, 100, hip.Q8_0]
+    return {
+        "KV_APPEND": (bufs(m["k"], m["v"], m["kpool"], m["vpool"], m["table"], m["norm"], m["rope"]),
+                      [2, 0, 128, KVD, 3, 0], au + [_U(64)], hip.FLAG_OWN_POS),
+        "KV_READ": (bufs(m["kpool"], m["vpool"], m["k"], m["v"], m["table"]), [2, 0, 128, KVD, 3, 0], au + [_U()], 0),
+        "ATTN_DECODE": (bufs(m["q"], m["kpool"], m["vpool"], m["out"], m["table"]), n, au + [_U(0)], hip.FLAG_OWN_POS),
+        "ATTN_VERIFY": (bufs(_Mem(6 * 4 * 256 * 4), m["k"], m["v"], m["kpool"], m["vpool"], m["out"], m["table"],
+                             m["norm"], m["norm"], m["rope"]), n, au + [_U(64)], hip.FLAG_OWN_POS),
+        "KV_WRITE_PAGED": ([m["k"], m["v"], m["kpool"], m["vpool"], m["table"]], [KVD], au, 0),
+        "KV_WRITE_BATCH_PAGED": ([m["k"], m["v"], m["kpool"], m["vpool"], m["table"]], [KVD, 6], au, 0),
+        "ATTENTION_PAGED": ([m["q"], m["kpool"], m["vpool"], m["out"], None, m["table"]], [2, 4, 128, KVD, 100],
+                            au + [1], 0),
+        "ATTENTION_PREFILL_PAGED": ([m["q"], m["kpool"], m["vpool"], m["out"], m["table"]], [2, 4, 128, KVD, 6, 0],
+                                    au + [1], 0),
+    }
+
+
+@pytest.mark.parametrize("name", sorted(_ops(_memory())))
+def test_plan_ops_over_q8_0_pools(name):
+    plan = _Plan()
+    bufs, n, u, flags = _ops(_memory())[name]
+    assert plan.add(name, bufs, n, u, flags=flags) == hip.OK, hip.lib().yuuka_last_error()
+    # a width that is not the heads', an unknown dtype, no capacity
+    wrong = list(n)
+    wrong[0 if "WRITE" in name else 3] += 32
+    assert plan.add(name, bufs, wrong, u, flags=flags) == hip.INVALID_ARGUMENT
+    assert plan.add(name, bufs, n, [16, 100, 77] + list(u[3:]), flags=flags) == hip.UNSUPPORTED
+    assert plan.add(name, bufs, n, [16, 0, hip.Q8_0] + list(u[3:]), flags=flags) == hip.INVALID_ARGUMENT
+    assert plan.add(name, bufs, n, [0, 100, hip.Q8_0] + list(u[3:]), flags=flags) == hip.INVALID_ARGUMENT
+    # each buffer: missing, too short, and at an offset that leaves too little or is misaligned
+    for i, b in enumerate(bufs):
+        if b is None or (b is bufs[-1] and not flags):
+            continue
+        if (name, i) not in (("KV_APPEND", 5),):
+            less = list(bufs)
+            less[i] = None
+            assert plan.add(name, less, n, u, flags=flags) == hip.INVALID_ARGUMENT, (name, i, "missing")
+        offs = [0] * 16
+        offs[i] = b.handle.bytes
+        assert plan.add(name, bufs, n, u, offs=offs, flags=flags) == hip.INVALID_ARGUMENT, (name, i, "offset")
+        offs[i] = 2
+        assert plan.add(name, bufs, n, u, offs=offs, flags=flags) == hip.INVALID_ARGUMENT, (name, i, "aligned")
+
+
+@pytest.mark.parametrize("name", ["KV_APPEND", "ATTN_DECODE", "ATTN_VERIFY"])
+def test_several_requests_need_their_own_positions(name):
+    plan = _Plan()
+    bufs, n, u, _ = _ops(_memory())[name]
+    assert plan.add(name, bufs, n, u, flags=0) == hip.INVALID_ARGUMENT
+
+
+@pytest.mark.parametrize("disp,status", [(2 ** 64 - 3, hip.OK), (5, hip.OK), (2 ** 40, hip.INVALID_ARGUMENT),
+                                         (2 ** 63, hip.INVALID_ARGUMENT), (2 ** 31, hip.INVALID_ARGUMENT)])
+def test_displacements_are_signed(disp, status):
+    plan = _Plan()
+    bufs, n, u, flags = _ops(_memory())["KV_READ"]
+    assert plan.add("KV_READ", bufs, n[:5] + [disp], u, flags=flags) == status
+
+
+def test_prefill_attention_takes_16_rows():
+    plan = _Plan()
+    m = _memory()
+    m["q"], m["out"] = _Mem(17 * 4 * 128 * 4), _Mem(17 * 4 * 128 * 4)
+    bufs, n, u, flags = _ops(m)["ATTENTION_PREFILL_PAGED"]
+    for rows, status in ((16, hip.OK), (17, hip.INVALID_ARGUMENT)):
+        assert plan.add("ATTENTION_PREFILL_PAGED", bufs, n[:4] + [rows, 0], u, flags=flags) == status

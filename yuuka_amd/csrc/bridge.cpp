@@ -17,6 +17,7 @@
 #include <vector>
 
 #include "internal.h"
+#include "kv.h"
 #include "model_kernels.h"
 #include "ops.h"
 #include "plan.h"
@@ -56,6 +57,7 @@ yuuka_status ensure_scratch(yuuka_stream *stream, yk_scratch *area, uint64_t byt
                     hip_error(err));
     }
     err = hipMemset(area->ptr, 0, want);
+    if (err == hipSuccess) err = hipStreamSynchronize(nullptr);  // the stream does not wait for the default one
     if (err != hipSuccess) return fail(YUUKA_ERR_DEVICE, "workspace clear: %s", hip_error(err));
     area->bytes = want;
     return YUUKA_OK;
@@ -632,6 +634,130 @@ yuuka_status yuuka_verify_accept_noalloc(yuuka_stream *stream, const yuuka_buffe
             reinterpret_cast<int32_t *>(static_cast<uint8_t *>(result->ptr) + result_offset), nullptr, p,
             stream->dev->noalloc_scratch, stream->stream);
         if (err != hipSuccess) return fail(YUUKA_ERR_DEVICE, "accept launch: %s", hip_error(err));
+        return record(stream, completion);
+    });
+}
+
+// The launch arguments of a KV-cache call, checked.
+static yuuka_status kv_args(const yuuka_kv_params &p, bool attention, KvArgs *a) {
+    *a = KvArgs{};
+    a->block_size = p.block_size;
+    a->capacity = p.capacity;
+    a->requests = p.requests;
+    a->rows = p.rows;
+    a->rq_rows = p.request_rows;
+    a->heads = attention ? p.heads : 0;
+    a->kv_heads = p.kv_heads;
+    a->head_dim = p.head_dim;
+    a->rope_dim = attention ? 0 : p.rope_dim;
+    a->gated = attention && p.gated;
+    a->displacement = p.displacement;
+    a->scale = p.scale;
+    a->eps = p.eps;
+    if (p.request_rows < 0) return fail(YUUKA_ERR_INVALID_ARGUMENT, "KV cache: %d rows between requests", p.request_rows);
+    return kv_check(a, p.dtype, attention);
+}
+
+// The buffers' device: the stream's, made current for the launches.
+static yuuka_status kv_device(yuuka_stream *stream, std::initializer_list<const yuuka_buffer *> bufs) {
+    for (const yuuka_buffer *b : bufs)
+        if (b && b->dev && stream->dev && b->dev->index != stream->dev->index)
+            return fail(YUUKA_ERR_INVALID_ARGUMENT, "KV cache: a buffer of device %d on a stream of device %d",
+                        b->dev->index, stream->dev->index);
+    if (stream->dev) {
+        const hipError_t err = hipSetDevice(stream->dev->index);
+        if (err != hipSuccess) return fail(YUUKA_ERR_DEVICE, "set device: %s", hip_error(err));
+    }
+    return YUUKA_OK;
+}
+
+uint64_t yuuka_kv_page_bytes(const yuuka_kv_params *params) {
+    KvArgs a;
+    return params && kv_args(*params, false, &a) == YUUKA_OK ? (uint64_t)kv_page_bytes(a) : 0;
+}
+
+yuuka_status yuuka_kv_append(yuuka_stream *stream, const yuuka_buffer *k, const yuuka_buffer *v, yuuka_buffer *kpool,
+                             yuuka_buffer *vpool, const yuuka_buffer *table, const yuuka_buffer *positions,
+                             const yuuka_buffer *k_norm, const yuuka_buffer *rope, const yuuka_kv_params *params,
+                             yuuka_event *completion) {
+    return guard("kv_append", [&]() -> yuuka_status {
+        if (!stream || !k || !v || !kpool || !vpool || !table || !positions || !params)
+            return fail(YUUKA_ERR_INVALID_ARGUMENT, "null argument");
+        KvArgs a;
+        yuuka_status st = kv_args(*params, false, &a);
+        if (st != YUUKA_OK) return st;
+        if ((a.rope_dim != 0) != (rope != nullptr))
+            return fail(YUUKA_ERR_INVALID_ARGUMENT, "kv_append: a rotation needs rope_dim and its table");
+        const uint64_t rows = kv_span_rows(a);
+        a.pages = kv_pages(a, kpool->bytes, vpool->bytes);
+        if (!range_ok(k, 0, rows * a.kv_dim * 4) || !range_ok(v, 0, rows * a.kv_dim * 4) || !a.pages ||
+            !range_ok(table, 0, kv_table_entries(a) * 4) || !range_ok(positions, 0, 8ull * a.requests) ||
+            (k_norm && !range_ok(k_norm, 0, a.head_dim * 4ull)) ||
+            (rope && !range_ok(rope, 0, rows * (a.rope_dim / 2) * 8)))
+            return fail(YUUKA_ERR_INVALID_ARGUMENT, "kv_append buffers too small");
+        st = kv_device(stream, {k, v, kpool, vpool, table, positions, k_norm, rope});
+        if (st != YUUKA_OK) return st;
+        const ModelDyn dyn{static_cast<int32_t *>(positions->ptr) + 1, 0};
+        const hipError_t err = launch_kv_append(
+            static_cast<const float *>(k->ptr), static_cast<const float *>(v->ptr), kpool->ptr, vpool->ptr,
+            static_cast<const int32_t *>(table->ptr), k_norm ? static_cast<const float *>(k_norm->ptr) : nullptr,
+            rope ? static_cast<const float2 *>(rope->ptr) : nullptr, nullptr, nullptr, nullptr, a, dyn, stream->stream);
+        if (err != hipSuccess) return fail(YUUKA_ERR_DEVICE, "kv_append launch: %s", hip_error(err));
+        return record(stream, completion);
+    });
+}
+
+yuuka_status yuuka_kv_read(yuuka_stream *stream, yuuka_buffer *k_out, yuuka_buffer *v_out, const yuuka_buffer *kpool,
+                           const yuuka_buffer *vpool, const yuuka_buffer *table, const yuuka_buffer *positions,
+                           const yuuka_kv_params *params, yuuka_event *completion) {
+    return guard("kv_read", [&]() -> yuuka_status {
+        if (!stream || !table || !params || !k_out != !kpool || !v_out != !vpool || (!kpool && !vpool))
+            return fail(YUUKA_ERR_INVALID_ARGUMENT, "null argument");
+        KvArgs a;
+        yuuka_status st = kv_args(*params, false, &a);
+        if (st != YUUKA_OK) return st;
+        const uint64_t out = kv_span_rows(a) * a.kv_dim * 4;
+        a.pages = kv_pages(a, kpool ? kpool->bytes : ~0ull, vpool ? vpool->bytes : ~0ull);
+        if ((k_out && !range_ok(k_out, 0, out)) || (v_out && !range_ok(v_out, 0, out)) || !a.pages ||
+            !range_ok(table, 0, kv_table_entries(a) * 4) || (positions && !range_ok(positions, 0, 8ull * a.requests)))
+            return fail(YUUKA_ERR_INVALID_ARGUMENT, "kv_read buffers too small");
+        st = kv_device(stream, {k_out, v_out, kpool, vpool, table, positions});
+        if (st != YUUKA_OK) return st;
+        const ModelDyn dyn{positions ? static_cast<int32_t *>(positions->ptr) + 1 : nullptr, 0};
+        const hipError_t err =
+            launch_kv_read(kpool ? kpool->ptr : nullptr, vpool ? vpool->ptr : nullptr,
+                           static_cast<const int32_t *>(table->ptr), k_out ? static_cast<float *>(k_out->ptr) : nullptr,
+                           v_out ? static_cast<float *>(v_out->ptr) : nullptr, a, dyn, stream->stream);
+        if (err != hipSuccess) return fail(YUUKA_ERR_DEVICE, "kv_read launch: %s", hip_error(err));
+        return record(stream, completion);
+    });
+}
+
+yuuka_status yuuka_attn_decode(yuuka_stream *stream, yuuka_buffer *out, const yuuka_buffer *q,
+                               const yuuka_buffer *kpool, const yuuka_buffer *vpool, const yuuka_buffer *table,
+                               const yuuka_buffer *positions, const yuuka_kv_params *params, yuuka_event *completion) {
+    return guard("attn_decode", [&]() -> yuuka_status {
+        if (!stream || !out || !q || !kpool || !vpool || !table || !positions || !params)
+            return fail(YUUKA_ERR_INVALID_ARGUMENT, "null argument");
+        KvArgs a;
+        yuuka_status st = kv_args(*params, true, &a);
+        if (st != YUUKA_OK) return st;
+        const uint64_t rows = kv_span_rows(a), width = (uint64_t)a.heads * a.head_dim;
+        a.pages = kv_pages(a, kpool->bytes, vpool->bytes);
+        if (!range_ok(q, 0, rows * width * (a.gated ? 2 : 1) * 4) || !range_ok(out, 0, rows * width * 4) || !a.pages ||
+            !range_ok(table, 0, kv_table_entries(a) * 4) || !range_ok(positions, 0, 8ull * a.requests))
+            return fail(YUUKA_ERR_INVALID_ARGUMENT, "attn_decode buffers too small");
+        st = kv_device(stream, {out, q, kpool, vpool, table, positions});
+        if (st == YUUKA_OK) st = ensure_scratch(stream, &stream->scratch, kv_attention_scratch_bytes(a));
+        if (st != YUUKA_OK) return st;
+        const ModelDyn dyn{static_cast<int32_t *>(positions->ptr) + 1, 0};
+        const float *qp = static_cast<const float *>(q->ptr);
+        const int stride = a.gated ? 2 * a.head_dim : a.head_dim;
+        const hipError_t err = launch_kv_attention(
+            qp, stride, a.gated ? qp + a.head_dim : nullptr, stride, kpool->ptr, vpool->ptr,
+            static_cast<const int32_t *>(table->ptr), static_cast<float *>(out->ptr), a, stream->scratch.ptr, dyn,
+            stream->stream);
+        if (err != hipSuccess) return fail(YUUKA_ERR_DEVICE, "attn_decode launch: %s", hip_error(err));
         return record(stream, completion);
     });
 }

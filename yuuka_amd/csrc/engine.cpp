@@ -31,6 +31,7 @@
 
 #include "fgemm.h"
 #include "internal.h"
+#include "kv.h"
 #include "model_kernels.h"
 #include "plan.h"
 
@@ -332,8 +333,9 @@ yuuka_status build_plan(yuuka_q35 *q, const PlanKey &key, yuuka_plan **out) {
             const uint32_t packed = (uint32_t)c.rope_dim | ((uint32_t)nreq << 8) | ((uint32_t)R1 << 20);
             // the MFMA kernel walks up to 32 rows in one launch (the key chunk
             // read once); the other kernel takes kAttnRows at a time
-            const uint64_t per = yk::attn_verify_mfma(c.kv_dtype == YUUKA_DTYPE_F16 ? 1 : 0, c.heads, c.kv_heads,
-                                                      (int)hd, c.rope_dim, (int)kvdim)
+            const uint64_t per = c.kv_dtype == YUUKA_DTYPE_Q8_0 ||
+                                         yk::attn_verify_mfma(c.kv_dtype == YUUKA_DTYPE_F16 ? 1 : 0, c.heads, c.kv_heads,
+                                                              (int)hd, c.rope_dim, (int)kvdim)
                                      ? 32
                                      : kAttnRows;
             for (uint64_t c0 = 0; c0 < R1; c0 += per) {
@@ -688,8 +690,7 @@ yuuka_status yuuka_q35_create(yuuka_device *dev, const yuuka_q35_config *cfg, co
         if (moe && (c.n_experts_used <= 0 || c.n_experts_used > c.n_experts || c.expert_ffn <= 0 || c.shared_ffn <= 0))
             return fail(YUUKA_ERR_INVALID_ARGUMENT, "invalid MoE configuration");
         if (!moe && c.ffn <= 0) return fail(YUUKA_ERR_INVALID_ARGUMENT, "dense FFN size must be positive");
-        if (c.kv_dtype != YUUKA_DTYPE_F16 && c.kv_dtype != YUUKA_DTYPE_F32)
-            return fail(YUUKA_ERR_UNSUPPORTED, "KV dtype %u", c.kv_dtype);
+        if (yk::kv_fmt_of(c.kv_dtype) < 0) return fail(YUUKA_ERR_UNSUPPORTED, "KV dtype %u", c.kv_dtype);
         std::unique_ptr<yuuka_q35> q(new yuuka_q35());
         q->dev = dev;
         q->cfg = c;
@@ -726,7 +727,8 @@ yuuka_status yuuka_q35_create(yuuka_device *dev, const yuuka_q35_config *cfg, co
         CHK(upload_tensor(q.get(), w->output, c.vocab, H, "output", &q->output));
         CHK(upload_vec(q.get(), w->output_norm, H, "output_norm", &q->output_norm));
         q->layers.resize(c.n_layers);
-        const uint64_t kv_bytes = (uint64_t)pool_blocks * c.block_size * kvdim * (c.kv_dtype == YUUKA_DTYPE_F16 ? 2 : 4);
+        const uint64_t kv_bytes =
+            (uint64_t)pool_blocks * c.block_size * yk::kv_token_bytes(yk::kv_fmt_of(c.kv_dtype), (int64_t)kvdim);
         for (int i = 0; i < c.n_layers; i++) {
             const yuuka_q35_layer_weights &lw = w->layers[i];
             Layer &L = q->layers[i];
@@ -920,7 +922,7 @@ yuuka_status yuuka_q35_fork(yuuka_q35 *q, int32_t src, int32_t dst) {
             if (st != YUUKA_OK) return st;
             const int32_t from = q->req[src].blocks[full], to = d.blocks[full];
             const uint64_t kvdim = (uint64_t)q->cfg.kv_heads * q->cfg.head_dim;
-            const uint64_t blk_bytes = (uint64_t)bs * kvdim * (q->cfg.kv_dtype == YUUKA_DTYPE_F16 ? 2 : 4);
+            const uint64_t blk_bytes = (uint64_t)bs * yk::kv_token_bytes(yk::kv_fmt_of(q->cfg.kv_dtype), (int64_t)kvdim);
             for (auto &L : q->layers) {
                 if (L.recurrent) continue;
                 for (yuuka_buffer *pool : {L.kpool, L.vpool}) {

@@ -4,7 +4,10 @@
 // documented in include/yuuka_hip.h.
 #include "ops.h"
 
+#include <algorithm>
+
 #include "fgemm.h"
+#include "kv.h"
 #include "model_kernels.h"
 
 namespace yk {
@@ -32,6 +35,245 @@ static ModelDyn dyn_of(const ExecCtx &ctx, const yuuka_op &op) {
 static uint32_t kv_fmt(uint32_t dtype, bool *ok) {
     *ok = dtype == YUUKA_DTYPE_F32 || dtype == YUUKA_DTYPE_F16;
     return dtype == YUUKA_DTYPE_F16 ? 1u : 0u;
+}
+
+// ------------------------------------------------------------------------
+// Ops over the paged cache of a batch of requests (kv.h): the KV_* and
+// ATTN_DECODE extension ops, and the v10 cache ops and ATTN_VERIFY over Q8_0
+// pools.
+
+static KvArgs kv_op_args(const yuuka_op &op) {
+    KvArgs a{};
+    auto clip = [](uint64_t v) { return (int)std::min<uint64_t>(v, 0x7fffffff); };
+    a.kv_heads = clip(op.n[0]);
+    a.heads = clip(op.n[1]);
+    a.head_dim = clip(op.n[2]);
+    a.rows = clip(op.n[4]);
+    // a displacement is signed; one that does not fit 32 bits is refused by kv_check
+    const int64_t disp = (int64_t)op.n[5];
+    a.displacement = disp < -0x7fffffff || disp > 0x7fffffff ? 0x7fffffff : (int)disp;
+    a.block_size = clip(op.u[0]);
+    a.capacity = clip(op.u[1]);
+    a.requests = std::max(1, (int)((op.u[3] >> 8) & 0xfffu));
+    a.rq_rows = (int)(op.u[3] >> 20);
+    a.scale = op.f[0];
+    a.eps = op.f[1];
+    return a;
+}
+
+// The op's arguments as the kernels take them, and its dtype: the v10 ops
+// describe one request, and their writes give kv_dim without its heads (which
+// do not matter there: every 64 dims are stored alike).
+static KvArgs kv_any_args(const yuuka_op &op) {
+    KvArgs a = kv_op_args(op);
+    switch (op.code) {
+    case YUUKA_EXT_OP_KV_APPEND:
+    case YUUKA_EXT_OP_ATTN_VERIFY:
+        a.rope_dim = (int)(op.u[3] & 0xffu);
+        a.gated = op.code == YUUKA_EXT_OP_ATTN_VERIFY;
+        break;
+    case YUUKA_EXT_OP_ATTN_DECODE:
+        a.gated = (op.u[3] & 0xffu) != 0;
+        break;
+    case YUUKA_OP_KV_WRITE_PAGED:
+    case YUUKA_OP_KV_WRITE_BATCH_PAGED:
+        a.head_dim = 64;
+        a.kv_heads = (int)std::min<uint64_t>(op.n[0] / 64, 0x7fffffff);
+        a.heads = 0;
+        a.rows = op.code == YUUKA_OP_KV_WRITE_PAGED ? 1 : (int)std::min<uint64_t>(op.n[1], 0x7fffffff);
+        a.requests = 1;
+        a.rq_rows = a.displacement = 0;
+        break;
+    case YUUKA_OP_ATTENTION_PAGED:
+    case YUUKA_OP_ATTENTION_PREFILL_PAGED:
+        if (op.code == YUUKA_OP_ATTENTION_PAGED) {
+            a.rows = 1;
+            a.displacement = 0;
+        }
+        a.requests = 1;
+        a.rq_rows = 0;
+        a.gated = op.u[3] == 0;
+        break;
+    default:
+        break;
+    }
+    return a;
+}
+
+static bool kv_is_q8(const yuuka_op &op) { return op.u[2] == YUUKA_DTYPE_Q8_0; }
+
+// Checks shared by every op over a paged cache: shape, table (buf `table`),
+// pools (bufs `kp`, `kp + 1`) and positions. `own`: the op's requests may carry
+// their positions.
+static yuuka_status kv_check_op(const yuuka_op &op, bool attention, int kp, int table, bool own, KvArgs *a) {
+    *a = kv_any_args(op);
+    yuuka_status st = kv_check(a, op.u[2], attention);
+    if (st != YUUKA_OK) return st;
+    if (own && (op.flags & YUUKA_EXT_FLAG_OWN_POS)) {
+        if (!buf_ok(op.buf[15], op.off[15], 8ull * a->requests) || op.off[15] % 4)
+            return fail(YUUKA_ERR_INVALID_ARGUMENT, "KV cache op %u: own position buffer", op.code);
+    } else if (a->requests > 1 && op.code != YUUKA_EXT_OP_KV_READ) {
+        return fail(YUUKA_ERR_INVALID_ARGUMENT, "KV cache op %u: several requests need their own positions", op.code);
+    }
+    uint64_t bytes[2] = {~0ull, ~0ull};
+    for (int i = 0; i < 2; i++) {
+        if (!op.buf[kp + i]) continue;
+        if (op.off[kp + i] > op.buf[kp + i]->bytes || op.off[kp + i] % 16)
+            return fail(YUUKA_ERR_INVALID_ARGUMENT, "KV cache op %u: pool offset", op.code);
+        bytes[i] = op.buf[kp + i]->bytes - op.off[kp + i];
+    }
+    a->pages = kv_pages(*a, bytes[0], bytes[1]);
+    if ((!op.buf[kp] && !op.buf[kp + 1]) || !a->pages || op.off[table] % 4 ||
+        !buf_ok(op.buf[table], op.off[table], kv_table_entries(*a) * 4))
+        return fail(YUUKA_ERR_INVALID_ARGUMENT, "KV cache op %u: pool or block table too small", op.code);
+    return YUUKA_OK;
+}
+
+static yuuka_status validate_kv_append(const yuuka_op &op) {
+    KvArgs a;
+    yuuka_status st = kv_check_op(op, false, 2, 4, op.code == YUUKA_EXT_OP_KV_APPEND, &a);
+    if (st != YUUKA_OK) return st;
+    const bool ext = op.code == YUUKA_EXT_OP_KV_APPEND;
+    if (ext ? op.n[3] != (uint64_t)a.kv_dim : op.n[0] != (uint64_t)a.kv_dim)
+        return fail(YUUKA_ERR_INVALID_ARGUMENT, "KV write: row width %llu", (unsigned long long)(ext ? op.n[3] : op.n[0]));
+    const uint64_t rows = kv_span_rows(a);
+    const bool norm = ext && op.buf[5], rope = ext && op.buf[6];
+    if (!op.buf[2] || !op.buf[3] || !buf_ok(op.buf[0], op.off[0], rows * a.kv_dim * 4) || op.off[0] % 4 ||
+        !buf_ok(op.buf[1], op.off[1], rows * a.kv_dim * 4) || op.off[1] % 4 ||
+        (norm && (!buf_ok(op.buf[5], op.off[5], a.head_dim * 4ull) || op.off[5] % 4)) ||
+        (rope && (!buf_ok(op.buf[6], op.off[6], rows * (a.rope_dim / 2) * 8) || op.off[6] % 8)) ||
+        (ext && rope != (a.rope_dim != 0)))
+        return fail(YUUKA_ERR_INVALID_ARGUMENT, "KV write buffers too small");
+    return YUUKA_OK;
+}
+
+static yuuka_status validate_kv_attention(const yuuka_op &op, uint64_t *ws) {
+    const bool ext = op.code == YUUKA_EXT_OP_ATTN_DECODE;
+    const int out = 3, table = op.code == YUUKA_OP_ATTENTION_PAGED ? 5 : 4;
+    KvArgs a;
+    yuuka_status st = kv_check_op(op, true, 1, table, ext, &a);
+    if (st != YUUKA_OK) return st;
+    const uint64_t rows = kv_span_rows(a), width = (uint64_t)a.heads * a.head_dim;
+    if (op.n[3] != (uint64_t)a.kv_dim || (!ext && op.code == YUUKA_OP_ATTENTION_PREFILL_PAGED && a.rows > 16))
+        return fail(YUUKA_ERR_INVALID_ARGUMENT, "invalid paged attention dimensions");
+    if (!op.buf[1] || !op.buf[2] || !buf_ok(op.buf[0], op.off[0], rows * width * (a.gated ? 2 : 1) * 4) || op.off[0] % 4 ||
+        !buf_ok(op.buf[out], op.off[out], rows * width * 4) || op.off[out] % 4)
+        return fail(YUUKA_ERR_INVALID_ARGUMENT, "paged attention buffers too small");
+    *ws = kv_attention_scratch_bytes(a);
+    return YUUKA_OK;
+}
+
+// ATTN_VERIFY over Q8_0 pools: the rows are appended and their queries
+// prepared in one launch, then attention reads the prepared queries (first in
+// the workspace) and the gates where they are.
+static uint64_t kv_verify_query_bytes(const KvArgs &a) {
+    return (kv_span_rows(a) * a.heads * a.head_dim * 4 + 255) & ~255ull;
+}
+
+static yuuka_status validate_kv_verify(const yuuka_op &op, uint64_t *ws) {
+    KvArgs a;
+    yuuka_status st = kv_check_op(op, true, 3, 6, true, &a);
+    if (st != YUUKA_OK) return st;
+    const uint64_t rows = kv_span_rows(a), width = (uint64_t)a.heads * a.head_dim;
+    if (op.n[3] != (uint64_t)a.kv_dim || !a.rope_dim)
+        return fail(YUUKA_ERR_INVALID_ARGUMENT, "invalid verify attention dimensions");
+    bool aligned = op.off[9] % 8 == 0;
+    for (int i : {0, 1, 2, 5, 7, 8}) aligned = aligned && op.off[i] % 4 == 0;
+    if (!aligned || !op.buf[3] || !op.buf[4] || !buf_ok(op.buf[0], op.off[0], rows * width * 2 * 4) ||
+        !buf_ok(op.buf[1], op.off[1], rows * a.kv_dim * 4) || !buf_ok(op.buf[2], op.off[2], rows * a.kv_dim * 4) ||
+        !buf_ok(op.buf[5], op.off[5], rows * width * 4) || !buf_ok(op.buf[7], op.off[7], a.head_dim * 4ull) ||
+        !buf_ok(op.buf[8], op.off[8], a.head_dim * 4ull) || !buf_ok(op.buf[9], op.off[9], rows * (a.rope_dim / 2) * 8))
+        return fail(YUUKA_ERR_INVALID_ARGUMENT, "verify attention buffers too small");
+    *ws = kv_verify_query_bytes(a) + kv_attention_scratch_bytes(a);
+    return YUUKA_OK;
+}
+
+static hipError_t execute_kv_op(const yuuka_op &op, const ExecCtx &ctx) {
+    KvArgs a;
+    const hipStream_t s = ctx.stream;
+    switch (op.code) {
+    case YUUKA_EXT_OP_KV_APPEND:
+    case YUUKA_OP_KV_WRITE_PAGED:
+    case YUUKA_OP_KV_WRITE_BATCH_PAGED: {
+        const bool ext = op.code == YUUKA_EXT_OP_KV_APPEND;
+        (void)kv_check_op(op, false, 2, 4, ext, &a);
+        return launch_kv_append(at<const float>(op, 0), at<const float>(op, 1), at<void>(op, 2), at<void>(op, 3),
+                                at<const int32_t>(op, 4), ext ? at<const float>(op, 5) : nullptr,
+                                ext ? at<const float2>(op, 6) : nullptr, nullptr, nullptr, nullptr, a,
+                                ext ? dyn_of(ctx, op) : dyn_of(ctx), s);
+    }
+    case YUUKA_EXT_OP_KV_READ: {
+        (void)kv_check_op(op, false, 0, 4, true, &a);
+        const bool own = (op.flags & YUUKA_EXT_FLAG_OWN_POS) != 0;
+        return launch_kv_read(at<const void>(op, 0), at<const void>(op, 1), at<const int32_t>(op, 4), at<float>(op, 2),
+                              at<float>(op, 3), a, own ? dyn_of(ctx, op) : ModelDyn{nullptr, 0}, s);
+    }
+    case YUUKA_EXT_OP_ATTN_VERIFY: {
+        (void)kv_check_op(op, true, 3, 6, true, &a);
+        float *prepared = static_cast<float *>(ctx.ws);
+        uint8_t *partials = static_cast<uint8_t *>(ctx.ws) + kv_verify_query_bytes(a);
+        const ModelDyn dyn = dyn_of(ctx, op);
+        const hipError_t err = launch_kv_append(
+            at<const float>(op, 1), at<const float>(op, 2), at<void>(op, 3), at<void>(op, 4), at<const int32_t>(op, 6),
+            at<const float>(op, 8), at<const float2>(op, 9), at<const float>(op, 0), at<const float>(op, 7), prepared, a,
+            dyn, s);
+        if (err != hipSuccess) return err;
+        return launch_kv_attention(prepared, a.head_dim, at<const float>(op, 0) + a.head_dim, 2 * a.head_dim,
+                                   at<const void>(op, 3), at<const void>(op, 4), at<const int32_t>(op, 6),
+                                   at<float>(op, 5), a, partials, dyn, s);
+    }
+    default: {  // ATTN_DECODE, ATTENTION_PAGED, ATTENTION_PREFILL_PAGED
+        const bool ext = op.code == YUUKA_EXT_OP_ATTN_DECODE;
+        const int table = op.code == YUUKA_OP_ATTENTION_PAGED ? 5 : 4;
+        (void)kv_check_op(op, true, 1, table, ext, &a);
+        const int stride = a.gated ? 2 * a.head_dim : a.head_dim;
+        return launch_kv_attention(at<const float>(op, 0), stride, a.gated ? at<const float>(op, 0) + a.head_dim : nullptr,
+                                   stride, at<const void>(op, 1), at<const void>(op, 2), at<const int32_t>(op, table),
+                                   at<float>(op, 3), a, ctx.ws, ext ? dyn_of(ctx, op) : dyn_of(ctx), s);
+    }
+    }
+}
+
+// The ops that execute_kv_op runs.
+static bool kv_op(const yuuka_op &op) {
+    switch (op.code) {
+    case YUUKA_EXT_OP_KV_APPEND:
+    case YUUKA_EXT_OP_KV_READ:
+    case YUUKA_EXT_OP_ATTN_DECODE:
+        return true;
+    case YUUKA_OP_KV_WRITE_PAGED:
+    case YUUKA_OP_KV_WRITE_BATCH_PAGED:
+    case YUUKA_OP_ATTENTION_PAGED:
+    case YUUKA_OP_ATTENTION_PREFILL_PAGED:
+    case YUUKA_EXT_OP_ATTN_VERIFY:
+        return kv_is_q8(op);
+    default:
+        return false;
+    }
+}
+
+static yuuka_status validate_kv_op(const yuuka_op &op, uint64_t *ws) {
+    switch (op.code) {
+    case YUUKA_EXT_OP_KV_APPEND:
+    case YUUKA_OP_KV_WRITE_PAGED:
+    case YUUKA_OP_KV_WRITE_BATCH_PAGED:
+        return validate_kv_append(op);
+    case YUUKA_EXT_OP_KV_READ: {
+        KvArgs a;
+        yuuka_status st = kv_check_op(op, false, 0, 4, true, &a);
+        if (st != YUUKA_OK) return st;
+        const uint64_t out = kv_span_rows(a) * a.kv_dim * 4;
+        for (int i = 0; i < 2; i++)
+            if (!op.buf[i] != !op.buf[2 + i] || (op.buf[i] && (!buf_ok(op.buf[2 + i], op.off[2 + i], out) || op.off[2 + i] % 4)))
+                return fail(YUUKA_ERR_INVALID_ARGUMENT, "KV read buffers too small");
+        if (op.n[3] != (uint64_t)a.kv_dim) return fail(YUUKA_ERR_INVALID_ARGUMENT, "KV read: row width");
+        return YUUKA_OK;
+    }
+    case YUUKA_EXT_OP_ATTN_VERIFY:
+        return validate_kv_verify(op, ws);
+    default:
+        return validate_kv_attention(op, ws);
+    }
 }
 
 static AttnArgs attn_args(const yuuka_op &op) {
@@ -504,6 +746,8 @@ bool op_uses_position(const yuuka_op &op) {
     case YUUKA_OP_ATTENTION_PREFILL_PAGED:
     case YUUKA_EXT_OP_ROPE_TABLE:
     case YUUKA_EXT_OP_ATTN_VERIFY:
+    case YUUKA_EXT_OP_KV_APPEND:
+    case YUUKA_EXT_OP_ATTN_DECODE:
         return !(op.flags & YUUKA_EXT_FLAG_OWN_POS);
     case YUUKA_OP_EMBEDDING:  // the dynamic token
     case YUUKA_OP_ROPE:
@@ -517,6 +761,7 @@ bool op_uses_position(const yuuka_op &op) {
 
 yuuka_status validate_model_op(const yuuka_op &op, uint64_t *ws) {
     *ws = 0;
+    if (kv_op(op)) return validate_kv_op(op, ws);
     bool decode = false;
     const yuuka_status dst = validate_decode_op(op, ws, &decode);
     if (decode) return dst;
@@ -966,6 +1211,11 @@ yuuka_status execute_gdn_commit_run(const yuuka_op *ops, int count, const ExecCt
 }
 
 yuuka_status execute_model_op(const yuuka_op &op, const ExecCtx &ctx) {
+    if (kv_op(op)) {
+        const hipError_t err = execute_kv_op(op, ctx);
+        if (err != hipSuccess) return fail(YUUKA_ERR_DEVICE, "op %u launch: %s", op.code, hip_error(err));
+        return YUUKA_OK;
+    }
     bool decode = false;
     const yuuka_status dst = execute_decode_op(op, ctx, &decode);
     if (decode) return dst;

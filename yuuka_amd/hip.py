@@ -27,12 +27,13 @@ OP = dict(
     ROPE_BATCH=20, RECURRENT_CHUNK=23, EMBEDDING_BATCH=24, KV_WRITE_BATCH_PAGED=28,
     ATTENTION_PREFILL_PAGED=29, MOE_ROUTE=30, MOE_GATE_UP=31, MOE_DOWN=32, MOE_REDUCE_ADD=33, LM_HEAD=37,
     ACCEPT=66, GDN_COMMIT=67, ADVANCE=68, GEMM_FUSED=69, ROPE_TABLE=70, ATTN_VERIFY=71, MOE_ROUTER=72,
-    MOE_COMBINE=73, ROUTER_NORMAL=74,
+    MOE_COMBINE=73, ROUTER_NORMAL=74, KV_APPEND=75, KV_READ=76, ATTN_DECODE=77,
 )
 FLAG_MOE_SWIGLU = 0x800
 FLAG_MOE_PACKED = 0x2000
 EPI_STORE, EPI_RESIDUAL, EPI_SWIGLU = 0, 1, 2
 FLAG_TAIL = 0x1
+FLAG_OWN_POS = 0x1000
 
 ACCEPT_GREEDY, ACCEPT_STOCHASTIC = 0, 1
 
@@ -73,6 +74,12 @@ class yuuka_accept_params(C.Structure):
         ("step", C.c_uint64),
         ("row_stride", C.c_uint64),
     ]
+
+
+class yuuka_kv_params(C.Structure):
+    _fields_ = [("dtype", C.c_uint32)] + [(n, C.c_int32) for n in (
+        "block_size", "capacity", "requests", "rows", "request_rows", "heads", "kv_heads", "head_dim", "rope_dim",
+        "gated", "displacement")] + [("scale", C.c_float), ("eps", C.c_float)]
 
 
 class yuuka_device_info(C.Structure):
@@ -147,6 +154,10 @@ def _declare(L: C.CDLL) -> None:
         "yuuka_quantized_bytes": (u64, [u64, u64]),
         "yuuka_quantize_activations": (C.c_int, [vp, vp, vp, u64, u64, vp]),
         "yuuka_gemm_quantized": (C.c_int, [vp, vp, vp, vp, u64, u64, u64, u32, vp]),
+        "yuuka_kv_page_bytes": (u64, [C.POINTER(yuuka_kv_params)]),
+        "yuuka_kv_append": (C.c_int, [vp] * 9 + [C.POINTER(yuuka_kv_params), vp]),
+        "yuuka_kv_read": (C.c_int, [vp] * 7 + [C.POINTER(yuuka_kv_params), vp]),
+        "yuuka_attn_decode": (C.c_int, [vp] * 7 + [C.POINTER(yuuka_kv_params), vp]),
         "yuuka_plan_create": (C.c_int, [vp, C.POINTER(vp)]),
         "yuuka_plan_destroy": (None, [vp]),
         "yuuka_plan_add": (C.c_int, [vp, C.POINTER(yuuka_op)]),
@@ -326,6 +337,41 @@ def accept_params(mode: int, batch: int, drafts: int, vocab: int, temperature: f
                   request_base: int = 0, row_stride: int = 0) -> yuuka_accept_params:
     return yuuka_accept_params(mode, batch, drafts, vocab, temperature, top_k, top_p, request_base,
                                seed, step, row_stride)
+
+
+def kv_params(dtype: int, block_size: int, capacity: int, kv_heads: int, head_dim: int, rows: int, requests: int = 1,
+              heads: int = 0, gated: bool = False, scale: float = 1.0, displacement: int = 0, request_rows: int = 0,
+              rope_dim: int = 0, eps: float = 1e-6) -> yuuka_kv_params:
+    return yuuka_kv_params(dtype, block_size, capacity, requests, rows, request_rows, heads, kv_heads, head_dim,
+                           rope_dim, int(gated), displacement, scale, eps)
+
+
+def kv_page_bytes(params: yuuka_kv_params) -> int:
+    """Bytes of one page of one pool (0 when the parameters are not served)."""
+    return int(lib().yuuka_kv_page_bytes(C.byref(params)))
+
+
+def kv_append(stream: Stream, k: Buffer, v: Buffer, kpool: Buffer, vpool: Buffer, table: Buffer, positions: Buffer,
+              params: yuuka_kv_params, k_norm: Buffer | None = None, rope: Buffer | None = None,
+              event: Event | None = None) -> None:
+    """Rounds new key and value rows into the paged pools."""
+    check(lib().yuuka_kv_append(stream.ptr, _p(k), _p(v), _p(kpool), _p(vpool), _p(table), _p(positions), _p(k_norm),
+                                _p(rope), C.byref(params), _p(event)), "kv_append")
+
+
+def kv_read(stream: Stream, k_out: Buffer | None, v_out: Buffer | None, kpool: Buffer | None, vpool: Buffer | None,
+            table: Buffer, params: yuuka_kv_params, positions: Buffer | None = None,
+            event: Event | None = None) -> None:
+    """Cached rows back to float32."""
+    check(lib().yuuka_kv_read(stream.ptr, _p(k_out), _p(v_out), _p(kpool), _p(vpool), _p(table), _p(positions),
+                              C.byref(params), _p(event)), "kv_read")
+
+
+def attn_decode(stream: Stream, out: Buffer, q: Buffer, kpool: Buffer, vpool: Buffer, table: Buffer,
+                positions: Buffer, params: yuuka_kv_params, event: Event | None = None) -> None:
+    """Attention of the newest rows over the paged cache."""
+    check(lib().yuuka_attn_decode(stream.ptr, _p(out), _p(q), _p(kpool), _p(vpool), _p(table), _p(positions),
+                                  C.byref(params), _p(event)), "attn_decode")
 
 
 def gemm_fused_op(plan: "Plan", x: Buffer, n_in: int, rows: int, segments, epilogue: int = 0,
