@@ -172,12 +172,13 @@ def attention(c, q, rows, heads, scale, gated, request_rows=None, displacement=0
     return out
 
 
-def close(got, want, tol=TOL):
+def close(got, want, tol=TOL, floor=0.0):
+    """Equal up to tol of the norm, and `floor` an element."""
     got, want = got.astype(np.float64), np.asarray(want, np.float64)
     assert np.array_equal(np.isfinite(got), np.isfinite(want))
     ok = np.isfinite(want)
     d = np.linalg.norm(got[ok] - want[ok])
-    assert d <= tol * np.linalg.norm(want[ok]), d / np.linalg.norm(want[ok])
+    assert d <= tol * np.linalg.norm(want[ok]) + floor * math.sqrt(ok.sum()), d / np.linalg.norm(want[ok])
 
 
 # --------------------------------------------------------- append and read back
@@ -505,7 +506,10 @@ def test_magnitudes(dev, stream, dtype, qs, ks, vs):
     got = o.read(np.float32).reshape(q.shape)
     for odd in range(2):  # the small blocks on their own
         dims = np.arange(D) // 32 % 2 == odd
-        close(got[..., dims], want[..., dims])
+        # An MFMA aligns the products it sums by their exponent fields, and a subnormal half has that of 2^-14: with
+        # weights that sum to one, such values (steps of 2^-24) are summed to 2^-14 2^-24 = 2^-38. Q8_0 digits are
+        # normal halves; the last bits of 2^-38 a term, over the terms' 2^4 spread of weights, are 2^-36 at the most.
+        close(got[..., dims], want[..., dims], floor=2.0 ** -36 if dtype == F16 else 0.0)
 
 
 @pytest.mark.parametrize("dtype", [Q8, F16])

@@ -4,12 +4,31 @@
 //
 //   out = sum_t softmax_t(scale q . k_t) v_t,  t = 0 .. position of the row
 //
-// A request's keys are cut into `splits` ranges; a workgroup keeps the running
-// maximum m, sum l and unnormalised output o of its range, and the merge
-// kernel joins the ranges' records with weights exp(m - max m).
+// A workgroup takes one kv head of one request, up to 16 of its (row, query
+// head) pairs and a range of the keys; its eight waves walk the range's
+// 32-key tiles, each with a running reference, sum and output of its own, and
+// are joined at the end. With more ranges than one the records {o, m, l} of
+// the ranges are joined by a second kernel.
+//
+// Both products run on v_mfma_f32_16x16x32_f16 straight from the pages:
+//  * scores = K Q^T (keys are the rows of the tile, so that a lane ends with
+//    the scores of one query row and the keys 4 g .. 4 g + 3 of both 16-key
+//    halves), P V with those very keys as lane g's eight: probabilities go from
+//    the first product's result to the second's operand without leaving the lane;
+//  * int8 digits are exact halves. A query is two halves (scaled by a power of
+//    two to below 2^14), a probability times its key's scale too: products are good
+//    to 2^-22, sums are float32. Key scales multiply the scores block by block
+//    (an MFMA covers one block of 32 dims), value scales the probabilities.
+//  * up to eight pairs ("stacked") put both halves in one 16-wide operand, as rows
+//    n and n + 8; more take two MFMAs.
+//  * p = 2^(s - m') with the reference m' = running max + E - 10, E the
+//    exponent of the largest value scale so far: p times a scale stays below 2^14
+//    and the halves' 39 octaves are used; m' moves (and the accumulators are
+//    rescaled) when a tile passes it by 4.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <mutex>
 
 #include "internal.h"
 #include "kv_dev.h"
@@ -18,79 +37,541 @@
 namespace yk {
 namespace {
 
-constexpr int kChunk = 64;
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef float float2v __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+template <int N> struct Dwords {  // N dwords at dword alignment
+    typedef uint32_t V __attribute__((ext_vector_type(N), aligned(4)));
+};
+template <> struct Dwords<1> { typedef uint32_t V; };
+template <int N> __device__ __forceinline__ uint32_t dword(const typename Dwords<N>::V &v, int i) { return v[i]; }
+template <> __device__ __forceinline__ uint32_t dword<1>(const uint32_t &v, int) { return v; }
 
-// Keys a row sees: those at positions up to its own, within the capacity.
-__device__ __forceinline__ int row_keys(const KvArgs &a, const ModelDyn &dyn, int j, int r) {
-    const int64_t p = kv_position(a, dyn, j, r);
-    return p < 0 ? 0 : (int)min(p + 1, (int64_t)a.capacity);
+constexpr int kWaves = 8, kTile = 32;
+constexpr float kHeadroom = 10.0f, kSlack = 4.0f;
+
+__device__ __forceinline__ float max_rows(float x) {  // over the four 16-lane rows
+    auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+}
+__device__ __forceinline__ float sum_halves(float x) {  // lane l and l ^ 32
+    auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(a[0]) + __uint_as_float(a[1]);
+}
+__device__ __forceinline__ float sum_rows(float x) {
+    x = sum_halves(x);
+    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(a[0]) + __uint_as_float(a[1]);
+}
+__device__ __forceinline__ float ror8(float x) {  // lane (l + 8) % 16 of the row
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x128, 0xf, 0xf, true));
+}
+__device__ __forceinline__ half2v to_half2(float a, float b) {
+    return __builtin_convertvector((float2v){a, b}, half2v);
+}
+__device__ __forceinline__ half8 join(half2v a, half2v b, half2v c, half2v d) {
+    return half8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+__device__ __forceinline__ void wave_lds_fence() {  // the wave's LDS writes are in order before its reads
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
 }
 
-// Value of dim d of head h of a token.
-template <int FMT>
-__device__ __forceinline__ float kv_value(const KvArgs &a, const uint8_t *pool, int64_t at, int64_t sc, int h, int d) {
-    const int D = a.head_dim;
-    if constexpr (FMT == kKvF16) return h2f(reinterpret_cast<const uint16_t *>(pool + at)[h * D + d]);
-    return (float)(int8_t)pool[at + h * D + (d & ~63) + 4 * (d & 15) + ((d >> 4) & 3)] *
-           h2f(reinterpret_cast<const uint16_t *>(pool + sc)[h * (D / 32) + (d >> 5)]);
+// Two digits of a dword of keys as halves: 0x6400 | u is 1024 + u.
+template <int H>
+__device__ __forceinline__ half2v key_digits(uint32_t biased) {
+    const uint32_t u = __builtin_amdgcn_perm(0x64646464u, biased, H ? 0x04030402u : 0x04010400u);
+    return __builtin_bit_cast(half2v, u) + half2v{(_Float16)-1152.0f, (_Float16)-1152.0f};
+}
+// Digit J of two keys' dwords, times 2^-9: u as a subnormal half is u 2^-24.
+template <int J>
+__device__ __forceinline__ half2v value_digits(uint32_t x, uint32_t y) {
+    const uint32_t u = __builtin_amdgcn_perm(y, x, 0x0c000c00u | ((4u + J) << 16) | J);
+    return __builtin_elementwise_fma(__builtin_bit_cast(half2v, u), half2v{(_Float16)32768.0f, (_Float16)32768.0f},
+                                     half2v{(_Float16)-0.25f, (_Float16)-0.25f});
+}
+// Half J of two keys' four values.
+template <int J>
+__device__ __forceinline__ half2v value_halves(u32x2 x, u32x2 y) {
+    return __builtin_bit_cast(half2v, __builtin_amdgcn_perm(y[J >> 1], x[J >> 1], J & 1 ? 0x07060302u : 0x05040100u));
 }
 
-// One workgroup per (range, query head, request), the rows in turn.
-template <int FMT>
-__global__ __launch_bounds__(256) void kv_attention_kernel(const float *__restrict__ q, int q_stride,
-                                                           const uint8_t *__restrict__ kpool,
-                                                           const uint8_t *__restrict__ vpool,
-                                                           const int32_t *__restrict__ table, KvArgs a, int splits,
-                                                           float *__restrict__ part, ModelDyn dyn) {
-    __shared__ float qs[256], ps[kChunk], stat[2];
-    __shared__ int64_t at[kChunk], sc[kChunk];
-    const int split = blockIdx.x, h = blockIdx.y, j = blockIdx.z, D = a.head_dim, tid = threadIdx.x;
-    const int kvh = h / (a.heads / a.kv_heads);
-    for (int r = 0; r < a.rows; r++) {
-        const int n = row_keys(a, dyn, j, r);
-        const int chunks = (n + kChunk - 1) / kChunk, per = (chunks + splits - 1) / splits;
-        const int c0 = split * per, c1 = min(chunks, c0 + per);
-        const float *qr = q + (((int64_t)j * a.rq_rows + r) * a.heads + h) * q_stride;
-        __syncthreads();
-        if (tid < D) qs[tid] = qr[tid];
-        float m = -INFINITY, l = 0.0f, o = 0.0f;
-        for (int c = c0; c < c1; c++) {
-            __syncthreads();
-            if (tid < kChunk) {
-                const int t = c * kChunk + tid;
-                if (t >= n || !kv_slot(a, table, j, t, &at[tid], &sc[tid])) at[tid] = -1;
-            }
-            __syncthreads();
-            {
-                const int kk = tid >> 2, quarter = tid & 3;
-                float s = 0.0f;
-                if (at[kk] >= 0)
-                    for (int d = quarter; d < D; d += 4) s = fmaf(qs[d], kv_value<FMT>(a, kpool, at[kk], sc[kk], kvh, d), s);
-                s += __shfl_xor(s, 1);
-                s += __shfl_xor(s, 2);
-                if (quarter == 0) ps[kk] = at[kk] >= 0 ? s * a.scale : -INFINITY;
-            }
-            __syncthreads();
-            float mn = m;
-            for (int kk = 0; kk < kChunk; kk++) mn = fmaxf(mn, ps[kk]);
-            __syncthreads();
-            const float shrink = m == mn ? 1.0f : expf(m - mn);
-            if (tid < kChunk) ps[tid] = at[tid] >= 0 ? expf(ps[tid] - mn) : 0.0f;
-            __syncthreads();
-            l *= shrink;
-            o *= shrink;
-            for (int kk = 0; kk < kChunk; kk++) {
-                if (at[kk] < 0) continue;
-                l += ps[kk];
-                if (tid < D) o = fmaf(ps[kk], kv_value<FMT>(a, vpool, at[kk], sc[kk], kvh, tid), o);
-            }
-            m = mn;
+template <int FMT, int GROUPS, bool STACK, bool PAGED> struct Layout {
+    static constexpr bool Q8 = FMT == kKvQ8;
+    static constexpr int D = 64 * GROUPS, NB = 2 * GROUPS, ROWS = STACK ? 8 : 16;
+    static constexpr uint32_t plane = NB * 1024;                              // query operands, one half
+    static constexpr uint32_t scales = STACK ? plane : 2 * plane;             // [wave][key, value][32][GROUPS dwords]
+    static constexpr uint32_t addr = scales + (Q8 ? kWaves * 256 * GROUPS : 0);  // [wave][32] row offsets
+    static constexpr uint32_t loop = addr + (PAGED ? 0 : kWaves * 256);
+    static constexpr int slot_row = D + 4;                                    // floats; rows 4 g land 16 banks apart
+    static constexpr uint32_t slots = kWaves * ROWS * slot_row * 4;           // over the loop's areas, after it
+    static constexpr uint32_t stats = loop > slots ? loop : slots;            // m[8][16], l[8][16], factor[16]
+    static constexpr uint32_t total = stats + (2 * kWaves + 1) * 16 * 4;
+};
+
+struct AttnSplit {
+    int splits, row_blocks;
+    int page_shift;  // PAGED: log2(block_size / 16)
+};
+
+// 512 threads. PAGED: pages are 16 << page_shift tokens, so that a 16-key half
+// of a tile lies in one page, found by scalar loads and read through a
+// buffer resource of that page's bytes (none for an unmapped page or past the end:
+// such loads cost nothing and give zeros).
+template <int FMT, int GROUPS, bool STACK, bool PAGED>
+__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 2))) void kv_attention_kernel(
+    const float *__restrict__ q, int q_stride, const float *__restrict__ gate, int gate_stride,
+    const uint8_t *__restrict__ kpool, const uint8_t *__restrict__ vpool, const int32_t *__restrict__ table, KvArgs a,
+    AttnSplit sp, float *__restrict__ part, float *__restrict__ out, ModelDyn dyn) {
+    using L = Layout<FMT, GROUPS, STACK, PAGED>;
+    constexpr bool Q8 = L::Q8;
+    constexpr int D = L::D, NB = L::NB, ROWS = L::ROWS;
+    constexpr int KP = Q8 ? GROUPS : 2 * GROUPS;  // 16-byte pieces of a key per lane
+    extern __shared__ __align__(16) uint8_t lds[];
+    float *const st_m = reinterpret_cast<float *>(lds + L::stats), *const st_l = st_m + kWaves * 16;
+    float *const row_factor = st_l + kWaves * 16;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int r16 = lane & 15, g4 = lane >> 4;
+    int bx = blockIdx.x;
+    const int rb = bx % sp.row_blocks;
+    bx /= sp.row_blocks;
+    const int split = bx % sp.splits, kvh = bx / sp.splits, j = blockIdx.y;
+    const int G = a.heads / a.kv_heads;
+    const int n0 = rb * ROWS, nr = min(ROWS, G * a.rows - n0);  // pairs n = row * G + head of the group
+    const int64_t p0 = kv_position(a, dyn, j, 0);
+    // last key a row sees, -1 for none
+    auto limit = [&](int n) { return (int)max((int64_t)-1, min(p0 + n / G, (int64_t)a.capacity - 1)); };
+    const int len = limit(n0 + nr - 1) + 1, least = limit(n0);
+    const int tiles = (len + kTile - 1) / kTile;
+    const int per = max((tiles + sp.splits - 1) / sp.splits, kWaves);
+    const int c0 = split * per, c1 = min(tiles, c0 + per);
+    const int64_t out_row = (int64_t)j * a.rq_rows;
+    if (c0 >= c1 && sp.splits > 1) {  // nothing here: an empty record
+        if (threadIdx.x < (uint32_t)nr) {
+            const int n = n0 + threadIdx.x, r = n / G, h = kvh * G + n % G;
+            float *rec = part + ((((int64_t)j * a.rows + r) * a.heads + h) * sp.splits + split) * (D + 2);
+            rec[D] = -INFINITY;
+            rec[D + 1] = 0.0f;
         }
-        float *rec = part + ((((int64_t)j * a.rows + r) * a.heads + h) * splits + split) * (D + 2);
-        if (tid < D) rec[tid] = o;
-        if (tid == 0) {
-            rec[D] = m;
-            rec[D + 1] = l;
+        return;
+    }
+
+    // ---- pages of a tile's halves, and which of its keys there are
+    const int32_t *const table_j = table + (int64_t)j * kv_table_blocks(a);
+    const int64_t page_bytes = kv_page_bytes(a);
+    const uint32_t row_bytes = Q8 ? a.kv_dim : a.kv_dim * 2;
+    struct Tile {
+        int page[2];    // PAGED: -1 unmapped or past the end
+        uint32_t keys;  // bit k: key k of the tile is there
+    };
+    auto pages_of = [&](int c) {
+        Tile t;
+        t.keys = 0;
+        if constexpr (PAGED) {
+#pragma unroll
+            for (int T = 0; T < 2; T++) {
+                const int tok = kTile * c + 16 * T;
+                int page = -1;
+                if (c < c1 && tok < len) page = table_j[tok >> (4 + sp.page_shift)];
+                t.page[T] = (uint32_t)page < (uint32_t)a.pages ? page : -1;
+                if (t.page[T] >= 0) t.keys |= (0xffffu >> max(0, tok + 16 - len)) << (16 * T);
+            }
+        }
+        return t;
+    };
+    // ---- loads of one tile
+    u32x4 kreg[2][KP];
+    uint32_t vdig[Q8 ? 8 : 1][GROUPS];
+    u32x2 vhalf[Q8 ? 1 : 8][GROUPS];
+    typename Dwords<GROUPS>::V sreg;  // lanes 0..31: scales of key `lane`, 32..63: of value `lane - 32`
+    const uint8_t *krow[PAGED ? 1 : 2], *vrow[PAGED ? 1 : 8];  // rows of the tile to be loaded
+    const uint32_t koff = r16 * row_bytes + kvh * D * (Q8 ? 1 : 2) + 16 * g4;
+    const uint32_t voff = 4 * g4 * row_bytes + kvh * D * (Q8 ? 1 : 2) + r16 * (Q8 ? 4 : 8);
+    auto resource = [&](const uint8_t *pool, const Tile &t, int c, int T) {
+        const int in = ((2 * c + T) & ((1 << sp.page_shift) - 1)) * 16;  // tokens before the half in its page
+        const int64_t skip = (int64_t)in * row_bytes;
+        const int page = t.page[T];
+        return __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<uint8_t *>(pool) + (page >= 0 ? page * page_bytes + skip : 0), (short)0,
+            page >= 0 ? (int)(page_bytes - skip) : 0, 0x00020000);
+    };
+    uint8_t *const my_scales = lds + L::scales + wave * 256 * GROUPS;
+    int64_t *const my_addr = reinterpret_cast<int64_t *>(lds + L::addr) + wave * 32;
+    auto load_scales = [&](const Tile &t, int c) {
+        if constexpr (Q8 && PAGED) {
+            const int T = (lane >> 4) & 1, tok = lane & 15;
+            int64_t at[2];
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                const int in = ((2 * c + u) & ((1 << sp.page_shift) - 1)) * 16;
+                at[u] = t.page[u] * page_bytes + (int64_t)a.block_size * a.kv_dim + (int64_t)in * (a.kv_dim / 16);
+            }
+            const bool there = (t.keys >> (lane & 31)) & 1;
+            const int64_t off = there ? (T ? at[1] : at[0]) + tok * (a.kv_dim / 16) + kvh * NB * 2 : 0;
+            sreg = *reinterpret_cast<const typename Dwords<GROUPS>::V *>((lane < 32 ? kpool : vpool) + off);
+        }
+    };
+    // !PAGED: every lane finds the row (and the scales) of key `lane & 31`
+    auto find_rows = [&](int c) {
+        Tile t{};
+        if constexpr (!PAGED) {
+            const int key = kTile * c + (lane & 31);
+            int64_t row = 0, sc = 0;
+            const bool there = c < c1 && key < len && kv_slot(a, table, j, key, &row, &sc);
+            t.keys = (uint32_t)__builtin_amdgcn_ballot_w64(there);
+            wave_lds_fence();
+            if (lane < 32) my_addr[lane] = there ? row : 0;
+            wave_lds_fence();
+#pragma unroll
+            for (int T = 0; T < 2; T++) krow[T] = kpool + my_addr[16 * T + r16] + (koff - r16 * row_bytes);
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                vrow[i] = vpool + my_addr[16 * (i >> 2) + 4 * g4 + (i & 3)] + (voff - 4 * g4 * row_bytes);
+            if constexpr (Q8)
+                sreg = *reinterpret_cast<const typename Dwords<GROUPS>::V *>((lane < 32 ? kpool : vpool) +
+                                                                             (there ? sc + kvh * NB * 2 : 0));
+        }
+        return t;
+    };
+    auto load_key = [&](__amdgpu_buffer_rsrc_t rs, int T, int p) {
+        if constexpr (PAGED)
+            kreg[T][p] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, koff + 64 * p, 0, 0));
+        else
+            kreg[T][p] = *reinterpret_cast<const typename Dwords<4>::V *>(krow[T] + 64 * p);
+    };
+    auto load_value = [&](__amdgpu_buffer_rsrc_t rs, int i, int s) {
+        const uint32_t off = voff + (i & 3) * row_bytes;
+        if constexpr (Q8 && PAGED) vdig[i][s] = (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(rs, off + 64 * s, 0, 0);
+        else if constexpr (Q8) vdig[i][s] = *reinterpret_cast<const uint32_t *>(vrow[i] + 64 * s);
+        else if constexpr (PAGED)
+            vhalf[i][s] = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rs, off + 128 * s, 0, 0));
+        else
+            vhalf[i][s] = *reinterpret_cast<const typename Dwords<2>::V *>(vrow[i] + 128 * s);
+    };
+    auto first_resource = [&](const uint8_t *pool, const Tile &t, int c, int T) {
+        if constexpr (PAGED) return resource(pool, t, c, T);
+        else return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(pool), (short)0, 0, 0x00020000);
+    };
+
+    int c = c0 + wave;
+    Tile cur = PAGED ? pages_of(c) : find_rows(c);
+    load_scales(cur, c);
+    {
+        const auto k0 = first_resource(kpool, cur, c, 0), k1 = first_resource(kpool, cur, c, 1);
+        const auto v0 = first_resource(vpool, cur, c, 0), v1 = first_resource(vpool, cur, c, 1);
+#pragma unroll
+        for (int p = 0; p < KP; p++) {
+            load_key(k0, 0, p);
+            load_key(k1, 1, p);
+        }
+#pragma unroll
+        for (int s = 0; s < GROUPS; s++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) load_value(i < 4 ? v0 : v1, i, s);
+    }
+
+    // ---- queries as MFMA operands in LDS: wave w prepares rows w and w + 8
+#pragma unroll
+    for (int n = wave; n < ROWS; n += kWaves) {
+        float x[GROUPS], top = 0.0f;
+        const int r = (n0 + n) / G, h = kvh * G + (n0 + n) % G;
+#pragma unroll
+        for (int s = 0; s < GROUPS; s++) {
+            x[s] = n < nr ? q[((out_row + r) * a.heads + h) * q_stride + 64 * s + lane] : 0.0f;
+            top = fmaxf(top, fabsf(x[s]));
+        }
+#pragma unroll
+        for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
+        int e = 14;
+        if (top > 0.0f && top < INFINITY) (void)frexpf(top, &e);  // top < 2^e
+        const int in = Q8 ? lane : 0;
+        // dim 64 s + lane: block 2 s + h, lane group g, place k of the operand's eight
+        const int hb = Q8 ? in >> 5 : lane >> 5;
+        const int g = Q8 ? (lane & 15) >> 2 : (lane & 31) >> 3;
+        const int k = Q8 ? 2 * (lane & 3) + ((lane >> 4) & 1) : lane & 7;
+#pragma unroll
+        for (int s = 0; s < GROUPS; s++) {
+            const float y = ldexpf(x[s], 14 - e);
+            const _Float16 hi = (_Float16)y, lo = (_Float16)(y - (float)hi);
+            const uint32_t at = ((2 * s + hb) * 64 + 16 * g + n) * 16 + 2 * k;
+            *reinterpret_cast<_Float16 *>(lds + at) = hi;
+            *reinterpret_cast<_Float16 *>(lds + at + (STACK ? 8 * 16 : L::plane)) = lo;
+        }
+        // scores in units of log2: factor * (operand product)
+        if (lane == 0) row_factor[n] = ldexpf(a.scale * 1.44269504088896341f, e - 14);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+
+    const int my_n = STACK ? r16 & 7 : r16;
+    const float factor = row_factor[my_n];
+    const int my_limit = my_n < nr ? limit(n0 + my_n) : -1;
+    const float low_half = STACK && r16 >= 8 ? 1.0f : 0.0f;  // this lane's probabilities: the remainder's half
+    f32x4 acc[GROUPS][4];
+#pragma unroll
+    for (int s = 0; s < GROUPS; s++)
+#pragma unroll
+        for (int t = 0; t < 4; t++) acc[s][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float ref = -INFINITY, l = 0.0f;
+
+    Tile next{};
+    if constexpr (PAGED) next = pages_of(c + kWaves);
+    for (; c < c1; c += kWaves) {
+        float E = 0.0f;
+        if constexpr (Q8) {
+            // scales to LDS (those of missing keys as zeros), and the largest finite value scale's exponent
+            wave_lds_fence();
+            const bool there = (cur.keys >> (lane & 31)) & 1;
+            uint32_t most = 0;
+#pragma unroll
+            for (int s = 0; s < GROUPS; s++) {
+                const uint32_t d = there ? dword<GROUPS>(sreg, s) : 0u;
+                reinterpret_cast<uint32_t *>(my_scales)[lane * GROUPS + s] = d;
+                const uint32_t lo = d & 0x7fffu, hi = (d >> 16) & 0x7fffu;
+                most = max(most, max(lo < 0x7c00u ? lo : 0u, hi < 0x7c00u ? hi : 0u));
+            }
+            if (lane < 32) most = 0;
+            float m = __uint_as_float(most);  // non-negative: ordered as floats
+            m = fmaxf(m, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(m), 0xb1, 0xf, 0xf, true)));
+            m = fmaxf(m, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(m), 0x4e, 0xf, 0xf, true)));
+            m = fmaxf(m, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(m), 0x124, 0xf, 0xf, true)));
+            m = fmaxf(m, ror8(m));
+            m = max_rows(m);
+            E = (float)((int)(__float_as_uint(m) >> 10) - 14);  // scale < 2^E
+            wave_lds_fence();
+        }
+        Tile after{};
+        if constexpr (!PAGED) next = find_rows(c + kWaves);
+        // ---- scores: keys 4 g + e of half T against query row r16
+        float s[2][4] = {};
+        {
+            typename Dwords<GROUPS>::V ks[2][4];
+            if constexpr (Q8) {
+#pragma unroll
+                for (int T = 0; T < 2; T++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        ks[T][e] = *reinterpret_cast<const typename Dwords<GROUPS>::V *>(
+                            my_scales + (16 * T + 4 * g4 + e) * 4 * GROUPS);
+            }
+            const auto k0 = first_resource(kpool, next, c + kWaves, 0), k1 = first_resource(kpool, next, c + kWaves, 1);
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                const half8 qh = *reinterpret_cast<const half8 *>(lds + (b * 64 + lane) * 16);
+                half8 ql{};
+                if constexpr (!STACK) ql = *reinterpret_cast<const half8 *>(lds + L::plane + (b * 64 + lane) * 16);
+#pragma unroll
+                for (int T = 0; T < 2; T++) {
+                    half8 kk;
+                    if constexpr (Q8) {
+                        const u32x4 w = kreg[T][b >> 1] ^ 0x80808080u;
+                        kk = b & 1 ? join(key_digits<1>(w[0]), key_digits<1>(w[1]), key_digits<1>(w[2]), key_digits<1>(w[3]))
+                                   : join(key_digits<0>(w[0]), key_digits<0>(w[1]), key_digits<0>(w[2]), key_digits<0>(w[3]));
+                    } else {
+                        kk = __builtin_bit_cast(half8, kreg[T][b]);
+                    }
+                    f32x4 d = {0.f, 0.f, 0.f, 0.f};
+                    if constexpr (!Q8) d = f32x4{s[T][0], s[T][1], s[T][2], s[T][3]};
+                    d = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, qh, d, 0, 0, 0);
+                    if constexpr (!STACK) d = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, ql, d, 0, 0, 0);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        if constexpr (Q8)
+                            s[T][e] = fmaf(d[e], (float)__builtin_bit_cast(half2v, dword<GROUPS>(ks[T][e], b >> 1))[b & 1],
+                                           s[T][e]);
+                        else
+                            s[T][e] = d[e];
+                    }
+                }
+                if (!Q8 || (b & 1)) {
+                    load_key(k0, 0, Q8 ? b >> 1 : b);
+                    load_key(k1, 1, Q8 ? b >> 1 : b);
+                }
+            }
+        }
+        load_scales(next, c + kWaves);
+        if constexpr (PAGED) after = pages_of(c + 2 * kWaves);
+        // ---- softmax of the lane's row over its eight keys
+        const bool whole = cur.keys == ~0u && kTile * c + kTile - 1 <= least;
+        float top = -INFINITY;
+#pragma unroll
+        for (int T = 0; T < 2; T++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                if constexpr (STACK) s[T][e] += ror8(s[T][e]);
+                s[T][e] *= factor;
+                if (!whole) {
+                    const int kk = 16 * T + 4 * g4 + e;
+                    if (!((cur.keys >> kk) & 1) || kTile * c + kk > my_limit) s[T][e] = -INFINITY;
+                }
+                top = fmaxf(top, s[T][e]);
+            }
+        top = max_rows(top) + (E - kHeadroom);
+        if (__any(top > ref + kSlack)) {
+            const float moved = fmaxf(ref, top);
+            const float shrink = moved == ref ? 1.0f : __builtin_amdgcn_exp2f(ref - moved);
+            ref = moved;
+            l *= shrink;
+            float row_shrink[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) row_shrink[e] = __shfl(shrink, 4 * g4 + e);
+#pragma unroll
+            for (int u = 0; u < GROUPS; u++)
+#pragma unroll
+                for (int t = 0; t < 4; t++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) acc[u][t][e] *= row_shrink[e];
+        }
+        float p[8];
+        {
+            const float base = ref == -INFINITY ? 0.0f : ref;
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                p[i] = __builtin_amdgcn_exp2f(s[i >> 2][i & 3] - base);
+                l += p[i];
+            }
+        }
+        // ---- value product: keys 4 g + e of both halves are the lane's eight
+        {
+            typename Dwords<GROUPS>::V vs[8];
+            if constexpr (Q8) {
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                    vs[i] = *reinterpret_cast<const typename Dwords<GROUPS>::V *>(
+                        my_scales + (32 + 16 * (i >> 2) + 4 * g4 + (i & 3)) * 4 * GROUPS);
+            }
+            const auto v0 = first_resource(vpool, next, c + kWaves, 0), v1 = first_resource(vpool, next, c + kWaves, 1);
+            half8 ph, pl;
+            auto halves = [&](const float (&x)[8]) {
+                half2v h[4], o[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    h[i] = to_half2(x[2 * i], x[2 * i + 1]);
+                    const float m = STACK ? low_half : 1.0f;
+                    o[i] = to_half2(fmaf(-m, (float)h[i][0], x[2 * i]), fmaf(-m, (float)h[i][1], x[2 * i + 1]));
+                }
+                ph = join(h[0], h[1], h[2], h[3]);
+                pl = join(o[0], o[1], o[2], o[3]);
+            };
+            if constexpr (!Q8) {
+                halves(p);
+                if (!whole) {  // what is past the last key may be anything
+#pragma unroll
+                    for (int i = 0; i < 8; i++)
+                        if (!((cur.keys >> (16 * (i >> 2) + 4 * g4 + (i & 3))) & 1))
+#pragma unroll
+                            for (int u = 0; u < GROUPS; u++) vhalf[i][u] = u32x2{0, 0};
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < GROUPS; u++) {
+                uint32_t w[8];
+                if constexpr (Q8) {
+#pragma unroll
+                    for (int i = 0; i < 8; i++) w[i] = vdig[i][u] ^ 0x80808080u;
+                }
+#pragma unroll
+                for (int t = 0; t < 4; t++) {
+                    half8 vv;
+                    if constexpr (Q8) {
+                        if (!(t & 1)) {  // block 2 u + t / 2: p times its scales
+                            float x[8];
+#pragma unroll
+                            for (int i = 0; i < 8; i++)
+                                x[i] = p[i] * (float)__builtin_bit_cast(half2v, dword<GROUPS>(vs[i], u))[t >> 1];
+                            if (!whole) {  // a scale that the row does not see may be NaN
+#pragma unroll
+                                for (int i = 0; i < 8; i++) x[i] = p[i] == 0.0f ? 0.0f : x[i];
+                            }
+                            halves(x);
+                        }
+                        vv = t == 0   ? join(value_digits<0>(w[0], w[1]), value_digits<0>(w[2], w[3]), value_digits<0>(w[4], w[5]), value_digits<0>(w[6], w[7]))
+                             : t == 1 ? join(value_digits<1>(w[0], w[1]), value_digits<1>(w[2], w[3]), value_digits<1>(w[4], w[5]), value_digits<1>(w[6], w[7]))
+                             : t == 2 ? join(value_digits<2>(w[0], w[1]), value_digits<2>(w[2], w[3]), value_digits<2>(w[4], w[5]), value_digits<2>(w[6], w[7]))
+                                      : join(value_digits<3>(w[0], w[1]), value_digits<3>(w[2], w[3]), value_digits<3>(w[4], w[5]), value_digits<3>(w[6], w[7]));
+                    } else {
+                        auto pairs = [&](auto J) {
+                            return join(value_halves<J()>(vhalf[0][u], vhalf[1][u]), value_halves<J()>(vhalf[2][u], vhalf[3][u]),
+                                        value_halves<J()>(vhalf[4][u], vhalf[5][u]), value_halves<J()>(vhalf[6][u], vhalf[7][u]));
+                        };
+                        vv = t == 0   ? pairs(std::integral_constant<int, 0>{})
+                             : t == 1 ? pairs(std::integral_constant<int, 1>{})
+                             : t == 2 ? pairs(std::integral_constant<int, 2>{})
+                                      : pairs(std::integral_constant<int, 3>{});
+                    }
+                    if constexpr (!STACK) acc[u][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph, vv, acc[u][t], 0, 0, 0);
+                    acc[u][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pl, vv, acc[u][t], 0, 0, 0);
+                }
+#pragma unroll
+                for (int i = 0; i < 8; i++) load_value(i < 4 ? v0 : v1, i, u);
+            }
+        }
+        cur = next;
+        if constexpr (PAGED) next = after;
+    }
+
+    // ---- the waves' outputs joined: o = sum_w 2^(ref_w - max ref) o_w
+    l = sum_rows(l);
+    __syncthreads();  // every wave is done with the operands the slots lie over
+    {
+        float *const slot = reinterpret_cast<float *>(lds) + wave * ROWS * L::slot_row;
+        const float unit = Q8 ? 512.0f : 1.0f;  // the digits were times 2^-9
+#pragma unroll
+        for (int u = 0; u < GROUPS; u++)
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    float x = acc[u][t][e] * unit;
+                    if constexpr (STACK) x = sum_halves(x);  // rows n and n + 8
+                    if (!STACK || g4 < 2)
+                        slot[(4 * g4 + e) * L::slot_row + 64 * u + (Q8 ? 16 * t + r16 : 4 * r16 + t)] = x;
+                }
+        if (lane < ROWS) {
+            st_m[wave * 16 + lane] = ref;
+            st_l[wave * 16 + lane] = l;
+        }
+    }
+    __syncthreads();
+    for (int idx = threadIdx.x; idx < nr * (D / 4); idx += 64 * kWaves) {
+        const int n = idx / (D / 4), d = 4 * (idx % (D / 4));
+        float m = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kWaves; w++) m = fmaxf(m, st_m[w * 16 + n]);
+        f32x4 o = {0.f, 0.f, 0.f, 0.f};
+        float total = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWaves; w++) {
+            const float mw = st_m[w * 16 + n];
+            const float f = mw == m ? 1.0f : __builtin_amdgcn_exp2f(mw - m);
+            const f32x4 x = *reinterpret_cast<const f32x4 *>(lds + ((w * ROWS + n) * L::slot_row + d) * 4);
+            o += f * x;
+            total = fmaf(f, st_l[w * 16 + n], total);
+        }
+        const int r = (n0 + n) / G, h = kvh * G + (n0 + n) % G;
+        if (sp.splits == 1) {
+            const int64_t at = (out_row + r) * a.heads + h;
+            const float inv = 1.0f / total;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                float y = total == 0.0f ? 0.0f : o[i] * inv;  // a row that sees no key
+                if (gate) y *= sigmoid_ref(gate[at * gate_stride + d + i]);
+                out[at * D + d + i] = y;
+            }
+        } else {
+            float *rec = part + ((((int64_t)j * a.rows + r) * a.heads + h) * sp.splits + split) * (D + 2);
+#pragma unroll
+            for (int i = 0; i < 4; i++) rec[d + i] = o[i];
+            if (d == 0) {
+                rec[D] = m;
+                rec[D + 1] = total;
+            }
         }
     }
 }
@@ -108,7 +589,7 @@ __global__ __launch_bounds__(256) void kv_attention_merge_kernel(const float *__
     for (int s = 0; s < splits; s++) {
         const float *p = rec + (int64_t)s * (D + 2);
         if (p[D + 1] == 0.0f) continue;  // a range without keys
-        const float w = p[D] == m ? 1.0f : expf(p[D] - m);
+        const float w = p[D] == m ? 1.0f : __builtin_amdgcn_exp2f(p[D] - m);
         l = fmaf(w, p[D + 1], l);
         o = fmaf(w, p[d], o);
     }
@@ -118,28 +599,63 @@ __global__ __launch_bounds__(256) void kv_attention_merge_kernel(const float *__
     out[(row * a.heads + h) * D + d] = y;
 }
 
+bool stacked(const KvArgs &a) { return a.heads / a.kv_heads * a.rows <= 8; }
+int row_blocks(const KvArgs &a) {
+    const int pairs = a.heads / a.kv_heads * a.rows, per = stacked(a) ? 8 : 16;
+    return (pairs + per - 1) / per;
+}
+
 int kv_splits(const KvArgs &a) {
-    const int64_t work = (int64_t)a.heads * a.requests;
-    const int64_t want = (2048 + work - 1) / work, most = (a.capacity + 4 * kChunk - 1) / (4 * kChunk);
+    const int64_t work = (int64_t)a.kv_heads * a.requests * row_blocks(a);
+    const int64_t want = (512 + work - 1) / work, most = (a.capacity + kWaves * kTile - 1) / (kWaves * kTile);
     return (int)std::max<int64_t>(1, std::min(want, most));
 }
 
 }  // namespace
 
 uint64_t kv_attention_scratch_bytes(const KvArgs &a) {
-    return (uint64_t)a.requests * a.rows * a.heads * kv_splits(a) * (a.head_dim + 2) * 4;
+    const int splits = kv_splits(a);
+    return splits == 1 ? 0 : (uint64_t)a.requests * a.rows * a.heads * splits * (a.head_dim + 2) * 4;
 }
 
 hipError_t launch_kv_attention(const float *q, int q_stride, const float *gate, int gate_stride, const void *kpool,
                                const void *vpool, const int32_t *table, float *out, const KvArgs &a, void *scratch,
                                const ModelDyn &dyn, hipStream_t s) {
-    const int splits = kv_splits(a);
-    auto *kernel = a.fmt == kKvF16 ? kv_attention_kernel<kKvF16> : kv_attention_kernel<kKvQ8>;
+    AttnSplit sp{kv_splits(a), row_blocks(a), 0};
+    while ((16 << sp.page_shift) < a.block_size) sp.page_shift++;
+    const bool paged = (16 << sp.page_shift) == a.block_size;
     float *part = static_cast<float *>(scratch);
-    kernel<<<dim3(splits, a.heads, a.requests), 256, 0, s>>>(q, q_stride, static_cast<const uint8_t *>(kpool),
-                                                             static_cast<const uint8_t *>(vpool), table, a, splits,
-                                                             part, dyn);
-    kv_attention_merge_kernel<<<dim3(a.rows, a.heads, a.requests), 256, 0, s>>>(part, splits, gate, gate_stride, out, a);
+    hipError_t err = hipSuccess;
+    auto launch = [&](auto fmt, auto groups, auto stack, auto pages) {
+        constexpr auto kernel = kv_attention_kernel<fmt(), groups(), stack(), pages()>;
+        constexpr uint32_t bytes = Layout<fmt(), groups(), stack(), pages()>::total;
+        static std::once_flag once;
+        std::call_once(once, [&] {
+            (void)hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                      (int)bytes);
+        });
+        kernel<<<dim3((uint32_t)((int64_t)sp.splits * sp.row_blocks * a.kv_heads), a.requests), 64 * kWaves, bytes, s>>>(
+            q, q_stride, gate, gate_stride, static_cast<const uint8_t *>(kpool), static_cast<const uint8_t *>(vpool), table,
+            a, sp, part, out, dyn);
+        err = hipGetLastError();
+    };
+    auto by_pages = [&](auto fmt, auto groups) {
+        if (!paged) launch(fmt, groups, std::false_type{}, std::false_type{});
+        else if (stacked(a)) launch(fmt, groups, std::true_type{}, std::true_type{});
+        else launch(fmt, groups, std::false_type{}, std::true_type{});
+    };
+    auto by_width = [&](auto fmt) {
+        switch (a.head_dim / 64) {
+        case 1: by_pages(fmt, std::integral_constant<int, 1>{}); break;
+        case 2: by_pages(fmt, std::integral_constant<int, 2>{}); break;
+        case 3: by_pages(fmt, std::integral_constant<int, 3>{}); break;
+        default: by_pages(fmt, std::integral_constant<int, 4>{}); break;
+        }
+    };
+    if (a.fmt == kKvF16) by_width(std::integral_constant<int, kKvF16>{});
+    else by_width(std::integral_constant<int, kKvQ8>{});
+    if (err != hipSuccess || sp.splits == 1) return err;
+    kv_attention_merge_kernel<<<dim3(a.rows, a.heads, a.requests), 256, 0, s>>>(part, sp.splits, gate, gate_stride, out, a);
     return hipGetLastError();
 }
 
