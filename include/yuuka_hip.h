@@ -552,10 +552,11 @@ YUUKA_API yuuka_status yuuka_moe_pack_q4k(yuuka_stream * stream, yuuka_buffer * 
  * the v10 KV writes). A Q8_0 page is [block_size][kv_dim] int8 digits followed
  * by [block_size][kv_dim / 32] F16 scales; a value is digit * scale of its block
  * of 32 dims. Every 64 dims' digits are stored as a 16 x 4 matrix: byte
- * 4 r + j of the 64 holds dim 16 j + r. Rounding, in FP32 as the reference's
- * kv_format.go:93-137: s = max|x| / 127, scale = F16(s), half up; digit = x / s
- * to the nearest, halves away from zero. A block holding a NaN reads back as
- * NaN, one past the scale's range (|x| over 8.3e6) as infinities and NaN.
+ * 4 r + j of the 64 holds dim 16 j + r. Rounding, in FP32 (kv_format.go:93-137
+ * up to the last bit of s): s = max|x| * (1 / 127), scale = F16(s), half up;
+ * digit = x / s to the nearest, halves away from zero. A block holding a NaN
+ * reads back as NaN, one past the scale's range (|x| over 8.3e6) as infinities
+ * and NaN.
  *
  * Request j's block table is the j-th run of ceil(capacity / block_size) int32
  * page indices. An entry outside the pool (such as -1) is an unmapped page:

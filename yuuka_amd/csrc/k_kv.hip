@@ -2,12 +2,14 @@
 // reading it back (the reference's row codec model/qwen35/kv_format.go:93-168
 // behind kv_pool.go:131-170, on the device).
 //
-// Q8_0 rounding of a block of 32 values x, as the reference's EncodeRow
-// (kv_format.go:93-137), every step in float32, so that the cached values are
-// the CPU decoder's bit for bit:
-//   scale = max|x| / 127, stored as F16 (half up, as every F16 of the cache)
+// Q8_0 rounding of a block of 32 values x, every step in float32:
+//   scale = max|x| * (1 / 127), stored as F16 (half up, as every F16 of the cache)
 //   digit = x / scale to the nearest, halves away from zero; 0 where scale is 0
 //   value = digit * F16 scale (exact in float32: 7 + 11 significant bits)
+// The reference's EncodeRow (kv_format.go:93-137) divides max|x| by 127: the
+// product's last bit differs in one block of 22, which moves one digit in a
+// million by a step. A value is off by at most half a step, scale / 2, and by
+// |x| 2^-11 for the scale's own rounding.
 // A block that holds a NaN has a NaN scale (the reference leaves that case
 // undefined), so that it reads back as NaN instead of as finite values.
 #include <hip/hip_runtime.h>
@@ -162,7 +164,7 @@ __global__ __launch_bounds__(64 * kAppendWaves) void kv_append_kernel(
         for (int b = 0; b < 2; b++) {
 #pragma unroll
             for (int off = 1; off < 16; off <<= 1) m[b] = max_nan(m[b], __shfl_xor(m[b], off));
-            const float scale = __fdiv_rn(m[b], 127.0f);
+            const float scale = __fmul_rn(m[b], 1.0f / 127.0f);
             d16[b] = ref_f32_to_f16(scale);
 #pragma unroll
             for (int i = 0; i < 2; i++) {

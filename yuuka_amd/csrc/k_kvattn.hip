@@ -105,7 +105,7 @@ template <int FMT, int GROUPS, bool STACK, bool PAGED> struct Layout {
     static constexpr bool Q8 = FMT == kKvQ8;
     static constexpr int D = 64 * GROUPS, NB = 2 * GROUPS, ROWS = STACK ? 8 : 16;
     static constexpr uint32_t plane = NB * 1024;                              // query operands, one half
-    static constexpr uint32_t scales = STACK ? plane : 2 * plane;             // [wave][key, value][32][GROUPS dwords]
+    static constexpr uint32_t scales = STACK ? plane : 2 * plane;             // [wave][key, value][GROUPS][32] dwords
     static constexpr uint32_t addr = scales + (Q8 ? kWaves * 256 * GROUPS : 0);  // [wave][32] row offsets
     static constexpr uint32_t loop = addr + (PAGED ? 0 : kWaves * 256);
     static constexpr int slot_row = D + 4;                                    // floats; rows 4 g land 16 banks apart
@@ -146,7 +146,8 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
     const int64_t p0 = kv_position(a, dyn, j, 0);
     // last key a row sees, -1 for none
     auto limit = [&](int n) { return (int)max((int64_t)-1, min(p0 + n / G, (int64_t)a.capacity - 1)); };
-    const int len = limit(n0 + nr - 1) + 1, least = limit(n0);
+    const int len = __builtin_amdgcn_readfirstlane(limit(n0 + nr - 1) + 1);
+    const int least = __builtin_amdgcn_readfirstlane(limit(n0));
     const int tiles = (len + kTile - 1) / kTile;
     const int per = max((tiles + sp.splits - 1) / sp.splits, kWaves);
     const int c0 = split * per, c1 = min(tiles, c0 + per);
@@ -177,7 +178,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
             for (int T = 0; T < 2; T++) {
                 const int tok = kTile * c + 16 * T;
                 int page = -1;
-                if (c < c1 && tok < len) page = table_j[tok >> (4 + sp.page_shift)];
+                if (c < c1 && tok < len) page = __builtin_amdgcn_readfirstlane(table_j[tok >> (4 + sp.page_shift)]);
                 t.page[T] = (uint32_t)page < (uint32_t)a.pages ? page : -1;
                 if (t.page[T] >= 0) t.keys |= (0xffffu >> max(0, tok + 16 - len)) << (16 * T);
             }
@@ -196,9 +197,13 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
         const int in = ((2 * c + T) & ((1 << sp.page_shift) - 1)) * 16;  // tokens before the half in its page
         const int64_t skip = (int64_t)in * row_bytes;
         const int page = t.page[T];
-        return __builtin_amdgcn_make_buffer_rsrc(
-            const_cast<uint8_t *>(pool) + (page >= 0 ? page * page_bytes + skip : 0), (short)0,
-            page >= 0 ? (int)(page_bytes - skip) : 0, 0x00020000);
+        // uniform, but 64-bit products are vector instructions; without scalar
+        // registers each load would be a loop over the lanes
+        const uint64_t base = (uint64_t)(pool + (page >= 0 ? page * page_bytes + skip : 0));
+        const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)base);
+        const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)(base >> 32));
+        const int bytes = __builtin_amdgcn_readfirstlane(page >= 0 ? (int)(page_bytes - skip) : 0);
+        return __builtin_amdgcn_make_buffer_rsrc((void *)((uint64_t)hi << 32 | lo), (short)0, bytes, 0x00020000);
     };
     uint8_t *const my_scales = lds + L::scales + wave * 256 * GROUPS;
     int64_t *const my_addr = reinterpret_cast<int64_t *>(lds + L::addr) + wave * 32;
@@ -332,7 +337,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
 #pragma unroll
             for (int s = 0; s < GROUPS; s++) {
                 const uint32_t d = there ? dword<GROUPS>(sreg, s) : 0u;
-                reinterpret_cast<uint32_t *>(my_scales)[lane * GROUPS + s] = d;
+                reinterpret_cast<uint32_t *>(my_scales)[((lane >> 5) * GROUPS + s) * 32 + (lane & 31)] = d;
                 const uint32_t lo = d & 0x7fffu, hi = (d >> 16) & 0x7fffu;
                 most = max(most, max(lo < 0x7c00u ? lo : 0u, hi < 0x7c00u ? hi : 0u));
             }
@@ -351,18 +356,16 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
         // ---- scores: keys 4 g + e of half T against query row r16
         float s[2][4] = {};
         {
-            typename Dwords<GROUPS>::V ks[2][4];
-            if constexpr (Q8) {
-#pragma unroll
-                for (int T = 0; T < 2; T++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        ks[T][e] = *reinterpret_cast<const typename Dwords<GROUPS>::V *>(
-                            my_scales + (16 * T + 4 * g4 + e) * 4 * GROUPS);
-            }
+            u32x4 ks[2];  // two blocks' scales of the lane's keys
             const auto k0 = first_resource(kpool, next, c + kWaves, 0), k1 = first_resource(kpool, next, c + kWaves, 1);
 #pragma unroll
             for (int b = 0; b < NB; b++) {
+                if constexpr (Q8) {
+                    if (!(b & 1))
+#pragma unroll
+                        for (int T = 0; T < 2; T++)
+                            ks[T] = *reinterpret_cast<const u32x4 *>(my_scales + ((b >> 1) * 32 + 16 * T + 4 * g4) * 4);
+                }
                 const half8 qh = *reinterpret_cast<const half8 *>(lds + (b * 64 + lane) * 16);
                 half8 ql{};
                 if constexpr (!STACK) ql = *reinterpret_cast<const half8 *>(lds + L::plane + (b * 64 + lane) * 16);
@@ -383,8 +386,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
                         if constexpr (Q8)
-                            s[T][e] = fmaf(d[e], (float)__builtin_bit_cast(half2v, dword<GROUPS>(ks[T][e], b >> 1))[b & 1],
-                                           s[T][e]);
+                            s[T][e] = fmaf(d[e], (float)__builtin_bit_cast(half2v, (uint32_t)ks[T][e])[b & 1], s[T][e]);
                         else
                             s[T][e] = d[e];
                     }
@@ -439,13 +441,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
         }
         // ---- value product: keys 4 g + e of both halves are the lane's eight
         {
-            typename Dwords<GROUPS>::V vs[8];
-            if constexpr (Q8) {
-#pragma unroll
-                for (int i = 0; i < 8; i++)
-                    vs[i] = *reinterpret_cast<const typename Dwords<GROUPS>::V *>(
-                        my_scales + (32 + 16 * (i >> 2) + 4 * g4 + (i & 3)) * 4 * GROUPS);
-            }
+            u32x4 vs[2];  // two blocks' scales of the lane's keys
             const auto v0 = first_resource(vpool, next, c + kWaves, 0), v1 = first_resource(vpool, next, c + kWaves, 1);
             half8 ph, pl;
             auto halves = [&](const float (&x)[8]) {
@@ -474,6 +470,9 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
                 uint32_t w[8];
                 if constexpr (Q8) {
 #pragma unroll
+                    for (int T = 0; T < 2; T++)
+                        vs[T] = *reinterpret_cast<const u32x4 *>(my_scales + ((GROUPS + u) * 32 + 16 * T + 4 * g4) * 4);
+#pragma unroll
                     for (int i = 0; i < 8; i++) w[i] = vdig[i][u] ^ 0x80808080u;
                 }
 #pragma unroll
@@ -484,7 +483,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
                             float x[8];
 #pragma unroll
                             for (int i = 0; i < 8; i++)
-                                x[i] = p[i] * (float)__builtin_bit_cast(half2v, dword<GROUPS>(vs[i], u))[t >> 1];
+                                x[i] = p[i] * (float)__builtin_bit_cast(half2v, (uint32_t)vs[i >> 2][i & 3])[t >> 1];
                             if (!whole) {  // a scale that the row does not see may be NaN
 #pragma unroll
                                 for (int i = 0; i < 8; i++) x[i] = p[i] == 0.0f ? 0.0f : x[i];
