@@ -47,6 +47,9 @@ yuuka_status kv_check(KvArgs *a, uint32_t dtype, bool attention) {
     if (attention && (a->heads < 1 || a->heads % a->kv_heads || a->heads > 65535 || a->rows > 4096))
         return fail(YUUKA_ERR_INVALID_ARGUMENT, "decode attention of %d rows, %d heads over %d KV heads", a->rows,
                     a->heads, a->kv_heads);
+    if (attention && kv_page_bytes(*a) > 0x7fffffff)
+        return fail(YUUKA_ERR_UNSUPPORTED, "decode attention over pages of %lld bytes (below 2 GiB are served)",
+                    (long long)kv_page_bytes(*a));
     return YUUKA_OK;
 }
 

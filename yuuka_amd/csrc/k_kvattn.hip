@@ -164,24 +164,37 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
 
     // ---- pages of a tile's halves, and which of its keys there are
     const int32_t *const table_j = table + (int64_t)j * kv_table_blocks(a);
-    const int64_t page_bytes = kv_page_bytes(a);
+    const uint32_t page_bytes = (uint32_t)kv_page_bytes(a);
     const uint32_t row_bytes = Q8 ? a.kv_dim : a.kv_dim * 2;
+    // (PAGED: everything uniform, made scalar by hand; a buffer resource out of
+    // vector registers costs every load a loop over the lanes)
     struct Tile {
-        int page[2];    // PAGED: -1 unmapped or past the end
-        uint32_t keys;  // bit k: key k of the tile is there
+        uint64_t row[2], scales[2];  // offsets in the pools: first token of each half, and its scales
+        uint32_t bytes[2];           // from there to the end of the page; 0: unmapped or past the end
+        uint32_t keys;               // bit k: key k of the tile is there
+    };
+    auto scalar64 = [](uint64_t x) {  // (the builtin's result is a signed int)
+        const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)x);
+        const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)(x >> 32));
+        return (uint64_t)hi << 32 | lo;
     };
     auto pages_of = [&](int c) {
-        Tile t;
-        t.keys = 0;
+        Tile t{};
         if constexpr (PAGED) {
 #pragma unroll
             for (int T = 0; T < 2; T++) {
                 const int tok = kTile * c + 16 * T;
                 int page = -1;
                 if (c < c1 && tok < len) page = __builtin_amdgcn_readfirstlane(table_j[tok >> (4 + sp.page_shift)]);
-                t.page[T] = (uint32_t)page < (uint32_t)a.pages ? page : -1;
-                if (t.page[T] >= 0) t.keys |= (0xffffu >> max(0, tok + 16 - len)) << (16 * T);
+                const bool mapped = (uint32_t)page < (uint32_t)a.pages;
+                const uint32_t in = tok & ((16u << sp.page_shift) - 1);  // tokens before the half in its page
+                const uint64_t at = (uint64_t)(mapped ? (uint32_t)page : 0u) * page_bytes;
+                t.row[T] = scalar64(at + in * row_bytes);
+                t.scales[T] = scalar64(at + a.block_size * row_bytes + in * (a.kv_dim / 16));
+                t.bytes[T] = __builtin_amdgcn_readfirstlane(mapped ? page_bytes - in * row_bytes : 0u);
+                if (mapped) t.keys |= (0xffffu >> max(0, tok + 16 - len)) << (16 * T);
             }
+            t.keys = __builtin_amdgcn_readfirstlane(t.keys);
         }
         return t;
     };
@@ -191,34 +204,25 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
     u32x2 vhalf[Q8 ? 1 : 8][GROUPS];
     typename Dwords<GROUPS>::V sreg;  // lanes 0..31: scales of key `lane`, 32..63: of value `lane - 32`
     const uint8_t *krow[PAGED ? 1 : 2], *vrow[PAGED ? 1 : 8];  // rows of the tile to be loaded
-    const uint32_t koff = r16 * row_bytes + kvh * D * (Q8 ? 1 : 2) + 16 * g4;
+    uint32_t koff = r16 * row_bytes + kvh * D * (Q8 ? 1 : 2) + 16 * g4;
     const uint32_t voff = 4 * g4 * row_bytes + kvh * D * (Q8 ? 1 : 2) + r16 * (Q8 ? 4 : 8);
-    auto resource = [&](const uint8_t *pool, const Tile &t, int c, int T) {
-        const int in = ((2 * c + T) & ((1 << sp.page_shift) - 1)) * 16;  // tokens before the half in its page
-        const int64_t skip = (int64_t)in * row_bytes;
-        const int page = t.page[T];
-        // uniform, but 64-bit products are vector instructions; without scalar
-        // registers each load would be a loop over the lanes
-        const uint64_t base = (uint64_t)(pool + (page >= 0 ? page * page_bytes + skip : 0));
-        const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)base);
-        const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)(base >> 32));
-        const int bytes = __builtin_amdgcn_readfirstlane(page >= 0 ? (int)(page_bytes - skip) : 0);
-        return __builtin_amdgcn_make_buffer_rsrc((void *)((uint64_t)hi << 32 | lo), (short)0, bytes, 0x00020000);
+    uint32_t voff_row[4] = {voff, voff + row_bytes, voff + 2 * row_bytes, voff + 3 * row_bytes};
+    auto resource = [&](const uint8_t *pool, const Tile &t, int T) {
+        return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(pool) + (PAGED ? t.row[T] : 0), (short)0,
+                                                 PAGED ? (int)t.bytes[T] : 0, 0x00020000);
     };
-    uint8_t *const my_scales = lds + L::scales + wave * 256 * GROUPS;
+    // LDS offsets of the wave's scales: where the lane's key goes, and keys 4 g4 .. + 3
+    uint32_t scale_write = L::scales + wave * 256 * GROUPS + (lane >> 5) * 128 * GROUPS + (lane & 31) * 4;
+    uint32_t scale_read = L::scales + wave * 256 * GROUPS + g4 * 16;
+    uint32_t query_read = lane * 16;  // of the lane's operands
     int64_t *const my_addr = reinterpret_cast<int64_t *>(lds + L::addr) + wave * 32;
-    auto load_scales = [&](const Tile &t, int c) {
+    const uint32_t soff = (lane & 15) * (a.kv_dim / 16) + kvh * NB * 2;
+    auto load_scales = [&](const Tile &t) {  // (an unmapped half reads page 0's: not used)
         if constexpr (Q8 && PAGED) {
-            const int T = (lane >> 4) & 1, tok = lane & 15;
-            int64_t at[2];
-#pragma unroll
-            for (int u = 0; u < 2; u++) {
-                const int in = ((2 * c + u) & ((1 << sp.page_shift) - 1)) * 16;
-                at[u] = t.page[u] * page_bytes + (int64_t)a.block_size * a.kv_dim + (int64_t)in * (a.kv_dim / 16);
-            }
-            const bool there = (t.keys >> (lane & 31)) & 1;
-            const int64_t off = there ? (T ? at[1] : at[0]) + tok * (a.kv_dim / 16) + kvh * NB * 2 : 0;
-            sreg = *reinterpret_cast<const typename Dwords<GROUPS>::V *>((lane < 32 ? kpool : vpool) + off);
+            const uint8_t *k0 = kpool + t.scales[0], *k1 = kpool + t.scales[1];
+            const uint8_t *v0 = vpool + t.scales[0], *v1 = vpool + t.scales[1];
+            const uint8_t *at = (lane < 32 ? (lane & 16 ? k1 : k0) : (lane & 16 ? v1 : v0)) + soff;
+            sreg = *reinterpret_cast<const typename Dwords<GROUPS>::V *>(at);
         }
     };
     // !PAGED: every lane finds the row (and the scales) of key `lane & 31`
@@ -250,7 +254,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
             kreg[T][p] = *reinterpret_cast<const typename Dwords<4>::V *>(krow[T] + 64 * p);
     };
     auto load_value = [&](__amdgpu_buffer_rsrc_t rs, int i, int s) {
-        const uint32_t off = voff + (i & 3) * row_bytes;
+        const uint32_t off = voff_row[i & 3];
         if constexpr (Q8 && PAGED) vdig[i][s] = (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(rs, off + 64 * s, 0, 0);
         else if constexpr (Q8) vdig[i][s] = *reinterpret_cast<const uint32_t *>(vrow[i] + 64 * s);
         else if constexpr (PAGED)
@@ -258,17 +262,12 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
         else
             vhalf[i][s] = *reinterpret_cast<const typename Dwords<2>::V *>(vrow[i] + 128 * s);
     };
-    auto first_resource = [&](const uint8_t *pool, const Tile &t, int c, int T) {
-        if constexpr (PAGED) return resource(pool, t, c, T);
-        else return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(pool), (short)0, 0, 0x00020000);
-    };
-
     int c = c0 + wave;
     Tile cur = PAGED ? pages_of(c) : find_rows(c);
-    load_scales(cur, c);
+    load_scales(cur);
     {
-        const auto k0 = first_resource(kpool, cur, c, 0), k1 = first_resource(kpool, cur, c, 1);
-        const auto v0 = first_resource(vpool, cur, c, 0), v1 = first_resource(vpool, cur, c, 1);
+        const auto k0 = resource(kpool, cur, 0), k1 = resource(kpool, cur, 1);
+        const auto v0 = resource(vpool, cur, 0), v1 = resource(vpool, cur, 1);
 #pragma unroll
         for (int p = 0; p < KP; p++) {
             load_key(k0, 0, p);
@@ -317,7 +316,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
     const int my_n = STACK ? r16 & 7 : r16;
     const float factor = row_factor[my_n];
     const int my_limit = my_n < nr ? limit(n0 + my_n) : -1;
-    const float low_half = STACK && r16 >= 8 ? 1.0f : 0.0f;  // this lane's probabilities: the remainder's half
+    const bool low_half = STACK && r16 >= 8;  // this lane's probabilities are the remainders
     f32x4 acc[GROUPS][4];
 #pragma unroll
     for (int s = 0; s < GROUPS; s++)
@@ -328,21 +327,38 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
     Tile next{};
     if constexpr (PAGED) next = pages_of(c + kWaves);
     for (; c < c1; c += kWaves) {
+        // Opaque in every turn: the constant steps from these addresses then stay
+        // in the instructions' immediate offsets. Hoisted out of the loop they take a
+        // register each, loaded values spill, and every spill waits for all loads.
+        asm volatile("" : "+v"(koff), "+v"(voff_row[0]), "+v"(voff_row[1]), "+v"(voff_row[2]), "+v"(voff_row[3]));
+        asm volatile("" : "+v"(scale_write), "+v"(scale_read), "+v"(query_read));
+        // every row sees every key of the tile
+        const bool whole = cur.keys == ~0u && kTile * c + kTile - 1 <= least;
         float E = 0.0f;
+        uint32_t poison = 0;  // keys with a non-finite value that not every row sees: left out, their rows made NaN
         if constexpr (Q8) {
             // scales to LDS (those of missing keys as zeros), and the largest finite value scale's exponent
             wave_lds_fence();
             const bool there = (cur.keys >> (lane & 31)) & 1;
-            uint32_t most = 0;
+            uint32_t d[GROUPS], most = 0, over = 0;
 #pragma unroll
             for (int s = 0; s < GROUPS; s++) {
-                const uint32_t d = there ? dword<GROUPS>(sreg, s) : 0u;
-                reinterpret_cast<uint32_t *>(my_scales)[((lane >> 5) * GROUPS + s) * 32 + (lane & 31)] = d;
-                const uint32_t lo = d & 0x7fffu, hi = (d >> 16) & 0x7fffu;
+                d[s] = there ? dword<GROUPS>(sreg, s) : 0u;
+                const uint32_t lo = d[s] & 0x7fffu, hi = (d[s] >> 16) & 0x7fffu;
                 most = max(most, max(lo < 0x7c00u ? lo : 0u, hi < 0x7c00u ? hi : 0u));
+                over |= ((d[s] & 0x7fff7fffu) + 0x04000400u) & 0x80008000u;
             }
-            if (lane < 32) most = 0;
-            float m = __uint_as_float(most);  // non-negative: ordered as floats
+            if (!whole) {
+                const uint64_t b = __builtin_amdgcn_ballot_w64(over != 0 && kTile * c + (lane & 31) > least);
+                poison = (uint32_t)(b >> 32);
+                if (lane >= 32 && (poison >> (lane & 31)) & 1) {
+#pragma unroll
+                    for (int s = 0; s < GROUPS; s++) d[s] = 0;
+                }
+            }
+#pragma unroll
+            for (int s = 0; s < GROUPS; s++) *reinterpret_cast<uint32_t *>(lds + scale_write + 128 * s) = d[s];
+            float m = __uint_as_float(lane < 32 ? 0u : most);  // non-negative: ordered as floats
             m = fmaxf(m, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(m), 0xb1, 0xf, 0xf, true)));
             m = fmaxf(m, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(m), 0x4e, 0xf, 0xf, true)));
             m = fmaxf(m, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(m), 0x124, 0xf, 0xf, true)));
@@ -357,18 +373,18 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
         float s[2][4] = {};
         {
             u32x4 ks[2];  // two blocks' scales of the lane's keys
-            const auto k0 = first_resource(kpool, next, c + kWaves, 0), k1 = first_resource(kpool, next, c + kWaves, 1);
+            const auto k0 = resource(kpool, next, 0), k1 = resource(kpool, next, 1);
 #pragma unroll
             for (int b = 0; b < NB; b++) {
                 if constexpr (Q8) {
                     if (!(b & 1))
 #pragma unroll
                         for (int T = 0; T < 2; T++)
-                            ks[T] = *reinterpret_cast<const u32x4 *>(my_scales + ((b >> 1) * 32 + 16 * T + 4 * g4) * 4);
+                            ks[T] = *reinterpret_cast<const u32x4 *>(lds + scale_read + (b >> 1) * 128 + 64 * T);
                 }
-                const half8 qh = *reinterpret_cast<const half8 *>(lds + (b * 64 + lane) * 16);
+                const half8 qh = *reinterpret_cast<const half8 *>(lds + query_read + b * 1024);
                 half8 ql{};
-                if constexpr (!STACK) ql = *reinterpret_cast<const half8 *>(lds + L::plane + (b * 64 + lane) * 16);
+                if constexpr (!STACK) ql = *reinterpret_cast<const half8 *>(lds + query_read + L::plane + b * 1024);
 #pragma unroll
                 for (int T = 0; T < 2; T++) {
                     half8 kk;
@@ -394,13 +410,13 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
                 if (!Q8 || (b & 1)) {
                     load_key(k0, 0, Q8 ? b >> 1 : b);
                     load_key(k1, 1, Q8 ? b >> 1 : b);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
             }
         }
-        load_scales(next, c + kWaves);
+        load_scales(next);
         if constexpr (PAGED) after = pages_of(c + 2 * kWaves);
         // ---- softmax of the lane's row over its eight keys
-        const bool whole = cur.keys == ~0u && kTile * c + kTile - 1 <= least;
         float top = -INFINITY;
 #pragma unroll
         for (int T = 0; T < 2; T++)
@@ -408,12 +424,35 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
             for (int e = 0; e < 4; e++) {
                 if constexpr (STACK) s[T][e] += ror8(s[T][e]);
                 s[T][e] *= factor;
-                if (!whole) {
-                    const int kk = 16 * T + 4 * g4 + e;
-                    if (!((cur.keys >> kk) & 1) || kTile * c + kk > my_limit) s[T][e] = -INFINITY;
-                }
-                top = fmaxf(top, s[T][e]);
             }
+        if (!whole) {
+            int first = 4 * g4;  // opaque: what follows is not kept in registers for every tile
+            asm volatile("" : "+v"(first));
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const int kk = first + 16 * (i >> 2) + (i & 3);
+                bool there = (cur.keys >> kk) & 1, bad = (poison >> kk) & 1;
+                if constexpr (!Q8) {  // values that not every row sees must be finite for those that do not
+                    uint32_t over = 0;
+#pragma unroll
+                    for (int u = 0; u < GROUPS; u++)
+#pragma unroll
+                        for (int w = 0; w < 2; w++) over |= (vhalf[i][u][w] & 0x7fff7fffu) + 0x04000400u;
+                    const uint64_t b = __builtin_amdgcn_ballot_w64((over & 0x80008000u) != 0);
+                    bad = ((b >> (4 * first)) & 0xffffu) != 0 && kTile * c + kk > least;
+                    if (!there || bad) {
+#pragma unroll
+                        for (int u = 0; u < GROUPS; u++) vhalf[i][u] = u32x2{0, 0};
+                    }
+                }
+                const bool seen = there && kTile * c + kk <= my_limit;
+                s[i >> 2][i & 3] = !seen ? -INFINITY : bad ? NAN : s[i >> 2][i & 3];
+            }
+        }
+#pragma unroll
+        for (int T = 0; T < 2; T++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) top = fmaxf(top, s[T][e]);
         top = max_rows(top) + (E - kHeadroom);
         if (__any(top > ref + kSlack)) {
             const float moved = fmaxf(ref, top);
@@ -442,36 +481,31 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
         // ---- value product: keys 4 g + e of both halves are the lane's eight
         {
             u32x4 vs[2];  // two blocks' scales of the lane's keys
-            const auto v0 = first_resource(vpool, next, c + kWaves, 0), v1 = first_resource(vpool, next, c + kWaves, 1);
+            const auto v0 = resource(vpool, next, 0), v1 = resource(vpool, next, 1);
             half8 ph, pl;
-            auto halves = [&](const float (&x)[8]) {
+            // p[i] * d(i) as two halves (stacked: the one that the lane's row is)
+            auto halves = [&](auto d) {
                 half2v h[4], o[4];
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    h[i] = to_half2(x[2 * i], x[2 * i + 1]);
-                    const float m = STACK ? low_half : 1.0f;
-                    o[i] = to_half2(fmaf(-m, (float)h[i][0], x[2 * i]), fmaf(-m, (float)h[i][1], x[2 * i + 1]));
+                    const float x = d(2 * i), y = d(2 * i + 1);
+                    h[i] = half2v{(_Float16)fmaf(p[2 * i], x, 0.0f), (_Float16)fmaf(p[2 * i + 1], y, 0.0f)};
+                    o[i] = half2v{(_Float16)fmaf(p[2 * i], x, -(float)h[i][0]), (_Float16)fmaf(p[2 * i + 1], y, -(float)h[i][1])};
+                    // one value h in every lane: rounded twice by different
+                    // instructions, the two rows' halves need not be each other's
+                    if constexpr (STACK) o[i] = low_half ? o[i] : h[i];
                 }
                 ph = join(h[0], h[1], h[2], h[3]);
                 pl = join(o[0], o[1], o[2], o[3]);
             };
-            if constexpr (!Q8) {
-                halves(p);
-                if (!whole) {  // what is past the last key may be anything
-#pragma unroll
-                    for (int i = 0; i < 8; i++)
-                        if (!((cur.keys >> (16 * (i >> 2) + 4 * g4 + (i & 3))) & 1))
-#pragma unroll
-                            for (int u = 0; u < GROUPS; u++) vhalf[i][u] = u32x2{0, 0};
-                }
-            }
+            if constexpr (!Q8) halves([](int) { return 1.0f; });
 #pragma unroll
             for (int u = 0; u < GROUPS; u++) {
                 uint32_t w[8];
                 if constexpr (Q8) {
 #pragma unroll
                     for (int T = 0; T < 2; T++)
-                        vs[T] = *reinterpret_cast<const u32x4 *>(my_scales + ((GROUPS + u) * 32 + 16 * T + 4 * g4) * 4);
+                        vs[T] = *reinterpret_cast<const u32x4 *>(lds + scale_read + (GROUPS + u) * 128 + 64 * T);
 #pragma unroll
                     for (int i = 0; i < 8; i++) w[i] = vdig[i][u] ^ 0x80808080u;
                 }
@@ -479,17 +513,10 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
                 for (int t = 0; t < 4; t++) {
                     half8 vv;
                     if constexpr (Q8) {
-                        if (!(t & 1)) {  // block 2 u + t / 2: p times its scales
-                            float x[8];
-#pragma unroll
-                            for (int i = 0; i < 8; i++)
-                                x[i] = p[i] * (float)__builtin_bit_cast(half2v, (uint32_t)vs[i >> 2][i & 3])[t >> 1];
-                            if (!whole) {  // a scale that the row does not see may be NaN
-#pragma unroll
-                                for (int i = 0; i < 8; i++) x[i] = p[i] == 0.0f ? 0.0f : x[i];
-                            }
-                            halves(x);
-                        }
+                        if (!(t & 1))  // block 2 u + t / 2
+                            halves([&](int i) {
+                                return (float)__builtin_bit_cast(half2v, (uint32_t)vs[i >> 2][i & 3])[t >> 1];
+                            });
                         vv = t == 0   ? join(value_digits<0>(w[0], w[1]), value_digits<0>(w[2], w[3]), value_digits<0>(w[4], w[5]), value_digits<0>(w[6], w[7]))
                              : t == 1 ? join(value_digits<1>(w[0], w[1]), value_digits<1>(w[2], w[3]), value_digits<1>(w[4], w[5]), value_digits<1>(w[6], w[7]))
                              : t == 2 ? join(value_digits<2>(w[0], w[1]), value_digits<2>(w[2], w[3]), value_digits<2>(w[4], w[5]), value_digits<2>(w[6], w[7]))
@@ -509,6 +536,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
                 }
 #pragma unroll
                 for (int i = 0; i < 8; i++) load_value(i < 4 ? v0 : v1, i, u);
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
         cur = next;
@@ -606,7 +634,7 @@ int row_blocks(const KvArgs &a) {
 
 int kv_splits(const KvArgs &a) {
     const int64_t work = (int64_t)a.kv_heads * a.requests * row_blocks(a);
-    const int64_t want = (512 + work - 1) / work, most = (a.capacity + kWaves * kTile - 1) / (kWaves * kTile);
+    const int64_t want = (256 + work - 1) / work, most = (a.capacity + kWaves * kTile - 1) / (kWaves * kTile);
     return (int)std::max<int64_t>(1, std::min(want, most));
 }
 
