@@ -127,7 +127,7 @@ template <int FMT, int GROUPS, bool STACK, bool PAGED>
 __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 2))) void kv_attention_kernel(
     const float *__restrict__ q, int q_stride, const float *__restrict__ gate, int gate_stride,
     const uint8_t *__restrict__ kpool, const uint8_t *__restrict__ vpool, const int32_t *__restrict__ table, KvArgs a,
-    AttnSplit sp, float *__restrict__ part, float *__restrict__ out, ModelDyn dyn) {
+    AttnSplit sp, float *__restrict__ part, float2 *__restrict__ stats, float *__restrict__ out, ModelDyn dyn) {
     using L = Layout<FMT, GROUPS, STACK, PAGED>;
     constexpr bool Q8 = L::Q8;
     constexpr int D = L::D, NB = L::NB, ROWS = L::ROWS;
@@ -155,11 +155,22 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
     if (c0 >= c1 && sp.splits > 1) {  // nothing here: an empty record
         if (threadIdx.x < (uint32_t)nr) {
             const int n = n0 + threadIdx.x, r = n / G, h = kvh * G + n % G;
-            float *rec = part + ((((int64_t)j * a.rows + r) * a.heads + h) * sp.splits + split) * (D + 2);
-            rec[D] = -INFINITY;
-            rec[D + 1] = 0.0f;
+            stats[(((int64_t)j * a.rows + r) * a.heads + h) * sp.splits + split] = make_float2(-INFINITY, 0.0f);
         }
         return;
+    }
+
+    // the query rows that this wave prepares: loaded before the first tile, since
+    // loads return in order
+    float queries[ROWS / kWaves][GROUPS];
+#pragma unroll
+    for (int half = 0; half < ROWS / kWaves; half++) {
+        const int n = min(wave + kWaves * half, nr - 1), r = (n0 + n) / G, h = kvh * G + (n0 + n) % G;
+#pragma unroll
+        for (int s = 0; s < GROUPS; s++) {
+            const float x = q[((out_row + r) * a.heads + h) * q_stride + 64 * s + lane];
+            queries[half][s] = wave + kWaves * half < nr ? x : 0.0f;
+        }
     }
 
     // ---- pages of a tile's halves, and which of its keys there are
@@ -281,14 +292,12 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
 
     // ---- queries as MFMA operands in LDS: wave w prepares rows w and w + 8
 #pragma unroll
-    for (int n = wave; n < ROWS; n += kWaves) {
-        float x[GROUPS], top = 0.0f;
-        const int r = (n0 + n) / G, h = kvh * G + (n0 + n) % G;
+    for (int half = 0; half < ROWS / kWaves; half++) {
+        const int n = wave + kWaves * half;
+        const float(&x)[GROUPS] = queries[half];
+        float top = 0.0f;
 #pragma unroll
-        for (int s = 0; s < GROUPS; s++) {
-            x[s] = n < nr ? q[((out_row + r) * a.heads + h) * q_stride + 64 * s + lane] : 0.0f;
-            top = fmaxf(top, fabsf(x[s]));
-        }
+        for (int s = 0; s < GROUPS; s++) top = fmaxf(top, fabsf(x[s]));
 #pragma unroll
         for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
         int e = 14;
@@ -592,38 +601,73 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
                 out[at * D + d + i] = y;
             }
         } else {
-            float *rec = part + ((((int64_t)j * a.rows + r) * a.heads + h) * sp.splits + split) * (D + 2);
-#pragma unroll
-            for (int i = 0; i < 4; i++) rec[d + i] = o[i];
-            if (d == 0) {
-                rec[D] = m;
-                rec[D + 1] = total;
-            }
+            const int64_t rec = (((int64_t)j * a.rows + r) * a.heads + h) * sp.splits + split;
+            *reinterpret_cast<f32x4 *>(part + rec * D + d) = o;
+            if (d == 0) stats[rec] = make_float2(m, total);
         }
     }
 }
 
-// One workgroup per (row, head, request): joins the ranges' records.
-__global__ __launch_bounds__(256) void kv_attention_merge_kernel(const float *__restrict__ part, int splits,
+// One workgroup of four waves per (row, head, request): joins the ranges'
+// records. The weights come first, a range a thread; then wave w adds the
+// ranges w, w + 4, ... with four loads in flight, a lane four dims (or two, or
+// one: D / 64).
+constexpr int kMaxSplits = 256;
+
+template <int GROUPS>
+__global__ __launch_bounds__(256) void kv_attention_merge_kernel(const float *__restrict__ part,
+                                                                 const float2 *__restrict__ stats, int splits,
                                                                  const float *__restrict__ gate, int gate_stride,
                                                                  float *__restrict__ out, KvArgs a) {
-    const int r = blockIdx.x, h = blockIdx.y, j = blockIdx.z, D = a.head_dim, d = threadIdx.x;
-    if (d >= D) return;
-    const float *rec = part + (((int64_t)j * a.rows + r) * a.heads + h) * splits * (int64_t)(D + 2);
-    float m = -INFINITY;
-    for (int s = 0; s < splits; s++) m = fmaxf(m, rec[(int64_t)s * (D + 2) + D]);
-    float l = 0.0f, o = 0.0f;
-    for (int s = 0; s < splits; s++) {
-        const float *p = rec + (int64_t)s * (D + 2);
-        if (p[D + 1] == 0.0f) continue;  // a range without keys
-        const float w = p[D] == m ? 1.0f : __builtin_amdgcn_exp2f(p[D] - m);
-        l = fmaf(w, p[D + 1], l);
-        o = fmaf(w, p[d], o);
+    constexpr int D = 64 * GROUPS;
+    __shared__ float weight[kMaxSplits], red[2][4];
+    __shared__ float sum[4][D];
+    const int r = blockIdx.x, h = blockIdx.y, j = blockIdx.z, tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+    const int64_t rec = (((int64_t)j * a.rows + r) * a.heads + h) * splits;
+    const int64_t row = ((int64_t)j * a.rq_rows + r) * a.heads + h;
+    const float2 ml = tid < splits ? stats[rec + tid] : make_float2(-INFINITY, 0.0f);
+    float g = 0.0f;
+    if (gate && tid < D) g = gate[row * gate_stride + tid];
+    float m = ml.x;
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off));
+    if (lane == 0) red[0][wave] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+    // a range without keys (no sum) weighs nothing, whatever its output holds
+    const float w = ml.y == 0.0f ? 0.0f : ml.x == m ? 1.0f : __builtin_amdgcn_exp2f(ml.x - m);
+    weight[tid] = ml.y == 0.0f ? -1.0f : w;
+    float l = w * ml.y;
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) l += __shfl_xor(l, off);
+    if (lane == 0) red[1][wave] = l;
+    __syncthreads();
+    l = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
+    float o[GROUPS] = {};
+    for (int s0 = wave; s0 < splits; s0 += 16) {
+        float x[4][GROUPS], f[4];
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const int s = s0 + 4 * u;
+            f[u] = s < splits ? weight[s] : -1.0f;
+#pragma unroll
+            for (int i = 0; i < GROUPS; i++) x[u][i] = f[u] >= 0.0f ? part[(rec + s) * D + 64 * i + lane] : 0.0f;
+        }
+#pragma unroll
+        for (int u = 0; u < 4; u++)
+#pragma unroll
+            for (int i = 0; i < GROUPS; i++)
+                if (f[u] >= 0.0f) o[i] = fmaf(f[u], x[u][i], o[i]);
     }
-    float y = l == 0.0f ? 0.0f : o / l;  // a row that sees no key
-    const int64_t row = (int64_t)j * a.rq_rows + r;
-    if (gate) y *= sigmoid_ref(gate[(row * a.heads + h) * gate_stride + d]);
-    out[(row * a.heads + h) * D + d] = y;
+#pragma unroll
+    for (int i = 0; i < GROUPS; i++) sum[wave][64 * i + lane] = o[i];
+    __syncthreads();
+    if (tid < D) {
+        float y = (sum[0][tid] + sum[1][tid]) + (sum[2][tid] + sum[3][tid]);
+        y = l == 0.0f ? 0.0f : y / l;  // a row that sees no key
+        if (gate) y *= sigmoid_ref(g);
+        out[row * D + tid] = y;
+    }
 }
 
 bool stacked(const KvArgs &a) { return a.heads / a.kv_heads * a.rows <= 8; }
@@ -634,15 +678,17 @@ int row_blocks(const KvArgs &a) {
 
 int kv_splits(const KvArgs &a) {
     const int64_t work = (int64_t)a.kv_heads * a.requests * row_blocks(a);
-    const int64_t want = (256 + work - 1) / work, most = (a.capacity + kWaves * kTile - 1) / (kWaves * kTile);
+    const int64_t want = (kMaxSplits + work - 1) / work, most = (a.capacity + kWaves * kTile - 1) / (kWaves * kTile);
     return (int)std::max<int64_t>(1, std::min(want, most));
 }
+
+uint64_t kv_records(const KvArgs &a) { return (uint64_t)a.requests * a.rows * a.heads * kv_splits(a); }
 
 }  // namespace
 
 uint64_t kv_attention_scratch_bytes(const KvArgs &a) {
     const int splits = kv_splits(a);
-    return splits == 1 ? 0 : (uint64_t)a.requests * a.rows * a.heads * splits * (a.head_dim + 2) * 4;
+    return splits == 1 ? 0 : kv_records(a) * (a.head_dim + 2) * 4;  // outputs, then {m, l}
 }
 
 hipError_t launch_kv_attention(const float *q, int q_stride, const float *gate, int gate_stride, const void *kpool,
@@ -652,6 +698,7 @@ hipError_t launch_kv_attention(const float *q, int q_stride, const float *gate, 
     while ((16 << sp.page_shift) < a.block_size) sp.page_shift++;
     const bool paged = (16 << sp.page_shift) == a.block_size;
     float *part = static_cast<float *>(scratch);
+    float2 *stats = part ? reinterpret_cast<float2 *>(part + kv_records(a) * a.head_dim) : nullptr;
     hipError_t err = hipSuccess;
     auto launch = [&](auto fmt, auto groups, auto stack, auto pages) {
         constexpr auto kernel = kv_attention_kernel<fmt(), groups(), stack(), pages()>;
@@ -663,7 +710,7 @@ hipError_t launch_kv_attention(const float *q, int q_stride, const float *gate, 
         });
         kernel<<<dim3((uint32_t)((int64_t)sp.splits * sp.row_blocks * a.kv_heads), a.requests), 64 * kWaves, bytes, s>>>(
             q, q_stride, gate, gate_stride, static_cast<const uint8_t *>(kpool), static_cast<const uint8_t *>(vpool), table,
-            a, sp, part, out, dyn);
+            a, sp, part, stats, out, dyn);
         err = hipGetLastError();
     };
     auto by_pages = [&](auto fmt, auto groups) {
@@ -682,7 +729,11 @@ hipError_t launch_kv_attention(const float *q, int q_stride, const float *gate, 
     if (a.fmt == kKvF16) by_width(std::integral_constant<int, kKvF16>{});
     else by_width(std::integral_constant<int, kKvQ8>{});
     if (err != hipSuccess || sp.splits == 1) return err;
-    kv_attention_merge_kernel<<<dim3(a.rows, a.heads, a.requests), 256, 0, s>>>(part, sp.splits, gate, gate_stride, out, a);
+    auto merge = a.head_dim == 64    ? kv_attention_merge_kernel<1>
+                 : a.head_dim == 128 ? kv_attention_merge_kernel<2>
+                 : a.head_dim == 192 ? kv_attention_merge_kernel<3>
+                                     : kv_attention_merge_kernel<4>;
+    merge<<<dim3(a.rows, a.heads, a.requests), 256, 0, s>>>(part, stats, sp.splits, gate, gate_stride, out, a);
     return hipGetLastError();
 }
 
