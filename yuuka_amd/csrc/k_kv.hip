@@ -44,9 +44,13 @@ yuuka_status kv_check(KvArgs *a, uint32_t dtype, bool attention) {
         return fail(YUUKA_ERR_INVALID_ARGUMENT, "KV cache rotation of %d dimensions", a->rope_dim);
     if ((int64_t)a->rows * (2 * a->kv_heads + a->heads) > (1 << 25))  // vectors of one launch
         return fail(YUUKA_ERR_INVALID_ARGUMENT, "KV cache: %d rows of %d heads in one call", a->rows, a->kv_heads);
-    if (attention && (a->heads < 1 || a->heads % a->kv_heads || a->heads > 65535 || a->rows > 4096))
+    if (attention && (a->heads < 1 || a->heads % a->kv_heads || a->heads > 65535 ||
+                      a->heads / a->kv_heads > 256 || a->rows > 4096))
         return fail(YUUKA_ERR_INVALID_ARGUMENT, "decode attention of %d rows, %d heads over %d KV heads", a->rows,
                     a->heads, a->kv_heads);
+    if (attention && (int64_t)a->requests * a->kv_heads * ((a->heads / a->kv_heads * (int64_t)a->rows + 7) / 8) > (1 << 23))
+        return fail(YUUKA_ERR_INVALID_ARGUMENT, "decode attention: %d requests of %d rows, %d heads in one call",
+                    a->requests, a->rows, a->heads);  // (workgroups of one launch)
     if (attention && kv_page_bytes(*a) > 0x7fffffff)
         return fail(YUUKA_ERR_UNSUPPORTED, "decode attention over pages of %lld bytes (below 2 GiB are served)",
                     (long long)kv_page_bytes(*a));

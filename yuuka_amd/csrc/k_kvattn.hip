@@ -5,10 +5,12 @@
 //   out = sum_t softmax_t(scale q . k_t) v_t,  t = 0 .. position of the row
 //
 // A workgroup takes one kv head of one request, up to 16 of its (row, query
-// head) pairs and a range of the keys; its eight waves walk the range's
+// head) pairs and a part of the keys; its four waves walk the part's
 // 32-key tiles, each with a running reference, sum and output of its own, and
-// are joined at the end. With more ranges than one the records {o, m, l} of
-// the ranges are joined by a second kernel.
+// are joined at the end. With more parts than one the records {o, m, l} of
+// the parts are joined by a second kernel. Keys and values of a wave's next tile
+// are on their way while it works on one: a register is loaded again as soon as
+// it has been used.
 //
 // Both products run on v_mfma_f32_16x16x32_f16 straight from the pages:
 //  * scores = K Q^T (keys are the rows of the tile, so that a lane ends with
@@ -50,7 +52,7 @@ template <> struct Dwords<1> { typedef uint32_t V; };
 template <int N> __device__ __forceinline__ uint32_t dword(const typename Dwords<N>::V &v, int i) { return v[i]; }
 template <> __device__ __forceinline__ uint32_t dword<1>(const uint32_t &v, int) { return v; }
 
-constexpr int kWaves = 8, kTile = 32;
+constexpr int kWaves = 4, kTile = 32;
 constexpr float kHeadroom = 10.0f, kSlack = 4.0f;
 
 __device__ __forceinline__ float max_rows(float x) {  // over the four 16-lane rows
@@ -67,6 +69,24 @@ __device__ __forceinline__ float sum_rows(float x) {
     x = sum_halves(x);
     auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     return __uint_as_float(a[0]) + __uint_as_float(a[1]);
+}
+template <int CTRL>
+__device__ __forceinline__ float dpp(float x) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float max_wave(float x) {  // non-negative or not, no NaN kept
+    x = fmaxf(x, dpp<0xb1>(x));   // lanes l ^ 1, l ^ 2, then rotated by 4 and 8
+    x = fmaxf(x, dpp<0x4e>(x));
+    x = fmaxf(x, dpp<0x124>(x));
+    x = fmaxf(x, dpp<0x128>(x));
+    return max_rows(x);
+}
+__device__ __forceinline__ float sum_wave(float x) {
+    x += dpp<0xb1>(x);
+    x += dpp<0x4e>(x);
+    x += dpp<0x124>(x);
+    x += dpp<0x128>(x);
+    return sum_rows(x);
 }
 __device__ __forceinline__ float ror8(float x) {  // lane (l + 8) % 16 of the row
     return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x128, 0xf, 0xf, true));
@@ -114,20 +134,139 @@ template <int FMT, int GROUPS, bool STACK, bool PAGED> struct Layout {
     static constexpr uint32_t total = stats + (2 * kWaves + 1) * 16 * 4;
 };
 
+// How the work is cut. A "column" is one (row block, kv head) of a request; a
+// request's keys are cut into parts of at most `chunk` tiles, the same for all
+// requests. W = all columns' tiles over `target`, the workgroups that the GPU
+// holds at once. The smallest chunk of W .. 1.5 W (in four steps) whose parts are
+// one round is taken; where there is none (more columns than workgroups, or
+// very different lengths), W / 2, so that the last workgroups are short ones. The
+// lengths are on the device: every wave works the cut out for itself, a
+// request a lane.
 struct AttnSplit {
-    int splits, row_blocks;
-    int page_shift;  // PAGED: log2(block_size / 16)
+    int row_blocks, columns;  // columns = row_blocks * kv_heads
+    int group;                // query heads of a kv head
+    uint32_t group_inverse;   // ceil(2^32 / group): n / group = high word of the product, n < 2^24 (group 1: 0)
+    int target;
+    float share;              // columns / target
+    int whole;                // 1: every request is one part (twice as many columns as workgroups)
+    int page_shift;           // PAGED: log2(block_size / 16)
+};
+constexpr int kMaxParts = 256;
+
+__device__ __forceinline__ int wave_sum(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0xb1, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x4e, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x124, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x128, 0xf, 0xf, true);
+    return __builtin_amdgcn_readlane(x, 0) + __builtin_amdgcn_readlane(x, 16) + __builtin_amdgcn_readlane(x, 32) +
+           __builtin_amdgcn_readlane(x, 48);
+}
+__device__ __forceinline__ int wave_max(int x) {
+    x = max(x, __builtin_amdgcn_update_dpp(0, x, 0xb1, 0xf, 0xf, true));
+    x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x4e, 0xf, 0xf, true));
+    x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x124, 0xf, 0xf, true));
+    x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x128, 0xf, 0xf, true));
+    return max(max(__builtin_amdgcn_readlane(x, 0), __builtin_amdgcn_readlane(x, 16)),
+               max(__builtin_amdgcn_readlane(x, 32), __builtin_amdgcn_readlane(x, 48)));
+}
+
+// Sums of the lanes up to and with each.
+__device__ __forceinline__ int wave_scan(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr 1, 2, 4, 8
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast 15 into rows 1 and 3
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast 31 into rows 2 and 3
+    return x;
+}
+
+struct Cut {
+    int chunk, total;   // tiles of a part at most; parts of all requests
+    int first;          // the lane's tiles of requests 0 .. 63
+    int64_t position;   // and position of its first row
+};
+// (requests that are cut are at most 2^11)
+__device__ __forceinline__ int cut_tiles(const KvArgs &a, int64_t position) {
+    const int len = (int)max((int64_t)1, min(position + a.rows, (int64_t)a.capacity));
+    return min((len - 1) / kTile + 1, 1 << 19);
+}
+__device__ __forceinline__ int cut_tiles(const KvArgs &a, const ModelDyn &dyn, int base) {
+    const int j = base + (threadIdx.x & 63);
+    return j < a.requests ? cut_tiles(a, kv_position(a, dyn, j, 0)) : 0;
+}
+__device__ __forceinline__ int cut_parts(int tiles, int chunk) {
+    return tiles ? (uint32_t)(tiles - 1) / (uint32_t)chunk + 1 : 0;
+}
+
+__device__ __forceinline__ Cut cut_work(const KvArgs &a, const ModelDyn &dyn, const AttnSplit &sp) {
+    Cut cut{0, a.requests, 0, 0};
+    if (sp.whole) return cut;
+    {
+        const int lane = threadIdx.x & 63;
+        cut.position = kv_position(a, dyn, min(lane, a.requests - 1), 0);
+        cut.first = lane < a.requests ? cut_tiles(a, cut.position) : 0;
+    }
+    int sum = cut.first, top = cut.first;
+    for (int base = 64; base < a.requests; base += 64) {
+        const int t = cut_tiles(a, dyn, base);
+        sum += t;
+        top = max(top, t);
+    }
+    if (a.requests > 1) {
+        sum = wave_sum(sum);
+        top = wave_max(top);
+    }
+    sum = __builtin_amdgcn_readfirstlane(sum);
+    top = __builtin_amdgcn_readfirstlane(top);
+    const int least = max(kWaves, (top + kMaxParts - 1) / kMaxParts);
+    const int even = (int)ceilf((float)sum * sp.share);  // W: below 2^21, for at most 2 target columns are cut
+    for (int turn = 0; turn < 5; turn++) {
+        cut.chunk = max(least, turn < 4 ? (even * (8 + turn + (turn == 3)) + 7) / 8 : (even + 1) / 2);
+        int n = cut_parts(cut.first, cut.chunk);
+        for (int base = 64; base < a.requests; base += 64) n += cut_parts(cut_tiles(a, dyn, base), cut.chunk);
+        cut.total = a.requests > 1 ? wave_sum(n) : __builtin_amdgcn_readfirstlane(n);
+        if (cut.total * sp.columns <= sp.target) break;
+    }
+    return cut;
+}
+
+struct Part {
+    int j, index, parts;  // request, part of it, its number of parts
+    int record;           // parts before it of the requests with several
 };
 
-// 512 threads. PAGED: pages are 16 << page_shift tokens, so that a 16-key half
+// Part number `item` of all.
+__device__ __forceinline__ Part find_part(const KvArgs &a, const ModelDyn &dyn, const AttnSplit &sp, const Cut &cut,
+                                          int item) {
+    if (sp.whole) return {item, 0, 1, 0};
+    if (a.requests == 1) return {0, item, cut.total, 0};
+    int before = 0, records_before = 0;
+    for (int base = 0;; base += 64) {
+        const int n = cut_parts(base ? cut_tiles(a, dyn, base) : cut.first, cut.chunk);
+        // parts, and parts of requests with several, summed as one (64 * 256 of each at most)
+        const int own = n | (n > 1 ? n << 16 : 0), upto = wave_scan(own);
+        const int here = __builtin_amdgcn_readlane(upto, 63);
+        if (item < before + (here & 0xffff)) {
+            const int at = __ffsll((unsigned long long)__builtin_amdgcn_ballot_w64(before + (upto & 0xffff) > item)) - 1;
+            const int past = __builtin_amdgcn_readlane(upto - own, at);
+            return {base + at, item - before - (past & 0xffff), __builtin_amdgcn_readlane(n, at), records_before + (past >> 16)};
+        }
+        before += here & 0xffff;
+        records_before += here >> 16;
+    }
+}
+
+// PAGED: pages are 16 << page_shift tokens, so that a 16-key half
 // of a tile lies in one page, found by scalar loads and read through a
 // buffer resource of that page's bytes (none for an unmapped page or past the end:
 // such loads cost nothing and give zeros).
 template <int FMT, int GROUPS, bool STACK, bool PAGED>
-__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 2))) void kv_attention_kernel(
+__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(GROUPS == 1 ? 4 : GROUPS == 2 ? 3 : 2))) void kv_attention_kernel(
     const float *__restrict__ q, int q_stride, const float *__restrict__ gate, int gate_stride,
     const uint8_t *__restrict__ kpool, const uint8_t *__restrict__ vpool, const int32_t *__restrict__ table, KvArgs a,
-    AttnSplit sp, float *__restrict__ part, float2 *__restrict__ stats, float *__restrict__ out, ModelDyn dyn) {
+    AttnSplit sp, float *__restrict__ part, float2 *__restrict__ stats, int2 *__restrict__ plan, float *__restrict__ out,
+    ModelDyn dyn) {
     using L = Layout<FMT, GROUPS, STACK, PAGED>;
     constexpr bool Q8 = L::Q8;
     constexpr int D = L::D, NB = L::NB, ROWS = L::ROWS;
@@ -137,26 +276,49 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
     float *const row_factor = st_l + kWaves * 16;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int r16 = lane & 15, g4 = lane >> 4;
-    int bx = blockIdx.x;
-    const int rb = bx % sp.row_blocks;
-    bx /= sp.row_blocks;
-    const int split = bx % sp.splits, kvh = bx / sp.splits, j = blockIdx.y;
-    const int G = a.heads / a.kv_heads;
+    // Workgroups go to the eight XCDs in turn. Each XCD gets one run of the work
+    // items in the order (row block, kv head, part, request), so that what
+    // reads one run of tokens, all heads' scales in one line, shares an L2.
+    const Cut cut = cut_work(a, dyn, sp);
+    int item = blockIdx.x;
+    {
+        const int n = __builtin_amdgcn_readfirstlane(cut.total) * sp.columns, x = item & 7;
+        if (item >= n) return;
+        item = x * (n >> 3) + min(x, n & 7) + (item >> 3);
+    }
+    const int turn_of = (uint32_t)item / (uint32_t)sp.columns, column = item - turn_of * sp.columns;
+    const int kvh = sp.row_blocks == 1 ? column : (uint32_t)column / (uint32_t)sp.row_blocks;
+    const int rb = column - kvh * sp.row_blocks;
+    const Part pt = find_part(a, dyn, sp, cut, turn_of);
+    const int j = __builtin_amdgcn_readfirstlane(pt.j), split = __builtin_amdgcn_readfirstlane(pt.index);
+    const int parts = __builtin_amdgcn_readfirstlane(pt.parts);
+    const int G = sp.group;
+    auto row_of = [&](int n) { return sp.group_inverse ? (int)__umulhi((uint32_t)n, sp.group_inverse) : n; };
     const int n0 = rb * ROWS, nr = min(ROWS, G * a.rows - n0);  // pairs n = row * G + head of the group
-    const int64_t p0 = kv_position(a, dyn, j, 0);
+    int64_t p0;
+    if (sp.whole || j >= 64) p0 = kv_position(a, dyn, j, 0);
+    else p0 = (int64_t)__builtin_amdgcn_readlane((int)(cut.position >> 32), j) << 32 |
+              (uint32_t)__builtin_amdgcn_readlane((int)cut.position, j);
     // last key a row sees, -1 for none
-    auto limit = [&](int n) { return (int)max((int64_t)-1, min(p0 + n / G, (int64_t)a.capacity - 1)); };
+    auto limit = [&](int n) { return (int)max((int64_t)-1, min(p0 + row_of(n), (int64_t)a.capacity - 1)); };
     const int len = __builtin_amdgcn_readfirstlane(limit(n0 + nr - 1) + 1);
     const int least = __builtin_amdgcn_readfirstlane(limit(n0));
+    // (the parts are of the last row block's tiles; an earlier one may need fewer)
     const int tiles = (len + kTile - 1) / kTile;
-    const int per = max((tiles + sp.splits - 1) / sp.splits, kWaves);
-    const int c0 = split * per, c1 = min(tiles, c0 + per);
+    int c0 = 0, c1 = tiles;
+    if (parts > 1) {
+        const int last = (int)max((int64_t)1, min(p0 + a.rows, (int64_t)a.capacity));
+        const uint32_t all = (uint32_t)((last - 1) / kTile + 1), each = all / (uint32_t)parts, more = all - each * parts;
+        c0 = split * each + min(split, (int)more);
+        c1 = min(tiles, c0 + (int)each + (split < (int)more));
+    }
+    c0 = __builtin_amdgcn_readfirstlane(c0);
+    c1 = __builtin_amdgcn_readfirstlane(c1);
+    const int64_t record = ((int64_t)(__builtin_amdgcn_readfirstlane(pt.record) + split) * sp.columns + column) * ROWS;
     const int64_t out_row = (int64_t)j * a.rq_rows;
-    if (c0 >= c1 && sp.splits > 1) {  // nothing here: an empty record
-        if (threadIdx.x < (uint32_t)nr) {
-            const int n = n0 + threadIdx.x, r = n / G, h = kvh * G + n % G;
-            stats[(((int64_t)j * a.rows + r) * a.heads + h) * sp.splits + split] = make_float2(-INFINITY, 0.0f);
-        }
+    if (plan && split == 0 && column == 0 && threadIdx.x == 0) plan[j] = make_int2(parts, pt.record);
+    if (c0 >= c1 && parts > 1) {  // nothing here: empty records
+        if (threadIdx.x < (uint32_t)nr) stats[record + threadIdx.x] = make_float2(-INFINITY, 0.0f);
         return;
     }
 
@@ -165,7 +327,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
     float queries[ROWS / kWaves][GROUPS];
 #pragma unroll
     for (int half = 0; half < ROWS / kWaves; half++) {
-        const int n = min(wave + kWaves * half, nr - 1), r = (n0 + n) / G, h = kvh * G + (n0 + n) % G;
+        const int n = min(wave + kWaves * half, nr - 1), r = row_of(n0 + n), h = kvh * G + n0 + n - r * G;
 #pragma unroll
         for (int s = 0; s < GROUPS; s++) {
             const float x = q[((out_row + r) * a.heads + h) * q_stride + 64 * s + lane];
@@ -189,14 +351,25 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
         const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)(x >> 32));
         return (uint64_t)hi << 32 | lo;
     };
-    auto pages_of = [&](int c) {
+    // The pages of the wave's next 32 tiles, two a tile, a half a lane: one load in
+    // 32 turns. (A scalar load a turn stalls it: any wait for LDS is one for that load too.)
+    int page_queue = -1;
+    auto pages_of = [&](int turn) {
         Tile t{};
         if constexpr (PAGED) {
+            if ((turn & 31) == 0) {
+                int at = lane;  // opaque: nothing of this is kept in registers over the loop
+                asm volatile("" : "+v"(at));
+                const int mine = c0 + wave + kWaves * (turn + (at >> 1)), tok = kTile * mine + 16 * (at & 1);
+                const bool in = mine < c1 && tok < len;
+                const int page = table_j[(uint32_t)(in ? tok >> (4 + sp.page_shift) : 0)];
+                page_queue = in ? page : -1;
+            }
+            const int c = c0 + wave + kWaves * turn;
 #pragma unroll
             for (int T = 0; T < 2; T++) {
                 const int tok = kTile * c + 16 * T;
-                int page = -1;
-                if (c < c1 && tok < len) page = __builtin_amdgcn_readfirstlane(table_j[tok >> (4 + sp.page_shift)]);
+                const int page = __builtin_amdgcn_readlane(page_queue, 2 * (turn & 31) + T);
                 const bool mapped = (uint32_t)page < (uint32_t)a.pages;
                 const uint32_t in = tok & ((16u << sp.page_shift) - 1);  // tokens before the half in its page
                 const uint64_t at = (uint64_t)(mapped ? (uint32_t)page : 0u) * page_bytes;
@@ -227,13 +400,14 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
     uint32_t scale_read = L::scales + wave * 256 * GROUPS + g4 * 16;
     uint32_t query_read = lane * 16;  // of the lane's operands
     int64_t *const my_addr = reinterpret_cast<int64_t *>(lds + L::addr) + wave * 32;
-    const uint32_t soff = (lane & 15) * (a.kv_dim / 16) + kvh * NB * 2;
+    uint32_t soff = (lane & 15) * (a.kv_dim / 16) + kvh * NB * 2;
     auto load_scales = [&](const Tile &t) {  // (an unmapped half reads page 0's: not used)
         if constexpr (Q8 && PAGED) {
-            const uint8_t *k0 = kpool + t.scales[0], *k1 = kpool + t.scales[1];
-            const uint8_t *v0 = vpool + t.scales[0], *v1 = vpool + t.scales[1];
-            const uint8_t *at = (lane < 32 ? (lane & 16 ? k1 : k0) : (lane & 16 ? v1 : v0)) + soff;
-            sreg = *reinterpret_cast<const typename Dwords<GROUPS>::V *>(at);
+            uint64_t k0 = (uint64_t)kpool + t.scales[0], k1 = (uint64_t)kpool + t.scales[1];
+            uint64_t v0 = (uint64_t)vpool + t.scales[0], v1 = (uint64_t)vpool + t.scales[1];
+            asm volatile("" : "+s"(k0), "+s"(k1), "+s"(v0), "+s"(v1));  // (no lane's pool kept in registers)
+            const uint64_t at = (lane < 32 ? (lane & 16 ? k1 : k0) : (lane & 16 ? v1 : v0)) + soff;
+            sreg = *reinterpret_cast<const __attribute__((address_space(1))) typename Dwords<GROUPS>::V *>(at);
         }
     };
     // !PAGED: every lane finds the row (and the scales) of key `lane & 31`
@@ -273,21 +447,40 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
         else
             vhalf[i][s] = *reinterpret_cast<const typename Dwords<2>::V *>(vrow[i] + 128 * s);
     };
+    // 64-byte pieces p - 1 and p of the keys (the last may be alone), and 64-dim groups of
+    // the values: what shares a line is asked for together.
+    auto load_keys = [&](__amdgpu_buffer_rsrc_t rs, int T, int p) {
+        if (p & 1) load_key(rs, T, p - 1);
+        load_key(rs, T, p);
+    };
+    auto load_values = [&](__amdgpu_buffer_rsrc_t v0, __amdgpu_buffer_rsrc_t v1, int u) {
+        if (Q8 && !(u & 1) && u < GROUPS - 1) return;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            if (Q8 && (u & 1)) load_value(i < 4 ? v0 : v1, i, u - 1);
+            load_value(i < 4 ? v0 : v1, i, u);
+        }
+    };
     int c = c0 + wave;
-    Tile cur = PAGED ? pages_of(c) : find_rows(c);
+    Tile cur = PAGED ? pages_of(0) : find_rows(c);
+    // (in the loop's order: its waits count the loads issued since, on either way into it)
     load_scales(cur);
+    __builtin_amdgcn_sched_barrier(0);
     {
         const auto k0 = resource(kpool, cur, 0), k1 = resource(kpool, cur, 1);
         const auto v0 = resource(vpool, cur, 0), v1 = resource(vpool, cur, 1);
 #pragma unroll
-        for (int p = 0; p < KP; p++) {
-            load_key(k0, 0, p);
-            load_key(k1, 1, p);
+        for (int p = 0; p < KP; p++)
+            if ((p & 1) || p == KP - 1) {
+                load_keys(k0, 0, p);
+                load_keys(k1, 1, p);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+#pragma unroll
+        for (int u = 0; u < GROUPS; u++) {
+            load_values(v0, v1, u);
+            __builtin_amdgcn_sched_barrier(0);
         }
-#pragma unroll
-        for (int s = 0; s < GROUPS; s++)
-#pragma unroll
-            for (int i = 0; i < 8; i++) load_value(i < 4 ? v0 : v1, i, s);
     }
 
     // ---- queries as MFMA operands in LDS: wave w prepares rows w and w + 8
@@ -298,8 +491,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
         float top = 0.0f;
 #pragma unroll
         for (int s = 0; s < GROUPS; s++) top = fmaxf(top, fabsf(x[s]));
-#pragma unroll
-        for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
+        top = max_wave(top);
         int e = 14;
         if (top > 0.0f && top < INFINITY) (void)frexpf(top, &e);  // top < 2^e
         const int in = Q8 ? lane : 0;
@@ -334,13 +526,13 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
     float ref = -INFINITY, l = 0.0f;
 
     Tile next{};
-    if constexpr (PAGED) next = pages_of(c + kWaves);
-    for (; c < c1; c += kWaves) {
+    if constexpr (PAGED) next = pages_of(1);
+    for (int turn = 0; c < c1; c += kWaves, turn++) {
         // Opaque in every turn: the constant steps from these addresses then stay
         // in the instructions' immediate offsets. Hoisted out of the loop they take a
         // register each, loaded values spill, and every spill waits for all loads.
         asm volatile("" : "+v"(koff), "+v"(voff_row[0]), "+v"(voff_row[1]), "+v"(voff_row[2]), "+v"(voff_row[3]));
-        asm volatile("" : "+v"(scale_write), "+v"(scale_read), "+v"(query_read));
+        asm volatile("" : "+v"(scale_write), "+v"(scale_read), "+v"(query_read), "+v"(soff));
         // every row sees every key of the tile
         const bool whole = cur.keys == ~0u && kTile * c + kTile - 1 <= least;
         float E = 0.0f;
@@ -348,7 +540,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
         if constexpr (Q8) {
             // scales to LDS (those of missing keys as zeros), and the largest finite value scale's exponent
             wave_lds_fence();
-            const bool there = (cur.keys >> (lane & 31)) & 1;
+            const bool there = __builtin_amdgcn_inverse_ballot_w64((uint64_t)cur.keys << 32 | cur.keys);
             uint32_t d[GROUPS], most = 0, over = 0;
 #pragma unroll
             for (int s = 0; s < GROUPS; s++) {
@@ -358,9 +550,9 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
                 over |= ((d[s] & 0x7fff7fffu) + 0x04000400u) & 0x80008000u;
             }
             if (!whole) {
-                const uint64_t b = __builtin_amdgcn_ballot_w64(over != 0 && kTile * c + (lane & 31) > least);
+                uint64_t b = __builtin_amdgcn_ballot_w64(over != 0 && kTile * c + (lane & 31) > least);
                 poison = (uint32_t)(b >> 32);
-                if (lane >= 32 && (poison >> (lane & 31)) & 1) {
+                if (__builtin_amdgcn_inverse_ballot_w64((uint64_t)poison << 32)) {
 #pragma unroll
                     for (int s = 0; s < GROUPS; s++) d[s] = 0;
                 }
@@ -368,11 +560,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
 #pragma unroll
             for (int s = 0; s < GROUPS; s++) *reinterpret_cast<uint32_t *>(lds + scale_write + 128 * s) = d[s];
             float m = __uint_as_float(lane < 32 ? 0u : most);  // non-negative: ordered as floats
-            m = fmaxf(m, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(m), 0xb1, 0xf, 0xf, true)));
-            m = fmaxf(m, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(m), 0x4e, 0xf, 0xf, true)));
-            m = fmaxf(m, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(m), 0x124, 0xf, 0xf, true)));
-            m = fmaxf(m, ror8(m));
-            m = max_rows(m);
+            m = max_wave(m);
             E = (float)((int)(__float_as_uint(m) >> 10) - 14);  // scale < 2^E
             wave_lds_fence();
         }
@@ -416,15 +604,16 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
                             s[T][e] = d[e];
                     }
                 }
-                if (!Q8 || (b & 1)) {
-                    load_key(k0, 0, Q8 ? b >> 1 : b);
-                    load_key(k1, 1, Q8 ? b >> 1 : b);
+                const int p = Q8 ? b >> 1 : b;  // the piece that this block was in
+                if ((!Q8 || (b & 1)) && ((p & 1) || p == KP - 1)) {
+                    load_keys(k0, 0, p);
+                    load_keys(k1, 1, p);
                     __builtin_amdgcn_sched_barrier(0);
                 }
             }
         }
         load_scales(next);
-        if constexpr (PAGED) after = pages_of(c + 2 * kWaves);
+        if constexpr (PAGED) after = pages_of(turn + 2);
         // ---- softmax of the lane's row over its eight keys
         float top = -INFINITY;
 #pragma unroll
@@ -464,19 +653,22 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
             for (int e = 0; e < 4; e++) top = fmaxf(top, s[T][e]);
         top = max_rows(top) + (E - kHeadroom);
         if (__any(top > ref + kSlack)) {
+            const bool filled = __any(ref != -INFINITY);  // not in the wave's first tile
             const float moved = fmaxf(ref, top);
             const float shrink = moved == ref ? 1.0f : __builtin_amdgcn_exp2f(ref - moved);
             ref = moved;
-            l *= shrink;
-            float row_shrink[4];
+            if (filled) {
+                l *= shrink;
+                float row_shrink[4];
 #pragma unroll
-            for (int e = 0; e < 4; e++) row_shrink[e] = __shfl(shrink, 4 * g4 + e);
+                for (int e = 0; e < 4; e++) row_shrink[e] = __shfl(shrink, 4 * g4 + e);
 #pragma unroll
-            for (int u = 0; u < GROUPS; u++)
+                for (int u = 0; u < GROUPS; u++)
 #pragma unroll
-                for (int t = 0; t < 4; t++)
+                    for (int t = 0; t < 4; t++)
 #pragma unroll
-                    for (int e = 0; e < 4; e++) acc[u][t][e] *= row_shrink[e];
+                        for (int e = 0; e < 4; e++) acc[u][t][e] *= row_shrink[e];
+            }
         }
         float p[8];
         {
@@ -543,8 +735,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
                     if constexpr (!STACK) acc[u][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph, vv, acc[u][t], 0, 0, 0);
                     acc[u][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pl, vv, acc[u][t], 0, 0, 0);
                 }
-#pragma unroll
-                for (int i = 0; i < 8; i++) load_value(i < 4 ? v0 : v1, i, u);
+                load_values(v0, v1, u);
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
@@ -558,16 +749,23 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
     {
         float *const slot = reinterpret_cast<float *>(lds) + wave * ROWS * L::slot_row;
         const float unit = Q8 ? 512.0f : 1.0f;  // the digits were times 2^-9
+        auto dim = [&](int u, int t) { return 64 * u + (Q8 ? 16 * t + r16 : 4 * r16 + t); };
 #pragma unroll
         for (int u = 0; u < GROUPS; u++)
 #pragma unroll
-            for (int t = 0; t < 4; t++)
+            for (int t = 0; t < 4; t += STACK ? 2 : 1)
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    float x = acc[u][t][e] * unit;
-                    if constexpr (STACK) x = sum_halves(x);  // rows n and n + 8
-                    if (!STACK || g4 < 2)
-                        slot[(4 * g4 + e) * L::slot_row + 64 * u + (Q8 ? 16 * t + r16 : 4 * r16 + t)] = x;
+                    if constexpr (STACK) {
+                        // rows n and n + 8, 32 lanes apart: one swap puts t's two halves and t + 1's
+                        // side by side, their sums in the lower and the upper lanes
+                        const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(acc[u][t][e]),
+                                                                        __float_as_uint(acc[u][t + 1][e]), false, false);
+                        slot[(4 * (g4 & 1) + e) * L::slot_row + dim(u, t) + (Q8 ? 16 : 1) * (g4 >> 1)] =
+                            (__uint_as_float(x[0]) + __uint_as_float(x[1])) * unit;
+                    } else {
+                        slot[(4 * g4 + e) * L::slot_row + dim(u, t)] = acc[u][t][e] * unit;
+                    }
                 }
         if (lane < ROWS) {
             st_m[wave * 16 + lane] = ref;
@@ -590,8 +788,8 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
             o += f * x;
             total = fmaf(f, st_l[w * 16 + n], total);
         }
-        const int r = (n0 + n) / G, h = kvh * G + (n0 + n) % G;
-        if (sp.splits == 1) {
+        const int r = row_of(n0 + n), h = kvh * G + n0 + n - r * G;
+        if (parts == 1) {
             const int64_t at = (out_row + r) * a.heads + h;
             const float inv = 1.0f / total;
 #pragma unroll
@@ -601,104 +799,138 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
                 out[at * D + d + i] = y;
             }
         } else {
-            const int64_t rec = (((int64_t)j * a.rows + r) * a.heads + h) * sp.splits + split;
-            *reinterpret_cast<f32x4 *>(part + rec * D + d) = o;
-            if (d == 0) stats[rec] = make_float2(m, total);
+            *reinterpret_cast<f32x4 *>(part + (record + n) * D + d) = o;
+            if (d == 0) stats[record + n] = make_float2(m, total);
         }
     }
 }
 
-// One workgroup of four waves per (row, head, request): joins the ranges'
-// records. The weights come first, a range a thread; then wave w adds the
-// ranges w, w + 4, ... with four loads in flight, a lane four dims (or two, or
-// one: D / 64).
-constexpr int kMaxSplits = 256;
-
-template <int GROUPS>
+// One workgroup per (row, head, request) and `dims` dims: joins the parts' records. A
+// thread has four dims of every (1024 / dims)-th record, kDeep of them loaded while
+// the weights are worked out, a part a thread.
+template <int kDeep>
 __global__ __launch_bounds__(256) void kv_attention_merge_kernel(const float *__restrict__ part,
-                                                                 const float2 *__restrict__ stats, int splits,
+                                                                 const float2 *__restrict__ stats,
+                                                                 const int2 *__restrict__ plan,
                                                                  const float *__restrict__ gate, int gate_stride,
-                                                                 float *__restrict__ out, KvArgs a) {
-    constexpr int D = 64 * GROUPS;
-    __shared__ float weight[kMaxSplits], red[2][4];
-    __shared__ float sum[4][D];
-    const int r = blockIdx.x, h = blockIdx.y, j = blockIdx.z, tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-    const int64_t rec = (((int64_t)j * a.rows + r) * a.heads + h) * splits;
+                                                                 float *__restrict__ out, KvArgs a, int row_blocks,
+                                                                 int pairs_per_block, int dims) {
+    static_assert(kMaxParts <= 256, "a part a thread");
+    __shared__ float weight[256], red[2][4];
+    __shared__ f32x4 sum[256];
+    const int h = blockIdx.y, j = blockIdx.z, tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+    const int slices = a.head_dim / dims, r = blockIdx.x / slices, d0 = dims * (blockIdx.x % slices);
+    const int2 mine = plan[j];
+    const int parts = mine.x;
+    if (parts == 1) return;  // written by its workgroup
+    const int G = a.heads / a.kv_heads, kvh = h / G, pair = r * G + h - kvh * G, columns = row_blocks * a.kv_heads;
+    const int column = kvh * row_blocks + pair / pairs_per_block;
+    // record of part s: first + s * step
+    const int64_t first = ((int64_t)mine.y * columns + column) * pairs_per_block + pair % pairs_per_block;
+    const int64_t step = (int64_t)columns * pairs_per_block;
     const int64_t row = ((int64_t)j * a.rq_rows + r) * a.heads + h;
-    const float2 ml = tid < splits ? stats[rec + tid] : make_float2(-INFINITY, 0.0f);
-    float g = 0.0f;
-    if (gate && tid < D) g = gate[row * gate_stride + tid];
-    float m = ml.x;
+    const float2 ml = tid < parts ? stats[first + tid * step] : make_float2(-INFINITY, 0.0f);
+    const int quads = dims / 4, wide = 256 / quads, rec = tid / quads, d = d0 + 4 * (tid % quads);
+    const f32x4 none = {0.f, 0.f, 0.f, 0.f};
+    f32x4 x[kDeep], o = none;
+    auto load = [&](int s0) {
 #pragma unroll
-    for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off));
+        for (int u = 0; u < kDeep; u++) {
+            const int s = s0 + wide * u;
+            const bool in = rec < wide && s < parts;
+            x[u] = in ? *reinterpret_cast<const f32x4 *>(part + (first + s * step) * a.head_dim + d) : none;
+        }
+    };
+    load(rec);
+    float g = 0.0f;
+    if (gate && tid < dims) g = gate[row * gate_stride + d0 + tid];
+    float m = ml.x;
+    m = max_wave(m);
     if (lane == 0) red[0][wave] = m;
     __syncthreads();
     m = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
-    // a range without keys (no sum) weighs nothing, whatever its output holds
+    // a part without keys (no sum) weighs nothing, whatever its output holds
     const float w = ml.y == 0.0f ? 0.0f : ml.x == m ? 1.0f : __builtin_amdgcn_exp2f(ml.x - m);
     weight[tid] = ml.y == 0.0f ? -1.0f : w;
     float l = w * ml.y;
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) l += __shfl_xor(l, off);
+    l = sum_wave(l);
     if (lane == 0) red[1][wave] = l;
     __syncthreads();
     l = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
-    float o[GROUPS] = {};
-    for (int s0 = wave; s0 < splits; s0 += 16) {
-        float x[4][GROUPS], f[4];
+    for (int s0 = rec;;) {
 #pragma unroll
-        for (int u = 0; u < 4; u++) {
-            const int s = s0 + 4 * u;
-            f[u] = s < splits ? weight[s] : -1.0f;
-#pragma unroll
-            for (int i = 0; i < GROUPS; i++) x[u][i] = f[u] >= 0.0f ? part[(rec + s) * D + 64 * i + lane] : 0.0f;
+        for (int u = 0; u < kDeep; u++) {
+            const float f = weight[(s0 + wide * u) & 255];
+            if (s0 + wide * u < parts && f >= 0.0f) o += f * x[u];
         }
-#pragma unroll
-        for (int u = 0; u < 4; u++)
-#pragma unroll
-            for (int i = 0; i < GROUPS; i++)
-                if (f[u] >= 0.0f) o[i] = fmaf(f[u], x[u][i], o[i]);
+        s0 += wide * kDeep;
+        if (s0 - rec >= parts) break;
+        load(s0);
     }
-#pragma unroll
-    for (int i = 0; i < GROUPS; i++) sum[wave][64 * i + lane] = o[i];
+    sum[tid] = o;
     __syncthreads();
-    if (tid < D) {
-        float y = (sum[0][tid] + sum[1][tid]) + (sum[2][tid] + sum[3][tid]);
+    if (tid < dims) {
+        const float *const t = reinterpret_cast<const float *>(sum);
+        float y = 0.0f;
+        for (int i = 0; i < wide; i++) y += t[dims * i + tid];
         y = l == 0.0f ? 0.0f : y / l;  // a row that sees no key
         if (gate) y *= sigmoid_ref(g);
-        out[row * D + tid] = y;
+        out[row * a.head_dim + d0 + tid] = y;
     }
 }
 
-bool stacked(const KvArgs &a) { return a.heads / a.kv_heads * a.rows <= 8; }
+bool paged(const KvArgs &a) { return a.block_size % 16 == 0 && (a.block_size & (a.block_size - 1)) == 0; }
+bool stacked(const KvArgs &a) { return paged(a) && a.heads / a.kv_heads * a.rows <= 8; }
 int row_blocks(const KvArgs &a) {
     const int pairs = a.heads / a.kv_heads * a.rows, per = stacked(a) ? 8 : 16;
     return (pairs + per - 1) / per;
 }
 
-int kv_splits(const KvArgs &a) {
-    const int64_t work = (int64_t)a.kv_heads * a.requests * row_blocks(a);
-    const int64_t want = (kMaxSplits + work - 1) / work, most = (a.capacity + kWaves * kTile - 1) / (kWaves * kTile);
-    return (int)std::max<int64_t>(1, std::min(want, most));
+AttnSplit attn_split(const KvArgs &a) {
+    AttnSplit sp{};
+    sp.row_blocks = row_blocks(a);
+    sp.columns = sp.row_blocks * a.kv_heads;
+    sp.group = a.heads / a.kv_heads;
+    sp.group_inverse = sp.group == 1 ? 0 : (uint32_t)(((1ull << 32) + sp.group - 1) / sp.group);
+    const int held = a.head_dim <= 64 ? 4 : a.head_dim <= 128 ? 3 : 2;  // workgroups of a CU
+    sp.target = 256 * held;
+    sp.share = (float)sp.columns / (float)sp.target;
+    sp.whole = (int64_t)sp.columns * a.requests >= 2 * sp.target;
+    if (paged(a)) while ((16 << sp.page_shift) < a.block_size) sp.page_shift++;
+    return sp;
 }
-
-uint64_t kv_records(const KvArgs &a) { return (uint64_t)a.requests * a.rows * a.heads * kv_splits(a); }
+// Most parts of a request, by its capacity.
+int64_t most_parts(const KvArgs &a) {
+    const int64_t tiles = ((int64_t)a.capacity - 1) / kTile + 1;
+    return std::min<int64_t>(kMaxParts, (tiles - 1) / kWaves + 1);
+}
+// Workgroups, and records of requests in several parts: a part has more than half a
+// chunk of tiles there, and a chunk is 1 / (2 target) of all tiles at the least.
+int64_t most_items(const KvArgs &a, const AttnSplit &sp) {
+    const int64_t columns = (int64_t)sp.columns * a.requests;
+    return sp.whole ? columns : std::min(columns * most_parts(a), columns + 2 * sp.target);
+}
+int64_t most_records(const KvArgs &a, const AttnSplit &sp) {
+    if (sp.whole || most_parts(a) == 1) return 0;
+    const int64_t items = std::min((int64_t)sp.columns * a.requests * most_parts(a), (int64_t)4 * sp.target);
+    return items * (stacked(a) ? 8 : 16);
+}
 
 }  // namespace
 
 uint64_t kv_attention_scratch_bytes(const KvArgs &a) {
-    const int splits = kv_splits(a);
-    return splits == 1 ? 0 : kv_records(a) * (a.head_dim + 2) * 4;  // outputs, then {m, l}
+    const int64_t records = most_records(a, attn_split(a));  // outputs, {m, l}, then {parts, first record} of the requests
+    return records ? (uint64_t)records * (a.head_dim + 2) * 4 + (uint64_t)a.requests * 8 : 0;
 }
 
 hipError_t launch_kv_attention(const float *q, int q_stride, const float *gate, int gate_stride, const void *kpool,
                                const void *vpool, const int32_t *table, float *out, const KvArgs &a, void *scratch,
                                const ModelDyn &dyn, hipStream_t s) {
-    AttnSplit sp{kv_splits(a), row_blocks(a), 0};
-    while ((16 << sp.page_shift) < a.block_size) sp.page_shift++;
-    const bool paged = (16 << sp.page_shift) == a.block_size;
+    const AttnSplit sp = attn_split(a);
+    const int64_t records = most_records(a, sp);
     float *part = static_cast<float *>(scratch);
-    float2 *stats = part ? reinterpret_cast<float2 *>(part + kv_records(a) * a.head_dim) : nullptr;
+    float2 *stats = records ? reinterpret_cast<float2 *>(part + records * a.head_dim) : nullptr;
+    int2 *plan = records ? reinterpret_cast<int2 *>(stats + records) : nullptr;
     hipError_t err = hipSuccess;
     auto launch = [&](auto fmt, auto groups, auto stack, auto pages) {
         constexpr auto kernel = kv_attention_kernel<fmt(), groups(), stack(), pages()>;
@@ -708,13 +940,13 @@ hipError_t launch_kv_attention(const float *q, int q_stride, const float *gate, 
             (void)hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
                                       (int)bytes);
         });
-        kernel<<<dim3((uint32_t)((int64_t)sp.splits * sp.row_blocks * a.kv_heads), a.requests), 64 * kWaves, bytes, s>>>(
+        kernel<<<(uint32_t)most_items(a, sp), 64 * kWaves, bytes, s>>>(
             q, q_stride, gate, gate_stride, static_cast<const uint8_t *>(kpool), static_cast<const uint8_t *>(vpool), table,
-            a, sp, part, stats, out, dyn);
+            a, sp, part, stats, plan, out, dyn);
         err = hipGetLastError();
     };
     auto by_pages = [&](auto fmt, auto groups) {
-        if (!paged) launch(fmt, groups, std::false_type{}, std::false_type{});
+        if (!paged(a)) launch(fmt, groups, std::false_type{}, std::false_type{});
         else if (stacked(a)) launch(fmt, groups, std::true_type{}, std::true_type{});
         else launch(fmt, groups, std::false_type{}, std::true_type{});
     };
@@ -728,12 +960,13 @@ hipError_t launch_kv_attention(const float *q, int q_stride, const float *gate, 
     };
     if (a.fmt == kKvF16) by_width(std::integral_constant<int, kKvF16>{});
     else by_width(std::integral_constant<int, kKvQ8>{});
-    if (err != hipSuccess || sp.splits == 1) return err;
-    auto merge = a.head_dim == 64    ? kv_attention_merge_kernel<1>
-                 : a.head_dim == 128 ? kv_attention_merge_kernel<2>
-                 : a.head_dim == 192 ? kv_attention_merge_kernel<3>
-                                     : kv_attention_merge_kernel<4>;
-    merge<<<dim3(a.rows, a.heads, a.requests), 256, 0, s>>>(part, stats, sp.splits, gate, gate_stride, out, a);
+    if (err != hipSuccess || !records) return err;
+    // A slice of 64 dims a workgroup where that leaves few workgroups (their records are many,
+    // and what counts is the loads in flight), else whole rows.
+    const int dims = (int64_t)a.rows * a.heads * a.requests * (a.head_dim / 64) <= 1024 ? 64 : a.head_dim;
+    auto merge = dims == 64 ? kv_attention_merge_kernel<8> : kv_attention_merge_kernel<4>;
+    merge<<<dim3(a.rows * (a.head_dim / dims), a.heads, a.requests), 256, 0, s>>>(
+        part, stats, plan, gate, gate_stride, out, a, sp.row_blocks, stacked(a) ? 8 : 16, dims);
     return hipGetLastError();
 }
 
