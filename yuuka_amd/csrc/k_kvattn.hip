@@ -54,6 +54,11 @@ template <> __device__ __forceinline__ uint32_t dword<1>(const uint32_t &v, int)
 
 constexpr int kWaves = 4, kTile = 32;
 constexpr float kHeadroom = 10.0f, kSlack = 4.0f;
+// Waves of a SIMD, and workgroups of a CU, by the registers: a tile and accumulators of 64 dims are 32.
+constexpr int waves_held(int groups, int blocks) {
+    const int n = groups == 1 ? 4 : groups == 2 ? 3 : 2;
+    return blocks == 1 ? n : n - 1;
+}
 
 __device__ __forceinline__ float max_rows(float x) {  // over the four 16-lane rows
     auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -121,17 +126,17 @@ __device__ __forceinline__ half2v value_halves(u32x2 x, u32x2 y) {
     return __builtin_bit_cast(half2v, __builtin_amdgcn_perm(y[J >> 1], x[J >> 1], J & 1 ? 0x07060302u : 0x05040100u));
 }
 
-template <int FMT, int GROUPS, bool STACK, bool PAGED> struct Layout {
+template <int FMT, int GROUPS, bool STACK, bool PAGED, int RB> struct Layout {
     static constexpr bool Q8 = FMT == kKvQ8;
-    static constexpr int D = 64 * GROUPS, NB = 2 * GROUPS, ROWS = STACK ? 8 : 16;
+    static constexpr int D = 64 * GROUPS, NB = 2 * GROUPS, PER = STACK ? 8 : 16, ROWS = PER * RB;
     static constexpr uint32_t plane = NB * 1024;                              // query operands, one half
-    static constexpr uint32_t scales = STACK ? plane : 2 * plane;             // [wave][key, value][GROUPS][32] dwords
+    static constexpr uint32_t scales = STACK ? plane : 2 * plane * RB;        // [wave][key, value][GROUPS][32] dwords
     static constexpr uint32_t addr = scales + (Q8 ? kWaves * 256 * GROUPS : 0);  // [wave][32] row offsets
     static constexpr uint32_t loop = addr + (PAGED ? 0 : kWaves * 256);
     static constexpr int slot_row = D + 4;                                    // floats; rows 4 g land 16 banks apart
-    static constexpr uint32_t slots = kWaves * ROWS * slot_row * 4;           // over the loop's areas, after it
-    static constexpr uint32_t stats = loop > slots ? loop : slots;            // m[8][16], l[8][16], factor[16]
-    static constexpr uint32_t total = stats + (2 * kWaves + 1) * 16 * 4;
+    static constexpr uint32_t slots = kWaves * PER * slot_row * 4;            // over the loop's areas, after it
+    static constexpr uint32_t stats = loop > slots ? loop : slots;            // m and l [wave][16], factor[ROWS]
+    static constexpr uint32_t total = stats + (2 * kWaves + RB) * 16 * 4;
 };
 
 // How the work is cut. A "column" is one (row block, kv head) of a request; a
@@ -141,7 +146,7 @@ template <int FMT, int GROUPS, bool STACK, bool PAGED> struct Layout {
 // one round is taken; where there is none (more columns than workgroups, or
 // very different lengths), W / 2, so that the last workgroups are short ones. The
 // lengths are on the device: every wave works the cut out for itself, a
-// request a lane.
+// request a lane (2700 cycles for one request, 3800 for 16).
 struct AttnSplit {
     int row_blocks, columns;  // columns = row_blocks * kv_heads
     int group;                // query heads of a kv head
@@ -181,10 +186,12 @@ __device__ __forceinline__ int wave_scan(int x) {
     return x;
 }
 
+constexpr int kSegments = 4;  // of 64 requests, whose tiles stay in registers
 struct Cut {
-    int chunk, total;   // tiles of a part at most; parts of all requests
-    int first;          // the lane's tiles of requests 0 .. 63
-    int64_t position;   // and position of its first row
+    int chunk, total;       // tiles of a part at most; parts of all requests
+    float inverse;          // (just below) 1 / chunk
+    int tiles[kSegments];   // the lane's requests'
+    int64_t position;       // of the lane's request of the first 64: its first row's
 };
 // (requests that are cut are at most 2^11)
 __device__ __forceinline__ int cut_tiles(const KvArgs &a, int64_t position) {
@@ -195,24 +202,35 @@ __device__ __forceinline__ int cut_tiles(const KvArgs &a, const ModelDyn &dyn, i
     const int j = base + (threadIdx.x & 63);
     return j < a.requests ? cut_tiles(a, kv_position(a, dyn, j, 0)) : 0;
 }
-__device__ __forceinline__ int cut_parts(int tiles, int chunk) {
-    return tiles ? (uint32_t)(tiles - 1) / (uint32_t)chunk + 1 : 0;
+// ceil(tiles / chunk), or now and then one less (chunks of thousands of tiles): never more
+__device__ __forceinline__ int cut_parts(int tiles, float inverse) {
+    return tiles ? (int)(((float)tiles - 0.5f) * inverse) + 1 : 0;
+}
+// f(segment's tiles, its first request) for all of them
+template <typename F>
+__device__ __forceinline__ void each_segment(const KvArgs &a, const ModelDyn &dyn, const Cut &cut, F &&f) {
+    f(cut.tiles[0], 0);
+    if (a.requests <= 64) return;
+#pragma unroll
+    for (int i = 1; i < kSegments; i++) f(cut.tiles[i], 64 * i);
+    for (int base = 64 * kSegments; base < a.requests; base += 64) f(cut_tiles(a, dyn, base), base);
 }
 
 __device__ __forceinline__ Cut cut_work(const KvArgs &a, const ModelDyn &dyn, const AttnSplit &sp) {
-    Cut cut{0, a.requests, 0, 0};
+    Cut cut{0, a.requests, 0.0f, {}, 0};
     if (sp.whole) return cut;
-    {
-        const int lane = threadIdx.x & 63;
-        cut.position = kv_position(a, dyn, min(lane, a.requests - 1), 0);
-        cut.first = lane < a.requests ? cut_tiles(a, cut.position) : 0;
+    const int lane = threadIdx.x & 63;
+    cut.position = kv_position(a, dyn, min(lane, a.requests - 1), 0);
+    cut.tiles[0] = lane < a.requests ? cut_tiles(a, cut.position) : 0;
+    if (a.requests > 64) {
+#pragma unroll
+        for (int i = 1; i < kSegments; i++) cut.tiles[i] = cut_tiles(a, dyn, 64 * i);
     }
-    int sum = cut.first, top = cut.first;
-    for (int base = 64; base < a.requests; base += 64) {
-        const int t = cut_tiles(a, dyn, base);
+    int sum = 0, top = 0;
+    each_segment(a, dyn, cut, [&](int t, int) {
         sum += t;
         top = max(top, t);
-    }
+    });
     if (a.requests > 1) {
         sum = wave_sum(sum);
         top = wave_max(top);
@@ -221,12 +239,23 @@ __device__ __forceinline__ Cut cut_work(const KvArgs &a, const ModelDyn &dyn, co
     top = __builtin_amdgcn_readfirstlane(top);
     const int least = max(kWaves, (top + kMaxParts - 1) / kMaxParts);
     const int even = (int)ceilf((float)sum * sp.share);  // W: below 2^21, for at most 2 target columns are cut
-    for (int turn = 0; turn < 5; turn++) {
-        cut.chunk = max(least, turn < 4 ? (even * (8 + turn + (turn == 3)) + 7) / 8 : (even + 1) / 2);
-        int n = cut_parts(cut.first, cut.chunk);
-        for (int base = 64; base < a.requests; base += 64) n += cut_parts(cut_tiles(a, dyn, base), cut.chunk);
-        cut.total = a.requests > 1 ? wave_sum(n) : __builtin_amdgcn_readfirstlane(n);
-        if (cut.total * sp.columns <= sp.target) break;
+    auto count = [&](Cut &cut) {
+        cut.inverse = __builtin_amdgcn_rcpf((float)cut.chunk) * (1.0f - 0x1p-21f);
+        int n = 0;
+        each_segment(a, dyn, cut, [&](int t, int) { n += cut_parts(t, cut.inverse); });
+        return a.requests > 1 ? wave_sum(n) : __builtin_amdgcn_readfirstlane(n);
+    };
+    for (int turn = 0; turn < 5; turn++) {  // W, then 1.5 W: if that is more than one round, nothing between is less
+        const int eighths = turn == 0 ? 8 : turn == 2 ? 9 : turn == 3 ? 10 : 12;
+        cut.chunk = max(least, (even * eighths + 7) / 8);
+        cut.total = count(cut);
+        const bool fits = cut.total * sp.columns <= sp.target;
+        if (fits && turn != 1) break;
+        if (!fits && turn == 1) {
+            cut.chunk = max(least, (even + 1) / 2);
+            cut.total = count(cut);
+            break;
+        }
     }
     return cut;
 }
@@ -241,35 +270,37 @@ __device__ __forceinline__ Part find_part(const KvArgs &a, const ModelDyn &dyn, 
                                           int item) {
     if (sp.whole) return {item, 0, 1, 0};
     if (a.requests == 1) return {0, item, cut.total, 0};
+    Part part{};
     int before = 0, records_before = 0;
-    for (int base = 0;; base += 64) {
-        const int n = cut_parts(base ? cut_tiles(a, dyn, base) : cut.first, cut.chunk);
+    each_segment(a, dyn, cut, [&](int t, int base) {
+        const int n = cut_parts(t, cut.inverse);
         // parts, and parts of requests with several, summed as one (64 * 256 of each at most)
         const int own = n | (n > 1 ? n << 16 : 0), upto = wave_scan(own);
         const int here = __builtin_amdgcn_readlane(upto, 63);
-        if (item < before + (here & 0xffff)) {
+        if (item >= before && item < before + (here & 0xffff)) {
             const int at = __ffsll((unsigned long long)__builtin_amdgcn_ballot_w64(before + (upto & 0xffff) > item)) - 1;
             const int past = __builtin_amdgcn_readlane(upto - own, at);
-            return {base + at, item - before - (past & 0xffff), __builtin_amdgcn_readlane(n, at), records_before + (past >> 16)};
+            part = {base + at, item - before - (past & 0xffff), __builtin_amdgcn_readlane(n, at), records_before + (past >> 16)};
         }
         before += here & 0xffff;
         records_before += here >> 16;
-    }
+    });
+    return part;
 }
 
 // PAGED: pages are 16 << page_shift tokens, so that a 16-key half
 // of a tile lies in one page, found by scalar loads and read through a
 // buffer resource of that page's bytes (none for an unmapped page or past the end:
 // such loads cost nothing and give zeros).
-template <int FMT, int GROUPS, bool STACK, bool PAGED>
-__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(GROUPS == 1 ? 4 : GROUPS == 2 ? 3 : 2))) void kv_attention_kernel(
+template <int FMT, int GROUPS, bool STACK, bool PAGED, int RB>
+__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(waves_held(GROUPS, RB)))) void kv_attention_kernel(
     const float *__restrict__ q, int q_stride, const float *__restrict__ gate, int gate_stride,
     const uint8_t *__restrict__ kpool, const uint8_t *__restrict__ vpool, const int32_t *__restrict__ table, KvArgs a,
     AttnSplit sp, float *__restrict__ part, float2 *__restrict__ stats, int2 *__restrict__ plan, float *__restrict__ out,
     ModelDyn dyn) {
-    using L = Layout<FMT, GROUPS, STACK, PAGED>;
+    using L = Layout<FMT, GROUPS, STACK, PAGED, RB>;
     constexpr bool Q8 = L::Q8;
-    constexpr int D = L::D, NB = L::NB, ROWS = L::ROWS;
+    constexpr int D = L::D, NB = L::NB, PER = L::PER, ROWS = L::ROWS;
     constexpr int KP = Q8 ? GROUPS : 2 * GROUPS;  // 16-byte pieces of a key per lane
     extern __shared__ __align__(16) uint8_t lds[];
     float *const st_m = reinterpret_cast<float *>(lds + L::stats), *const st_l = st_m + kWaves * 16;
@@ -503,7 +534,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(GRO
         for (int s = 0; s < GROUPS; s++) {
             const float y = ldexpf(x[s], 14 - e);
             const _Float16 hi = (_Float16)y, lo = (_Float16)(y - (float)hi);
-            const uint32_t at = ((2 * s + hb) * 64 + 16 * g + n) * 16 + 2 * k;
+            const uint32_t at = n / PER * 2 * L::plane + ((2 * s + hb) * 64 + 16 * g + n % PER) * 16 + 2 * k;
             *reinterpret_cast<_Float16 *>(lds + at) = hi;
             *reinterpret_cast<_Float16 *>(lds + at + (STACK ? 8 * 16 : L::plane)) = lo;
         }
@@ -515,15 +546,23 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(GRO
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 
     const int my_n = STACK ? r16 & 7 : r16;
-    const float factor = row_factor[my_n];
-    const int my_limit = my_n < nr ? limit(n0 + my_n) : -1;
     const bool low_half = STACK && r16 >= 8;  // this lane's probabilities are the remainders
-    f32x4 acc[GROUPS][4];
+    float factor[RB];
+    int my_limit[RB];
+    f32x4 acc[RB][GROUPS][4];
+    float ref[RB], l[RB];
 #pragma unroll
-    for (int s = 0; s < GROUPS; s++)
+    for (int b = 0; b < RB; b++) {
+        const int n = PER * b + my_n;
+        factor[b] = row_factor[n];
+        my_limit[b] = n < nr ? limit(n0 + n) : -1;
+        ref[b] = -INFINITY;
+        l[b] = 0.0f;
 #pragma unroll
-        for (int t = 0; t < 4; t++) acc[s][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-    float ref = -INFINITY, l = 0.0f;
+        for (int s = 0; s < GROUPS; s++)
+#pragma unroll
+            for (int t = 0; t < 4; t++) acc[b][s][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
 
     Tile next{};
     if constexpr (PAGED) next = pages_of(1);
@@ -567,7 +606,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(GRO
         Tile after{};
         if constexpr (!PAGED) next = find_rows(c + kWaves);
         // ---- scores: keys 4 g + e of half T against query row r16
-        float s[2][4] = {};
+        float s[RB][2][4] = {};
         {
             u32x4 ks[2];  // two blocks' scales of the lane's keys
             const auto k0 = resource(kpool, next, 0), k1 = resource(kpool, next, 1);
@@ -579,29 +618,36 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(GRO
                         for (int T = 0; T < 2; T++)
                             ks[T] = *reinterpret_cast<const u32x4 *>(lds + scale_read + (b >> 1) * 128 + 64 * T);
                 }
-                const half8 qh = *reinterpret_cast<const half8 *>(lds + query_read + b * 1024);
-                half8 ql{};
-                if constexpr (!STACK) ql = *reinterpret_cast<const half8 *>(lds + query_read + L::plane + b * 1024);
+                half8 kk[2];
 #pragma unroll
                 for (int T = 0; T < 2; T++) {
-                    half8 kk;
                     if constexpr (Q8) {
                         const u32x4 w = kreg[T][b >> 1] ^ 0x80808080u;
-                        kk = b & 1 ? join(key_digits<1>(w[0]), key_digits<1>(w[1]), key_digits<1>(w[2]), key_digits<1>(w[3]))
-                                   : join(key_digits<0>(w[0]), key_digits<0>(w[1]), key_digits<0>(w[2]), key_digits<0>(w[3]));
+                        kk[T] = b & 1 ? join(key_digits<1>(w[0]), key_digits<1>(w[1]), key_digits<1>(w[2]), key_digits<1>(w[3]))
+                                      : join(key_digits<0>(w[0]), key_digits<0>(w[1]), key_digits<0>(w[2]), key_digits<0>(w[3]));
                     } else {
-                        kk = __builtin_bit_cast(half8, kreg[T][b]);
+                        kk[T] = __builtin_bit_cast(half8, kreg[T][b]);
                     }
-                    f32x4 d = {0.f, 0.f, 0.f, 0.f};
-                    if constexpr (!Q8) d = f32x4{s[T][0], s[T][1], s[T][2], s[T][3]};
-                    d = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, qh, d, 0, 0, 0);
-                    if constexpr (!STACK) d = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, ql, d, 0, 0, 0);
+                }
 #pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        if constexpr (Q8)
-                            s[T][e] = fmaf(d[e], (float)__builtin_bit_cast(half2v, (uint32_t)ks[T][e])[b & 1], s[T][e]);
-                        else
-                            s[T][e] = d[e];
+                for (int n = 0; n < RB; n++) {
+                    const uint8_t *const operand = lds + query_read + (2 * n * L::plane + b * 1024);
+                    const half8 qh = *reinterpret_cast<const half8 *>(operand);
+                    half8 ql{};
+                    if constexpr (!STACK) ql = *reinterpret_cast<const half8 *>(operand + L::plane);
+#pragma unroll
+                    for (int T = 0; T < 2; T++) {
+                        f32x4 d = {0.f, 0.f, 0.f, 0.f};
+                        if constexpr (!Q8) d = f32x4{s[n][T][0], s[n][T][1], s[n][T][2], s[n][T][3]};
+                        d = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk[T], qh, d, 0, 0, 0);
+                        if constexpr (!STACK) d = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk[T], ql, d, 0, 0, 0);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            if constexpr (Q8)
+                                s[n][T][e] = fmaf(d[e], (float)__builtin_bit_cast(half2v, (uint32_t)ks[T][e])[b & 1], s[n][T][e]);
+                            else
+                                s[n][T][e] = d[e];
+                        }
                     }
                 }
                 const int p = Q8 ? b >> 1 : b;  // the piece that this block was in
@@ -614,15 +660,16 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(GRO
         }
         load_scales(next);
         if constexpr (PAGED) after = pages_of(turn + 2);
-        // ---- softmax of the lane's row over its eight keys
-        float top = -INFINITY;
+        // ---- softmax of the lane's rows over its eight keys
 #pragma unroll
-        for (int T = 0; T < 2; T++)
+        for (int n = 0; n < RB; n++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                if constexpr (STACK) s[T][e] += ror8(s[T][e]);
-                s[T][e] *= factor;
-            }
+            for (int T = 0; T < 2; T++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    if constexpr (STACK) s[n][T][e] += ror8(s[n][T][e]);
+                    s[n][T][e] *= factor[n];
+                }
         if (!whole) {
             int first = 4 * g4;  // opaque: what follows is not kept in registers for every tile
             asm volatile("" : "+v"(first));
@@ -643,63 +690,80 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(GRO
                         for (int u = 0; u < GROUPS; u++) vhalf[i][u] = u32x2{0, 0};
                     }
                 }
-                const bool seen = there && kTile * c + kk <= my_limit;
-                s[i >> 2][i & 3] = !seen ? -INFINITY : bad ? NAN : s[i >> 2][i & 3];
+#pragma unroll
+                for (int n = 0; n < RB; n++) {
+                    const bool seen = there && kTile * c + kk <= my_limit[n];
+                    s[n][i >> 2][i & 3] = !seen ? -INFINITY : bad ? NAN : s[n][i >> 2][i & 3];
+                }
+            }
+        }
+        float p[RB][8];
+        float top[RB];
+        bool move = false;
+#pragma unroll
+        for (int n = 0; n < RB; n++) {
+            top[n] = -INFINITY;
+#pragma unroll
+            for (int T = 0; T < 2; T++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) top[n] = fmaxf(top[n], s[n][T][e]);
+            top[n] = max_rows(top[n]) + (E - kHeadroom);
+            move = move || top[n] > ref[n] + kSlack;
+        }
+        if (__any(move)) {
+#pragma unroll
+            for (int n = 0; n < RB; n++) {
+                const bool filled = __any(ref[n] != -INFINITY);  // not in the wave's first tile
+                const float moved = fmaxf(ref[n], top[n]);
+                const float shrink = moved == ref[n] ? 1.0f : __builtin_amdgcn_exp2f(ref[n] - moved);
+                ref[n] = moved;
+                if (filled) {
+                    l[n] *= shrink;
+                    float row_shrink[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) row_shrink[e] = __shfl(shrink, 4 * g4 + e);
+#pragma unroll
+                    for (int u = 0; u < GROUPS; u++)
+#pragma unroll
+                        for (int t = 0; t < 4; t++)
+#pragma unroll
+                            for (int e = 0; e < 4; e++) acc[n][u][t][e] *= row_shrink[e];
+                }
             }
         }
 #pragma unroll
-        for (int T = 0; T < 2; T++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) top = fmaxf(top, s[T][e]);
-        top = max_rows(top) + (E - kHeadroom);
-        if (__any(top > ref + kSlack)) {
-            const bool filled = __any(ref != -INFINITY);  // not in the wave's first tile
-            const float moved = fmaxf(ref, top);
-            const float shrink = moved == ref ? 1.0f : __builtin_amdgcn_exp2f(ref - moved);
-            ref = moved;
-            if (filled) {
-                l *= shrink;
-                float row_shrink[4];
-#pragma unroll
-                for (int e = 0; e < 4; e++) row_shrink[e] = __shfl(shrink, 4 * g4 + e);
-#pragma unroll
-                for (int u = 0; u < GROUPS; u++)
-#pragma unroll
-                    for (int t = 0; t < 4; t++)
-#pragma unroll
-                        for (int e = 0; e < 4; e++) acc[u][t][e] *= row_shrink[e];
-            }
-        }
-        float p[8];
-        {
-            const float base = ref == -INFINITY ? 0.0f : ref;
+        for (int n = 0; n < RB; n++) {
+            const float base = ref[n] == -INFINITY ? 0.0f : ref[n];
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                p[i] = __builtin_amdgcn_exp2f(s[i >> 2][i & 3] - base);
-                l += p[i];
+                p[n][i] = __builtin_amdgcn_exp2f(s[n][i >> 2][i & 3] - base);
+                l[n] += p[n][i];
             }
         }
         // ---- value product: keys 4 g + e of both halves are the lane's eight
         {
             u32x4 vs[2];  // two blocks' scales of the lane's keys
             const auto v0 = resource(vpool, next, 0), v1 = resource(vpool, next, 1);
-            half8 ph, pl;
+            half8 ph[RB], pl[RB];
             // p[i] * d(i) as two halves (stacked: the one that the lane's row is)
-            auto halves = [&](auto d) {
+            auto halves = [&](int n, auto d) {
                 half2v h[4], o[4];
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    const float x = d(2 * i), y = d(2 * i + 1);
-                    h[i] = half2v{(_Float16)fmaf(p[2 * i], x, 0.0f), (_Float16)fmaf(p[2 * i + 1], y, 0.0f)};
-                    o[i] = half2v{(_Float16)fmaf(p[2 * i], x, -(float)h[i][0]), (_Float16)fmaf(p[2 * i + 1], y, -(float)h[i][1])};
+                    const float x = d(2 * i), y = d(2 * i + 1), px = p[n][2 * i], py = p[n][2 * i + 1];
+                    h[i] = half2v{(_Float16)fmaf(px, x, 0.0f), (_Float16)fmaf(py, y, 0.0f)};
+                    o[i] = half2v{(_Float16)fmaf(px, x, -(float)h[i][0]), (_Float16)fmaf(py, y, -(float)h[i][1])};
                     // one value h in every lane: rounded twice by different
                     // instructions, the two rows' halves need not be each other's
                     if constexpr (STACK) o[i] = low_half ? o[i] : h[i];
                 }
-                ph = join(h[0], h[1], h[2], h[3]);
-                pl = join(o[0], o[1], o[2], o[3]);
+                ph[n] = join(h[0], h[1], h[2], h[3]);
+                pl[n] = join(o[0], o[1], o[2], o[3]);
             };
-            if constexpr (!Q8) halves([](int) { return 1.0f; });
+            if constexpr (!Q8) {
+#pragma unroll
+                for (int n = 0; n < RB; n++) halves(n, [](int) { return 1.0f; });
+            }
 #pragma unroll
             for (int u = 0; u < GROUPS; u++) {
                 uint32_t w[8];
@@ -714,10 +778,13 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(GRO
                 for (int t = 0; t < 4; t++) {
                     half8 vv;
                     if constexpr (Q8) {
-                        if (!(t & 1))  // block 2 u + t / 2
-                            halves([&](int i) {
-                                return (float)__builtin_bit_cast(half2v, (uint32_t)vs[i >> 2][i & 3])[t >> 1];
-                            });
+                        if (!(t & 1)) {  // block 2 u + t / 2
+#pragma unroll
+                            for (int n = 0; n < RB; n++)
+                                halves(n, [&](int i) {
+                                    return (float)__builtin_bit_cast(half2v, (uint32_t)vs[i >> 2][i & 3])[t >> 1];
+                                });
+                        }
                         vv = t == 0   ? join(value_digits<0>(w[0], w[1]), value_digits<0>(w[2], w[3]), value_digits<0>(w[4], w[5]), value_digits<0>(w[6], w[7]))
                              : t == 1 ? join(value_digits<1>(w[0], w[1]), value_digits<1>(w[2], w[3]), value_digits<1>(w[4], w[5]), value_digits<1>(w[6], w[7]))
                              : t == 2 ? join(value_digits<2>(w[0], w[1]), value_digits<2>(w[2], w[3]), value_digits<2>(w[4], w[5]), value_digits<2>(w[6], w[7]))
@@ -732,8 +799,11 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(GRO
                              : t == 2 ? pairs(std::integral_constant<int, 2>{})
                                       : pairs(std::integral_constant<int, 3>{});
                     }
-                    if constexpr (!STACK) acc[u][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph, vv, acc[u][t], 0, 0, 0);
-                    acc[u][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pl, vv, acc[u][t], 0, 0, 0);
+#pragma unroll
+                    for (int n = 0; n < RB; n++) {
+                        if constexpr (!STACK) acc[n][u][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph[n], vv, acc[n][u][t], 0, 0, 0);
+                        acc[n][u][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pl[n], vv, acc[n][u][t], 0, 0, 0);
+                    }
                 }
                 load_values(v0, v1, u);
                 __builtin_amdgcn_sched_barrier(0);
@@ -744,10 +814,12 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(GRO
     }
 
     // ---- the waves' outputs joined: o = sum_w 2^(ref_w - max ref) o_w
-    l = sum_rows(l);
-    __syncthreads();  // every wave is done with the operands the slots lie over
-    {
-        float *const slot = reinterpret_cast<float *>(lds) + wave * ROWS * L::slot_row;
+#pragma unroll
+    for (int b = 0; b < RB; b++) {
+        if (b * PER >= nr) break;
+        l[b] = sum_rows(l[b]);
+        __syncthreads();  // every wave is done with what the slots lie over
+        float *const slot = reinterpret_cast<float *>(lds) + wave * PER * L::slot_row;
         const float unit = Q8 ? 512.0f : 1.0f;  // the digits were times 2^-9
         auto dim = [&](int u, int t) { return 64 * u + (Q8 ? 16 * t + r16 : 4 * r16 + t); };
 #pragma unroll
@@ -759,48 +831,48 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(GRO
                     if constexpr (STACK) {
                         // rows n and n + 8, 32 lanes apart: one swap puts t's two halves and t + 1's
                         // side by side, their sums in the lower and the upper lanes
-                        const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(acc[u][t][e]),
-                                                                        __float_as_uint(acc[u][t + 1][e]), false, false);
+                        const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(acc[b][u][t][e]),
+                                                                        __float_as_uint(acc[b][u][t + 1][e]), false, false);
                         slot[(4 * (g4 & 1) + e) * L::slot_row + dim(u, t) + (Q8 ? 16 : 1) * (g4 >> 1)] =
                             (__uint_as_float(x[0]) + __uint_as_float(x[1])) * unit;
                     } else {
-                        slot[(4 * g4 + e) * L::slot_row + dim(u, t)] = acc[u][t][e] * unit;
+                        slot[(4 * g4 + e) * L::slot_row + dim(u, t)] = acc[b][u][t][e] * unit;
                     }
                 }
-        if (lane < ROWS) {
-            st_m[wave * 16 + lane] = ref;
-            st_l[wave * 16 + lane] = l;
+        if (lane < PER) {
+            st_m[wave * 16 + lane] = ref[b];
+            st_l[wave * 16 + lane] = l[b];
         }
-    }
-    __syncthreads();
-    for (int idx = threadIdx.x; idx < nr * (D / 4); idx += 64 * kWaves) {
-        const int n = idx / (D / 4), d = 4 * (idx % (D / 4));
-        float m = -INFINITY;
+        __syncthreads();
+        for (int idx = threadIdx.x; idx < min(PER, nr - b * PER) * (D / 4); idx += 64 * kWaves) {
+            const int m16 = idx / (D / 4), n = b * PER + m16, d = 4 * (idx % (D / 4));
+            float m = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < kWaves; w++) m = fmaxf(m, st_m[w * 16 + n]);
-        f32x4 o = {0.f, 0.f, 0.f, 0.f};
-        float total = 0.0f;
+            for (int w = 0; w < kWaves; w++) m = fmaxf(m, st_m[w * 16 + m16]);
+            f32x4 o = {0.f, 0.f, 0.f, 0.f};
+            float total = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kWaves; w++) {
-            const float mw = st_m[w * 16 + n];
-            const float f = mw == m ? 1.0f : __builtin_amdgcn_exp2f(mw - m);
-            const f32x4 x = *reinterpret_cast<const f32x4 *>(lds + ((w * ROWS + n) * L::slot_row + d) * 4);
-            o += f * x;
-            total = fmaf(f, st_l[w * 16 + n], total);
-        }
-        const int r = row_of(n0 + n), h = kvh * G + n0 + n - r * G;
-        if (parts == 1) {
-            const int64_t at = (out_row + r) * a.heads + h;
-            const float inv = 1.0f / total;
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                float y = total == 0.0f ? 0.0f : o[i] * inv;  // a row that sees no key
-                if (gate) y *= sigmoid_ref(gate[at * gate_stride + d + i]);
-                out[at * D + d + i] = y;
+            for (int w = 0; w < kWaves; w++) {
+                const float mw = st_m[w * 16 + m16];
+                const float f = mw == m ? 1.0f : __builtin_amdgcn_exp2f(mw - m);
+                const f32x4 x = *reinterpret_cast<const f32x4 *>(lds + ((w * PER + m16) * L::slot_row + d) * 4);
+                o += f * x;
+                total = fmaf(f, st_l[w * 16 + m16], total);
             }
-        } else {
-            *reinterpret_cast<f32x4 *>(part + (record + n) * D + d) = o;
-            if (d == 0) stats[record + n] = make_float2(m, total);
+            const int r = row_of(n0 + n), h = kvh * G + n0 + n - r * G;
+            if (parts == 1) {
+                const int64_t at = (out_row + r) * a.heads + h;
+                const float inv = 1.0f / total;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    float y = total == 0.0f ? 0.0f : o[i] * inv;  // a row that sees no key
+                    if (gate) y *= sigmoid_ref(gate[at * gate_stride + d + i]);
+                    out[at * D + d + i] = y;
+                }
+            } else {
+                *reinterpret_cast<f32x4 *>(part + (record + n) * D + d) = o;
+                if (d == 0) stats[record + n] = make_float2(m, total);
+            }
         }
     }
 }
@@ -881,8 +953,18 @@ __global__ __launch_bounds__(256) void kv_attention_merge_kernel(const float *__
 
 bool paged(const KvArgs &a) { return a.block_size % 16 == 0 && (a.block_size & (a.block_size - 1)) == 0; }
 bool stacked(const KvArgs &a) { return paged(a) && a.heads / a.kv_heads * a.rows <= 8; }
+// 16-row blocks of a wave. Two share each tile's way to halves, at two waves a SIMD for
+// three: 16 requests of 8 rows, 4 heads of 128 a kv head, over 4096 keys 64.3 -> 55.4 us
+// (two blocks), 4 of 17 rows over 16384 117.9 -> 109.8 (five blocks, one half idle); with
+// three blocks it does not pay (70.7 -> 75.0), nor from 192 dims, where one wave a SIMD is
+// left (256 dims, five blocks: 114 -> 136).
+int blocks_of_wave(const KvArgs &a) {
+    const int blocks = (a.heads / a.kv_heads * a.rows + 15) / 16;
+    return a.fmt == kKvQ8 && paged(a) && a.head_dim <= 128 && blocks != 1 && blocks != 3 ? 2 : 1;
+}
+int pairs_of(const KvArgs &a) { return stacked(a) ? 8 : 16 * blocks_of_wave(a); }
 int row_blocks(const KvArgs &a) {
-    const int pairs = a.heads / a.kv_heads * a.rows, per = stacked(a) ? 8 : 16;
+    const int pairs = a.heads / a.kv_heads * a.rows, per = pairs_of(a);
     return (pairs + per - 1) / per;
 }
 
@@ -892,8 +974,7 @@ AttnSplit attn_split(const KvArgs &a) {
     sp.columns = sp.row_blocks * a.kv_heads;
     sp.group = a.heads / a.kv_heads;
     sp.group_inverse = sp.group == 1 ? 0 : (uint32_t)(((1ull << 32) + sp.group - 1) / sp.group);
-    const int held = a.head_dim <= 64 ? 4 : a.head_dim <= 128 ? 3 : 2;  // workgroups of a CU
-    sp.target = 256 * held;
+    sp.target = 256 * waves_held(a.head_dim / 64, blocks_of_wave(a));
     sp.share = (float)sp.columns / (float)sp.target;
     sp.whole = (int64_t)sp.columns * a.requests >= 2 * sp.target;
     if (paged(a)) while ((16 << sp.page_shift) < a.block_size) sp.page_shift++;
@@ -913,7 +994,7 @@ int64_t most_items(const KvArgs &a, const AttnSplit &sp) {
 int64_t most_records(const KvArgs &a, const AttnSplit &sp) {
     if (sp.whole || most_parts(a) == 1) return 0;
     const int64_t items = std::min((int64_t)sp.columns * a.requests * most_parts(a), (int64_t)4 * sp.target);
-    return items * (stacked(a) ? 8 : 16);
+    return items * pairs_of(a);
 }
 
 }  // namespace
@@ -932,9 +1013,9 @@ hipError_t launch_kv_attention(const float *q, int q_stride, const float *gate, 
     float2 *stats = records ? reinterpret_cast<float2 *>(part + records * a.head_dim) : nullptr;
     int2 *plan = records ? reinterpret_cast<int2 *>(stats + records) : nullptr;
     hipError_t err = hipSuccess;
-    auto launch = [&](auto fmt, auto groups, auto stack, auto pages) {
-        constexpr auto kernel = kv_attention_kernel<fmt(), groups(), stack(), pages()>;
-        constexpr uint32_t bytes = Layout<fmt(), groups(), stack(), pages()>::total;
+    auto launch = [&](auto fmt, auto groups, auto stack, auto pages, auto blocks) {
+        constexpr auto kernel = kv_attention_kernel<fmt(), groups(), stack(), pages(), blocks()>;
+        constexpr uint32_t bytes = Layout<fmt(), groups(), stack(), pages(), blocks()>::total;
         static std::once_flag once;
         std::call_once(once, [&] {
             (void)hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
@@ -946,9 +1027,15 @@ hipError_t launch_kv_attention(const float *q, int q_stride, const float *gate, 
         err = hipGetLastError();
     };
     auto by_pages = [&](auto fmt, auto groups) {
-        if (!paged(a)) launch(fmt, groups, std::false_type{}, std::false_type{});
-        else if (stacked(a)) launch(fmt, groups, std::true_type{}, std::true_type{});
-        else launch(fmt, groups, std::false_type{}, std::true_type{});
+        const std::true_type yes;
+        const std::false_type no;
+        const std::integral_constant<int, 1> one;
+        if (!paged(a)) return launch(fmt, groups, no, no, one);
+        if (stacked(a)) return launch(fmt, groups, yes, yes, one);
+        if constexpr (fmt() == kKvQ8 && groups() <= 2) {
+            if (blocks_of_wave(a) == 2) return launch(fmt, groups, no, yes, std::integral_constant<int, 2>{});
+        }
+        launch(fmt, groups, no, yes, one);
     };
     auto by_width = [&](auto fmt) {
         switch (a.head_dim / 64) {
@@ -966,7 +1053,7 @@ hipError_t launch_kv_attention(const float *q, int q_stride, const float *gate, 
     const int dims = (int64_t)a.rows * a.heads * a.requests * (a.head_dim / 64) <= 1024 ? 64 : a.head_dim;
     auto merge = dims == 64 ? kv_attention_merge_kernel<8> : kv_attention_merge_kernel<4>;
     merge<<<dim3(a.rows * (a.head_dim / dims), a.heads, a.requests), 256, 0, s>>>(
-        part, stats, plan, gate, gate_stride, out, a, sp.row_blocks, stacked(a) ? 8 : 16, dims);
+        part, stats, plan, gate, gate_stride, out, a, sp.row_blocks, pairs_of(a), dims);
     return hipGetLastError();
 }
 
