@@ -577,9 +577,9 @@ typedef struct yuuka_kv_params {
     int32_t block_size;   /* tokens per page */
     int32_t capacity;     /* tokens a request can hold */
     int32_t requests;     /* 1..65535 */
-    int32_t rows;         /* rows of every request */
+    int32_t rows;         /* rows of every request (attention: 4096 at most) */
     int32_t request_rows; /* rows between consecutive requests (0: rows) */
-    int32_t heads;        /* query heads, a multiple of kv_heads (attention) */
+    int32_t heads;        /* attention: query heads, a multiple of kv_heads, 256 times them at most */
     int32_t kv_heads;
     int32_t head_dim;     /* 64, 128, 192 or 256 */
     int32_t rope_dim;     /* append: rotated dimensions of a key, <= 128 (0: none) */

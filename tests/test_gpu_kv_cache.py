@@ -307,6 +307,31 @@ def test_append_rounding_at_the_borders(dev, stream, nk, D):
         assert np.isnan(got.reshape(-1, 32)[np.isnan(x.reshape(-1, 32)).any(1)]).all()
 
 
+@pytest.mark.parametrize("D", [64, 128, 192, 256])
+def test_append_over_the_whole_float_range(dev, stream, D):
+    """Blocks from the smallest subnormal to the largest float, and with infinities: bit for bit."""
+    tops = [1e-45, 1e-42, 1e-38, 3e-32, 1e-30, 7e-31, 1e-20, 6e-6, 7.5e-6, 1e-3, 1.0, 127.0, 8.3e6, 8.4e6, 1e20, 5e30, 2e31,
+            1e37, 3.4e38, 0.0]
+    rng = np.random.default_rng(D)
+    x = rng.uniform(-1, 1, (2, len(tops), 4 * D))
+    x = (x * np.array(tops)[:, None]).astype(np.float32)
+    x[0, 3, 5], x[1, 9, D], x[0, 12, 2 * D + 1] = np.inf, -np.inf, np.nan
+    c = Cache(dev, Q8, 16, 64, 4, D, 1, [10])
+    hip.kv_append(stream, dev.upload(x[0]), dev.upload(x[1]), *c.b_pool, c.b_table, c.b_pos, c.params(len(tops)))
+    stream.sync()
+    for side in range(2):
+        for r in range(len(tops)):
+            c.put(side, 0, 10 + r, x[side, r])
+        got, want = c.read_pool(side), c.pool[side]
+        nan = np.isnan(x[side]).any()
+        if nan:  # the scale of a block with a NaN is a NaN, of whichever payload
+            page, t = c.at(0, 22)
+            o = 16 * c.kvd + t * c.kvd // 16 + (2 * D // 32) * 2
+            assert np.isnan(got[page, o:o + 2].copy().view(np.float16)).all()
+            got[page, o:o + 2] = want[page, o:o + 2]
+        assert np.array_equal(got, want)
+
+
 @pytest.mark.parametrize("dtype", [Q8, F16, F32])
 @pytest.mark.parametrize("nk,D,rot", [(3, 64, 64), (3, 128, 20), (2, 192, 128), (4, 256, 64), (1, 256, 2)])
 def test_append_with_norm_and_rotation(dev, stream, dtype, nk, D, rot):
@@ -548,6 +573,66 @@ def test_long_contexts_and_shared_pages(dev, stream, dtype):
         hip.attn_decode(stream, o, dev.upload(q), *c.b_pool, c.b_table, c.b_pos, p)
         stream.sync()
         assert np.array_equal(o.read(np.uint32), first.view(np.uint32))
+
+
+MANY = [  # requests, heads, kv heads, head width, page, rows, longest
+    (17, 8, 2, 256, 16, 1, 700),    # a round of workgroups holds every part
+    (70, 2, 1, 256, 16, 1, 900),    # more requests than lanes; joined by whole rows
+    (70, 6, 2, 192, 16, 1, 500),
+    (65, 12, 3, 128, 16, 3, 300),
+    (300, 4, 1, 128, 16, 1, 260),   # more requests than are kept in registers
+    (300, 4, 2, 64, 16, 1, 150),
+    (260, 4, 4, 64, 6, 2, 100),     # pages of no power of two
+    (200, 16, 8, 128, 32, 1, 400),  # more columns than two rounds: no request is cut
+    (33, 8, 2, 128, 16, 9, 600),    # 36 pairs of a kv head: three blocks of 16, each a wave's
+    (21, 16, 4, 128, 16, 8, 500),   # two blocks a wave
+    (9, 16, 4, 64, 16, 17, 400),    # five, in pairs
+]
+
+
+@pytest.mark.parametrize("dtype", [Q8, F16])
+@pytest.mark.parametrize("requests,heads,nk,D,bs,rows,longest", MANY)
+def test_batches_of_ragged_requests(dev, stream, dtype, requests, heads, nk, D, bs, rows, longest):
+    """Every way that the work of a batch is cut: lengths from none to the longest, which one request has alone."""
+    rng = np.random.default_rng(requests + D)
+    positions = rng.integers(-rows - 1, longest // 3, requests)
+    positions[0], positions[-1], positions[requests // 2] = 0, -rows - 3, longest
+    c = Cache(dev, dtype, bs, longest + rows, nk, D, requests, positions, seed=rows, shared=True,
+              pages=-(-(longest + rows) // bs) + 3, fill=q8_fill() if dtype == Q8 else f16_fill)
+    n = requests * rows
+    q = rng.normal(0, 1, (n, heads, D)).astype(np.float32)
+    o = dev.upload(np.full(n * heads * D, 7.5, np.float32))
+    p = c.params(rows, heads=heads, scale=D ** -0.5)
+    hip.attn_decode(stream, o, dev.upload(q), *c.b_pool, c.b_table, c.b_pos, p)
+    stream.sync()
+    got, want = o.read(np.float32).reshape(q.shape), attention(c, q, rows, heads, D ** -0.5, False)
+    close(got, want)
+    for j in range(requests):  # no request hides in the others' norm
+        close(got[j * rows:(j + 1) * rows], want[j * rows:(j + 1) * rows])
+    hip.attn_decode(stream, o, dev.upload(q), *c.b_pool, c.b_table, c.b_pos, p)
+    stream.sync()
+    assert np.array_equal(o.read(np.uint32), got.reshape(-1).view(np.uint32))
+
+
+@pytest.mark.parametrize("dtype", [Q8, F16])
+@pytest.mark.parametrize("heads,nk,D,rows", [(8, 2, 128, 8), (8, 2, 64, 5), (8, 2, 256, 6), (4, 2, 128, 3)])
+def test_an_infinity_that_only_later_rows_see(dev, stream, dtype, heads, nk, D, rows):
+    """A value that is not finite, at the position of a row in the middle: the earlier rows keep theirs."""
+    c = Cache(dev, dtype, 16, 300, nk, D, 2, [250, 31], fill=q8_fill() if dtype == Q8 else f16_fill)
+    q = np.random.default_rng(2).normal(0, 1, (2 * rows, heads, D)).astype(np.float32)
+    mid = rows // 2
+    bad = np.ones(c.kvd, np.float32)
+    bad[:D] = np.inf           # the first kv head's
+    for j in range(2):
+        c.put(1, j, int(c.positions[j, 1]) + mid, bad)
+    c.upload()
+    want = attention(c, q, rows, heads, D ** -0.5, False)
+    o = dev.alloc(q.nbytes)
+    hip.attn_decode(stream, o, dev.upload(q), *c.b_pool, c.b_table, c.b_pos, c.params(rows, heads=heads, scale=D ** -0.5))
+    stream.sync()
+    got = o.read(np.float32).reshape(q.shape)
+    assert np.isfinite(want[:mid]).all() and not np.isfinite(want[mid:rows, : heads // nk]).any()
+    close(got, want)
 
 
 @pytest.mark.parametrize("dtype", [Q8, F16])

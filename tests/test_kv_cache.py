@@ -168,6 +168,18 @@ def test_attention_refuses_heads_and_rows(change, status):
     assert _call("attn", _memory(), hip.kv_params(**{**GOOD, "heads": 4, **change})) == status
 
 
+@pytest.mark.parametrize("change,words", [
+    (dict(heads=2 * 257), b"514 heads over 2 KV heads"),
+    (dict(requests=65535, rows=4096, heads=64), b"in one call"),        # 65535 * 2 * 4096 * 32 / 8 workgroups
+    (dict(requests=4097, rows=512, heads=32), b"in one call")])         # 2^23 and 2048 more
+def test_attention_refuses_more_than_one_launch(change, words):
+    m = _memory()
+    for b in m.values():  # no buffer is too small
+        b.handle.bytes = 1 << 60
+    assert _call("attn", m, hip.kv_params(**{**GOOD, **change})) == hip.INVALID_ARGUMENT
+    assert words in hip.lib().yuuka_last_error()
+
+
 @pytest.mark.parametrize("name,small", [(n, b) for n, bs in dict(
     append=("k", "v", "kpool", "vpool", "table", "positions", "norm", "rope"),
     read=("k", "v", "kpool", "vpool", "table", "positions"),

@@ -1016,11 +1016,15 @@ hipError_t launch_kv_attention(const float *q, int q_stride, const float *gate, 
     auto launch = [&](auto fmt, auto groups, auto stack, auto pages, auto blocks) {
         constexpr auto kernel = kv_attention_kernel<fmt(), groups(), stack(), pages(), blocks()>;
         constexpr uint32_t bytes = Layout<fmt(), groups(), stack(), pages(), blocks()>::total;
-        static std::once_flag once;
-        std::call_once(once, [&] {
-            (void)hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
-                                      (int)bytes);
-        });
+        if constexpr (bytes > 64 * 1024) {  // (a device's own setting)
+            static std::once_flag once[64];
+            int device = 0;
+            (void)hipGetDevice(&device);
+            std::call_once(once[device & 63], [] {
+                (void)hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                          (int)bytes);
+            });
+        }
         kernel<<<(uint32_t)most_items(a, sp), 64 * kWaves, bytes, s>>>(
             q, q_stride, gate, gate_stride, static_cast<const uint8_t *>(kpool), static_cast<const uint8_t *>(vpool), table,
             a, sp, part, stats, plan, out, dyn);
