@@ -1052,10 +1052,12 @@ hipError_t launch_kv_attention(const float *q, int q_stride, const float *gate, 
     if (a.fmt == kKvF16) by_width(std::integral_constant<int, kKvF16>{});
     else by_width(std::integral_constant<int, kKvQ8>{});
     if (err != hipSuccess || !records) return err;
-    // A slice of 64 dims a workgroup where that leaves few workgroups (their records are many,
-    // and what counts is the loads in flight), else whole rows.
-    const int dims = (int64_t)a.rows * a.heads * a.requests * (a.head_dim / 64) <= 1024 ? 64 : a.head_dim;
-    auto merge = dims == 64 ? kv_attention_merge_kernel<8> : kv_attention_merge_kernel<4>;
+    // Whole rows, or where a request can have many parts slices of 64 dims: then what counts is the
+    // records in flight. (5 parts: 12.1 us with the attention, in slices 12.6; 8 parts 42.4 and
+    // 44.0; 125 parts 69.3 and 65.3.)
+    const int64_t parts = std::min<int64_t>(most_parts(a), sp.target / ((int64_t)sp.columns * a.requests));
+    const int dims = parts > 32 ? 64 : a.head_dim;
+    auto merge = parts > 32 ? kv_attention_merge_kernel<8> : kv_attention_merge_kernel<4>;
     merge<<<dim3(a.rows * (a.head_dim / dims), a.heads, a.requests), 256, 0, s>>>(
         part, stats, plan, gate, gate_stride, out, a, sp.row_blocks, pairs_of(a), dims);
     return hipGetLastError();
