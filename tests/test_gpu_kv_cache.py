@@ -57,7 +57,8 @@ def encode(x):
 
 def decode(digits, scales):
     v = digits.reshape(*digits.shape[:-1], -1, 16, 4).swapaxes(-1, -2).reshape(*digits.shape[:-1], -1, 32)
-    return (v.astype(np.float32) * scales.view(np.float16).astype(np.float32)[..., None]).reshape(digits.shape)
+    with np.errstate(invalid="ignore"):  # 0 * inf
+        return (v.astype(np.float32) * scales.view(np.float16).astype(np.float32)[..., None]).reshape(digits.shape)
 
 
 class Cache:

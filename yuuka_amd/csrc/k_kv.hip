@@ -129,7 +129,7 @@ __device__ __forceinline__ uint32_t transpose_digits(uint32_t mine, int r) {
 // One wave per 256 dims of kAppendRows rows: keys, values, or queries (those
 // only with q). Bound by the float32 rows it reads once (past the caches), those of all the
 // wave's rows asked for before any is used, and by vector instructions: 8191 rows of 8
-// heads of 128, keys normalised and rotated, to Q8_0 (89 MB): 26 us, 3.4 TB/s. Two rows a
+// heads of 128, keys normalised and rotated, to Q8_0 (89 MB): 28 us, 3.2 TB/s. Two rows a
 // wave: with the read back 45.8 us, one 51.2, four 48.4.
 constexpr int kAppendWaves = 4, kAppendRows = 2;
 

@@ -27,6 +27,15 @@
 //    exponent of the largest value scale so far: p times a scale stays below 2^14
 //    and the halves' 39 octaves are used; m' moves (and the accumulators are
 //    rescaled) when a tile passes it by 4.
+//
+// Measured, with the join: one row of one request over 120001 keys of 4 heads of 256, 16 query
+// heads (261 MB of Q8_0) 65 us, 4.0 TB/s, of which 5 before the first tile, 4 after the last
+// and 5 for the join; 16 requests of 4096 such keys 42 us; 16 of 4096 keys of 8 heads of 128
+// in F16 (269 MB) 58 us, 4.6 TB/s. Vector instructions issue in 50 % of a SIMD's cycles at
+// 256 dims (700 a tile), 64 % at 128, 16 % over F16: bound by the reads and, from Q8_0, by two
+// waves a SIMD (256 registers) that wait for them in turn. 4 requests of 17 rows over 16384
+// keys of 4 heads of 256 take 105 us: instructions (73 %), for every 16-row block turns each
+// tile's digits to halves again.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
