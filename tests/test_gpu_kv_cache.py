@@ -616,6 +616,21 @@ def test_batches_of_ragged_requests(dev, stream, dtype, requests, heads, nk, D, 
 
 
 @pytest.mark.parametrize("dtype", [Q8, F16])
+@pytest.mark.parametrize("scale,size", [(0.0, 1.0), (-0.0, 1.0), (-0.09, 1.0), (1e-25, 1e-25), (-1e-30, 1e-15), (1e-40, 1.0)])
+def test_scales_of_zero_below_and_next_to_nothing(dev, stream, dtype, scale, size):
+    """The mean of the values, or the signed scores; keys a row does not see stay out."""
+    heads, nk, D, rows = 8, 2, 128, 3
+    c = Cache(dev, dtype, 16, 200, nk, D, 3, [130, 0, -2], fill=q8_fill() if dtype == Q8 else f16_fill)
+    q = (size * np.random.default_rng(3).normal(0, 1, (3 * rows, heads, D))).astype(np.float32)
+    o = dev.upload(np.full(q.shape, 2.5, np.float32))
+    hip.attn_decode(stream, o, dev.upload(q), *c.b_pool, c.b_table, c.b_pos, c.params(rows, heads=heads, scale=scale))
+    stream.sync()
+    want = attention(c, q, rows, heads, scale, False)
+    assert (want[6:8] == 0).all() and (want[8] != 0).any()
+    close(o.read(np.float32).reshape(q.shape), want)
+
+
+@pytest.mark.parametrize("dtype", [Q8, F16])
 @pytest.mark.parametrize("heads,nk,D,rows", [(8, 2, 128, 8), (8, 2, 64, 5), (8, 2, 256, 6), (4, 2, 128, 3)])
 def test_an_infinity_that_only_later_rows_see(dev, stream, dtype, heads, nk, D, rows):
     """A value that is not finite, at the position of a row in the middle: the earlier rows keep theirs."""

@@ -34,7 +34,7 @@
 // in F16 (269 MB) 58 us, 4.6 TB/s. Vector instructions issue in 50 % of a SIMD's cycles at
 // 256 dims (700 a tile), 64 % at 128, 16 % over F16: bound by the reads and, from Q8_0, by two
 // waves a SIMD (256 registers) that wait for them in turn. 4 requests of 17 rows over 16384
-// keys of 4 heads of 256 take 105 us: instructions (73 %), for every 16-row block turns each
+// keys of 4 heads of 256 take 103 us: instructions (73 %), for every 16-row block turns each
 // tile's digits to halves again.
 #include <hip/hip_runtime.h>
 
@@ -52,6 +52,7 @@ typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef float float2v __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint16_t ushort2v __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 template <int N> struct Dwords {  // N dwords at dword alignment
@@ -94,6 +95,16 @@ __device__ __forceinline__ float max_wave(float x) {  // non-negative or not, no
     x = fmaxf(x, dpp<0x124>(x));
     x = fmaxf(x, dpp<0x128>(x));
     return max_rows(x);
+}
+__device__ __forceinline__ uint32_t max_wave(uint32_t x) {
+    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0xb1, 0xf, 0xf, true));
+    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x4e, 0xf, 0xf, true));
+    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x124, 0xf, 0xf, true));
+    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x128, 0xf, 0xf, true));
+    auto a = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    x = max(a[0], a[1]);
+    a = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    return max(a[0], a[1]);
 }
 __device__ __forceinline__ float sum_wave(float x) {
     x += dpp<0xb1>(x);
@@ -523,6 +534,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(wav
         }
     }
 
+    const float sign = a.scale > 0.0f ? 1.0f : a.scale < 0.0f ? -1.0f : a.scale;
     // ---- queries as MFMA operands in LDS: wave w prepares rows w and w + 8
 #pragma unroll
     for (int half = 0; half < ROWS / kWaves; half++) {
@@ -541,14 +553,16 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(wav
         const int k = Q8 ? 2 * (lane & 3) + ((lane >> 4) & 1) : lane & 7;
 #pragma unroll
         for (int s = 0; s < GROUPS; s++) {
-            const float y = ldexpf(x[s], 14 - e);
+            const float y = ldexpf(x[s] * sign, 14 - e);
             const _Float16 hi = (_Float16)y, lo = (_Float16)(y - (float)hi);
             const uint32_t at = n / PER * 2 * L::plane + ((2 * s + hb) * 64 + 16 * g + n % PER) * 16 + 2 * k;
             *reinterpret_cast<_Float16 *>(lds + at) = hi;
             *reinterpret_cast<_Float16 *>(lds + at + (STACK ? 8 * 16 : L::plane)) = lo;
         }
-        // scores in units of log2: factor * (operand product)
-        if (lane == 0) row_factor[n] = ldexpf(a.scale * 1.44269504088896341f, e - 14);
+        // scores in units of log2: factor * (operand product). The factor is above zero (a key left
+        // out has -infinity times it): the sign, or the whole of a scale of zero, goes to the
+        // query. (Products are below 2^45: times 2^-126 they are nothing to the exponential.)
+        if (lane == 0) row_factor[n] = fmaxf(ldexpf(fabsf(a.scale) * 1.44269504088896341f, e - 14), 0x1p-126f);
     }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
     __builtin_amdgcn_s_barrier();
@@ -589,16 +603,25 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(wav
             // scales to LDS (those of missing keys as zeros), and the largest finite value scale's exponent
             wave_lds_fence();
             const bool there = __builtin_amdgcn_inverse_ballot_w64((uint64_t)cur.keys << 32 | cur.keys);
-            uint32_t d[GROUPS], most = 0, over = 0;
+            uint32_t d[GROUPS];
+            ushort2v two = {0, 0};  // largest of each half, as integers
 #pragma unroll
             for (int s = 0; s < GROUPS; s++) {
                 d[s] = there ? dword<GROUPS>(sreg, s) : 0u;
-                const uint32_t lo = d[s] & 0x7fffu, hi = (d[s] >> 16) & 0x7fffu;
-                most = max(most, max(lo < 0x7c00u ? lo : 0u, hi < 0x7c00u ? hi : 0u));
-                over |= ((d[s] & 0x7fff7fffu) + 0x04000400u) & 0x80008000u;
+                two = __builtin_elementwise_max(two, __builtin_bit_cast(ushort2v, d[s] & 0x7fff7fffu));
+            }
+            uint32_t most = max((uint32_t)two[0], (uint32_t)two[1]);
+            const bool over = most >= 0x7c00u;  // an infinity or a NaN
+            if (__any(over)) {
+                most = 0;
+#pragma unroll
+                for (int s = 0; s < GROUPS; s++) {
+                    const uint32_t lo = d[s] & 0x7fffu, hi = (d[s] >> 16) & 0x7fffu;
+                    most = max(most, max(lo < 0x7c00u ? lo : 0u, hi < 0x7c00u ? hi : 0u));
+                }
             }
             if (!whole) {
-                uint64_t b = __builtin_amdgcn_ballot_w64(over != 0 && kTile * c + (lane & 31) > least);
+                uint64_t b = __builtin_amdgcn_ballot_w64(over && kTile * c + (lane & 31) > least);
                 poison = (uint32_t)(b >> 32);
                 if (__builtin_amdgcn_inverse_ballot_w64((uint64_t)poison << 32)) {
 #pragma unroll
@@ -607,9 +630,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(wav
             }
 #pragma unroll
             for (int s = 0; s < GROUPS; s++) *reinterpret_cast<uint32_t *>(lds + scale_write + 128 * s) = d[s];
-            float m = __uint_as_float(lane < 32 ? 0u : most);  // non-negative: ordered as floats
-            m = max_wave(m);
-            E = (float)((int)(__float_as_uint(m) >> 10) - 14);  // scale < 2^E
+            E = (float)((int)(max_wave(lane < 32 ? 0u : most) >> 10) - 14);  // scale < 2^E
             wave_lds_fence();
         }
         Tile after{};
@@ -677,7 +698,6 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(wav
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     if constexpr (STACK) s[n][T][e] += ror8(s[n][T][e]);
-                    s[n][T][e] *= factor[n];
                 }
         if (!whole) {
             int first = 4 * g4;  // opaque: what follows is not kept in registers for every tile
@@ -716,7 +736,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(wav
             for (int T = 0; T < 2; T++)
 #pragma unroll
                 for (int e = 0; e < 4; e++) top[n] = fmaxf(top[n], s[n][T][e]);
-            top[n] = max_rows(top[n]) + (E - kHeadroom);
+            top[n] = fmaf(max_rows(top[n]), factor[n], E - kHeadroom);
             move = move || top[n] > ref[n] + kSlack;
         }
         if (__any(move)) {
@@ -745,7 +765,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(wav
             const float base = ref[n] == -INFINITY ? 0.0f : ref[n];
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                p[n][i] = __builtin_amdgcn_exp2f(s[n][i >> 2][i & 3] - base);
+                p[n][i] = __builtin_amdgcn_exp2f(fmaf(s[n][i >> 2][i & 3], factor[n], -base));
                 l[n] += p[n][i];
             }
         }
