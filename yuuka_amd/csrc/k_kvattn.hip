@@ -34,7 +34,7 @@
 // in F16 (269 MB) 58 us, 4.6 TB/s. Vector instructions issue in 50 % of a SIMD's cycles at
 // 256 dims (700 a tile), 64 % at 128, 16 % over F16: bound by the reads and, from Q8_0, by two
 // waves a SIMD (256 registers) that wait for them in turn. 4 requests of 17 rows over 16384
-// keys of 4 heads of 256 take 103 us: instructions (73 %), for every 16-row block turns each
+// keys of 4 heads of 256 take 102 us: instructions (73 %), for every 16-row block turns each
 // tile's digits to halves again.
 #include <hip/hip_runtime.h>
 
@@ -52,6 +52,7 @@ typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef float float2v __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float Floats4 __attribute__((ext_vector_type(4), aligned(4)));  // at float alignment
 typedef uint16_t ushort2v __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -535,7 +536,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(wav
     }
 
     const float sign = a.scale > 0.0f ? 1.0f : a.scale < 0.0f ? -1.0f : a.scale;
-    // ---- queries as MFMA operands in LDS: wave w prepares rows w and w + 8
+    // ---- queries as MFMA operands in LDS: wave w prepares rows w, w + kWaves, ...
 #pragma unroll
     for (int half = 0; half < ROWS / kWaves; half++) {
         const int n = wave + kWaves * half;
@@ -906,74 +907,157 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(wav
     }
 }
 
-// One workgroup per (row, head, request) and `dims` dims: joins the parts' records. A
-// thread has four dims of every (1024 / dims)-th record, kDeep of them loaded while
-// the weights are worked out, a part a thread.
-template <int kDeep>
+// Where the records of one (row, head) of a request are: part s's at first + s * step.
+struct Records {
+    int parts;
+    int64_t first, step;
+};
+__device__ __forceinline__ Records records_of(const int2 *plan, const KvArgs &a, int row_blocks, int pairs_per_block, int j,
+                                              int r, int h) {
+    const int2 mine = plan[j];
+    const int G = a.heads / a.kv_heads, kvh = h / G, pair = r * G + h - kvh * G, columns = row_blocks * a.kv_heads;
+    const int column = kvh * row_blocks + pair / pairs_per_block;
+    return {mine.x, ((int64_t)mine.y * columns + column) * pairs_per_block + pair % pairs_per_block,
+            (int64_t)columns * pairs_per_block};
+}
+
+// Joins a request's parts, few of them: one wave per (row, head, request), a part a lane for the
+// weights, four dims a lane for the outputs, with kDeep records in flight from before the
+// weights are known.
+template <int GROUPS>
+__global__ __launch_bounds__(256) void kv_attention_join_kernel(const float *__restrict__ part,
+                                                                const float2 *__restrict__ stats,
+                                                                const int2 *__restrict__ plan,
+                                                                const float *__restrict__ gate, int gate_stride,
+                                                                float *__restrict__ out, KvArgs a, int row_blocks,
+                                                                int pairs_per_block) {
+    constexpr int D = 64 * GROUPS, kQuads = D / 4, kWide = 64 / kQuads, kDeep = 8;  // kWide records side by side
+    const int lane = threadIdx.x & 63, j = blockIdx.y;
+    const int item = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (item >= a.rows * a.heads) return;  // whole waves: no barrier below
+    const int r = item / a.heads, h = item - r * a.heads;
+    const Records rec = records_of(plan, a, row_blocks, pairs_per_block, j, r, h);
+    if (rec.parts == 1) return;  // written by its workgroup
+    const int64_t row = ((int64_t)j * a.rq_rows + r) * a.heads + h;
+    const int sub = lane / kQuads, d = 4 * (lane % kQuads);
+    const f32x4 none = {0.f, 0.f, 0.f, 0.f};
+    f32x4 x[kDeep], o = none, g = none;
+    auto load = [&](int s0) {
+#pragma unroll
+        for (int u = 0; u < kDeep; u++) {
+            const int s = min(s0 + kWide * u + sub, rec.parts - 1);  // (no branches between the loads)
+            x[u] = *reinterpret_cast<const f32x4 *>(part + (rec.first + s * rec.step) * D + d);
+        }
+    };
+    // weights of the parts base + lane; 64 of them at a time, the maximum over all first
+    auto stat = [&](int base) {
+        return base + lane < rec.parts ? stats[rec.first + (base + lane) * rec.step] : make_float2(-INFINITY, 0.0f);
+    };
+    float2 ml = stat(0);
+    load(0);
+    if (gate && lane < kQuads) g = *reinterpret_cast<const Floats4 *>(gate + row * gate_stride + d);
+    float m = ml.x;
+    for (int base = 64; base < rec.parts; base += 64) m = fmaxf(m, stat(base).x);
+    m = max_wave(m);
+    float l = 0.0f;
+    for (int base = 0;;) {
+        // a part without keys (no sum) weighs nothing, whatever its output holds
+        const float w = ml.y == 0.0f ? 0.0f : ml.x == m ? 1.0f : __builtin_amdgcn_exp2f(ml.x - m);
+        const float weight = ml.y == 0.0f ? -1.0f : w;
+        l += w * ml.y;
+        const int upto = min(64, rec.parts - base);
+        for (int s0 = 0;;) {
+#pragma unroll
+            for (int u = 0; u < kDeep; u++) {
+                const int s = s0 + kWide * u + sub;
+                const float f = __shfl(weight, s & 63);
+                if (s < upto && f >= 0.0f) o += f * x[u];
+            }
+            s0 += kWide * kDeep;
+            if (s0 >= upto) break;
+            load(base + s0);
+        }
+        base += 64;
+        if (base >= rec.parts) break;
+        ml = stat(base);
+        load(base);
+    }
+    l = sum_wave(l);
+#pragma unroll
+    for (int i = 0; i < 4; i++) o[i] = kWide == 4 ? sum_rows(o[i]) : kWide == 2 ? sum_halves(o[i]) : o[i];
+    if (lane < kQuads) {
+        const float inv = 1.0f / l;
+        f32x4 y;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            y[i] = l == 0.0f ? 0.0f : o[i] * inv;  // a row that sees no key
+            if (gate) y[i] *= sigmoid_ref(g[i]);
+        }
+        *reinterpret_cast<Floats4 *>(out + row * D + d) = y;
+    }
+}
+
+// The same for many parts: one workgroup per (row, head, request) and 64 dims. A thread has
+// four dims of every 16th record, eight of them loaded while the weights are worked
+// out, a part a thread.
 __global__ __launch_bounds__(256) void kv_attention_merge_kernel(const float *__restrict__ part,
                                                                  const float2 *__restrict__ stats,
                                                                  const int2 *__restrict__ plan,
                                                                  const float *__restrict__ gate, int gate_stride,
                                                                  float *__restrict__ out, KvArgs a, int row_blocks,
-                                                                 int pairs_per_block, int dims) {
+                                                                 int pairs_per_block) {
     static_assert(kMaxParts <= 256, "a part a thread");
+    constexpr int kDeep = 8;
     __shared__ float weight[256], red[2][4];
-    __shared__ f32x4 sum[256];
+    __shared__ f32x4 sum[4][16];
     const int h = blockIdx.y, j = blockIdx.z, tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-    const int slices = a.head_dim / dims, r = blockIdx.x / slices, d0 = dims * (blockIdx.x % slices);
-    const int2 mine = plan[j];
-    const int parts = mine.x;
+    const int slices = a.head_dim / 64, r = blockIdx.x / slices, d0 = 64 * (blockIdx.x % slices);
+    const Records recs = records_of(plan, a, row_blocks, pairs_per_block, j, r, h);
+    const int parts = recs.parts;
     if (parts == 1) return;  // written by its workgroup
-    const int G = a.heads / a.kv_heads, kvh = h / G, pair = r * G + h - kvh * G, columns = row_blocks * a.kv_heads;
-    const int column = kvh * row_blocks + pair / pairs_per_block;
-    // record of part s: first + s * step
-    const int64_t first = ((int64_t)mine.y * columns + column) * pairs_per_block + pair % pairs_per_block;
-    const int64_t step = (int64_t)columns * pairs_per_block;
     const int64_t row = ((int64_t)j * a.rq_rows + r) * a.heads + h;
-    const float2 ml = tid < parts ? stats[first + tid * step] : make_float2(-INFINITY, 0.0f);
-    const int quads = dims / 4, wide = 256 / quads, rec = tid / quads, d = d0 + 4 * (tid % quads);
+    const float2 ml = tid < parts ? stats[recs.first + tid * recs.step] : make_float2(-INFINITY, 0.0f);
+    const int rec = tid >> 4, d = d0 + 4 * (tid & 15);
     const f32x4 none = {0.f, 0.f, 0.f, 0.f};
     f32x4 x[kDeep], o = none;
     auto load = [&](int s0) {
 #pragma unroll
         for (int u = 0; u < kDeep; u++) {
-            const int s = s0 + wide * u;
-            const bool in = rec < wide && s < parts;
-            x[u] = in ? *reinterpret_cast<const f32x4 *>(part + (first + s * step) * a.head_dim + d) : none;
+            const int s = s0 + 16 * u;
+            x[u] = s < parts ? *reinterpret_cast<const f32x4 *>(part + (recs.first + s * recs.step) * a.head_dim + d) : none;
         }
     };
     load(rec);
     float g = 0.0f;
-    if (gate && tid < dims) g = gate[row * gate_stride + d0 + tid];
-    float m = ml.x;
-    m = max_wave(m);
+    if (gate && tid < 64) g = gate[row * gate_stride + d0 + tid];
+    float m = max_wave(ml.x);
     if (lane == 0) red[0][wave] = m;
     __syncthreads();
     m = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
     // a part without keys (no sum) weighs nothing, whatever its output holds
     const float w = ml.y == 0.0f ? 0.0f : ml.x == m ? 1.0f : __builtin_amdgcn_exp2f(ml.x - m);
     weight[tid] = ml.y == 0.0f ? -1.0f : w;
-    float l = w * ml.y;
-    l = sum_wave(l);
+    float l = sum_wave(w * ml.y);
     if (lane == 0) red[1][wave] = l;
     __syncthreads();
     l = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
     for (int s0 = rec;;) {
 #pragma unroll
         for (int u = 0; u < kDeep; u++) {
-            const float f = weight[(s0 + wide * u) & 255];
-            if (s0 + wide * u < parts && f >= 0.0f) o += f * x[u];
+            const float f = weight[(s0 + 16 * u) & 255];
+            if (s0 + 16 * u < parts && f >= 0.0f) o += f * x[u];
         }
-        s0 += wide * kDeep;
+        s0 += 16 * kDeep;
         if (s0 - rec >= parts) break;
         load(s0);
     }
-    sum[tid] = o;
+#pragma unroll
+    for (int i = 0; i < 4; i++) o[i] = sum_rows(o[i]);
+    if (lane < 16) sum[wave][lane] = o;
     __syncthreads();
-    if (tid < dims) {
+    if (tid < 64) {
         const float *const t = reinterpret_cast<const float *>(sum);
-        float y = 0.0f;
-        for (int i = 0; i < wide; i++) y += t[dims * i + tid];
+        float y = (t[tid] + t[64 + tid]) + (t[128 + tid] + t[192 + tid]);
         y = l == 0.0f ? 0.0f : y / l;  // a row that sees no key
         if (gate) y *= sigmoid_ref(g);
         out[row * a.head_dim + d0 + tid] = y;
@@ -1081,14 +1165,22 @@ hipError_t launch_kv_attention(const float *q, int q_stride, const float *gate, 
     if (a.fmt == kKvF16) by_width(std::integral_constant<int, kKvF16>{});
     else by_width(std::integral_constant<int, kKvQ8>{});
     if (err != hipSuccess || !records) return err;
-    // Whole rows, or where a request can have many parts slices of 64 dims: then what counts is the
-    // records in flight. (5 parts: 12.1 us with the attention, in slices 12.6; 8 parts 42.4 and
-    // 44.0; 125 parts 69.3 and 65.3.)
+    // A wave a row, or where a request can have many parts a workgroup each 64 dims: then what counts
+    // is the records in flight. (us with the attention, a wave a row and a workgroup a row: 96 requests of
+    // up to 6 parts, 8 heads of 128 a KV head, 91.5 and 94.5; 16 of 8 parts 42.1 and 42.3; 5 rows of 9
+    // parts 14.6 and 13.8. 125 parts: a workgroup a row 69.3, each 64 dims 64.6.)
     const int64_t parts = std::min<int64_t>(most_parts(a), sp.target / ((int64_t)sp.columns * a.requests));
-    const int dims = parts > 32 ? 64 : a.head_dim;
-    auto merge = parts > 32 ? kv_attention_merge_kernel<8> : kv_attention_merge_kernel<4>;
-    merge<<<dim3(a.rows * (a.head_dim / dims), a.heads, a.requests), 256, 0, s>>>(
-        part, stats, plan, gate, gate_stride, out, a, sp.row_blocks, pairs_of(a), dims);
+    if (parts > 32) {
+        kv_attention_merge_kernel<<<dim3(a.rows * (a.head_dim / 64), a.heads, a.requests), 256, 0, s>>>(
+            part, stats, plan, gate, gate_stride, out, a, sp.row_blocks, pairs_of(a));
+        return hipGetLastError();
+    }
+    auto join = a.head_dim == 64    ? kv_attention_join_kernel<1>
+                : a.head_dim == 128 ? kv_attention_join_kernel<2>
+                : a.head_dim == 192 ? kv_attention_join_kernel<3>
+                                    : kv_attention_join_kernel<4>;
+    join<<<dim3((a.rows * a.heads + 3) / 4, a.requests), 256, 0, s>>>(part, stats, plan, gate, gate_stride, out, a,
+                                                                      sp.row_blocks, pairs_of(a));
     return hipGetLastError();
 }
 
