@@ -616,6 +616,26 @@ def test_batches_of_ragged_requests(dev, stream, dtype, requests, heads, nk, D, 
 
 
 @pytest.mark.parametrize("dtype", [Q8, F16])
+@pytest.mark.parametrize("requests,heads,nk,D,rows", [(17, 8, 2, 256, 1), (18, 4, 2, 192, 2), (13, 6, 3, 128, 1), (37, 2, 1, 64, 3)])
+def test_one_long_request_among_short_ones(dev, stream, dtype, requests, heads, nk, D, rows):
+    """The long one is cut into more parts than a wave has lanes, though a request of the batch has few on average."""
+    longest = 9000
+    positions = np.random.default_rng(D).integers(0, 60, requests)
+    positions[requests // 3] = longest
+    c = Cache(dev, dtype, 64, longest + rows, nk, D, requests, positions, seed=rows, shared=True,
+              pages=-(-(longest + rows) // 64) + 2, fill=q8_fill() if dtype == Q8 else f16_fill)
+    q = np.random.default_rng(2).normal(0, 1, (requests * rows, heads, 2 * D)).astype(np.float32)
+    o = dev.alloc(requests * rows * heads * D * 4)
+    p = c.params(rows, heads=heads, gated=True, scale=D ** -0.5)
+    hip.attn_decode(stream, o, dev.upload(q), *c.b_pool, c.b_table, c.b_pos, p)
+    stream.sync()
+    got = o.read(np.float32).reshape(requests * rows, heads, D)
+    want = attention(c, q, rows, heads, D ** -0.5, True)
+    for j in range(requests):
+        close(got[j * rows:(j + 1) * rows], want[j * rows:(j + 1) * rows])
+
+
+@pytest.mark.parametrize("dtype", [Q8, F16])
 @pytest.mark.parametrize("scale,size", [(0.0, 1.0), (-0.0, 1.0), (-0.09, 1.0), (1e-25, 1e-25), (-1e-30, 1e-15), (1e-40, 1.0)])
 def test_scales_of_zero_below_and_next_to_nothing(dev, stream, dtype, scale, size):
     """The mean of the values, or the signed scores; keys a row does not see stay out."""
