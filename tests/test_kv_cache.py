@@ -344,3 +344,33 @@ def test_prefill_attention_takes_16_rows():
     bufs, n, u, flags = _ops(m)["ATTENTION_PREFILL_PAGED"]
     for rows, status in ((16, hip.OK), (17, hip.INVALID_ARGUMENT)):
         assert plan.add("ATTENTION_PREFILL_PAGED", bufs, n[:4] + [rows, 0], u, flags=flags) == status
+
+
+# ------------------------------------------------------- rows between requests
+
+WRAP = [  # the rows' bytes are 2^64 and a little: requests, rows between them, heads, kv heads
+    ("append", 4097, 1 << 30, 0, 4096),            # 4096 2^30 rows of 2^22 bytes
+    ("read", 4097, 1 << 30, 0, 4096),
+    ("append", 16385, 1 << 28, 0, 4096),
+    ("attn", 513, 1 << 30, 32768, 128),            # 512 2^30 rows of 2^25 bytes
+    ("attn", 1025, 1 << 29, 32768, 128),
+]
+
+
+@pytest.mark.parametrize("name,requests,stride,heads,kv_heads", WRAP)
+def test_rows_that_wrap_around_64_bits_are_refused(name, requests, stride, heads, kv_heads):
+    """Buffers of one request's size do not pass for those of thousands."""
+    m = _memory()
+    m.update(norm=None, rope=None)
+    row = 4 * 256 * (heads or kv_heads)
+    assert (requests - 1) * stride * row % 2 ** 64 == 0
+    for b in m.values():
+        if b is not None:
+            b.handle.bytes = 1 << 26
+    for b in ("k", "v", "q", "out"):
+        m[b].handle.bytes = row
+    for b in ("kpool", "vpool"):
+        m[b].handle.bytes = 1 << 40
+    p = hip.kv_params(hip.Q8_0, 16, 100, kv_heads, 256, 1, requests, heads=heads, request_rows=stride)
+    assert _call(name, m, p) == hip.INVALID_ARGUMENT
+    assert b"rows" in hip.lib().yuuka_last_error()

@@ -40,6 +40,11 @@ yuuka_status kv_check(KvArgs *a, uint32_t dtype, bool attention) {
     if (a->head_dim < 64 || a->head_dim % 64 || a->head_dim > 256)
         return fail(YUUKA_ERR_UNSUPPORTED, "KV cache head dimension %d (64, 128, 192 and 256 are served)", a->head_dim);
     a->kv_dim = a->kv_heads * a->head_dim;
+    // 2^36 rows of 64 dims are 16 TiB, more than any buffer: below that a row's bytes
+    // (2^27 at the most: 2^16 heads of 256 and their gates) times the rows stay under 2^63
+    if (kv_span_rows(*a) > 1ull << 36)
+        return fail(YUUKA_ERR_INVALID_ARGUMENT, "KV cache: %d requests of %d rows, %d rows apart", a->requests, a->rows,
+                    a->rq_rows);
     if (a->rope_dim < 0 || a->rope_dim % 2 || a->rope_dim > a->head_dim || a->rope_dim > 128)
         return fail(YUUKA_ERR_INVALID_ARGUMENT, "KV cache rotation of %d dimensions", a->rope_dim);
     if ((int64_t)a->rows * (2 * a->kv_heads + a->heads) > (1 << 25))  // vectors of one launch
