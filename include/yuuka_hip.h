@@ -578,7 +578,7 @@ typedef struct yuuka_kv_params {
     int32_t capacity;     /* tokens a request can hold */
     int32_t requests;     /* 1..65535 */
     int32_t rows;         /* rows of every request (attention: 4096 at most) */
-    int32_t request_rows; /* rows between consecutive requests (0: rows) */
+    int32_t request_rows; /* rows between consecutive requests (0: rows), not less than rows */
     int32_t heads;        /* attention: query heads, a multiple of kv_heads, 256 times them at most */
     int32_t kv_heads;
     int32_t head_dim;     /* 64, 128, 192 or 256 */

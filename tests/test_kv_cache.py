@@ -374,3 +374,25 @@ def test_rows_that_wrap_around_64_bits_are_refused(name, requests, stride, heads
     p = hip.kv_params(hip.Q8_0, 16, 100, kv_heads, 256, 1, requests, heads=heads, request_rows=stride)
     assert _call(name, m, p) == hip.INVALID_ARGUMENT
     assert b"rows" in hip.lib().yuuka_last_error()
+
+
+@pytest.mark.parametrize("name", ["append", "read", "attn"])
+def test_requests_do_not_overlap(name):
+    """Rows between requests are none (the rows themselves) or at least the rows: 3 here."""
+    m = _memory()
+    m.update(norm=None, rope=None)
+    for stride in (1, 2):
+        assert _call(name, m, hip.kv_params(**GOOD, heads=4, request_rows=stride)) == hip.INVALID_ARGUMENT
+        assert b"rows between requests of 3" in hip.lib().yuuka_last_error()
+    assert hip.kv_page_bytes(hip.kv_params(**GOOD, request_rows=2)) == 0
+    for stride in (0, 3):
+        assert hip.kv_page_bytes(hip.kv_params(**GOOD, request_rows=stride)) > 0
+
+
+@pytest.mark.parametrize("name", ["KV_APPEND", "KV_READ", "ATTN_DECODE", "ATTN_VERIFY"])
+def test_requests_of_an_op_do_not_overlap(name):
+    plan = _Plan()
+    bufs, n, u, flags = _ops(_memory())[name]
+    low = u[3] & 0xff
+    for stride, status in ((0, hip.OK), (1, hip.INVALID_ARGUMENT), (2, hip.INVALID_ARGUMENT), (3, hip.OK)):
+        assert plan.add(name, bufs, n, list(u[:3]) + [_U(low, 2, stride)], flags=flags) == status, stride

@@ -654,7 +654,6 @@ static yuuka_status kv_args(const yuuka_kv_params &p, bool attention, KvArgs *a)
     a->displacement = p.displacement;
     a->scale = p.scale;
     a->eps = p.eps;
-    if (p.request_rows < 0) return fail(YUUKA_ERR_INVALID_ARGUMENT, "KV cache: %d rows between requests", p.request_rows);
     return kv_check(a, p.dtype, attention);
 }
 

@@ -34,7 +34,9 @@ yuuka_status kv_check(KvArgs *a, uint32_t dtype, bool attention) {
         a->displacement > kBig)
         return fail(YUUKA_ERR_INVALID_ARGUMENT, "KV cache: %d requests of %d rows at displacement %d", a->requests,
                     a->rows, a->displacement);
-    if (a->rq_rows < a->rows) a->rq_rows = a->rows;
+    if (!a->rq_rows) a->rq_rows = a->rows;
+    if (a->rq_rows < a->rows)
+        return fail(YUUKA_ERR_INVALID_ARGUMENT, "KV cache: %d rows between requests of %d", a->rq_rows, a->rows);
     if (a->kv_heads < 1 || a->kv_heads > 4096)
         return fail(YUUKA_ERR_INVALID_ARGUMENT, "KV cache of %d heads", a->kv_heads);
     if (a->head_dim < 64 || a->head_dim % 64 || a->head_dim > 256)
