@@ -4,11 +4,13 @@ decided before anything is launched."""
 import ctypes as C
 import shutil
 import subprocess
+from dataclasses import replace
 from pathlib import Path
 
 import pytest
 
 from yuuka_amd import hip
+from yuuka_amd import model as Mdl
 
 CSRC = Path(__file__).resolve().parent.parent / "yuuka_amd" / "csrc"
 
@@ -396,3 +398,30 @@ def test_requests_of_an_op_do_not_overlap(name):
     low = u[3] & 0xff
     for stride, status in ((0, hip.OK), (1, hip.INVALID_ARGUMENT), (2, hip.INVALID_ARGUMENT), (3, hip.OK)):
         assert plan.add(name, bufs, n, list(u[:3]) + [_U(low, 2, stride)], flags=flags) == status, stride
+
+
+# ------------------------------------------------------------------ the engine
+
+def _create(**change):
+    """The status of an engine creation on a device that there is not."""
+    cfg = replace(Mdl.TINY, kv_dtype=hip.Q8_0, batch=2, **change)
+    if not hasattr(hip.lib(), "_q35_declared"):
+        Mdl._declare(hip.lib())
+        hip.lib()._q35_declared = True
+    cs, ws, layers = Mdl.config_struct(cfg), Mdl.yuuka_q35_weights(), (Mdl.yuuka_q35_layer_weights * cfg.n_layers)()
+    ws.layers = C.cast(layers, C.POINTER(Mdl.yuuka_q35_layer_weights))
+    dev, out = C.c_int32(1 << 20), C.c_void_p()  # yuuka_device starts with its index
+    return hip.lib().yuuka_q35_create(C.addressof(dev), C.byref(cs), C.byref(ws), C.byref(out))
+
+
+@pytest.mark.parametrize("change,status", [
+    (dict(head_dim=96), hip.UNSUPPORTED), (dict(head_dim=320), hip.UNSUPPORTED), (dict(head_dim=32), hip.UNSUPPORTED),
+    (dict(rope_dim=0), hip.INVALID_ARGUMENT), (dict(rope_dim=130), hip.INVALID_ARGUMENT),
+    (dict(rope_dim=31), hip.INVALID_ARGUMENT), (dict(heads=514, kv_heads=2), hip.INVALID_ARGUMENT),
+    (dict(block_size=1 << 21), hip.INVALID_ARGUMENT)])
+def test_an_engine_over_q8_0_pages_refuses_what_its_attention_does(change, status):
+    """At its creation, before a weight is uploaded, not in its first step; what is served gets as far as the device."""
+    assert _create(**change) == status
+    assert _create() == hip.DEVICE
+    # without a layer of attention there is no cache
+    assert _create(**change, full_interval=Mdl.TINY.n_layers + 1) == hip.DEVICE

@@ -691,6 +691,20 @@ yuuka_status yuuka_q35_create(yuuka_device *dev, const yuuka_q35_config *cfg, co
             return fail(YUUKA_ERR_INVALID_ARGUMENT, "invalid MoE configuration");
         if (!moe && c.ffn <= 0) return fail(YUUKA_ERR_INVALID_ARGUMENT, "dense FFN size must be positive");
         if (yk::kv_fmt_of(c.kv_dtype) < 0) return fail(YUUKA_ERR_UNSUPPORTED, "KV dtype %u", c.kv_dtype);
+        if (c.kv_dtype == YUUKA_DTYPE_Q8_0 && c.full_interval <= c.n_layers) {  // layers of attention: what their op takes
+            yk::KvArgs a{};
+            a.block_size = c.block_size;
+            a.capacity = c.capacity;
+            a.requests = c.batch;
+            a.rows = c.max_rows;
+            a.heads = c.heads;
+            a.kv_heads = c.kv_heads;
+            a.head_dim = c.head_dim;
+            a.rope_dim = c.rope_dim;
+            const yuuka_status served = yk::kv_check(&a, c.kv_dtype, true);
+            if (served != YUUKA_OK) return served;
+            if (!c.rope_dim) return fail(YUUKA_ERR_INVALID_ARGUMENT, "Q8_0 KV cache: no rotated dimensions");
+        }
         std::unique_ptr<yuuka_q35> q(new yuuka_q35());
         q->dev = dev;
         q->cfg = c;
