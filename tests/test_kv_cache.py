@@ -95,6 +95,48 @@ def test_no_table_or_position_leads_outside_the_pool(tmp_path):
     assert out.split() == ["1", "1", "0"]
 
 
+ALIGNMENT = r"""
+#include "kv_addr.h"
+#include <cstdio>
+#include <initializer_list>
+
+using namespace yk;
+
+int main() {
+    int64_t common = 0;  // of all rows' and scales' offsets
+    auto fold = [&](int64_t x) {
+        for (int64_t y = common; y;) { const int64_t r = x % y; x = y; y = r; }
+        common = x;
+    };
+    const int32_t table[] = {1, 2, 3, 4};
+    for (int fmt : {kKvF32, kKvF16, kKvQ8})
+        for (int kv_dim = 64; kv_dim <= 512; kv_dim += 64)
+            for (int block = 1; block <= 17; block++) {
+                KvLayout a{fmt, block, 4 * block, kv_dim, 5};
+                for (int p = 0; p < a.capacity; p++) {
+                    int64_t row, scales;
+                    if (!kv_slot(a, table, 0, p, &row, &scales)) return 1;
+                    fold(row);
+                    if (fmt == kKvQ8) fold(scales);
+                }
+            }
+    printf("%lld %d\n", (long long)common, kKvAlign);
+}
+"""
+
+
+def test_the_alignment_of_rows(tmp_path):
+    """What the read back's loads may ask for is what every row has, and no more."""
+    cxx = shutil.which("g++") or shutil.which("clang++")
+    if not cxx:
+        pytest.skip("no host C++ compiler")
+    src = tmp_path / "align.cpp"
+    src.write_text(ALIGNMENT)
+    subprocess.run([cxx, "-O1", "-std=c++17", "-Wall", f"-I{CSRC}", str(src), "-o", str(tmp_path / "align")], check=True)
+    out = subprocess.run([str(tmp_path / "align")], check=True, capture_output=True, text=True).stdout
+    assert out.split() == ["4", "4"]
+
+
 # Handles as the library lays them out (internal.h), over no device memory: a
 # call that gets past its checks would be refused by the missing device, with
 # another status than the ones asked for here.

@@ -86,7 +86,8 @@ __device__ __forceinline__ LaneDims lane_dims(int lane) {
 constexpr int heads_per_wave(int groups) { return groups == 1 ? 4 : groups == 2 ? 2 : 1; }
 
 typedef float floats4 __attribute__((ext_vector_type(4), aligned(4)));  // rows are 4-byte aligned
-typedef uint32_t dwords4 __attribute__((ext_vector_type(4)));
+typedef uint32_t dwords4 __attribute__((ext_vector_type(4), aligned(4)));  // Q8_0 pages start at any dword
+static_assert(alignof(dwords4) <= kKvAlign, "a row's loads need more than a row has");
 
 // ref_f32_to_f16, short for what becomes a normal half.
 __device__ __forceinline__ uint32_t f32_to_f16(float f) {

@@ -23,6 +23,9 @@ namespace yk {
 // have one scale each key; in the natural order the 16 columns of a tile
 // would be spread over all the scales.
 constexpr int kKvF32 = 0, kKvF16 = 1, kKvQ8 = 2;
+// Rows and scales start at multiples of these bytes, whatever the shape: a Q8_0 page
+// of one token of 64 dims is 68 bytes.
+constexpr int kKvAlign = 4;
 
 struct KvLayout {
     int fmt;
