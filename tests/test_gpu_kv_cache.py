@@ -953,3 +953,43 @@ def test_engine_over_a_q8_0_cache(dev):
     assert np.array_equal(got[:4], got[4:])
     eng.close()
     orc.close()
+
+
+# ----------------------------------------------- keys and values that are not finite
+
+ODD = [  # heads, kv heads, head width, page, rows, context: one operand for both halves, one and two blocks a wave, ...
+    (4, 2, 128, 16, 3, 90),
+    (8, 2, 128, 16, 3, 90),
+    (16, 4, 128, 16, 8, 500),
+    (8, 2, 64, 64, 9, 40),
+    (6, 2, 192, 16, 4, 200),
+    (8, 2, 256, 16, 6, 1500),   # several parts
+    (8, 2, 256, 16, 2, 64),
+    (8, 2, 128, 48, 5, 300),    # pages of no power of two
+]
+
+
+@pytest.mark.parametrize("dtype", [Q8, F16])
+@pytest.mark.parametrize("bad", [np.inf, -np.inf, np.nan, 1e10])
+@pytest.mark.parametrize("heads,nk,D,bs,rows,context", ODD)
+def test_a_value_that_is_not_finite_keeps_to_its_dims(dev, stream, dtype, bad, heads, nk, D, bs, rows, context):
+    """In the rows that see it, its dim (F16) or its block of 32 dims (Q8_0), wherever its token lies: among the newest
+    rows, where some see it and some do not, before them, and long before."""
+    ends = [context + rows // 2, context + rows - 1, context, context - 1, context // 2, 0]
+    c = Cache(dev, dtype, bs, context + rows + 2, nk, D, len(ends), [context] * len(ends), seed=D,
+              fill=q8_fill() if dtype == Q8 else f16_fill)
+    for j, p in enumerate(ends):
+        row = c.row(1, j, p).copy()
+        row[D + 40] = bad   # of the second kv head
+        c.put(1, j, p, row)
+    c.upload()
+    q = np.random.default_rng(rows).normal(0, 1, (len(ends) * rows, heads, D)).astype(np.float32)
+    o = dev.upload(np.full(q.shape, 2.5, np.float32))
+    hip.attn_decode(stream, o, dev.upload(q), *c.b_pool, c.b_table, c.b_pos, c.params(rows, heads=heads, scale=D ** -0.5))
+    stream.sync()
+    got, want = o.read(np.float32).reshape(q.shape), attention(c, q, rows, heads, D ** -0.5, False)
+    width = 32 if dtype == Q8 else 1
+    for j, p in enumerate(ends):
+        seen = sum(context + r >= p for r in range(rows))
+        assert (~np.isfinite(want[j * rows:(j + 1) * rows])).sum() == seen * heads // nk * width
+        close(got[j * rows:(j + 1) * rows], want[j * rows:(j + 1) * rows])

@@ -147,6 +147,18 @@ __device__ __forceinline__ half2v value_halves(u32x2 x, u32x2 y) {
     return __builtin_bit_cast(half2v, __builtin_amdgcn_perm(y[J >> 1], x[J >> 1], J & 1 ? 0x07060302u : 0x05040100u));
 }
 
+// The lane's number, worked out where it stands. What is rarely used and kept over the loop is spilled,
+// and a reload waits for all loads in flight.
+__device__ __forceinline__ int lane_anew() {
+    int zero = 0;
+    asm volatile("" : "+v"(zero));
+    return __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, zero));
+}
+// Two halves, zeros in the place of infinities and NaN.
+__device__ __forceinline__ uint32_t finite_halves(uint32_t x) {
+    return ((x & 0x7c00u) == 0x7c00u ? 0u : x & 0xffffu) | ((x & 0x7c000000u) == 0x7c000000u ? 0u : x & 0xffff0000u);
+}
+
 template <int FMT, int GROUPS, bool STACK, bool PAGED, int RB> struct Layout {
     static constexpr bool Q8 = FMT == kKvQ8;
     static constexpr int D = 64 * GROUPS, NB = 2 * GROUPS, PER = STACK ? 8 : 16, ROWS = PER * RB;
@@ -156,8 +168,9 @@ template <int FMT, int GROUPS, bool STACK, bool PAGED, int RB> struct Layout {
     static constexpr uint32_t loop = addr + (PAGED ? 0 : kWaves * 256);
     static constexpr int slot_row = D + 4;                                    // floats; rows 4 g land 16 banks apart
     static constexpr uint32_t slots = kWaves * PER * slot_row * 4;            // over the loop's areas, after it
-    static constexpr uint32_t stats = loop > slots ? loop : slots;            // m and l [wave][16], factor[ROWS]
-    static constexpr uint32_t total = stats + (2 * kWaves + RB) * 16 * 4;
+    static constexpr uint32_t stats = loop > slots ? loop : slots;            // m and l [wave][16], factor[ROWS], late[wave]
+    static constexpr uint32_t late = stats + (2 * kWaves + RB) * 16 * 4;
+    static constexpr uint32_t total = late + kWaves * 4;
 };
 
 // How the work is cut. A "column" is one (row block, kv head) of a request; a
@@ -327,6 +340,9 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(wav
     float *const st_m = reinterpret_cast<float *>(lds + L::stats), *const st_l = st_m + kWaves * 16;
     float *const row_factor = st_l + kWaves * 16;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    // the wave's values that are not finite, and that not every row sees, were taken as zeros (in LDS, which
+    // costs the loop no register)
+    auto late = [&]() -> int & { return *reinterpret_cast<int *>(lds + L::late + 4 * wave); };
     const int r16 = lane & 15, g4 = lane >> 4;
     // Workgroups go to the eight XCDs in turn. Each XCD gets one run of the work
     // items in the order (row block, kv head, part, request), so that what
@@ -370,7 +386,8 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(wav
     const int64_t out_row = (int64_t)j * a.rq_rows;
     if (plan && split == 0 && column == 0 && threadIdx.x == 0) plan[j] = make_int2(parts, pt.record);
     if (c0 >= c1 && parts > 1) {  // nothing here: empty records
-        if (threadIdx.x < (uint32_t)nr) stats[record + threadIdx.x] = make_float2(-INFINITY, 0.0f);
+        const int tid = 64 * wave + lane_anew();
+        if (tid < nr) stats[record + tid] = make_float2(-INFINITY, 0.0f);
         return;
     }
 
@@ -565,6 +582,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(wav
         // query. (Products are below 2^45: times 2^-126 they are nothing to the exponential.)
         if (lane == 0) row_factor[n] = fmaxf(ldexpf(fabsf(a.scale) * 1.44269504088896341f, e - 14), 0x1p-126f);
     }
+    late() = 0;
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
@@ -599,7 +617,6 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(wav
         // every row sees every key of the tile
         const bool whole = cur.keys == ~0u && kTile * c + kTile - 1 <= least;
         float E = 0.0f;
-        uint32_t poison = 0;  // keys with a non-finite value that not every row sees: left out, their rows made NaN
         if constexpr (Q8) {
             // scales to LDS (those of missing keys as zeros), and the largest finite value scale's exponent
             wave_lds_fence();
@@ -621,12 +638,12 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(wav
                     most = max(most, max(lo < 0x7c00u ? lo : 0u, hi < 0x7c00u ? hi : 0u));
                 }
             }
-            if (!whole) {
-                uint64_t b = __builtin_amdgcn_ballot_w64(over && kTile * c + (lane & 31) > least);
-                poison = (uint32_t)(b >> 32);
-                if (__builtin_amdgcn_inverse_ballot_w64((uint64_t)poison << 32)) {
+            if (!whole && __any(over)) {  // a value's scale that not every row sees
+                const bool put_off = over && lane_anew() >= 32 && kTile * c + (lane_anew() & 31) > least;
+                if (__any(put_off)) late() = 1;
+                if (put_off) {
 #pragma unroll
-                    for (int s = 0; s < GROUPS; s++) d[s] = 0;
+                    for (int s = 0; s < GROUPS; s++) d[s] = finite_halves(d[s]);
                 }
             }
 #pragma unroll
@@ -701,30 +718,35 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(wav
                     if constexpr (STACK) s[n][T][e] += ror8(s[n][T][e]);
                 }
         if (!whole) {
-            int first = 4 * g4;  // opaque: what follows is not kept in registers for every tile
-            asm volatile("" : "+v"(first));
+            const int first = 4 * (lane_anew() >> 4);  // (what follows is not kept in registers for every tile)
+            int off = 0;
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 const int kk = first + 16 * (i >> 2) + (i & 3);
-                bool there = (cur.keys >> kk) & 1, bad = (poison >> kk) & 1;
+                const bool there = (cur.keys >> kk) & 1;
                 if constexpr (!Q8) {  // values that not every row sees must be finite for those that do not
                     uint32_t over = 0;
 #pragma unroll
                     for (int u = 0; u < GROUPS; u++)
 #pragma unroll
                         for (int w = 0; w < 2; w++) over |= (vhalf[i][u][w] & 0x7fff7fffu) + 0x04000400u;
-                    const uint64_t b = __builtin_amdgcn_ballot_w64((over & 0x80008000u) != 0);
-                    bad = ((b >> (4 * first)) & 0xffffu) != 0 && kTile * c + kk > least;
-                    if (!there || bad) {
+                    const bool put_off = there && (over & 0x80008000u) != 0 && kTile * c + kk > least;
+                    off |= put_off;
+                    if (!there || put_off) {
 #pragma unroll
-                        for (int u = 0; u < GROUPS; u++) vhalf[i][u] = u32x2{0, 0};
+                        for (int u = 0; u < GROUPS; u++)
+#pragma unroll
+                            for (int w = 0; w < 2; w++) vhalf[i][u][w] = there ? finite_halves(vhalf[i][u][w]) : 0u;
                     }
                 }
 #pragma unroll
                 for (int n = 0; n < RB; n++) {
                     const bool seen = there && kTile * c + kk <= my_limit[n];
-                    s[n][i >> 2][i & 3] = !seen ? -INFINITY : bad ? NAN : s[n][i >> 2][i & 3];
+                    s[n][i >> 2][i & 3] = seen ? s[n][i >> 2][i & 3] : -INFINITY;
                 }
+            }
+            if constexpr (!Q8) {
+                if (__any(off)) late() = 1;
             }
         }
         float p[RB][8];
@@ -843,65 +865,90 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(wav
         if constexpr (PAGED) next = after;
     }
 
-    // ---- the waves' outputs joined: o = sum_w 2^(ref_w - max ref) o_w
+    {
+        const int lane = lane_anew(), r16 = lane & 15, g4 = lane >> 4, tid = 64 * wave + lane;
+        // ---- the values put off: their dims of the rows that see them are not finite, as where every row does
+        if (least + 1 < len && __builtin_amdgcn_readfirstlane(late())) {
+            KvLayout cache = a;
+            asm volatile("" : "+s"(cache.block_size));  // (its reciprocal is not kept over the loop either)
+            for (int key = max(least + 1, kTile * c0); key < min(len, kTile * c1); key++) {
+                int64_t row, sc;
+                if ((key / kTile - c0) % kWaves != wave || !kv_slot(cache, table, j, key, &row, &sc)) continue;
+                const uint16_t *const halves = reinterpret_cast<const uint16_t *>(vpool + (Q8 ? sc : row)) + kvh * (Q8 ? NB : D);
 #pragma unroll
-    for (int b = 0; b < RB; b++) {
-        if (b * PER >= nr) break;
-        l[b] = sum_rows(l[b]);
-        __syncthreads();  // every wave is done with what the slots lie over
-        float *const slot = reinterpret_cast<float *>(lds) + wave * PER * L::slot_row;
-        const float unit = Q8 ? 512.0f : 1.0f;  // the digits were times 2^-9
-        auto dim = [&](int u, int t) { return 64 * u + (Q8 ? 16 * t + r16 : 4 * r16 + t); };
+                for (int u = 0; u < GROUPS; u++)
 #pragma unroll
-        for (int u = 0; u < GROUPS; u++)
+                    for (int t = 0; t < 4; t++) {
+                        const bool bad = (halves[Q8 ? 2 * u + (t >> 1) : 64 * u + 4 * r16 + t] & 0x7c00u) == 0x7c00u;
 #pragma unroll
-            for (int t = 0; t < 4; t += STACK ? 2 : 1)
+                        for (int b = 0; b < RB; b++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    if constexpr (STACK) {
-                        // rows n and n + 8, 32 lanes apart: one swap puts t's two halves and t + 1's
-                        // side by side, their sums in the lower and the upper lanes
-                        const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(acc[b][u][t][e]),
-                                                                        __float_as_uint(acc[b][u][t + 1][e]), false, false);
-                        slot[(4 * (g4 & 1) + e) * L::slot_row + dim(u, t) + (Q8 ? 16 : 1) * (g4 >> 1)] =
-                            (__uint_as_float(x[0]) + __uint_as_float(x[1])) * unit;
-                    } else {
-                        slot[(4 * g4 + e) * L::slot_row + dim(u, t)] = acc[b][u][t][e] * unit;
+                            for (int e = 0; e < 4; e++)
+                                if (__shfl(my_limit[b], 4 * g4 + e) >= key && bad) acc[b][u][t][e] = NAN;
                     }
-                }
-        if (lane < PER) {
-            st_m[wave * 16 + lane] = ref[b];
-            st_l[wave * 16 + lane] = l[b];
-        }
-        __syncthreads();
-        for (int idx = threadIdx.x; idx < min(PER, nr - b * PER) * (D / 4); idx += 64 * kWaves) {
-            const int m16 = idx / (D / 4), n = b * PER + m16, d = 4 * (idx % (D / 4));
-            float m = -INFINITY;
-#pragma unroll
-            for (int w = 0; w < kWaves; w++) m = fmaxf(m, st_m[w * 16 + m16]);
-            f32x4 o = {0.f, 0.f, 0.f, 0.f};
-            float total = 0.0f;
-#pragma unroll
-            for (int w = 0; w < kWaves; w++) {
-                const float mw = st_m[w * 16 + m16];
-                const float f = mw == m ? 1.0f : __builtin_amdgcn_exp2f(mw - m);
-                const f32x4 x = *reinterpret_cast<const f32x4 *>(lds + ((w * PER + m16) * L::slot_row + d) * 4);
-                o += f * x;
-                total = fmaf(f, st_l[w * 16 + m16], total);
             }
-            const int r = row_of(n0 + n), h = kvh * G + n0 + n - r * G;
-            if (parts == 1) {
-                const int64_t at = (out_row + r) * a.heads + h;
-                const float inv = 1.0f / total;
+        }
+
+        // ---- the waves' outputs joined: o = sum_w 2^(ref_w - max ref) o_w
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    float y = total == 0.0f ? 0.0f : o[i] * inv;  // a row that sees no key
-                    if (gate) y *= sigmoid_ref(gate[at * gate_stride + d + i]);
-                    out[at * D + d + i] = y;
+        for (int b = 0; b < RB; b++) {
+            if (b * PER >= nr) break;
+            l[b] = sum_rows(l[b]);
+            __syncthreads();  // every wave is done with what the slots lie over
+            float *const slot = reinterpret_cast<float *>(lds) + wave * PER * L::slot_row;
+            const float unit = Q8 ? 512.0f : 1.0f;  // the digits were times 2^-9
+            auto dim = [&](int u, int t) { return 64 * u + (Q8 ? 16 * t + r16 : 4 * r16 + t); };
+#pragma unroll
+            for (int u = 0; u < GROUPS; u++)
+#pragma unroll
+                for (int t = 0; t < 4; t += STACK ? 2 : 1)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        if constexpr (STACK) {
+                            // rows n and n + 8, 32 lanes apart: one swap puts t's two halves and t + 1's
+                            // side by side, their sums in the lower and the upper lanes
+                            const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(acc[b][u][t][e]),
+                                                                            __float_as_uint(acc[b][u][t + 1][e]), false, false);
+                            slot[(4 * (g4 & 1) + e) * L::slot_row + dim(u, t) + (Q8 ? 16 : 1) * (g4 >> 1)] =
+                                (__uint_as_float(x[0]) + __uint_as_float(x[1])) * unit;
+                        } else {
+                            slot[(4 * g4 + e) * L::slot_row + dim(u, t)] = acc[b][u][t][e] * unit;
+                        }
+                    }
+            if (lane < PER) {
+                st_m[wave * 16 + lane] = ref[b];
+                st_l[wave * 16 + lane] = l[b];
+            }
+            __syncthreads();
+            for (int idx = tid; idx < min(PER, nr - b * PER) * (D / 4); idx += 64 * kWaves) {
+                const int m16 = idx / (D / 4), n = b * PER + m16, d = 4 * (idx % (D / 4));
+                float m = -INFINITY;
+#pragma unroll
+                for (int w = 0; w < kWaves; w++) m = fmaxf(m, st_m[w * 16 + m16]);
+                f32x4 o = {0.f, 0.f, 0.f, 0.f};
+                float total = 0.0f;
+#pragma unroll
+                for (int w = 0; w < kWaves; w++) {
+                    const float mw = st_m[w * 16 + m16];
+                    const float f = mw == m ? 1.0f : __builtin_amdgcn_exp2f(mw - m);
+                    const f32x4 x = *reinterpret_cast<const f32x4 *>(lds + ((w * PER + m16) * L::slot_row + d) * 4);
+                    o += f * x;
+                    total = fmaf(f, st_l[w * 16 + m16], total);
                 }
-            } else {
-                *reinterpret_cast<f32x4 *>(part + (record + n) * D + d) = o;
-                if (d == 0) stats[record + n] = make_float2(m, total);
+                const int r = row_of(n0 + n), h = kvh * G + n0 + n - r * G;
+                if (parts == 1) {
+                    const int64_t at = (out_row + r) * a.heads + h;
+                    const float inv = 1.0f / total;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        float y = total == 0.0f ? 0.0f : o[i] * inv;  // a row that sees no key
+                        if (gate) y *= sigmoid_ref(gate[at * gate_stride + d + i]);
+                        out[at * D + d + i] = y;
+                    }
+                } else {
+                    *reinterpret_cast<f32x4 *>(part + (record + n) * D + d) = o;
+                    if (d == 0) stats[record + n] = make_float2(m, total);
+                }
             }
         }
     }
