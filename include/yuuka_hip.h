@@ -612,8 +612,10 @@ YUUKA_API yuuka_status yuuka_kv_read(yuuka_stream * stream, yuuka_buffer * k_out
  *   out[h] = sum_t softmax_t(scale q[h] . k_t) v_t [* sigmoid(gate[h])]
  * with kv head h / (heads / kv_heads). q is [.][heads][head_dim] FP32, or
  * [.][heads][2 * head_dim] holding [q | gate]; out [.][heads][head_dim]. F16 and
- * Q8_0 pools. At most 4096 rows. A row that sees no key is zero. A non-finite
- * query or visible key or value makes its rows NaN. */
+ * Q8_0 pools. At most 4096 rows. A row that sees no key is zero. A query that is
+ * not finite makes its row NaN, and so does any key that the row sees, the score's
+ * sign whatever it is. A value that is not finite makes its dim (F16) or its block of
+ * 32 dims (Q8_0) of the rows that see it infinite or NaN, and no other. */
 YUUKA_API yuuka_status yuuka_attn_decode(yuuka_stream * stream, yuuka_buffer * out, const yuuka_buffer * q,
                         const yuuka_buffer * kpool, const yuuka_buffer * vpool, const yuuka_buffer * table,
                         const yuuka_buffer * positions, const yuuka_kv_params * params, yuuka_event * completion);

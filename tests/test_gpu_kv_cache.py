@@ -993,3 +993,37 @@ def test_a_value_that_is_not_finite_keeps_to_its_dims(dev, stream, dtype, bad, h
         seen = sum(context + r >= p for r in range(rows))
         assert (~np.isfinite(want[j * rows:(j + 1) * rows])).sum() == seen * heads // nk * width
         close(got[j * rows:(j + 1) * rows], want[j * rows:(j + 1) * rows])
+
+
+@pytest.mark.parametrize("dtype", [Q8, F16])
+@pytest.mark.parametrize("heads,nk,D,bs,rows,context", ODD)
+def test_a_key_that_is_not_finite_makes_its_rows_nan(dev, stream, dtype, heads, nk, D, bs, rows, context):
+    """Whether its score would be an infinity of either sign or a NaN: the rows that see it, of its kv head."""
+    rng = np.random.default_rng(rows)
+    ends = [context + rows // 2, context + rows - 1, context - 1, context // 2, 0, None]
+    c = Cache(dev, dtype, bs, context + rows + 2, nk, D, len(ends), [context] * len(ends), seed=D,
+              fill=q8_fill() if dtype == Q8 else f16_fill)
+    q = rng.normal(0, 1, (len(ends) * rows, heads, D)).astype(np.float32)
+    # dim 17: both halves of the query are of one sign, which differs between the heads
+    q[..., 17] = np.where(np.arange(heads) % 2, 1, -1) * np.float32(1 + 2.0 ** -12)
+    scale = np.float32(D ** -0.5)
+    for j, p in enumerate(ends):
+        for t in range(context + rows) if p is None else [p]:  # the last request: every key
+            row = c.row(0, j, t).copy()
+            if dtype == Q8:
+                row[D:D + 32] *= 1e12   # an infinite scale, digits of both signs
+            else:
+                row[D + 17] = -np.inf
+            c.put(0, j, t, row)
+    c.upload()
+    want = attention(c, q, rows, heads, scale, False)
+    for j, p in enumerate(ends):
+        for r in range(rows):
+            if p is None or context + r >= p:
+                want[j * rows + r, heads // nk:2 * heads // nk] = np.nan
+    o = dev.upload(np.full(q.shape, 2.5, np.float32))
+    hip.attn_decode(stream, o, dev.upload(q), *c.b_pool, c.b_table, c.b_pos, c.params(rows, heads=heads, scale=scale))
+    stream.sync()
+    got = o.read(np.float32).reshape(q.shape)
+    assert np.array_equal(np.isnan(got), np.isnan(want))
+    close(got, want)

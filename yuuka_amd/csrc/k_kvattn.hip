@@ -636,6 +636,8 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(wav
                 for (int s = 0; s < GROUPS; s++) {
                     const uint32_t lo = d[s] & 0x7fffu, hi = (d[s] >> 16) & 0x7fffu;
                     most = max(most, max(lo < 0x7c00u ? lo : 0u, hi < 0x7c00u ? hi : 0u));
+                    // infinities become NaN: with one, a score could be -infinity and leave its key out
+                    d[s] |= (lo < 0x7c00u ? 0u : 0x200u) | (hi < 0x7c00u ? 0u : 0x2000000u);
                 }
             }
             if (!whole && __any(over)) {  // a value's scale that not every row sees
@@ -716,6 +718,9 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(wav
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     if constexpr (STACK) s[n][T][e] += ror8(s[n][T][e]);
+                    // An infinite score, of a key that holds one (others are below 2^45), becomes NaN:
+                    // one of -infinity would leave its key out.
+                    if constexpr (!Q8) s[n][T][e] = fmaf(s[n][T][e], 0.0f, s[n][T][e]);
                 }
         if (!whole) {
             const int first = 4 * (lane_anew() >> 4);  // (what follows is not kept in registers for every tile)
