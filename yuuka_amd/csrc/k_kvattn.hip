@@ -724,7 +724,6 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(wav
                 }
         if (!whole) {
             const int first = 4 * (lane_anew() >> 4);  // (what follows is not kept in registers for every tile)
-            int off = 0;
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 const int kk = first + 16 * (i >> 2) + (i & 3);
@@ -736,12 +735,18 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(wav
 #pragma unroll
                         for (int w = 0; w < 2; w++) over |= (vhalf[i][u][w] & 0x7fff7fffu) + 0x04000400u;
                     const bool put_off = there && (over & 0x80008000u) != 0 && kTile * c + kk > least;
-                    off |= put_off;
-                    if (!there || put_off) {
+                    if (__any(put_off)) {
+                        late() = 1;
+                        if (put_off) {
 #pragma unroll
-                        for (int u = 0; u < GROUPS; u++)
+                            for (int u = 0; u < GROUPS; u++)
 #pragma unroll
-                            for (int w = 0; w < 2; w++) vhalf[i][u][w] = there ? finite_halves(vhalf[i][u][w]) : 0u;
+                                for (int w = 0; w < 2; w++) vhalf[i][u][w] = finite_halves(vhalf[i][u][w]);
+                        }
+                    }
+                    if (!there) {
+#pragma unroll
+                        for (int u = 0; u < GROUPS; u++) vhalf[i][u] = u32x2{0, 0};
                     }
                 }
 #pragma unroll
@@ -749,9 +754,6 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(wav
                     const bool seen = there && kTile * c + kk <= my_limit[n];
                     s[n][i >> 2][i & 3] = seen ? s[n][i >> 2][i & 3] : -INFINITY;
                 }
-            }
-            if constexpr (!Q8) {
-                if (__any(off)) late() = 1;
             }
         }
         float p[RB][8];
