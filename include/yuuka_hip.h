@@ -552,9 +552,10 @@ YUUKA_API yuuka_status yuuka_moe_pack_q4k(yuuka_stream * stream, yuuka_buffer * 
  * the v10 KV writes). A Q8_0 page is [block_size][kv_dim] int8 digits followed
  * by [block_size][kv_dim / 32] F16 scales; a value is digit * scale of its block
  * of 32 dims. Every 64 dims' digits are stored as a 16 x 4 matrix: byte
- * 4 r + j of the 64 holds dim 16 j + r. Rounding, in FP32 (kv_format.go:93-137
- * up to the last bit of s): s = max|x| * (1 / 127), scale = F16(s), half up;
- * digit = x / s to the nearest, halves away from zero. A block holding a NaN
+ * 4 r + j of the 64 holds dim 16 j + r. Rounding, in FP32: s = max|x| * (1 / 127),
+ * scale = F16(s), half up; digit = x / s to the nearest, halves away from zero.
+ * (kv_format.go:93-137 divides by 127: the last bit of s differs in one block of
+ * 23, and with it one digit in 7 million, by one.) A block holding a NaN
  * reads back as NaN, one past the scale's range (|x| over 8.3e6) as infinities
  * and NaN.
  *

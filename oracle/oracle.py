@@ -229,6 +229,7 @@ def _declare_q35(L):
     sig = {
         "orc_q35_pool_new": (vp, [C.POINTER(orc_q35_config), i32, i32, i32]),
         "orc_q35_pool_free": (None, [vp]),
+        "orc_kv_encode_row": (None, [i32, vp, vp, i32]),
         "orc_q35_pool_data": (vp, [vp, i32, i32, C.POINTER(C.c_uint64)]),
         "orc_q35_state_new": (vp, [C.POINTER(orc_q35_config), vp, vp, i32, i32]),
         "orc_q35_state_free": (None, [vp]),
@@ -246,6 +247,19 @@ def _declare_q35(L):
     for name, (res, args) in sig.items():
         fn = getattr(L, name)
         fn.restype, fn.argtypes = res, args
+
+
+def kv_encode_rows(x) -> tuple[np.ndarray, np.ndarray]:
+    """Rows as the reference's Q8_0 cache holds them: int8 digits [rows][n] and half scales' bits [rows][n / 32]."""
+    L = lib()
+    if not hasattr(L, "_q35_declared"):
+        _declare_q35(L)
+        L._q35_declared = True
+    x = np.ascontiguousarray(x, np.float32)
+    out = np.zeros((x.shape[0], x.shape[1] // 32, 34), np.uint8)
+    for row, to in zip(x, out):
+        L.orc_kv_encode_row(2, _ptr(to), _ptr(row), row.size)
+    return out[..., 2:].reshape(x.shape).view(np.int8), np.ascontiguousarray(out[..., :2]).view(np.uint16)[..., 0]
 
 
 def _mat(t):

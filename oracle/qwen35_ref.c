@@ -186,6 +186,8 @@ static void encode_row(int32_t format, uint8_t *dst, const float *src, int32_t n
     }
 }
 
+void orc_kv_encode_row(int32_t format, uint8_t *dst, const float *src, int32_t n) { encode_row(format, dst, src, n); }
+
 /* kv_format.go:140-168 DecodeRow */
 static void decode_row(int32_t format, float *dst, const uint8_t *src, int32_t n) {
     if (format == 0) {

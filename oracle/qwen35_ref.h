@@ -91,6 +91,8 @@ void orc_q35_pool_free(orc_q35_pool *pool);
 /* Raw stored bytes of layer's K (which=0) or V (which=1) rows, or NULL. */
 uint8_t *orc_q35_pool_data(orc_q35_pool *pool, int32_t layer, int32_t which, uint64_t *bytes);
 int32_t orc_q35_pool_row_bytes(const orc_q35_pool *pool);
+/* One cached row of n values in the pool's format (kv_format.go:93-137 EncodeRow). */
+void orc_kv_encode_row(int32_t format, uint8_t *dst, const float *src, int32_t n);
 
 /* model/qwen35/state.go:104-169 NewPagedState: binds a block table (copied)
  * mapping ceil(capacity/block_size) logical blocks to pool blocks. */

@@ -1027,3 +1027,47 @@ def test_a_key_that_is_not_finite_makes_its_rows_nan(dev, stream, dtype, heads, 
     got = o.read(np.float32).reshape(q.shape)
     assert np.array_equal(np.isnan(got), np.isnan(want))
     close(got, want)
+
+
+# ----------------------------------------------------------- the reference's codec
+
+def test_append_next_to_the_references_quotient(dev, stream):
+    """The cached bytes are those of the reference's codec, which takes s as max / 127 where the append takes max * (1 / 127),
+    but for what the last bits of s decide. Each s is within 2^-24 (the quotient) and 2 * 2^-24 (the constant and the
+    product) of max / 127, so that they differ by at most 3 * 2^-24 of it: the stored halves differ only where max / 127 is
+    that close to the middle of two. x / s is rounded to 2^-24 again, twice 2^-24 for the pair: two digits differ, by one,
+    only where x / s, up to 128, is within 5 * 128 * 2^-24 of a half."""
+    rng = np.random.default_rng(9)
+    x = rng.normal(0, 1, (600, 2, 256)) * np.exp(rng.normal(0, 2, (600, 2, 1)))
+    special = _special_blocks()
+    special = special[np.isfinite(special).all(1) & (np.abs(special).max(1) > 2.0 ** -100)]
+    special = special[:len(special) // 8 * 8].reshape(-1, 256)
+    x[0, 0, :32] = 0
+    x = np.concatenate([x.reshape(-1, 256).astype(np.float32), special])
+    c = Cache(dev, Q8, 16, len(x), 2, 128, 1, [0])
+    hip.kv_append(stream, dev.upload(x), dev.upload(x), *c.b_pool, c.b_table, c.b_pos, c.params(len(x)))
+    stream.sync()
+    c.pool = [c.read_pool(0), c.read_pool(1)]
+    assert np.array_equal(*c.pool)
+    n = c.kvd
+    digits, scales = np.zeros(x.shape, np.int8), np.zeros((len(x), n // 32), np.uint16)
+    for p in range(len(x)):
+        page, t = c.at(0, p)
+        stored = c.pool[0][page, t * n:(t + 1) * n].view(np.int8)
+        digits[p] = stored.reshape(-1, 16, 4).swapaxes(1, 2).reshape(-1)
+        scales[p] = c.pool[0][page, 16 * n + t * n // 16:16 * n + (t + 1) * n // 16].copy().view(np.uint16)
+    want_digits, want_scales = O.kv_encode_rows(x)
+    s = np.abs(x.astype(np.float64)).reshape(len(x), -1, 32).max(2) / 127
+    other = scales != want_scales
+    low = np.minimum(scales, want_scales)
+    assert (np.maximum(scales, want_scales) - low)[other].max(initial=0) <= 1
+    with np.errstate(over="ignore", invalid="ignore"):
+        middle = (low.view(np.float16).astype(np.float64) + (low + 1).astype(np.uint16).view(np.float16)) / 2
+    assert (np.abs(s - middle)[other] <= 3 * 2.0 ** -24 * s[other]).all()
+    with np.errstate(invalid="ignore"):
+        t = np.abs(x.astype(np.float64)).reshape(*s.shape, 32) / s[..., None]
+    other = (digits != want_digits).reshape(t.shape)
+    assert np.abs(digits.astype(int) - want_digits).max() <= 1
+    assert (np.abs(t - np.floor(t) - 0.5)[other] <= 5 * 128 * 2.0 ** -24).all()
+    ordinary = np.arange(len(x)) < 1200
+    assert (digits == want_digits)[ordinary].mean() > 0.99999 and (scales == want_scales)[ordinary].mean() > 0.999

@@ -6,10 +6,13 @@
 //   scale = max|x| * (1 / 127), stored as F16 (half up, as every F16 of the cache)
 //   digit = x / scale to the nearest, halves away from zero; 0 where scale is 0
 //   value = digit * F16 scale (exact in float32: 7 + 11 significant bits)
-// The reference's EncodeRow (kv_format.go:93-137) divides max|x| by 127: the
-// product's last bit differs in one block of 22, which moves one digit in a
-// million by a step. A value is off by at most half a step, scale / 2, and by
-// |x| 2^-11 for the scale's own rounding.
+// The reference's EncodeRow (kv_format.go:93-137) divides max|x| by 127. The product is what
+// torch computes for that division on the GPU (a constant divisor is inverted first), so that
+// pages written from there and from here hold the same bytes; it is as near to max / 127 for
+// what is cached. Over normal values its last bit differs from the quotient's in one block of
+// 23, a stored scale in one block of 2.5 million and a digit, by one, in one value of 7 million,
+// only where x / scale is within 5 * 2^-17 of a half. A value is off by at most half a step,
+// scale / 2, and by |x| 2^-11 for the scale's own rounding.
 // A block that holds a NaN has a NaN scale (the reference leaves that case
 // undefined), so that it reads back as NaN instead of as finite values.
 #include <hip/hip_runtime.h>
