@@ -1071,3 +1071,37 @@ def test_append_next_to_the_references_quotient(dev, stream):
     assert (np.abs(t - np.floor(t) - 0.5)[other] <= 5 * 128 * 2.0 ** -24).all()
     ordinary = np.arange(len(x)) < 1200
     assert (digits == want_digits)[ordinary].mean() > 0.99999 and (scales == want_scales)[ordinary].mean() > 0.999
+
+
+def test_two_captures_of_one_plan_at_once(dev, stream):
+    """The second capture, of the plan after it grew, runs what the first does and more; both fill the shared output with
+    the same values, so that only a workspace in common could make them wrong."""
+    heads, nk, D, rounds = 8, 2, 128, 12
+    s2 = hip.Stream(dev)
+    rng = np.random.default_rng(1)
+    plan, caches, outs, wants = hip.Plan(dev), [], [], []
+    streams, graphs = (stream, s2), []
+    for positions, s in zip(([2900, 1500], [700, 2600]), streams):
+        c = Cache(dev, Q8, 16, 3000, nk, D, 2, positions, seed=positions[0], fill=q8_fill())
+        q = rng.normal(0, 1, (2, heads, D)).astype(np.float32)
+        o = dev.upload(np.zeros(q.shape, np.float32))
+        plan.add(hip.OP["ATTN_DECODE"], [dev.upload(q), *c.b_pool, o, c.b_table] + [None] * 10 + [c.b_pos],
+                 n=[nk, heads, D, c.kvd, 1, 0], u=[16, 3000, Q8, 2 << 8], f=[D ** -0.5], flags=hip.FLAG_OWN_POS)
+        graphs.append(hip.Graph(plan, s, None))
+        caches.append(c)
+        outs.append(o)
+        wants.append(attention(c, q, 1, heads, D ** -0.5, False))
+    for _ in range(rounds):
+        for o in outs:
+            o.write(np.full(wants[0].shape, np.nan, np.float32))
+        for _ in range(8):
+            for g, s in zip(graphs, streams):
+                g.replay(s)
+        stream.sync()
+        s2.sync()
+        for o, w in zip(outs, wants):
+            close(o.read(np.float32).reshape(w.shape), w)
+    for g in graphs:
+        g.destroy()
+    plan.destroy()
+    s2.destroy()
