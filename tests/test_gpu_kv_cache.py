@@ -1105,3 +1105,21 @@ def test_two_captures_of_one_plan_at_once(dev, stream):
         g.destroy()
     plan.destroy()
     s2.destroy()
+
+
+@pytest.mark.parametrize("dtype", [Q8, F16])
+@pytest.mark.parametrize("requests,heads,nk,D,rows", [(260, 16, 4, 256, 1), (52, 16, 4, 256, 17), (520, 8, 4, 64, 1)])
+def test_one_long_request_among_more_than_are_cut(dev, stream, dtype, requests, heads, nk, D, rows):
+    """So many requests that each is one part, whatever its length."""
+    longest = 2500
+    positions = np.random.default_rng(D).integers(0, 30, requests)
+    positions[requests // 3] = longest
+    c = Cache(dev, dtype, 64, longest + rows, nk, D, requests, positions, seed=rows, shared=True,
+              pages=-(-(longest + rows) // 64) + 2, fill=q8_fill() if dtype == Q8 else f16_fill)
+    q = np.random.default_rng(2).normal(0, 1, (requests * rows, heads, D)).astype(np.float32)
+    o = dev.upload(np.full(q.shape, 7.5, np.float32))
+    hip.attn_decode(stream, o, dev.upload(q), *c.b_pool, c.b_table, c.b_pos, c.params(rows, heads=heads, scale=D ** -0.5))
+    stream.sync()
+    got, want = o.read(np.float32).reshape(q.shape), attention(c, q, rows, heads, D ** -0.5, False)
+    for j in range(requests):
+        close(got[j * rows:(j + 1) * rows], want[j * rows:(j + 1) * rows])
