@@ -578,7 +578,8 @@ typedef struct yuuka_kv_params {
     int32_t block_size;   /* tokens per page */
     int32_t capacity;     /* tokens a request can hold */
     int32_t requests;     /* 1..65535 */
-    int32_t rows;         /* rows of every request (attention: 4096 at most) */
+    int32_t rows;         /* rows of every request (attention: 4096 at most; rows x
+                           * (2 kv_heads + heads) 2^25 at most) */
     int32_t request_rows; /* rows between consecutive requests (0: rows), not less than rows */
     int32_t heads;        /* attention: query heads, a multiple of kv_heads, 256 times them at most */
     int32_t kv_heads;
@@ -616,7 +617,12 @@ YUUKA_API yuuka_status yuuka_kv_read(yuuka_stream * stream, yuuka_buffer * k_out
  * Q8_0 pools. At most 4096 rows. A row that sees no key is zero. A query that is
  * not finite makes its row NaN, and so does any key that the row sees, the score's
  * sign whatever it is. A value that is not finite makes its dim (F16) or its block of
- * 32 dims (Q8_0) of the rows that see it infinite or NaN, and no other. */
+ * 32 dims (Q8_0) of the rows that see it infinite or NaN, and no other.
+ * Precision: FP32 sums; a query is taken to 2^-23 of its largest element, a weight
+ * times its Q8_0 value scale to 2^-22, but not below 2^-34 of the largest weight times
+ * the largest value scale that the row sees: blocks of values whose scale is more than 12
+ * octaves below that lose precision by so much. F16 values below 2^-14 are summed
+ * to 2^-36. */
 YUUKA_API yuuka_status yuuka_attn_decode(yuuka_stream * stream, yuuka_buffer * out, const yuuka_buffer * q,
                         const yuuka_buffer * kpool, const yuuka_buffer * vpool, const yuuka_buffer * table,
                         const yuuka_buffer * positions, const yuuka_kv_params * params, yuuka_event * completion);

@@ -1123,3 +1123,38 @@ def test_one_long_request_among_more_than_are_cut(dev, stream, dtype, requests, 
     got, want = o.read(np.float32).reshape(q.shape), attention(c, q, rows, heads, D ** -0.5, False)
     for j in range(requests):
         close(got[j * rows:(j + 1) * rows], want[j * rows:(j + 1) * rows])
+
+
+@pytest.mark.parametrize("heads,nk,D,rows", [(8, 2, 128, 1), (8, 2, 256, 5), (16, 4, 64, 8)])
+@pytest.mark.parametrize("octaves", [6, 13, 20, 27])
+def test_value_scales_octaves_apart(dev, stream, octaves, heads, nk, D, rows):
+    """What the header states of blocks next to much larger ones. A weight times a value scale is two halves: off by 2^-22
+    of itself, or by half a step of 2^-24. Weights are in units in which the largest, 1, times the power of two above the
+    largest scale S is 2^10 at the least: half a step is at most 2^-25 2^-10 2 S = 2^-34 S there. So an output, sum of
+    w_k s_k digit_k over sum of w_k, is off by 2^-34 S sum |digit_k| / sum w_k beside the relative 2^-18 of every term."""
+    c = Cache(dev, Q8, 16, 400, nk, D, 2, [350, 33], fill=q8_fill())
+    rng = np.random.default_rng(octaves)
+    n = 16 * c.kvd
+    s = rng.uniform(1, 2, (c.pages, 16, c.kvd // 32)) * 2.0 ** 10
+    s[..., ::2] *= 2.0 ** -octaves
+    c.pool[1][:, n:] = s.astype(np.float16).reshape(c.pages, -1).view(np.uint8)
+    c.upload()
+    q = rng.normal(0, 1, (2 * rows, heads, D)).astype(np.float32)
+    o = dev.alloc(q.nbytes)
+    for scale in (0.0, D ** -0.5):
+        hip.attn_decode(stream, o, dev.upload(q), *c.b_pool, c.b_table, c.b_pos, c.params(rows, heads=heads, scale=scale))
+        stream.sync()
+        got, want = o.read(np.float32).reshape(q.shape), attention(c, q, rows, heads, scale, False)
+        for j in range(2):
+            K, V = (np.array([c.row(side, j, p) for p in range(c.positions[j, 1] + rows)], np.float64).reshape(-1, nk, D)
+                    for side in range(2))
+            steps = np.array([s[c.at(j, p)].repeat(32) for p in range(len(V))]).reshape(V.shape)  # a digit's
+            for r in range(rows):
+                m = c.positions[j, 1] + r + 1
+                for h in range(heads):
+                    g = h // (heads // nk)
+                    t = K[:m, g] @ q[j * rows + r, h].astype(np.float64) * scale
+                    w = np.exp(t - t.max())
+                    off = 2.0 ** -34 * steps.max() * (np.abs(V[:m, g]) / steps[:m, g]).sum(0) + TOL * (w @ np.abs(V[:m, g]))
+                    d = np.abs(got[j * rows + r, h] - want[j * rows + r, h])
+                    assert (d <= off / w.sum()).all(), (j, r, h, scale, (d * w.sum() / off).max())
