@@ -8,11 +8,11 @@
 //   value = digit * F16 scale (exact in float32: 7 + 11 significant bits)
 // The reference's EncodeRow (kv_format.go:93-137) divides max|x| by 127. The product is what
 // torch computes for that division on the GPU (a constant divisor is inverted first), so that
-// pages written from there and from here hold the same bytes; it is as near to max / 127 for
-// what is cached. Over normal values its last bit differs from the quotient's in one block of
-// 23, a stored scale in one block of 2.5 million and a digit, by one, in one value of 7 million,
-// only where x / scale is within 5 * 2^-17 of a half. A value is off by at most half a step,
-// scale / 2, and by |x| 2^-11 for the scale's own rounding.
+// pages written from there and from here hold the same bytes, and costs less (8191 rows of 8
+// heads of 128: 27.9 us, with the quotient 28.6). Over normal values its last bit differs from
+// the quotient's in one block of 23, a stored scale in one block of 2.5 million and a digit, by
+// one, in one value of 7 million, only where x / scale is within 5 * 2^-17 of a half. A value is
+// off by at most half a step, scale / 2, and by |x| 2^-11 for the scale's own rounding.
 // A block that holds a NaN has a NaN scale (the reference leaves that case
 // undefined), so that it reads back as NaN instead of as finite values.
 #include <hip/hip_runtime.h>
@@ -139,9 +139,10 @@ __device__ __forceinline__ uint32_t transpose_digits(uint32_t mine, int r) {
 
 // One wave per 256 dims of kAppendRows rows: keys, values, or queries (those
 // only with q). Bound by the float32 rows it reads once (past the caches), those of all the
-// wave's rows asked for before any is used, and by vector instructions: 8191 rows of 8
-// heads of 128, keys normalised and rotated, to Q8_0 (89 MB): 28 us, 3.2 TB/s. Two rows a
-// wave: with the read back 45.8 us, one 51.2, four 48.4.
+// wave's rows asked for before any is used, and by vector instructions (49 % of a SIMD's cycles):
+// 8191 rows of 8 heads of 128 to Q8_0 (85 MB) 28 us, 3.0 TB/s; with the key norm and 64 dims
+// rotated (87 MB) 34 us, 64 %. To F16 28 and 33, to F32 26 and 31. Two rows a wave: with the
+// read back 45.8 us, one 51.2, four 48.4.
 constexpr int kAppendWaves = 4, kAppendRows = 2;
 
 template <int FMT, int GROUPS>
@@ -291,7 +292,9 @@ __global__ __launch_bounds__(64 * kAppendWaves) void kv_append_kernel(
 // One wave per 256 dims of kReadRows tokens' keys or values, all loads before the
 // first store; unmapped positions read as zeros. Bound by the float32 rows it writes,
 // past the caches: 16 requests of 4000 tokens of 4 heads of 256 from Q8_0 (664 MB): 117 us,
-// 5.7 TB/s; through the caches 127; with one token a wave 189, two 141, eight 129.
+// 5.7 TB/s (132 at the clock that many passes in a row leave); through the caches 127; with one
+// token a wave 189, two 141, eight 129. 8191 tokens of 8 heads of 128 from Q8_0 and F16 18 us,
+// from F32 22.
 constexpr int kReadRows = 4;
 
 template <int FMT, int GROUPS>

@@ -18,9 +18,12 @@
 //    halves), P V with those very keys as lane g's eight: probabilities go from
 //    the first product's result to the second's operand without leaving the lane;
 //  * int8 digits are exact halves. A query is two halves (scaled by a power of
-//    two to below 2^14), a probability times its key's scale too: products are good
-//    to 2^-22, sums are float32. Key scales multiply the scores block by block
-//    (an MFMA covers one block of 32 dims), value scales the probabilities.
+//    two to below 2^14), 22 bits of its largest element; a probability times its value
+//    scale too, 22 bits in steps of 2^-24 at the least. The largest weight times the largest
+//    scale is 2^9 or more in these units, so that blocks of values whose scale is more than 12
+//    octaves below the largest lose precision by so much. Subnormal F16 values are summed to
+//    2^-36 (an MFMA aligns them as if they were 2^-14). Sums are float32. Key scales
+//    multiply the scores block by block (an MFMA covers one block of 32 dims).
 //  * up to eight pairs ("stacked") put both halves in one 16-wide operand, as rows
 //    n and n + 8; more take two MFMAs.
 //  * p = 2^(s - m') with the reference m' = running max + E - 10, E the
@@ -29,13 +32,14 @@
 //    rescaled) when a tile passes it by 4.
 //
 // Measured, with the join: one row of one request over 120001 keys of 4 heads of 256, 16 query
-// heads (261 MB of Q8_0) 65 us, 4.0 TB/s, of which 5 before the first tile, 4 after the last
-// and 5 for the join; 16 requests of 4096 such keys 42 us; 16 of 4096 keys of 8 heads of 128
-// in F16 (269 MB) 58 us, 4.6 TB/s. Vector instructions issue in 50 % of a SIMD's cycles at
-// 256 dims (700 a tile), 64 % at 128, 16 % over F16: bound by the reads and, from Q8_0, by two
-// waves a SIMD (256 registers) that wait for them in turn. 4 requests of 17 rows over 16384
-// keys of 4 heads of 256 take 102 us: instructions (73 %), for every 16-row block turns each
-// tile's digits to halves again.
+// heads (261 MB of Q8_0) 62 us, 4.2 TB/s, of which some 12 before the first tile, after the
+// last and for the join; 16 requests of 4096 such keys 40 us; 16 of 4096 keys of 8 heads of 128
+// in F16 (269 MB) 58 us, 4.6 TB/s. Vector instructions issue in 52 % of a SIMD's cycles at
+// 256 dims (700 a tile in the loop, 800 to 900 with what a wave does once), 61 % at 128, 17 %
+// over F16: bound by the reads and, from Q8_0, by two waves a SIMD (256 registers) that wait
+// for them in turn. 4 requests of 17 rows over 16384 keys of 4 heads of 256 take 101 us, and 114
+// at the clock that a profiled run leaves: instructions (71 %), for every 16-row block turns
+// each tile's digits to halves again.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -187,7 +191,11 @@ struct AttnSplit {
     uint32_t group_inverse;   // ceil(2^32 / group): n / group = high word of the product, n < 2^24 (group 1: 0)
     int target;
     float share;              // columns / target
-    int whole;                // 1: every request is one part (twice as many columns as workgroups)
+    // 1: every request is one part, from twice as many columns as workgroups on. Nothing is worked out or
+    // joined then, which is faster where the lengths are alike and far slower where one stands out: requests of
+    // one row, 4 heads of 256 a KV head and 4 KV heads, 500 keys each: 255 (cut) 66.5 us, 256 (whole) 60.7; with
+    // 120001 keys in one of them 158 and 2155 us.
+    int whole;
     int page_shift;           // PAGED: log2(block_size / 16)
 };
 constexpr int kMaxParts = 256;
@@ -1118,6 +1126,10 @@ __global__ __launch_bounds__(256) void kv_attention_merge_kernel(const float *__
     }
 }
 
+// A 16-key half of a tile lies in one page. Other page sizes have the rows of every tile found a lane a key,
+// and never share an operand between a query's halves: 16 requests of 4096 keys, pages of 16, 48 and 64 tokens, 16
+// query heads: Q8_0, 4 heads of 256 37.5, 38.9 and 37.2 us for one row, 84.7, 93.6 and 84.9 for nine; F16 58.4, 60.9 and
+// 58.1, 111.8, 116.7 and 112.0.
 bool paged(const KvArgs &a) { return a.block_size % 16 == 0 && (a.block_size & (a.block_size - 1)) == 0; }
 bool stacked(const KvArgs &a) { return paged(a) && a.heads / a.kv_heads * a.rows <= 8; }
 // 16-row blocks of a wave. Two share each tile's way to halves, at two waves a SIMD for
@@ -1222,7 +1234,9 @@ hipError_t launch_kv_attention(const float *q, int q_stride, const float *gate, 
     // A wave a row, or where a request can have many parts a workgroup each 64 dims: then what counts
     // is the records in flight. (us with the attention, a wave a row and a workgroup a row: 96 requests of
     // up to 6 parts, 8 heads of 128 a KV head, 91.5 and 94.5; 16 of 8 parts 42.1 and 42.3; 5 rows of 9
-    // parts 14.6 and 13.8. 125 parts: a workgroup a row 69.3, each 64 dims 64.6.)
+    // parts 14.6 and 13.8. 125 parts: a workgroup a row 69.3, each 64 dims 64.6.
+    // The estimate goes by the tables' length: 517 and 1029 keys in tables of 131072 tokens take 12.6 and 14.3, in
+    // tables that they fill 12.3 and 14.8.)
     const int64_t parts = std::min<int64_t>(most_parts(a), sp.target / ((int64_t)sp.columns * a.requests));
     if (parts > 32) {
         kv_attention_merge_kernel<<<dim3(a.rows * (a.head_dim / 64), a.heads, a.requests), 256, 0, s>>>(
