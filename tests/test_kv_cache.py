@@ -2,10 +2,13 @@
 for the host) and the refusals of the direct calls and plan ops, which are
 decided before anything is launched."""
 import ctypes as C
+import gc
 import shutil
 import subprocess
+import weakref
 from dataclasses import replace
 from pathlib import Path
+from types import SimpleNamespace
 
 import pytest
 
@@ -467,3 +470,29 @@ def test_an_engine_over_q8_0_pages_refuses_what_its_attention_does(change, statu
     assert _create() == hip.DEVICE
     # without a layer of attention there is no cache
     assert _create(**change, full_interval=Mdl.TINY.n_layers + 1) == hip.DEVICE
+
+
+# ------------------------------------------------------------------- the binding
+
+def test_a_graph_keeps_the_buffers_it_was_captured_over(monkeypatch):
+    """It holds their addresses, and may outlive its plan."""
+    class Owner:
+        pass
+
+    plan, dynamic, buffers = Owner(), Owner(), [Owner() for _ in range(3)]
+    plan.ptr, plan.keep, dynamic.ptr = None, list(buffers), None
+    calls = []
+    monkeypatch.setattr(hip, "lib", lambda: SimpleNamespace(yuuka_graph_create=lambda *a: calls.append(a) or hip.OK,
+                                                            yuuka_graph_destroy=lambda p: calls.append(p)))
+    graph = hip.Graph(plan, SimpleNamespace(ptr=None), dynamic)
+    graph.ptr = 1
+    alive = [weakref.ref(b) for b in buffers + [dynamic]]
+    later = Owner()
+    plan.keep.append(later)       # of an op that is not in the graph
+    alive_later = weakref.ref(later)
+    del plan, dynamic, buffers, later
+    gc.collect()
+    assert all(a() is not None for a in alive) and alive_later() is None
+    graph.destroy()
+    gc.collect()
+    assert len(calls) == 2 and all(a() is None for a in alive)

@@ -449,6 +449,7 @@ class Graph:
         check(lib().yuuka_graph_create(plan.ptr, stream.ptr, _p(dynamic), int(run_tail), C.byref(p)),
               "graph_create")
         self.ptr = p
+        self.keep = [*plan.keep, dynamic]  # the captured addresses: the plan may end before the graph
 
     def replay(self, stream: Stream, event: Event | None = None) -> None:
         check(lib().yuuka_graph_replay(self.ptr, stream.ptr, _p(event)), "graph_replay")
@@ -457,3 +458,4 @@ class Graph:
         if self.ptr:
             lib().yuuka_graph_destroy(self.ptr)
             self.ptr = None
+            self.keep = []
