@@ -1158,3 +1158,36 @@ def test_value_scales_octaves_apart(dev, stream, octaves, heads, nk, D, rows):
                     off = 2.0 ** -34 * steps.max() * (np.abs(V[:m, g]) / steps[:m, g]).sum(0) + TOL * (w @ np.abs(V[:m, g]))
                     d = np.abs(got[j * rows + r, h] - want[j * rows + r, h])
                     assert (d <= off / w.sum()).all(), (j, r, h, scale, (d * w.sum() / off).max())
+
+
+@pytest.mark.parametrize("dtype", [Q8, F16])
+def test_v10_single_token_ops_refuse_positions_past_the_capacity(dev, stream, dtype):
+    """In every format; the last position is served, and a refused write leaves the pools as they were."""
+    heads, nk, D, bs, cap = 8, 2, 128, 16, 70
+    c = Cache(dev, dtype, bs, cap, nk, D, 1, [cap - 1], fill=q8_fill() if dtype == Q8 else f16_fill)
+    rng = np.random.default_rng(3)
+    k, v = rng.normal(0, 1, (2, 1, c.kvd)).astype(np.float32)
+    q = rng.normal(0, 1, (1, heads, D)).astype(np.float32)
+    o = dev.upload(np.zeros(q.shape, np.float32))
+    scores = dev.alloc(heads * cap * 4)
+    write, attend = hip.Plan(dev), hip.Plan(dev)
+    write.add(26, [dev.upload(k), dev.upload(v), *c.b_pool, c.b_table], n=[c.kvd], u=[bs, cap, dtype])
+    attend.add(27, [dev.upload(q), *c.b_pool, o, scores, c.b_table], n=[nk, heads, D, c.kvd, cap], u=[bs, cap, dtype, 1],
+               f=[D ** -0.5])
+    for plan in (write, attend):
+        for position in (cap, cap + 9, 2 ** 31 - 1):
+            with pytest.raises(hip.HipError, match="capacity"):
+                plan.execute(stream, position=position)
+    stream.sync()
+    for side in range(2):
+        assert np.array_equal(c.read_pool(side), c.pool[side])
+    write.execute(stream, position=cap - 1)
+    attend.execute(stream, position=cap - 1)
+    stream.sync()
+    c.put(0, 0, cap - 1, k[0])
+    c.put(1, 0, cap - 1, v[0])
+    for side in range(2):
+        assert np.array_equal(c.read_pool(side), c.pool[side])
+    close(o.read(np.float32).reshape(q.shape), attention(c, q, 1, heads, D ** -0.5, False))
+    write.destroy()
+    attend.destroy()

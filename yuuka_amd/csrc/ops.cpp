@@ -1212,6 +1212,11 @@ yuuka_status execute_gdn_commit_run(const yuuka_op *ops, int count, const ExecCt
 
 yuuka_status execute_model_op(const yuuka_op &op, const ExecCtx &ctx) {
     if (kv_op(op)) {
+        // the single-token ops refuse a position past the capacity, as over F32 and F16 pools
+        if ((op.code == YUUKA_OP_KV_WRITE_PAGED || op.code == YUUKA_OP_ATTENTION_PAGED) && !ctx.dyn &&
+            ctx.position >= op.u[1])
+            return fail(YUUKA_ERR_INVALID_ARGUMENT, "paged KV op %u at %u exceeds capacity %u", op.code, ctx.position,
+                        op.u[1]);
         const hipError_t err = execute_kv_op(op, ctx);
         if (err != hipSuccess) return fail(YUUKA_ERR_DEVICE, "op %u launch: %s", op.code, hip_error(err));
         return YUUKA_OK;
