@@ -67,10 +67,12 @@ static KvArgs kv_op_args(const yuuka_op &op) {
 static KvArgs kv_any_args(const yuuka_op &op) {
     KvArgs a = kv_op_args(op);
     switch (op.code) {
-    case YUUKA_EXT_OP_KV_APPEND:
     case YUUKA_EXT_OP_ATTN_VERIFY:
+        a.gated = 1;
+        a.rq_rows = std::max(a.rq_rows, a.rows);  // as over F32 and F16 pools
+        [[fallthrough]];
+    case YUUKA_EXT_OP_KV_APPEND:
         a.rope_dim = (int)(op.u[3] & 0xffu);
-        a.gated = op.code == YUUKA_EXT_OP_ATTN_VERIFY;
         break;
     case YUUKA_EXT_OP_ATTN_DECODE:
         a.gated = (op.u[3] & 0xffu) != 0;
