@@ -444,8 +444,9 @@ YUUKA_API yuuka_status yuuka_verify_accept_noalloc(yuuka_stream * stream,
  *               f={scale, eps}. Writes the rows' K/V to the pool at position
  *               + displacement + row. With requests > 1 (and OWN_POS) request
  *               j's rows start request_rows rows (rows, if that is more) after
- *               request j-1's, its block table ceil(capacity / block_size) entries later and its
- *               {token, position} pair 8 bytes later (one launch).
+ *               request j-1's, its block table ceil(capacity / block_size)
+ *               entries later and its {token, position} pair 8 bytes later
+ *               (one launch).
  *   MOE_ROUTER: FP32 router of the MoE FFN (ffn_gate_inp, forward.go:328):
  *               buf0 FP32 y [rows][hidden], buf1 FP32 router weight
  *               [experts][hidden], buf2 FP32 logits [rows][experts];
