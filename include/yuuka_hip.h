@@ -203,7 +203,8 @@ typedef enum yuuka_dtype {
     YUUKA_DTYPE_Q8_0 = 8,
     YUUKA_DTYPE_Q4_K = 12,
     YUUKA_DTYPE_Q5_K = 13,
-    YUUKA_DTYPE_Q6_K = 14
+    YUUKA_DTYPE_Q6_K = 14,
+    YUUKA_DTYPE_BF16 = 30 /* extension: rows of the ragged GDN calls only */
 } yuuka_dtype;
 
 /* reference :209-212. Single-row decode GEMV: served by the verify GEMM with
@@ -507,6 +508,29 @@ YUUKA_API yuuka_status yuuka_verify_accept_noalloc(yuuka_stream * stream,
 #define YUUKA_EXT_OP_KV_APPEND 75u
 #define YUUKA_EXT_OP_KV_READ 76u
 #define YUUKA_EXT_OP_ATTN_DECODE 77u
+/* Ragged batches (the direct calls yuuka_batch_plan, yuuka_kv_append_slots,
+ * yuuka_gdn_conv, yuuka_gdn_prompt and yuuka_gdn_step below say what each
+ * computes). Buffer offsets are multiples of 16.
+ *   BATCH_PLAN: buf0 positions, buf1 counts, buf2 blocks, buf3 tables, buf4 free
+ *               pages, buf5 pool, buf6 offsets, buf7 row info, buf8 slots, buf9
+ *               blocks out, buf10 pool out; n={requests, rows};
+ *               u={block_size, capacity}.
+ *   KV_APPEND_SLOTS: buf0 FP32 k rows, buf1 v rows, buf2 K pool, buf3 V pool, buf4
+ *               slots, optional buf5 k_norm, optional buf6 rotation table;
+ *               n={kv_heads, 0, head_dim, kv_dim, rows};
+ *               u={block_size, 0, dtype, rot_dim}; f1 eps.
+ *   GDN_CONV:   buf0 out, buf1 x, buf2 weight, buf3 windows, buf4 offsets, buf5
+ *               slots; n={requests, rows, groups, heads, head_dim, row stride};
+ *               u={dtype, kernel}; f={scale, eps}.
+ *   GDN_PROMPT: buf0 out, buf1 qkv, buf2 alpha, buf3 beta, buf4 states, buf5
+ *               offsets, buf6 slots, buf7 dt, buf8 a (both null with u2); n as
+ *               GDN_CONV; u={dtype, 0, log_decay}; f0 scale.
+ *   GDN_STEP:   as GDN_PROMPT with buf5 null: row j is request j's. */
+#define YUUKA_EXT_OP_BATCH_PLAN 78u
+#define YUUKA_EXT_OP_KV_APPEND_SLOTS 79u
+#define YUUKA_EXT_OP_GDN_CONV 80u
+#define YUUKA_EXT_OP_GDN_PROMPT 81u
+#define YUUKA_EXT_OP_GDN_STEP 82u
 #define YUUKA_EXT_FLAG_DEFER 0x100u
 /* With YUUKA_EXT_FLAG_DEFER: buf10 receives the raw per-head scan outputs;
  * the gated RMSNorm is left to the consumer (GEMM_FUSED gated head norm). */
@@ -627,6 +651,108 @@ YUUKA_API yuuka_status yuuka_kv_read(yuuka_stream * stream, yuuka_buffer * k_out
 YUUKA_API yuuka_status yuuka_attn_decode(yuuka_stream * stream, yuuka_buffer * out, const yuuka_buffer * q,
                         const yuuka_buffer * kpool, const yuuka_buffer * vpool, const yuuka_buffer * table,
                         const yuuka_buffer * positions, const yuuka_kv_params * params, yuuka_event * completion);
+
+/* ----------------------------------------------------------------------
+ * Ragged batches (extension): requests with different numbers of new rows,
+ * laid one after another without padding. Rows offsets[j] .. offsets[j + 1] - 1
+ * (int32) are request j's; rows behind the last are neither read nor written.
+ * Offsets outside 0 .. rows are taken as the nearest of those, a request that
+ * ends before it starts as empty. Every buffer has to be on the stream's device;
+ * an output must not overlap an input or another output, except where said.
+ * ---------------------------------------------------------------------- */
+typedef struct yuuka_batch_params {
+    int32_t requests;   /* 1..65535 */
+    int32_t rows;       /* rows that the row arrays hold; 2^30 at most */
+    int32_t block_size; /* tokens per page, 2^20 at most */
+    int32_t capacity;   /* tokens a request can hold; its table has
+                         * ceil(capacity / block_size) entries */
+} yuuka_batch_params;
+
+/* Where the rows of a batch go, worked out on the device.
+ *   positions  {token, position} of every request (position p_j: its cached tokens)
+ *   counts     int32 [requests]: new rows n_j (below 0: none)
+ *   blocks     int32 [requests]: entries in use at the front of its table
+ *   table      int32 [requests][entries] block tables, extended
+ *   free_pages int32: page indices; pool = int32 {next, count}: entries next ..
+ *              count - 1 of the list are free
+ *   offsets    int32 [requests + 1] <- sums of the counts, `rows` at most
+ *   row_info   int32 [rows][2] <- {request, position p_j + i}
+ *   slots      int64 [rows] <- page * block_size + position % block_size
+ *   blocks_out int32 [requests] <- entries in use after it (may be blocks itself)
+ *   pool_out   int32 <- {next, pages that were missing}; with pool itself only next
+ *              moves, and the next call goes on from there
+ * Blocks from max(blocks_j, p_j / block_size) to that of the last new row get a page
+ * each, in the order of the requests; other entries stay. Once the list is
+ * empty they get -1, as do the slots of their rows, and blocks_out ends before
+ * them. A row whose position is below 0 or from `capacity` on, or whose entry is
+ * below 0, has the slot -1. Rows that the arrays have no room for take no page.
+ * Rows behind the last get {-1, -1} and -1. */
+YUUKA_API yuuka_status yuuka_batch_plan(yuuka_stream * stream, const yuuka_buffer * positions,
+                        const yuuka_buffer * counts, const yuuka_buffer * blocks, yuuka_buffer * table,
+                        const yuuka_buffer * free_pages, const yuuka_buffer * pool, yuuka_buffer * offsets,
+                        yuuka_buffer * row_info, yuuka_buffer * slots, yuuka_buffer * blocks_out,
+                        yuuka_buffer * pool_out, const yuuka_batch_params * params, yuuka_event * completion);
+
+/* yuuka_kv_append of `rows` rows that each go to a slot of their own: slots int64
+ * [rows] as yuuka_batch_plan writes them; a slot outside the pool drops its
+ * row, and of two rows with one slot the pool holds either's bytes. `rope` has a
+ * row's {cos, sin} each row. Of the parameters capacity, requests, request_rows and
+ * displacement are not used. */
+YUUKA_API yuuka_status yuuka_kv_append_slots(yuuka_stream * stream, const yuuka_buffer * k, const yuuka_buffer * v,
+                        yuuka_buffer * kpool, yuuka_buffer * vpool, const yuuka_buffer * slots,
+                        const yuuka_buffer * k_norm, const yuuka_buffer * rope, const yuuka_kv_params * params,
+                        yuuka_event * completion);
+
+typedef struct yuuka_gdn_params {
+    uint32_t dtype;     /* of x, qkv and out: YUUKA_DTYPE_F32, F16 or BF16 */
+    int32_t requests;   /* 1..65535 */
+    int32_t rows;       /* rows that x, qkv, alpha, beta and out hold; 2^30 at most */
+    int32_t groups;     /* q and k heads; head h takes those of group h % groups */
+    int32_t heads;      /* v heads, a multiple of groups, 1024 at most */
+    int32_t head_dim;   /* 64 or 128 */
+    int32_t kernel;     /* convolution: taps, 2..8 */
+    int32_t row_stride; /* elements between rows of x / qkv, a multiple of 8 (0: none
+                         * between them) */
+    int32_t log_decay;  /* alpha and beta are the log of the decay and the step size */
+    float scale;        /* factor of q */
+    float eps;          /* convolution: of the q / k norm */
+} yuuka_gdn_params;
+
+/* Slots of the three calls below: int32 {from, to} of every request, indices into the
+ * pool of states. The request starts from slot `from` and its new state goes to
+ * slot `to`, which may be the same; an index outside the pool (such as -1) is a start
+ * from zeros, or a state that is not kept. A request without rows has its
+ * state moved. A slot that a request writes must not be another's `from` or `to`
+ * (its content is then undefined).
+ *
+ * Causal convolution of rows [q | k | v] of (2 groups + heads) * head_dim channels
+ * (forward.go:248-268, 484-493):
+ *   y = SiLU(sum_i weight[c][i] x[t - kernel + 1 + i][c])
+ * then q and k heads y / sqrt(|y|^2 + eps), q times scale. weight FP32
+ * [channels][kernel]; windows FP32 [.][channels][kernel - 1], oldest input
+ * first; out has no space between its rows. */
+YUUKA_API yuuka_status yuuka_gdn_conv(yuuka_stream * stream, yuuka_buffer * out, const yuuka_buffer * x,
+                        const yuuka_buffer * weight, yuuka_buffer * windows, const yuuka_buffer * offsets,
+                        const yuuka_buffer * slots, const yuuka_gdn_params * params, yuuka_event * completion);
+
+/* The gated delta rule over rows [q | k | v] (recurrent.go:56-105), for every head
+ * with its state S FP32 [head_dim][head_dim] (rows: k's dims):
+ *   S = e^g S + k (beta (v - (e^g S)^T k))^T,   out = scale S^T q
+ * with g = softplus(alpha + dt) a and beta = sigmoid(beta), alpha and beta FP32
+ * [rows][heads], dt and a FP32 [heads]; or with log_decay g = alpha and beta
+ * themselves, and dt and a null. States are [.][heads][head_dim][head_dim], out
+ * [rows][heads][head_dim], rounded once to the nearest.
+ * Keys of norm 1 (as the convolution leaves them), beta in 0..1 and g <= 0 are what the
+ * rule is stable for. yuuka_gdn_step takes one row of every request, row j
+ * of request j (`rows` is not less than `requests`). */
+YUUKA_API yuuka_status yuuka_gdn_prompt(yuuka_stream * stream, yuuka_buffer * out, const yuuka_buffer * qkv,
+                        const yuuka_buffer * alpha, const yuuka_buffer * beta, const yuuka_buffer * dt,
+                        const yuuka_buffer * a, yuuka_buffer * states, const yuuka_buffer * offsets,
+                        const yuuka_buffer * slots, const yuuka_gdn_params * params, yuuka_event * completion);
+YUUKA_API yuuka_status yuuka_gdn_step(yuuka_stream * stream, yuuka_buffer * out, const yuuka_buffer * qkv,
+                        const yuuka_buffer * alpha, const yuuka_buffer * beta, const yuuka_buffer * dt,
+                        const yuuka_buffer * a, yuuka_buffer * states, const yuuka_buffer * slots,
+                        const yuuka_gdn_params * params, yuuka_event * completion);
 
 /* Timing events (extension): an event created with timing enabled, recorded
  * on a stream, and the elapsed milliseconds between two recorded events. */

@@ -658,16 +658,21 @@ static yuuka_status kv_args(const yuuka_kv_params &p, bool attention, KvArgs *a)
 }
 
 // The buffers' device: the stream's, made current for the launches.
-static yuuka_status kv_device(yuuka_stream *stream, std::initializer_list<const yuuka_buffer *> bufs) {
-    for (const yuuka_buffer *b : bufs)
+static yuuka_status kv_device(yuuka_stream *stream, const yuuka_buffer *const *bufs, size_t n) {
+    for (size_t i = 0; i < n; i++) {
+        const yuuka_buffer *const b = bufs[i];
         if (b && b->dev && stream->dev && b->dev->index != stream->dev->index)
-            return fail(YUUKA_ERR_INVALID_ARGUMENT, "KV cache: a buffer of device %d on a stream of device %d",
+            return fail(YUUKA_ERR_INVALID_ARGUMENT, "a buffer of device %d on a stream of device %d",
                         b->dev->index, stream->dev->index);
+    }
     if (stream->dev) {
         const hipError_t err = hipSetDevice(stream->dev->index);
         if (err != hipSuccess) return fail(YUUKA_ERR_DEVICE, "set device: %s", hip_error(err));
     }
     return YUUKA_OK;
+}
+static yuuka_status kv_device(yuuka_stream *stream, std::initializer_list<const yuuka_buffer *> bufs) {
+    return kv_device(stream, bufs.begin(), bufs.size());
 }
 
 uint64_t yuuka_kv_page_bytes(const yuuka_kv_params *params) {
@@ -758,6 +763,111 @@ yuuka_status yuuka_attn_decode(yuuka_stream *stream, yuuka_buffer *out, const yu
             stream->stream);
         if (err != hipSuccess) return fail(YUUKA_ERR_DEVICE, "attn_decode launch: %s", hip_error(err));
         return record(stream, completion);
+    });
+}
+
+// A direct call as the plan op that it is: checked the same way, its workspace the stream's.
+static yuuka_status run_direct(yuuka_stream *stream, const yuuka_op &op, yuuka_event *completion) {
+    uint64_t ws = 0;
+    yuuka_status st = validate_ragged_op(op, &ws);
+    if (st == YUUKA_OK) st = kv_device(stream, op.buf, 16);
+    if (st == YUUKA_OK) st = ensure_scratch(stream, &stream->scratch, ws);
+    if (st != YUUKA_OK) return st;
+    ExecCtx ctx{stream->stream, 0, 0, nullptr, stream->scratch.ptr, nullptr};
+    st = execute_ragged_op(op, ctx);
+    return st == YUUKA_OK ? record(stream, completion) : st;
+}
+// (the op only names its buffers)
+static void op_buffers(yuuka_op *op, std::initializer_list<const yuuka_buffer *> bufs) {
+    int i = 0;
+    for (const yuuka_buffer *b : bufs) op->buf[i++] = const_cast<yuuka_buffer *>(b);
+}
+static uint64_t op_count(int32_t v) { return (uint64_t)(int64_t)v; }
+
+yuuka_status yuuka_batch_plan(yuuka_stream *stream, const yuuka_buffer *positions, const yuuka_buffer *counts,
+                              const yuuka_buffer *blocks, yuuka_buffer *table, const yuuka_buffer *free_pages,
+                              const yuuka_buffer *pool, yuuka_buffer *offsets, yuuka_buffer *row_info,
+                              yuuka_buffer *slots, yuuka_buffer *blocks_out, yuuka_buffer *pool_out,
+                              const yuuka_batch_params *params, yuuka_event *completion) {
+    return guard("batch_plan", [&]() -> yuuka_status {
+        if (!stream || !params) return fail(YUUKA_ERR_INVALID_ARGUMENT, "null argument");
+        yuuka_op op{};
+        op.code = YUUKA_EXT_OP_BATCH_PLAN;
+        op_buffers(&op, {positions, counts, blocks, table, free_pages, pool, offsets, row_info, slots, blocks_out, pool_out});
+        op.n[0] = op_count(params->requests);
+        op.n[1] = op_count(params->rows);
+        op.u[0] = (uint32_t)params->block_size;
+        op.u[1] = (uint32_t)params->capacity;
+        return run_direct(stream, op, completion);
+    });
+}
+
+yuuka_status yuuka_kv_append_slots(yuuka_stream *stream, const yuuka_buffer *k, const yuuka_buffer *v,
+                                   yuuka_buffer *kpool, yuuka_buffer *vpool, const yuuka_buffer *slots,
+                                   const yuuka_buffer *k_norm, const yuuka_buffer *rope, const yuuka_kv_params *params,
+                                   yuuka_event *completion) {
+    return guard("kv_append_slots", [&]() -> yuuka_status {
+        if (!stream || !params) return fail(YUUKA_ERR_INVALID_ARGUMENT, "null argument");
+        yuuka_op op{};
+        op.code = YUUKA_EXT_OP_KV_APPEND_SLOTS;
+        op_buffers(&op, {k, v, kpool, vpool, slots, k_norm, rope});
+        op.n[0] = op_count(params->kv_heads);
+        op.n[2] = op_count(params->head_dim);
+        op.n[3] = (uint64_t)((int64_t)params->kv_heads * params->head_dim);
+        op.n[4] = op_count(params->rows);
+        op.u[0] = (uint32_t)params->block_size;
+        op.u[2] = params->dtype;
+        op.u[3] = (uint32_t)params->rope_dim;
+        op.f[1] = params->eps;
+        return run_direct(stream, op, completion);
+    });
+}
+
+static yuuka_op gdn_rows_op(uint32_t code, const yuuka_gdn_params &p) {
+    yuuka_op op{};
+    op.code = code;
+    const int32_t n[6] = {p.requests, p.rows, p.groups, p.heads, p.head_dim, p.row_stride};
+    for (int i = 0; i < 6; i++) op.n[i] = op_count(n[i]);
+    op.u[0] = p.dtype;
+    op.u[1] = (uint32_t)p.kernel;
+    op.u[2] = p.log_decay != 0;
+    op.f[0] = p.scale;
+    op.f[1] = p.eps;
+    return op;
+}
+
+yuuka_status yuuka_gdn_conv(yuuka_stream *stream, yuuka_buffer *out, const yuuka_buffer *x, const yuuka_buffer *weight,
+                            yuuka_buffer *windows, const yuuka_buffer *offsets, const yuuka_buffer *slots,
+                            const yuuka_gdn_params *params, yuuka_event *completion) {
+    return guard("gdn_conv", [&]() -> yuuka_status {
+        if (!stream || !params) return fail(YUUKA_ERR_INVALID_ARGUMENT, "null argument");
+        yuuka_op op = gdn_rows_op(YUUKA_EXT_OP_GDN_CONV, *params);
+        op_buffers(&op, {out, x, weight, windows, offsets, slots});
+        return run_direct(stream, op, completion);
+    });
+}
+
+yuuka_status yuuka_gdn_prompt(yuuka_stream *stream, yuuka_buffer *out, const yuuka_buffer *qkv,
+                              const yuuka_buffer *alpha, const yuuka_buffer *beta, const yuuka_buffer *dt,
+                              const yuuka_buffer *a, yuuka_buffer *states, const yuuka_buffer *offsets,
+                              const yuuka_buffer *slots, const yuuka_gdn_params *params, yuuka_event *completion) {
+    return guard("gdn_prompt", [&]() -> yuuka_status {
+        if (!stream || !params) return fail(YUUKA_ERR_INVALID_ARGUMENT, "null argument");
+        yuuka_op op = gdn_rows_op(YUUKA_EXT_OP_GDN_PROMPT, *params);
+        op_buffers(&op, {out, qkv, alpha, beta, states, offsets, slots, dt, a});
+        return run_direct(stream, op, completion);
+    });
+}
+
+yuuka_status yuuka_gdn_step(yuuka_stream *stream, yuuka_buffer *out, const yuuka_buffer *qkv, const yuuka_buffer *alpha,
+                            const yuuka_buffer *beta, const yuuka_buffer *dt, const yuuka_buffer *a,
+                            yuuka_buffer *states, const yuuka_buffer *slots, const yuuka_gdn_params *params,
+                            yuuka_event *completion) {
+    return guard("gdn_step", [&]() -> yuuka_status {
+        if (!stream || !params) return fail(YUUKA_ERR_INVALID_ARGUMENT, "null argument");
+        yuuka_op op = gdn_rows_op(YUUKA_EXT_OP_GDN_STEP, *params);
+        op_buffers(&op, {out, qkv, alpha, beta, states, nullptr, slots, dt, a});
+        return run_direct(stream, op, completion);
     });
 }
 

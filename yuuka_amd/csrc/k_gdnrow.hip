@@ -1,0 +1,353 @@
+// k_gdnrow.hip — Gated DeltaNet layers over ragged rows: the causal
+// convolution with SiLU and the q / k norm (forward.go:248-268, 484-493), and the
+// delta rule row by row (recurrent.go:56-105).
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "gdn_ragged_dev.h"
+#include "internal.h"
+
+namespace yk {
+
+yuuka_status ragged_check(RaggedArgs *a, uint32_t dtype, bool conv) {
+    constexpr int kBig = 1 << 30;
+    if (dtype != YUUKA_DTYPE_F32 && dtype != YUUKA_DTYPE_F16 && dtype != YUUKA_DTYPE_BF16)
+        return fail(YUUKA_ERR_UNSUPPORTED, "GDN rows of dtype %u (F32, F16 and BF16 are served)", dtype);
+    if (a->requests < 1 || a->requests > 65535 || a->rows < 1 || a->rows > kBig)
+        return fail(YUUKA_ERR_INVALID_ARGUMENT, "GDN rows: %d requests, %d rows", a->requests, a->rows);
+    if (a->groups < 1 || a->heads < 1 || a->heads > 1024 || a->heads % a->groups)
+        return fail(YUUKA_ERR_INVALID_ARGUMENT, "GDN rows: %d heads of %d groups", a->heads, a->groups);
+    if (a->head_dim != 64 && a->head_dim != 128)
+        return fail(YUUKA_ERR_UNSUPPORTED, "GDN head dimension %d (64 and 128 are served)", a->head_dim);
+    a->channels = (2 * a->groups + a->heads) * a->head_dim;
+    if (!a->stride) a->stride = a->channels;
+    if (a->stride < a->channels || a->stride % 8 || a->stride > kBig)
+        return fail(YUUKA_ERR_INVALID_ARGUMENT, "GDN rows of %d channels, %d elements apart (a multiple of 8)",
+                    a->channels, a->stride);
+    if (conv && (a->kernel < 2 || a->kernel > 8))
+        return fail(YUUKA_ERR_UNSUPPORTED, "GDN convolution of %d taps (2 to 8 are served)", a->kernel);
+    return YUUKA_OK;
+}
+
+namespace {
+
+// Sum over aligned groups of N lanes, in every lane.
+template <int CTRL> __device__ __forceinline__ float add_dpp(float x) {
+    return x + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, true));
+}
+template <int N> __device__ __forceinline__ float lanes_sum(float x) {
+    x = add_dpp<0xb1>(x);   // lanes l ^ 1, l ^ 2, 7 - l of eight
+    x = add_dpp<0x4e>(x);
+    x = add_dpp<0x141>(x);
+    if constexpr (N >= 16) x = add_dpp<0x128>(x);  // rotated by 8
+    if constexpr (N >= 32) {
+        const auto y = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+        x = __uint_as_float(y[0]) + __uint_as_float(y[1]);
+    }
+    return x;
+}
+
+// Convolution: y_t = SiLU(sum_i w_i x_{t - K + 1 + i}), then q and k over their head's
+// norm, q times `scale`. A wave takes 64 x 16 bytes of channels (whole heads) of `run`
+// rows and keeps the last KT - 1 of them in registers; the wave with a request's first
+// row reads its window and leaves its new one, which may be in the same slot.
+// Requests without rows have their window moved by waves of their own.
+template <typename E, int KT, int D>
+__global__ __launch_bounds__(256) void ragged_conv_kernel(typename E::T *__restrict__ out,
+                                                          const typename E::T *__restrict__ x,
+                                                          const float *__restrict__ weight, float *__restrict__ state,
+                                                          const int32_t *__restrict__ offsets,
+                                                          const int2 *__restrict__ slots, RaggedArgs a, int run,
+                                                          int row_blocks) {
+    constexpr int V = E::kWide;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int c = (blockIdx.y * 64 + lane) * V;
+    const bool live = c < a.channels;
+    const int K1 = a.kernel - 1;
+    const int64_t window = (int64_t)a.channels * K1;
+    // the request's window before its rows, oldest first, zeros in front where K < KT
+    float past[KT - 1][V] = {};
+    auto load_window = [&](int j) {
+        const int from = slots[j].x;
+#pragma unroll
+        for (int t = 0; t < KT - 1; t++)
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                const int at = t - (KT - 1 - K1);
+                past[t][i] = live && at >= 0 && (uint32_t)from < (uint32_t)a.states
+                                 ? state[from * window + (int64_t)(c + i) * K1 + at] : 0.0f;
+            }
+    };
+    auto load_row = [&](int row, float (&y)[V]) {
+        const Bytes16 none = {0, 0, 0, 0};
+        unpack<E>(live ? *reinterpret_cast<const Bytes16 *>(x + (int64_t)row * a.stride + c) : none, y);
+    };
+    // The window after the request's rows: the last K - 1 of [window, rows].
+    auto store_window = [&](int j, RowRange r) {
+        const int to = slots[j].y, n = r.end - r.begin;
+        if ((uint32_t)to >= (uint32_t)a.states) return;
+        float next[KT - 1][V];
+#pragma unroll
+        for (int t = 0; t < KT - 1; t++) {
+            const int back = KT - 1 - t;  // of the newest row: 1
+            if (back <= n) {
+                load_row(r.end - back, next[t]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < V; i++) next[t][i] = 0.0f;
+#pragma unroll
+                for (int u = 0; u < KT - 1; u++)
+                    if (u == t + n)
+#pragma unroll
+                        for (int i = 0; i < V; i++) next[t][i] = past[u][i];
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < KT - 1; t++)
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                const int at = t - (KT - 1 - K1);
+                if (live && at >= 0) state[to * window + (int64_t)(c + i) * K1 + at] = next[t][i];
+            }
+    };
+    if ((int)blockIdx.x >= row_blocks) {  // requests without rows
+        const int j = ((int)blockIdx.x - row_blocks) * 4 + wave;
+        if (j >= a.requests) return;
+        const RowRange r = row_range(offsets, a.rows, j);
+        if (r.end > r.begin) return;
+        load_window(j);
+        store_window(j, r);
+        return;
+    }
+    const int64_t first = ((int64_t)blockIdx.x * 4 + wave) * run;
+    if (first >= a.rows) return;
+    int row = (int)first;
+    const int last = (int)min(first + run, (int64_t)a.rows);
+    int j = wave_request_of_row(offsets, a.requests, row);
+    if (j >= a.requests) return;
+    float w[KT][V];
+#pragma unroll
+    for (int t = 0; t < KT; t++)
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+            const int at = t - (KT - a.kernel);
+            w[t][i] = live && at >= 0 ? weight[(int64_t)(c + i) * a.kernel + at] : 0.0f;
+        }
+    const int keys = a.groups * D;
+    RowRange r = row_range(offsets, a.rows, j);
+    bool fresh = true;  // the window is not in the registers
+    // A request's first K - 1 rows, which need its window, are the wave's that has the first of them: nobody
+    // else reads the slot that it may write.
+    for (;; row++) {
+        while (row >= r.end) {
+            if (row >= last || ++j >= a.requests) return;
+            r = row_range(offsets, a.rows, j);
+            fresh = true;
+        }
+        const bool early = row - r.begin < K1, begun = r.begin >= first;
+        if (row >= last && !(early && begun)) return;
+        if (row < r.begin || (early && !begun)) continue;  // (descending offsets leave rows between requests)
+        if (fresh) {
+            if (row == r.begin) {
+                load_window(j);
+                store_window(j, r);
+            }
+            // rows of the request before this one
+            const int have = min(row - r.begin, KT - 1);
+            float near[KT - 1][V];
+#pragma unroll
+            for (int t = 0; t < KT - 1; t++) {
+                const int back = KT - 1 - t;
+                if (back <= have) {
+                    load_row(row - back, near[t]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < V; i++) near[t][i] = 0.0f;
+#pragma unroll
+                    for (int u = 0; u < KT - 1; u++)
+                        if (u == t + have)
+#pragma unroll
+                            for (int i = 0; i < V; i++) near[t][i] = past[u][i];
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < KT - 1; t++)
+#pragma unroll
+                for (int i = 0; i < V; i++) past[t][i] = near[t][i];
+            fresh = false;
+        }
+        float now[V], y[V], squares = 0.0f;
+        load_row(row, now);
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int t = 0; t < KT - 1; t++)
+                if (t >= KT - 1 - K1) sum = fmaf(w[t][i], past[t][i], sum);
+            y[i] = silu_f32(fmaf(w[KT - 1][i], now[i], sum));
+            squares = fmaf(y[i], y[i], squares);
+        }
+        if (c < 2 * keys) {  // whole heads: a group of lanes takes one way
+            const float norm = (c < keys ? a.scale : 1.0f) / sqrtf(lanes_sum<D / V>(squares) + a.eps);
+#pragma unroll
+            for (int i = 0; i < V; i++) y[i] *= norm;
+        }
+        if (live) *reinterpret_cast<Bytes16 *>(out + (int64_t)row * a.channels + c) = pack<E>(y);
+#pragma unroll
+        for (int t = 0; t < KT - 2; t++)
+#pragma unroll
+            for (int i = 0; i < V; i++) past[t][i] = past[t + 1][i];
+#pragma unroll
+        for (int i = 0; i < V; i++) past[KT - 2][i] = now[i];
+    }
+}
+
+// The delta rule row by row: a workgroup holds COLS columns of one head's state, a
+// thread four of them in every (256 / (COLS / 4))th row.
+//   S = e^g S;  d = beta (v - S^T k);  S += k d^T;  o = S^T q
+template <typename E, int D, int COLS>
+__global__ __launch_bounds__(256) void ragged_scan_kernel(GdnRows b, RaggedArgs a) {
+    constexpr int C4 = COLS / 4, RG = 256 / C4, NR = D / RG, SPAN = C4 < 64 ? C4 : 64;
+    static_assert(D % RG == 0, "whole rows");
+    __shared__ float qk[2][D], vs[COLS];
+    __shared__ float4 part[2][4][C4];
+    typedef typename E::T T;
+    const int h = blockIdx.x, col0 = blockIdx.y * COLS, j = blockIdx.z;
+    const int t = threadIdx.x, wave = t >> 6, lane = t & 63, c4 = t % C4, rg = t / C4;
+    const RowRange r = b.offsets ? row_range(b.offsets, a.rows, j) : RowRange{j, j + 1};
+    const int2 slot = b.slots[j];
+    const int64_t size = (int64_t)a.heads * D * D, mine = (int64_t)h * D * D + col0 + 4 * c4;
+    float4 s[NR];
+#pragma unroll
+    for (int m = 0; m < NR; m++)
+        s[m] = (uint32_t)slot.x < (uint32_t)a.states
+                   ? *reinterpret_cast<const float4 *>(b.state + slot.x * size + mine + (int64_t)(rg + RG * m) * D)
+                   : make_float4(0.f, 0.f, 0.f, 0.f);
+    const T *const qkv = static_cast<const T *>(b.qkv);
+    const int group = h % a.groups;
+    // sum over the row groups of every column, in every thread
+    auto total = [&](float4 x, int which) {
+#pragma unroll
+        for (int off = C4; off < 64; off <<= 1) {
+            x.x += __shfl_xor(x.x, off);
+            x.y += __shfl_xor(x.y, off);
+            x.z += __shfl_xor(x.z, off);
+            x.w += __shfl_xor(x.w, off);
+        }
+        if (lane < SPAN) part[which][wave][c4] = x;
+        __syncthreads();
+        float4 sum = part[which][0][c4];
+#pragma unroll
+        for (int w = 1; w < 4; w++) {
+            const float4 y = part[which][w][c4];
+            sum.x += y.x; sum.y += y.y; sum.z += y.z; sum.w += y.w;
+        }
+        return sum;
+    };
+    for (int row = r.begin; row < r.end; row++) {
+        const T *const x = qkv + (int64_t)row * a.stride;
+        if (t < D) qk[0][t] = (float)x[group * D + t] * a.scale;
+        else if (t < 2 * D) qk[1][t - D] = (float)x[(a.groups + group) * D + t - D];
+        const float own_v = t < COLS ? (float)x[(2 * a.groups + h) * D + col0 + t] : 0.0f;
+        if (t < COLS) vs[t] = own_v;
+        const float decay = expf(log_decay_of(b, a, (int64_t)row * a.heads + h, h));
+        const float beta = beta_of(b, a, (int64_t)row * a.heads + h);
+        __syncthreads();
+        float4 seen = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int m = 0; m < NR; m++) {
+            const float k = qk[1][rg + RG * m];
+            s[m].x *= decay; s[m].y *= decay; s[m].z *= decay; s[m].w *= decay;
+            seen.x = fmaf(s[m].x, k, seen.x);
+            seen.y = fmaf(s[m].y, k, seen.y);
+            seen.z = fmaf(s[m].z, k, seen.z);
+            seen.w = fmaf(s[m].w, k, seen.w);
+        }
+        seen = total(seen, 0);
+        const float4 d = make_float4((vs[4 * c4] - seen.x) * beta, (vs[4 * c4 + 1] - seen.y) * beta,
+                                     (vs[4 * c4 + 2] - seen.z) * beta, (vs[4 * c4 + 3] - seen.w) * beta);
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int m = 0; m < NR; m++) {
+            const float k = qk[1][rg + RG * m], q = qk[0][rg + RG * m];
+            s[m].x = fmaf(k, d.x, s[m].x);
+            s[m].y = fmaf(k, d.y, s[m].y);
+            s[m].z = fmaf(k, d.z, s[m].z);
+            s[m].w = fmaf(k, d.w, s[m].w);
+            o.x = fmaf(s[m].x, q, o.x);
+            o.y = fmaf(s[m].y, q, o.y);
+            o.z = fmaf(s[m].z, q, o.z);
+            o.w = fmaf(s[m].w, q, o.w);
+        }
+        o = total(o, 1);
+        if (t < C4) {
+            T *const to = static_cast<T *>(b.out) + ((int64_t)row * a.heads + h) * D + col0 + 4 * t;
+            to[0] = (T)o.x;
+            to[1] = (T)o.y;
+            to[2] = (T)o.z;
+            to[3] = (T)o.w;
+        }
+        __syncthreads();
+    }
+    if ((uint32_t)slot.y < (uint32_t)a.states) {
+#pragma unroll
+        for (int m = 0; m < NR; m++)
+            *reinterpret_cast<float4 *>(b.state + slot.y * size + mine + (int64_t)(rg + RG * m) * D) = s[m];
+    }
+}
+
+template <typename F> void by_type(uint32_t dtype, F &&f) {
+    if (dtype == YUUKA_DTYPE_F32) f(RowF32{});
+    else if (dtype == YUUKA_DTYPE_F16) f(RowF16{});
+    else f(RowBF16{});
+}
+
+hipError_t launch_scan(const GdnRows &b, uint32_t dtype, const RaggedArgs &a, hipStream_t s) {
+    by_type(dtype, [&](auto e) {
+        using E = decltype(e);
+        auto go = [&](auto d, auto cols) {
+            ragged_scan_kernel<E, d(), cols()><<<dim3(a.heads, d() / cols(), a.requests), 256, 0, s>>>(b, a);
+        };
+        if (a.head_dim == 128) go(std::integral_constant<int, 128>{}, std::integral_constant<int, 32>{});
+        else go(std::integral_constant<int, 64>{}, std::integral_constant<int, 32>{});
+    });
+    return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_gdn_ragged_conv(void *out, const void *x, uint32_t dtype, const float *weight, float *state,
+                                  const int32_t *offsets, const int2 *slots, const RaggedArgs &a, hipStream_t s) {
+    by_type(dtype, [&](auto e) {
+        using E = decltype(e);
+        typedef typename E::T T;
+        const int run = 16;
+        const int row_blocks = (int)(((int64_t)a.rows + 4 * run - 1) / (4 * run));
+        const dim3 grid(row_blocks + (a.requests + 3) / 4, (a.channels + 64 * E::kWide - 1) / (64 * E::kWide));
+        auto go = [&](auto taps, auto d) {
+            ragged_conv_kernel<E, taps(), d()><<<grid, 256, 0, s>>>(static_cast<T *>(out), static_cast<const T *>(x), weight,
+                                                                    state, offsets, slots, a, run, row_blocks);
+        };
+        auto by_dim = [&](auto taps) {
+            if (a.head_dim == 128) go(taps, std::integral_constant<int, 128>{});
+            else go(taps, std::integral_constant<int, 64>{});
+        };
+        if (a.kernel <= 4) by_dim(std::integral_constant<int, 4>{});
+        else by_dim(std::integral_constant<int, 8>{});
+    });
+    return hipGetLastError();
+}
+
+hipError_t launch_gdn_step(const GdnRows &b, uint32_t dtype, const RaggedArgs &a, hipStream_t s) {
+    return launch_scan(b, dtype, a, s);
+}
+
+uint64_t gdn_prompt_scratch_bytes(const RaggedArgs &) { return 0; }
+
+hipError_t launch_gdn_prompt(const GdnRows &b, uint32_t dtype, const RaggedArgs &a, void *, hipStream_t s) {
+    return launch_scan(b, dtype, a, s);
+}
+
+}  // namespace yk

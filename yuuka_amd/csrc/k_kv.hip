@@ -145,11 +145,13 @@ __device__ __forceinline__ uint32_t transpose_digits(uint32_t mine, int r) {
 // read back 45.8 us, one 51.2, four 48.4.
 constexpr int kAppendWaves = 4, kAppendRows = 2;
 
-template <int FMT, int GROUPS>
+// SLOTS: `slots` says where each row goes, instead of the table and the position.
+template <int FMT, int GROUPS, bool SLOTS>
 __global__ __launch_bounds__(64 * kAppendWaves) void kv_append_kernel(
     const float *__restrict__ k, const float *__restrict__ v, uint8_t *__restrict__ kpool, uint8_t *__restrict__ vpool,
     const int32_t *__restrict__ table, const float *__restrict__ k_norm, const float2 *__restrict__ rope,
-    const float *__restrict__ q, const float *__restrict__ q_norm, float *__restrict__ q_out, KvArgs a, ModelDyn dyn) {
+    const float *__restrict__ q, const float *__restrict__ q_norm, float *__restrict__ q_out, KvArgs a, ModelDyn dyn,
+    const int64_t *__restrict__ slots) {
     constexpr int D = 64 * GROUPS, HPW = heads_per_wave(GROUPS);
     __shared__ float swap[kAppendWaves][256];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -174,12 +176,16 @@ __global__ __launch_bounds__(64 * kAppendWaves) void kv_append_kernel(
         rows[n] = live && first_row + n < a.rows ? __builtin_nontemporal_load(reinterpret_cast<const floats4 *>(src + n * stride)) : none;
     const float *norm = query ? q_norm : value ? nullptr : k_norm;
     const floats4 weight = norm && ld.live ? *reinterpret_cast<const floats4 *>(norm + ld.first) : none;
-    const int64_t p0 = query ? 0 : kv_position(a, dyn, j, first_row);
+    const int64_t p0 = query || SLOTS ? 0 : kv_position(a, dyn, j, first_row);
 #pragma unroll
     for (int n = 0; n < kAppendRows; n++) {
         if (first_row + n >= a.rows) return;
         int64_t at = 0, sc = 0;
-        if (!query && !kv_slot(a, table, j, p0 + n, &at, &sc)) continue;
+        if constexpr (SLOTS) {
+            if (!kv_row_of_slot(a, slots[first_row + n], &at, &sc)) continue;
+        } else {
+            if (!query && !kv_slot(a, table, j, p0 + n, &at, &sc)) continue;
+        }
         const int64_t row = row0 + n;
         float x[4] = {rows[n][0], rows[n][1], rows[n][2], rows[n][3]};
         if (norm) {  // x * (1 / rms * w), forward.go:472-482
@@ -383,9 +389,21 @@ hipError_t launch_kv_append(const float *k, const float *v, void *kpool, void *v
     const int64_t items = ((int64_t)a.rows + kAppendRows - 1) / kAppendRows * (2 * ((a.kv_heads + hpw - 1) / hpw) + (q ? (a.heads + hpw - 1) / hpw : 0));
     const int64_t blocks = (items + kAppendWaves - 1) / kAppendWaves;
     return by_format(a, [&](auto fmt, auto n) {
-        kv_append_kernel<fmt(), n()><<<dim3((uint32_t)blocks, (uint32_t)a.requests), 64 * kAppendWaves, 0, s>>>(
+        kv_append_kernel<fmt(), n(), false><<<dim3((uint32_t)blocks, (uint32_t)a.requests), 64 * kAppendWaves, 0, s>>>(
             k, v, static_cast<uint8_t *>(kpool), static_cast<uint8_t *>(vpool), table, k_norm,
-            a.rope_dim ? rope : nullptr, q, q_norm, q_out, a, dyn);
+            a.rope_dim ? rope : nullptr, q, q_norm, q_out, a, dyn, nullptr);
+    });
+}
+
+hipError_t launch_kv_append_slots(const float *k, const float *v, void *kpool, void *vpool, const int64_t *slots,
+                                  const float *k_norm, const float2 *rope, const KvArgs &a, hipStream_t s) {
+    const int hpw = heads_per_wave(a.head_dim / 64);
+    const int64_t items = ((int64_t)a.rows + kAppendRows - 1) / kAppendRows * (2 * ((a.kv_heads + hpw - 1) / hpw));
+    const int64_t blocks = (items + kAppendWaves - 1) / kAppendWaves;
+    return by_format(a, [&](auto fmt, auto n) {
+        kv_append_kernel<fmt(), n(), true><<<(uint32_t)blocks, 64 * kAppendWaves, 0, s>>>(
+            k, v, static_cast<uint8_t *>(kpool), static_cast<uint8_t *>(vpool), nullptr, k_norm,
+            a.rope_dim ? rope : nullptr, nullptr, nullptr, nullptr, a, ModelDyn{}, slots);
     });
 }
 

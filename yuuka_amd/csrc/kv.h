@@ -43,6 +43,9 @@ inline uint64_t kv_span_rows(const KvArgs &a) { return (uint64_t)(a.requests - 1
 hipError_t launch_kv_append(const float *k, const float *v, void *kpool, void *vpool, const int32_t *table,
                             const float *k_norm, const float2 *rope, const float *q, const float *q_norm,
                             float *q_out, const KvArgs &a, const ModelDyn &dyn, hipStream_t s);
+// The same for a.rows rows that go to slots[row] each (k and v only).
+hipError_t launch_kv_append_slots(const float *k, const float *v, void *kpool, void *vpool, const int64_t *slots,
+                                  const float *k_norm, const float2 *rope, const KvArgs &a, hipStream_t s);
 // Positions base + displacement + r of every request as float32 rows; a null
 // pool or output leaves that side out.
 hipError_t launch_kv_read(const void *kpool, const void *vpool, const int32_t *table, float *k_out, float *v_out,

@@ -60,4 +60,16 @@ YK_HD bool kv_slot(const KvLayout &a, const int32_t *table, int j, int64_t p, in
     return true;
 }
 
+// The same for a row that goes to `slot`, token slot % block_size of page slot / block_size; false for a
+// slot outside the pool, such as -1.
+YK_HD bool kv_row_of_slot(const KvLayout &a, int64_t slot, int64_t *row, int64_t *scales) {
+    if (slot < 0 || slot >= (int64_t)a.pages * a.block_size) return false;
+    const int64_t page = slot <= 0x7fffffff ? (uint32_t)slot / (uint32_t)a.block_size : slot / a.block_size;
+    const int64_t t = slot - page * a.block_size, base = page * kv_page_bytes(a);
+    const bool q8 = a.fmt == kKvQ8;
+    *row = base + t * (q8 ? (int64_t)a.kv_dim : kv_token_bytes(a.fmt, a.kv_dim));
+    *scales = q8 ? base + (int64_t)a.block_size * a.kv_dim + t * (a.kv_dim / 32) * 2 : 0;
+    return true;
+}
+
 }  // namespace yk

@@ -764,6 +764,7 @@ bool op_uses_position(const yuuka_op &op) {
 yuuka_status validate_model_op(const yuuka_op &op, uint64_t *ws) {
     *ws = 0;
     if (kv_op(op)) return validate_kv_op(op, ws);
+    if (ragged_op(op)) return validate_ragged_op(op, ws);
     bool decode = false;
     const yuuka_status dst = validate_decode_op(op, ws, &decode);
     if (decode) return dst;
@@ -1223,6 +1224,7 @@ yuuka_status execute_model_op(const yuuka_op &op, const ExecCtx &ctx) {
         if (err != hipSuccess) return fail(YUUKA_ERR_DEVICE, "op %u launch: %s", op.code, hip_error(err));
         return YUUKA_OK;
     }
+    if (ragged_op(op)) return execute_ragged_op(op, ctx);
     bool decode = false;
     const yuuka_status dst = execute_decode_op(op, ctx, &decode);
     if (decode) return dst;

@@ -13,6 +13,10 @@ namespace yk {
 // workspace bytes it needs. Unknown codes fail with YUUKA_ERR_UNSUPPORTED.
 yuuka_status validate_model_op(const yuuka_op &op, uint64_t *ws);
 yuuka_status execute_model_op(const yuuka_op &op, const ExecCtx &ctx);
+// The ops over ragged batches (ops_ragged.cpp).
+bool ragged_op(const yuuka_op &op);
+yuuka_status validate_ragged_op(const yuuka_op &op, uint64_t *ws);
+yuuka_status execute_ragged_op(const yuuka_op &op, const ExecCtx &ctx);
 // True when the op reads the execution position (graph capture then needs
 // the dynamic-parameter buffer).
 bool op_uses_position(const yuuka_op &op);

@@ -19,7 +19,7 @@ HEADER = Path(__file__).resolve().parent.parent / "include" / "yuuka_hip.h"
 OK, INVALID_ARGUMENT, UNSUPPORTED, DEVICE, ALLOCATION, INTERNAL = range(6)
 
 # yuuka_dtype (include/yuuka_hip.h)
-F32, F16, Q4_0, Q5_0, Q8_0, Q4_K, Q5_K, Q6_K = 0, 1, 2, 6, 8, 12, 13, 14
+F32, F16, Q4_0, Q5_0, Q8_0, Q4_K, Q5_K, Q6_K, BF16 = 0, 1, 2, 6, 8, 12, 13, 14, 30
 
 # op codes used by the verify plan
 OP = dict(
@@ -28,6 +28,7 @@ OP = dict(
     ATTENTION_PREFILL_PAGED=29, MOE_ROUTE=30, MOE_GATE_UP=31, MOE_DOWN=32, MOE_REDUCE_ADD=33, LM_HEAD=37,
     ACCEPT=66, GDN_COMMIT=67, ADVANCE=68, GEMM_FUSED=69, ROPE_TABLE=70, ATTN_VERIFY=71, MOE_ROUTER=72,
     MOE_COMBINE=73, ROUTER_NORMAL=74, KV_APPEND=75, KV_READ=76, ATTN_DECODE=77,
+    BATCH_PLAN=78, KV_APPEND_SLOTS=79, GDN_CONV=80, GDN_PROMPT=81, GDN_STEP=82,
 )
 FLAG_MOE_SWIGLU = 0x800
 FLAG_MOE_PACKED = 0x2000
@@ -80,6 +81,16 @@ class yuuka_kv_params(C.Structure):
     _fields_ = [("dtype", C.c_uint32)] + [(n, C.c_int32) for n in (
         "block_size", "capacity", "requests", "rows", "request_rows", "heads", "kv_heads", "head_dim", "rope_dim",
         "gated", "displacement")] + [("scale", C.c_float), ("eps", C.c_float)]
+
+
+class yuuka_batch_params(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("requests", "rows", "block_size", "capacity")]
+
+
+class yuuka_gdn_params(C.Structure):
+    _fields_ = [("dtype", C.c_uint32)] + [(n, C.c_int32) for n in (
+        "requests", "rows", "groups", "heads", "head_dim", "kernel", "row_stride", "log_decay")] + [
+        ("scale", C.c_float), ("eps", C.c_float)]
 
 
 class yuuka_device_info(C.Structure):
@@ -158,6 +169,11 @@ def _declare(L: C.CDLL) -> None:
         "yuuka_kv_append": (C.c_int, [vp] * 9 + [C.POINTER(yuuka_kv_params), vp]),
         "yuuka_kv_read": (C.c_int, [vp] * 7 + [C.POINTER(yuuka_kv_params), vp]),
         "yuuka_attn_decode": (C.c_int, [vp] * 7 + [C.POINTER(yuuka_kv_params), vp]),
+        "yuuka_batch_plan": (C.c_int, [vp] * 12 + [C.POINTER(yuuka_batch_params), vp]),
+        "yuuka_kv_append_slots": (C.c_int, [vp] * 8 + [C.POINTER(yuuka_kv_params), vp]),
+        "yuuka_gdn_conv": (C.c_int, [vp] * 7 + [C.POINTER(yuuka_gdn_params), vp]),
+        "yuuka_gdn_prompt": (C.c_int, [vp] * 10 + [C.POINTER(yuuka_gdn_params), vp]),
+        "yuuka_gdn_step": (C.c_int, [vp] * 9 + [C.POINTER(yuuka_gdn_params), vp]),
         "yuuka_plan_create": (C.c_int, [vp, C.POINTER(vp)]),
         "yuuka_plan_destroy": (None, [vp]),
         "yuuka_plan_add": (C.c_int, [vp, C.POINTER(yuuka_op)]),
@@ -372,6 +388,56 @@ def attn_decode(stream: Stream, out: Buffer, q: Buffer, kpool: Buffer, vpool: Bu
     """Attention of the newest rows over the paged cache."""
     check(lib().yuuka_attn_decode(stream.ptr, _p(out), _p(q), _p(kpool), _p(vpool), _p(table), _p(positions),
                                   C.byref(params), _p(event)), "attn_decode")
+
+
+def batch_params(requests: int, rows: int, block_size: int, capacity: int) -> yuuka_batch_params:
+    return yuuka_batch_params(requests, rows, block_size, capacity)
+
+
+def batch_plan(stream: Stream, positions: Buffer, counts: Buffer, blocks: Buffer, table: Buffer, free_pages: Buffer,
+               pool: Buffer, offsets: Buffer, row_info: Buffer, slots: Buffer, blocks_out: Buffer, pool_out: Buffer,
+               params: yuuka_batch_params, event: Event | None = None) -> None:
+    """Offsets, row requests and positions, slots and new pages of a ragged batch."""
+    check(lib().yuuka_batch_plan(stream.ptr, _p(positions), _p(counts), _p(blocks), _p(table), _p(free_pages), _p(pool),
+                                 _p(offsets), _p(row_info), _p(slots), _p(blocks_out), _p(pool_out), C.byref(params),
+                                 _p(event)), "batch_plan")
+
+
+def kv_append_slots(stream: Stream, k: Buffer, v: Buffer, kpool: Buffer, vpool: Buffer, slots: Buffer,
+                    params: yuuka_kv_params, k_norm: Buffer | None = None, rope: Buffer | None = None,
+                    event: Event | None = None) -> None:
+    """Rounds key and value rows into the slots of the paged pools."""
+    check(lib().yuuka_kv_append_slots(stream.ptr, _p(k), _p(v), _p(kpool), _p(vpool), _p(slots), _p(k_norm), _p(rope),
+                                      C.byref(params), _p(event)), "kv_append_slots")
+
+
+def gdn_params(dtype: int, requests: int, rows: int, groups: int, heads: int, head_dim: int, kernel: int = 4,
+               row_stride: int = 0, log_decay: bool = False, scale: float = 1.0, eps: float = 1e-6) -> yuuka_gdn_params:
+    return yuuka_gdn_params(dtype, requests, rows, groups, heads, head_dim, kernel, row_stride, int(log_decay), scale,
+                            eps)
+
+
+def gdn_conv(stream: Stream, out: Buffer, x: Buffer, weight: Buffer, windows: Buffer, offsets: Buffer, slots: Buffer,
+             params: yuuka_gdn_params, event: Event | None = None) -> None:
+    """Causal convolution, SiLU and q / k norm of ragged rows, with the requests' windows."""
+    check(lib().yuuka_gdn_conv(stream.ptr, _p(out), _p(x), _p(weight), _p(windows), _p(offsets), _p(slots),
+                               C.byref(params), _p(event)), "gdn_conv")
+
+
+def gdn_prompt(stream: Stream, out: Buffer, qkv: Buffer, alpha: Buffer, beta: Buffer, states: Buffer, offsets: Buffer,
+               slots: Buffer, params: yuuka_gdn_params, dt: Buffer | None = None, a: Buffer | None = None,
+               event: Event | None = None) -> None:
+    """The gated delta rule over ragged rows, with the requests' states."""
+    check(lib().yuuka_gdn_prompt(stream.ptr, _p(out), _p(qkv), _p(alpha), _p(beta), _p(dt), _p(a), _p(states),
+                                 _p(offsets), _p(slots), C.byref(params), _p(event)), "gdn_prompt")
+
+
+def gdn_step(stream: Stream, out: Buffer, qkv: Buffer, alpha: Buffer, beta: Buffer, states: Buffer, slots: Buffer,
+             params: yuuka_gdn_params, dt: Buffer | None = None, a: Buffer | None = None,
+             event: Event | None = None) -> None:
+    """The gated delta rule over one row of every request."""
+    check(lib().yuuka_gdn_step(stream.ptr, _p(out), _p(qkv), _p(alpha), _p(beta), _p(dt), _p(a), _p(states), _p(slots),
+                               C.byref(params), _p(event)), "gdn_step")
 
 
 def gemm_fused_op(plan: "Plan", x: Buffer, n_in: int, rows: int, segments, epilogue: int = 0,
