@@ -344,10 +344,4 @@ hipError_t launch_gdn_step(const GdnRows &b, uint32_t dtype, const RaggedArgs &a
     return launch_scan(b, dtype, a, s);
 }
 
-uint64_t gdn_prompt_scratch_bytes(const RaggedArgs &) { return 0; }
-
-hipError_t launch_gdn_prompt(const GdnRows &b, uint32_t dtype, const RaggedArgs &a, void *, hipStream_t s) {
-    return launch_scan(b, dtype, a, s);
-}
-
 }  // namespace yk
