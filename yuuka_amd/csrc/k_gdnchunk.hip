@@ -37,6 +37,13 @@ __device__ __forceinline__ f32x4 mma(f32x4 a, f32x4 b, f32x4 c) {
 }
 constexpr f32x4 kZero = {0.f, 0.f, 0.f, 0.f};
 
+// A barrier for what is in LDS: loads from memory stay under way.
+__device__ __forceinline__ void lds_barrier() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
 // What the first kernel leaves for a chunk and head: operands as the second loads them, 64 lanes
 // of 16 bytes each.
 template <int D> struct Left {
@@ -247,7 +254,7 @@ __global__ __launch_bounds__(256) void chunk_prepare_kernel(GdnRows b, RaggedArg
 // A workgroup has CT tiles of 16 columns of one head's state; wave w the state's rows D / 4 w .. and the
 // chunk's rows 16 w .. + 15.
 template <typename E, int D, int CT>
-__global__ __launch_bounds__(256) void chunk_scan_kernel(GdnRows b, RaggedArgs a, const float *__restrict__ left,
+__global__ __launch_bounds__(256, 1) void chunk_scan_kernel(GdnRows b, RaggedArgs a, const float *__restrict__ left,
                                                          const float *__restrict__ keys) {
     typedef typename E::T T;
     constexpr int KT = D / 16, ST = D / 64;
@@ -270,60 +277,94 @@ __global__ __launch_bounds__(256) void chunk_scan_kernel(GdnRows b, RaggedArgs a
                 s[t][c][e] = (uint32_t)slot.x < (uint32_t)a.states
                                  ? b.state[slot.x * size + at0 + (int64_t)(16 * (wave * ST + t) + 4 * g4 + e) * D + 16 * c]
                                  : 0.0f;
-    int number = first_chunk<kC>(r.begin, j);
-    for (int row0 = r.begin; row0 < r.end; row0 += kC, number++) {
-        const int n = min(kC, r.end - row0);
-        const float *const mine = left + ((int64_t)number * a.heads + h) * L::floats;
-        const float *const group_keys = keys + ((int64_t)number * a.groups + group) * L::keys;
-        const T *const q = static_cast<const T *>(b.qkv) + (int64_t)(row0 + 16 * wave + r16) * a.stride + group * D + 4 * g4;
+    // A chunk's operands are loaded while the one before it is worked on, each as soon as its registers are free.
+    typedef T T4 __attribute__((ext_vector_type(4)));
+    f32x4 w[KT], u[CT], p[4], k[ST][4], front, tail;
+    T4 q[KT];
+    float fall;
+    const int number0 = first_chunk<kC>(r.begin, j), last = (r.end - r.begin + kC - 1) / kC - 1;
+    auto chunk_at = [&](int i) { return left + ((int64_t)(number0 + min(i, last)) * a.heads + h) * L::floats; };
+    auto load_row = [&](int i, int t) {
+        const int row = r.begin + i * kC + 16 * wave + r16;
+        q[t] = T4{0, 0, 0, 0};
+        if (row < r.end)
+            q[t] = *reinterpret_cast<const T4 *>(static_cast<const T *>(b.qkv) + (int64_t)row * a.stride + group * D + 16 * t + 4 * g4);
+        w[t] = *reinterpret_cast<const f32x4 *>(chunk_at(i) + L::w + ((wave * KT + t) * 64 + lane) * 4);
+    };
+    auto load_rest = [&](int i) {
+        const float *const mine = chunk_at(i);
+#pragma unroll
+        for (int c = 0; c < CT; c++)
+            u[c] = *reinterpret_cast<const f32x4 *>(mine + L::u + ((wave * KT + col0 / 16 + c) * 64 + lane) * 4);
+        front = *reinterpret_cast<const f32x4 *>(mine + L::v + 16 * wave + 4 * g4);
+        tail = *reinterpret_cast<const f32x4 *>(mine + L::v + kC + 16 * wave + 4 * g4);
+        fall = mine[L::v + 2 * kC];
+    };
+    auto load_p = [&](int i, int t) {
+        if (t <= wave) p[t] = *reinterpret_cast<const f32x4 *>(chunk_at(i) + L::p + (p_tile(wave, t) * 64 + lane) * 4);
+    };
+    auto load_k = [&](int i, int x, int t) {
+        k[x][t] = *reinterpret_cast<const f32x4 *>(keys + ((int64_t)(number0 + min(i, last)) * a.groups + group) * L::keys +
+                                                   ((t * KT + wave * ST + x) * 64 + lane) * 4);
+    };
+    if (last >= 0) {
+#pragma unroll
+        for (int t = 0; t < KT; t++) load_row(0, t);
+        load_rest(0);
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            load_p(0, t);
+#pragma unroll
+            for (int x = 0; x < ST; x++) load_k(0, x, t);
+        }
+    }
+    for (int i = 0; i <= last; i++) {
+        const int row0 = r.begin + i * kC, n = min(kC, r.end - row0);
 #pragma unroll
         for (int t = 0; t < ST; t++)
 #pragma unroll
             for (int c = 0; c < CT; c++) ls[wave * ST + t][c][lane] = s[t][c];
-        __syncthreads();
+        lds_barrier();
         f32x4 ws[CT], o[CT];
 #pragma unroll
         for (int c = 0; c < CT; c++) ws[c] = o[c] = kZero;
 #pragma unroll
         for (int t = 0; t < KT; t++) {
-            const f32x4 w = *reinterpret_cast<const f32x4 *>(mine + L::w + ((wave * KT + t) * 64 + lane) * 4);
-            const f32x4 x = four<E>(q + 16 * t, 16 * wave + r16 < n);
+            const f32x4 x = {(float)q[t][0], (float)q[t][1], (float)q[t][2], (float)q[t][3]};
 #pragma unroll
             for (int c = 0; c < CT; c++) {
                 const f32x4 y = ls[t][c][lane];
-                ws[c] = mma(w, y, ws[c]);
+                ws[c] = mma(w[t], y, ws[c]);
                 o[c] = mma(x, y, o[c]);
             }
+            load_row(i + 1, t);
         }
-        const f32x4 front = *reinterpret_cast<const f32x4 *>(mine + L::v + 16 * wave + 4 * g4);
-        const f32x4 tail = *reinterpret_cast<const f32x4 *>(mine + L::v + kC + 16 * wave + 4 * g4);
-        const float fall = mine[L::v + 2 * kC];
+        const float before = fall;
 #pragma unroll
         for (int c = 0; c < CT; c++) {
-            const f32x4 u = *reinterpret_cast<const f32x4 *>(mine + L::u + ((wave * KT + col0 / 16 + c) * 64 + lane) * 4);
-            const f32x4 x = u - ws[c];
+            const f32x4 x = u[c] - ws[c];
             lv[wave][c][lane] = x;
             lt[wave][c][lane] = x * tail;
             o[c] *= front;
         }
-        __syncthreads();
+        load_rest(i + 1);
+        lds_barrier();
+#pragma unroll
+        for (int x = 0; x < ST; x++)
+#pragma unroll
+            for (int c = 0; c < CT; c++) s[x][c] *= before;
 #pragma unroll
         for (int t = 0; t < 4; t++) {
-            if (t > wave) break;
-            const f32x4 p = *reinterpret_cast<const f32x4 *>(mine + L::p + (p_tile(wave, t) * 64 + lane) * 4);
 #pragma unroll
-            for (int c = 0; c < CT; c++) o[c] = mma(p, lv[t][c][lane], o[c]);
-        }
+            for (int c = 0; c < CT; c++) {
+                const f32x4 y = lt[t][c][lane];
 #pragma unroll
-        for (int u = 0; u < ST; u++) {
-#pragma unroll
-            for (int c = 0; c < CT; c++) s[u][c] *= fall;
-#pragma unroll
-            for (int t = 0; t < 4; t++) {
-                const f32x4 x = *reinterpret_cast<const f32x4 *>(group_keys + ((t * KT + wave * ST + u) * 64 + lane) * 4);
-#pragma unroll
-                for (int c = 0; c < CT; c++) s[u][c] = mma(x, lt[t][c][lane], s[u][c]);
+                for (int x = 0; x < ST; x++) s[x][c] = mma(k[x][t], y, s[x][c]);
+                if (t <= wave) o[c] = mma(p[t], lv[t][c][lane], o[c]);
             }
+#pragma unroll
+            for (int x = 0; x < ST; x++) load_k(i + 1, x, t);
+            load_p(i + 1, t);
         }
         T *const out = static_cast<T *>(b.out) + ((int64_t)(row0 + 16 * wave + 4 * g4) * a.heads + h) * D + col0 + r16;
 #pragma unroll
