@@ -2,16 +2,16 @@
 // 64 rows at a time.
 //
 // With c_i the sum of the log decays of a chunk's rows up to i, and S the state before it,
-//   A_ij = beta_i (k_i . k_j) e^(c_i - c_j)  for i > j
-//   (I + A) U = diag(beta) V,   (I + A) W = diag(beta e^c) K
-//   V' = U - W S                                 the rows' corrections, d_i in the rule
+//   A_ij = beta_i (k_i . k_j) e^(c_i - c_j)  for i > j,    T = (I + A)^-1
+//   V' = T (beta V - beta e^c (K S))             the rows' corrections, d_i in the rule
 //   out = e^c (Q S) + P V',     P_ij = (q_i . k_j) e^(c_i - c_j)  for i >= j
 //   S <- e^(c_last) S + K^T diag(e^(c_last - c)) V'
-// The first kernel makes U, W and P of every chunk and head, all chunks at once; the second
+// The first kernel makes T and P of every chunk and head, all chunks at once; the second
 // walks the chunks of a request with S in registers.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <mutex>
 #include <type_traits>
 
 #include "gdn_ragged_dev.h"
@@ -21,10 +21,15 @@ namespace yk {
 namespace {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kC = 64;           // rows of a chunk
+constexpr int kC = 64;             // rows of a chunk
 constexpr int kRowPitch = kC + 4;  // floats of a row of A in LDS
 constexpr float kLeast = -200.0f;  // e^-200 is zero in float32, and the sums of 64 stay exact to 1e-12 in float64
+constexpr f32x4 kZero = {0.f, 0.f, 0.f, 0.f};
 
 // Products on v_mfma_f32_16x16x4_f32. Lane l has row (A) or column (B) l % 16 and, of 16 terms of
 // the sum, 4 (l / 16) + e in the e-th of four instructions; the result's lane has column l % 16 and
@@ -35,7 +40,58 @@ __device__ __forceinline__ f32x4 mma(f32x4 a, f32x4 b, f32x4 c) {
     for (int e = 0; e < 4; e++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], c, 0, 0, 0);
     return c;
 }
-constexpr f32x4 kZero = {0.f, 0.f, 0.f, 0.f};
+
+// The same for 32 terms on v_mfma_f32_16x16x32_bf16, lane l with terms 4 (l / 16) + e of two tiles of 16:
+// a float32 is the sum of three bf16 (8 bits each, cut off), a half of two. Of the products of parts those
+// below 2^-23 of the whole are left out: six instructions of 16 cycles for eight of 32.
+// The first part's product with the first is summed apart from the small ones.
+struct Sum {
+    f32x4 big, small;
+    __device__ __forceinline__ f32x4 all() const { return big + small; }
+};
+template <int NA, int NB>
+__device__ __forceinline__ void mma32(const u32x4 (&a)[NA], const u32x4 (&b)[NB], Sum &c) {
+#pragma unroll
+    for (int order = 2; order >= 0; order--)
+#pragma unroll
+        for (int i = 0; i < NA; i++)
+#pragma unroll
+            for (int k = 0; k < NB; k++) {
+                if (i + k != order) continue;
+                f32x4 &to = order ? c.small : c.big;
+                to = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a[i]), __builtin_bit_cast(bf16x8, b[k]),
+                                                             to, 0, 0, 0);
+            }
+}
+// The first N parts of two values, one dword each.
+template <int N> __device__ __forceinline__ void split(float x, float y, uint32_t (&p)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        const uint32_t u = __float_as_uint(x), v = __float_as_uint(y);
+        p[i] = __builtin_amdgcn_perm(v, u, 0x07060302u);
+        if (i == N - 1) break;
+        x -= __uint_as_float(u & 0xffff0000u);
+        y -= __uint_as_float(v & 0xffff0000u);
+    }
+}
+template <int N> __device__ __forceinline__ void split(f32x4 x, u32x2 (&p)[N]) {
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        uint32_t d[N];
+        split(x[2 * i], x[2 * i + 1], d);
+#pragma unroll
+        for (int k = 0; k < N; k++) p[k][i] = d[k];
+    }
+}
+template <int N> __device__ __forceinline__ void split(f32x4 x, f32x4 y, u32x4 (&p)[N]) {
+    u32x2 a[N], b[N];
+    split(x, a);
+    split(y, b);
+#pragma unroll
+    for (int k = 0; k < N; k++) p[k] = u32x4{a[k][0], a[k][1], b[k][0], b[k][1]};
+}
+// bf16 parts that hold a row's element exactly.
+template <typename E> constexpr int kParts = std::is_same<E, RowF32>::value ? 3 : std::is_same<E, RowF16>::value ? 2 : 1;
 
 // A barrier for what is in LDS: loads from memory stay under way.
 __device__ __forceinline__ void lds_barrier() {
@@ -44,36 +100,65 @@ __device__ __forceinline__ void lds_barrier() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
-// What the first kernel leaves for a chunk and head: operands as the second loads them, 64 lanes
-// of 16 bytes each.
-template <int D> struct Left {
-    static constexpr int kTiles = D / 16;
-    static constexpr int w = 0;                      // [row tile][tile of k's dims]: A of W S
-    static constexpr int u = w + 4 * kTiles * 256;   // [row tile][tile of v's dims]: C layout
-    static constexpr int p = u + 4 * kTiles * 256;   // [row tile i, tile j <= i]: A of P V'
-    static constexpr int v = p + 10 * 256;           // scale e^c of every row, e^(c_last - c), e^c_last
-    static constexpr int floats = v + 2 * kC + 64;
-    static constexpr int keys = 4 * kTiles * 256;    // of a group: [row tile][tile of k's dims], A of K^T V'
-};
-constexpr int p_tile(int i, int j) { return i * (i + 1) / 2 + j; }
-
-// Four consecutive elements of a row, zeros for a row that is not there.
-template <typename E> __device__ __forceinline__ f32x4 four(const typename E::T *at, bool there) {
-    typedef typename E::T T4 __attribute__((ext_vector_type(4)));
-    T4 x = {0, 0, 0, 0};
-    if (there) x = *reinterpret_cast<const T4 *>(at);
-    return f32x4{(float)x[0], (float)x[1], (float)x[2], (float)x[3]};
+// 16 lanes give the addresses of four rows of 16 elements, four elements each; a lane gets a column.
+__device__ __forceinline__ u32x2 columns_of(const uint8_t *at) {
+    typedef short s16x4 __attribute__((ext_vector_type(4)));
+    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (__attribute__((address_space(3))) s16x4 *)(const_cast<uint8_t *>(at))));
 }
 
+// What the first kernel leaves for a chunk and head: operands as the second loads them, 64 lanes
+// of 16 bytes each (256 dwords).
+namespace left {
+constexpr int t = 0;              // [step][part] of T
+constexpr int p = 6 * 3 * 256;    // [step][part] of P
+constexpr int v = 2 * p;          // float32: beta, beta e^c, scale e^c, e^(c_last - c) of every row, e^c_last 64 times
+constexpr int dwords = v + 5 * kC;
+// Row tile i against rows 32 s .. (those up to its own are there).
+constexpr int step(int i, int s) { return i < 2 ? i : 2 * i - 2 + s; }
+}  // namespace left
+
+// Rows as operands of products over their dims, zeros for one that is not there.
+template <typename E, int D> struct RowOperand {  // 16-bit: products are exact
+    u32x4 x[D / 32];
+    __device__ __forceinline__ void load(const typename E::T *row, int g4, bool there) {
+#pragma unroll
+        for (int s = 0; s < D / 32; s++)
+            x[s] = there ? *reinterpret_cast<const u32x4 *>(row + 32 * s + 8 * g4) : u32x4{0, 0, 0, 0};
+    }
+    __device__ __forceinline__ f32x4 times(const RowOperand &o) const {
+        f32x4 c = kZero;
+#pragma unroll
+        for (int s = 0; s < D / 32; s++) {
+            if constexpr (std::is_same<E, RowF16>::value)
+                c = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, x[s]), __builtin_bit_cast(f16x8, o.x[s]), c, 0, 0, 0);
+            else
+                c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x[s]), __builtin_bit_cast(bf16x8, o.x[s]), c, 0, 0, 0);
+        }
+        return c;
+    }
+};
+template <int D> struct RowOperand<RowF32, D> {
+    f32x4 x[D / 16];
+    __device__ __forceinline__ void load(const float *row, int g4, bool there) {
+#pragma unroll
+        for (int s = 0; s < D / 16; s++) x[s] = there ? *reinterpret_cast<const f32x4 *>(row + 16 * s + 4 * g4) : kZero;
+    }
+    __device__ __forceinline__ f32x4 times(const RowOperand &o) const {
+        f32x4 c = kZero;
+#pragma unroll
+        for (int s = 0; s < D / 16; s++) c = mma(x[s], o.x[s], c);
+        return c;
+    }
+};
+
+// Eight waves: four for k_i . k_j and T, four for q_i . k_j.
 template <typename E, int D>
-__global__ __launch_bounds__(256) void chunk_prepare_kernel(GdnRows b, RaggedArgs a, float *__restrict__ left,
-                                                            float *__restrict__ keys) {
+__global__ __launch_bounds__(512) void chunk_prepare_kernel(GdnRows b, RaggedArgs a, uint32_t *__restrict__ left_all) {
     typedef typename E::T T;
-    constexpr int KT = D / 16;
-    using L = Left<D>;
     __shared__ double sum[kC];
-    __shared__ __align__(16) float beta[kC], grown[kC];  // e^c
-    __shared__ __align__(16) float am[kC][kRowPitch], tm[kC][kRowPitch];  // A with its diagonal blocks' inverses; T diag(beta)
+    __shared__ __align__(16) float beta[kC];
+    __shared__ __align__(16) float at[kC][kRowPitch];  // A^T, its diagonal blocks later those of T^T
     const int number = blockIdx.x, h = blockIdx.y;
     // the request whose chunk this is
     const int after = wave_first(a.requests, [&](int j) {
@@ -86,16 +171,18 @@ __global__ __launch_bounds__(256) void chunk_prepare_kernel(GdnRows b, RaggedArg
     if (n <= 0) return;
     const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g4 = lane >> 4;
     // the waves' parts differ in length: turned from chunk to chunk, so that no SIMD has the longest each time
-    const int wave = (__builtin_amdgcn_readfirstlane(tid >> 6) + number + h) & 3;
+    const int role = (__builtin_amdgcn_readfirstlane(tid >> 6) + number + h) & 7, wave = role & 3;
+    const bool keys = role < 4;
     const T *const rows = static_cast<const T *>(b.qkv) + (int64_t)row0 * a.stride;
     const int group = h % a.groups;
-    const T *const q = rows + group * D, *const k = rows + (a.groups + group) * D, *const v = rows + (2 * a.groups + h) * D;
-    float *const mine = left + ((int64_t)number * a.heads + h) * L::floats;
+    const T *const k = rows + (a.groups + group) * D, *const mine = keys ? k : rows + group * D;
+    uint32_t *const left_here = left_all + ((int64_t)number * a.heads + h) * left::dwords;
 
-    if (wave == 0) {  // a row a lane
+    if (role == 7) {  // a row a lane
+        float *const factors = reinterpret_cast<float *>(left_here + left::v);
         const bool there = lane < n;
-        const int64_t at = (int64_t)(row0 + (there ? lane : 0)) * a.heads + h;
-        const float g = there ? log_decay_of(b, a, at, h) : 0.0f;
+        const int64_t from = (int64_t)(row0 + (there ? lane : 0)) * a.heads + h;
+        const float g = there ? log_decay_of(b, a, from, h) : 0.0f, step = there ? beta_of(b, a, from) : 0.0f;
         double c = g < kLeast ? kLeast : g;
         for (int off = 1; off < 64; off <<= 1) {
             const double x = __shfl_up(c, off);
@@ -103,45 +190,49 @@ __global__ __launch_bounds__(256) void chunk_prepare_kernel(GdnRows b, RaggedArg
         }
         const double last = __shfl(c, 63);
         sum[lane] = c;
-        beta[lane] = there ? beta_of(b, a, at) : 0.0f;
-        grown[lane] = expf((float)c);
-        mine[L::v + lane] = expf((float)c) * a.scale;
-        mine[L::v + kC + lane] = expf((float)(last - c));
-        if (lane == 0) mine[L::v + 2 * kC] = expf((float)last);
+        beta[lane] = step;
+        const float grown = expf((float)c);
+        factors[lane] = step;
+        factors[kC + lane] = step * grown;
+        factors[2 * kC + lane] = grown * a.scale;
+        factors[3 * kC + lane] = expf((float)(last - c));
+        factors[4 * kC + lane] = expf((float)last);
     }
-    // ---- k_i . k_j and q_i . k_j by tiles of 16 x 16 on and below the diagonal, i the columns of a result
-    auto row_operand = [&](const T *x, int tile, f32x4 (&o)[KT]) {
-        const int row = 16 * tile + r16;
-#pragma unroll
-        for (int s = 0; s < KT; s++) o[s] = four<E>(x + (int64_t)row * a.stride + 16 * s + 4 * g4, row < n);
-    };
-    const int it0 = wave == 0 ? 0 : wave == 1 ? 2 : 3, it1 = wave == 0 ? 1 : it0;
-    f32x4 kk[3], qk[3];  // wave 0: (0,0) (1,0) (1,1); 1: (2,0..2); 2: (3,0) (3,1); 3: (3,2) (3,3)
+    // ---- products of rows by tiles of 16 x 16 on and below the diagonal, i the columns of a result:
+    // wave 0 has (0,0) (1,0) (1,1), 1 (2,0..2), 2 (3,0) (3,1), 3 (3,2) (3,3)
+    const int tiles = wave < 2 ? 3 : 2;
     auto tile_of = [&](int m, int *i, int *jt) {
-        *i = wave == 0 && m == 0 ? 0 : it1;
+        *i = wave == 0 ? (m == 0 ? 0 : 1) : wave == 1 ? 2 : 3;
         *jt = wave == 0 ? (m == 2 ? 1 : 0) : wave == 3 ? m + 2 : m;
     };
-    const int tiles = wave < 2 ? 3 : 2;
+    typedef RowOperand<E, D> Rows;
+    auto row_operand = [&](const T *x, int tile, Rows &o) {
+        o.load(x + (int64_t)(16 * tile + r16) * a.stride, g4, 16 * tile + r16 < n);
+    };
+    f32x4 dot[3];
     {
-        f32x4 ki[KT], qi[KT], kj[KT];
+        Rows xi, kj;
 #pragma unroll
         for (int m = 0; m < 3; m++) {
             if (m >= tiles) break;
             int i, jt;
             tile_of(m, &i, &jt);
-            if (m == 0 || (wave == 0 && m == 1)) {
-                row_operand(k, i, ki);
-                row_operand(q, i, qi);
-            }
+            if (m == 0 || (wave == 0 && m == 1)) row_operand(mine, i, xi);
             row_operand(k, jt, kj);
-            kk[m] = qk[m] = kZero;
-#pragma unroll
-            for (int s = 0; s < KT; s++) {
-                kk[m] = mma(kj[s], ki[s], kk[m]);
-                qk[m] = mma(kj[s], qi[s], qk[m]);
-            }
+            dot[m] = kj.times(xi);
         }
     }
+    // four terms of a row tile's sum over rows: half a step of 32
+    auto put = [&](int what, int i, int jt, f32x4 x) {
+        u32x2 part[3];
+        split(x, part);
+        uint32_t *const to = left_here + what + (left::step(i, jt >> 1) * 3 * 64 + lane) * 4;
+#pragma unroll
+        for (int u = 0; u < 3; u++) {
+            *reinterpret_cast<u32x2 *>(to + u * 256 + 2 * (jt & 1)) = part[u];
+            if (i == jt && !(i & 1)) *reinterpret_cast<u32x2 *>(to + u * 256 + 2) = u32x2{0, 0};  // above the diagonal
+        }
+    };
     __syncthreads();
 #pragma unroll
     for (int m = 0; m < 3; m++) {
@@ -149,124 +240,219 @@ __global__ __launch_bounds__(256) void chunk_prepare_kernel(GdnRows b, RaggedArg
         int it, jt;
         tile_of(m, &it, &jt);
         const int i = 16 * it + r16, j0 = 16 * jt + 4 * g4;
-        f32x4 x, p;
+        f32x4 x;
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-            const bool low = j0 + e <= i;
+            const bool low = keys ? j0 + e < i : j0 + e <= i;
             const float fall = low ? expf((float)(sum[i] - sum[j0 + e])) : 0.0f;
-            x[e] = j0 + e < i ? kk[m][e] * fall * beta[i] : 0.0f;
-            p[e] = low ? qk[m][e] * fall * a.scale : 0.0f;
+            x[e] = low ? dot[m][e] * fall * (keys ? beta[i] : a.scale) : 0.0f;
         }
-        *reinterpret_cast<f32x4 *>(&am[i][j0]) = x;
-        *reinterpret_cast<f32x4 *>(mine + L::p + (p_tile(it, jt) * 64 + lane) * 4) = p;
+        if (keys) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) at[j0 + e][i] = x[e];
+        } else {
+            put(left::p, it, jt, x);
+        }
     }
     __syncthreads();
-    // ---- T = (I + A)^-1: a wave inverts a diagonal block by substitution, a column a lane
+    // ---- T: a wave inverts a diagonal block, from T (I + A) = I, a row a lane
     const int diag = 16 * wave;
-    {
+    if (keys) {
         float t[16];
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
-            float x = i == r16 ? 1.0f : 0.0f;
+        for (int c = 15; c >= 0; c--) {
+            float x = c == r16 ? 1.0f : 0.0f;
 #pragma unroll
-            for (int m4 = 0; m4 < (i + 3) / 4; m4++) {
-                const f32x4 y = *reinterpret_cast<const f32x4 *>(&am[diag + i][diag + 4 * m4]);
+            for (int m4 = c / 4; m4 < 4; m4++) {
+                const f32x4 y = *reinterpret_cast<const f32x4 *>(&at[diag + c][diag + 4 * m4]);
 #pragma unroll
                 for (int e = 0; e < 4; e++)
-                    if (4 * m4 + e < i) x = fmaf(-y[e], t[4 * m4 + e], x);
+                    if (4 * m4 + e > c) x = fmaf(-y[e], t[4 * m4 + e], x);
             }
-            t[i] = x;
+            t[c] = x;
         }
         if (g4 == 0) {
 #pragma unroll
-            for (int i = 0; i < 16; i++) am[diag + i][diag + r16] = t[i];
+            for (int c = 0; c < 16; c++) at[diag + c][diag + r16] = t[c];
         }
     }
     __syncthreads();
-    // then the column of blocks below it: T_ij = -T_ii sum_m A_im T_mj
-    auto block_rows = [&](int i, int jt) { return *reinterpret_cast<const f32x4 *>(&am[16 * i + r16][16 * jt + 4 * g4]); };
-    {
-        f32x4 t[4];
+    if (!keys) return;
+    // then its row of blocks: T_ij^T = -T_jj^T sum_m A_mj^T T_im^T
+    auto block = [&](int jt, int m) { return *reinterpret_cast<const f32x4 *>(&at[16 * jt + r16][16 * m + 4 * g4]); };
+    f32x4 t[4];
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            if (i < wave) {
-                t[i] = kZero;
-            } else if (i == wave) {
-#pragma unroll
-                for (int e = 0; e < 4; e++) t[i][e] = am[diag + 4 * g4 + e][diag + r16];
-            } else {
-                f32x4 x = kZero;
-#pragma unroll
-                for (int m = 0; m < i; m++)
-                    if (m >= wave) x = mma(block_rows(i, m), t[m], x);
-                t[i] = mma(block_rows(i, i), -x, kZero);
-            }
-#pragma unroll
-            for (int e = 0; e < 4; e++) tm[16 * i + 4 * g4 + e][diag + r16] = t[i][e] * beta[diag + r16];
+    for (int jt = 3; jt >= 0; jt--) {
+        if (jt > wave) {
+            t[jt] = kZero;
+            continue;
         }
-    }
-    __syncthreads();
-    // ---- U = T diag(beta) V and W^T = K^T (T diag(beta e^c))^T, a tile of 16 columns at a time
-    f32x4 tv[10], tk[10];
+        if (jt == wave) {
 #pragma unroll
-    for (int i = 0; i < 4; i++)
+            for (int e = 0; e < 4; e++) t[jt][e] = at[diag + 4 * g4 + e][diag + r16];
+        } else {
+            f32x4 x = kZero;
 #pragma unroll
-        for (int t = 0; t <= i; t++) {
-            tv[p_tile(i, t)] = *reinterpret_cast<const f32x4 *>(&tm[16 * i + r16][16 * t + 4 * g4]);
-            tk[p_tile(i, t)] = tv[p_tile(i, t)] * *reinterpret_cast<const f32x4 *>(&grown[16 * t + 4 * g4]);
+            for (int m = jt + 1; m < 4; m++)
+                if (m <= wave) x = mma(block(jt, m), t[m], x);
+            t[jt] = mma(block(jt, jt), -x, kZero);
         }
-    auto column_operand = [&](const T *x, int tile, f32x4 (&o)[4]) {
-#pragma unroll
-        for (int t = 0; t < 4; t++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const int row = 16 * t + 4 * g4 + e;
-                o[t][e] = row < n ? (float)x[(int64_t)row * a.stride + 16 * tile + r16] : 0.0f;
-            }
-    };
-    float *const group_keys = keys + ((int64_t)number * a.groups + group) * L::keys;
-#pragma unroll
-    for (int c = wave; c < KT; c += 4) {
-        f32x4 x[4];
-        column_operand(k, c, x);
-        if (h < a.groups) {
-#pragma unroll
-            for (int t = 0; t < 4; t++) *reinterpret_cast<f32x4 *>(group_keys + ((t * KT + c) * 64 + lane) * 4) = x[t];
-        }
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            f32x4 y = kZero;
-#pragma unroll
-            for (int t = 0; t <= i; t++) y = mma(x[t], tk[p_tile(i, t)], y);
-            *reinterpret_cast<f32x4 *>(mine + L::w + ((i * KT + c) * 64 + lane) * 4) = y;
-        }
-        column_operand(v, c, x);
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            f32x4 y = kZero;
-#pragma unroll
-            for (int t = 0; t <= i; t++) y = mma(tv[p_tile(i, t)], x[t], y);
-            *reinterpret_cast<f32x4 *>(mine + L::u + ((i * KT + c) * 64 + lane) * 4) = y;
-        }
+        put(left::t, wave, jt, t[jt]);
     }
 }
 
-// A workgroup has CT tiles of 16 columns of one head's state; wave w the state's rows D / 4 w .. and the
-// chunk's rows 16 w .. + 15.
+// Rows of K in LDS, a plane a part: 16 bytes more than its elements, so that 16 rows of 8 bytes
+// spread over all banks.
+template <int D> constexpr int kKeyPitch = 2 * D + 16;
+
+template <typename E, int D, int CT> struct ScanLds {
+    static constexpr int KS = D / 32, NP = kParts<E>;
+    static constexpr uint32_t state = 0;                             // S, [32 dims of k][tile][part]
+    static constexpr uint32_t r = state + KS * CT * 3 * 1024;        // beta V - beta e^c K S, [32 rows][tile][part]
+    static constexpr uint32_t v = r + 2 * CT * 3 * 1024;             // V'
+    static constexpr uint32_t tail = v + 2 * CT * 3 * 1024;          // e^(c_last - c) V'
+    static constexpr uint32_t keys = tail + 2 * CT * 3 * 1024;       // [chunk & 1][part][row]
+    static constexpr uint32_t key_part = kC * kKeyPitch<D>, key_buffer = NP * key_part;
+    static constexpr uint32_t total = keys + 2 * key_buffer;
+};
+
+// A workgroup has CT tiles of 16 columns of one head's state, and eight waves: the first four walk the state, wave w
+// with the rows D / 4 w .. of it and the chunk's rows 16 w .. + 15; the others bring the keys to LDS, a chunk
+// ahead, and make the outputs of 16 rows each. Three barriers a chunk:
+//   S and K there | K S -> R; Q S | T R -> V' | S; P V'
 template <typename E, int D, int CT>
-__global__ __launch_bounds__(256, 1) void chunk_scan_kernel(GdnRows b, RaggedArgs a, const float *__restrict__ left,
-                                                         const float *__restrict__ keys) {
+__global__ __launch_bounds__(512) void chunk_scan_kernel(GdnRows b, RaggedArgs a, const uint32_t *__restrict__ left_all) {
     typedef typename E::T T;
-    constexpr int KT = D / 16, ST = D / 64;
-    using L = Left<D>;
-    __shared__ f32x4 ls[KT][CT][64], lv[4][CT][64], lt[4][CT][64];  // S, V' and e^(c_last - c) V' as B operands
+    typedef T T4 __attribute__((ext_vector_type(4)));
+    constexpr int KT = D / 16, KS = D / 32, ST = D / 64, NP = kParts<E>;
+    using L = ScanLds<E, D, CT>;
+    extern __shared__ __align__(16) uint8_t lds[];
     const int h = blockIdx.x, col0 = blockIdx.y * 16 * CT, j = blockIdx.z;
     const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g4 = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int role = __builtin_amdgcn_readfirstlane(tid >> 6), wave = role & 3;
     const RowRange r = row_range(b.offsets, a.rows, j);
+    const int group = h % a.groups;
+    const int number0 = first_chunk<kC>(r.begin, j), last = (r.end - r.begin + kC - 1) / kC - 1;
+    const T *const qkv = static_cast<const T *>(b.qkv);
+    auto chunk_at = [&](int i) { return left_all + ((int64_t)(number0 + min(i, last)) * a.heads + h) * left::dwords; };
+    auto factors_at = [&](int i, int which) {  // of the lane's four rows
+        return *reinterpret_cast<const f32x4 *>(chunk_at(i) + left::v + which * kC + 16 * wave + 4 * g4);
+    };
+    // an operand's parts in LDS: of a tile of 16 columns, 32 terms in a step
+    auto operand = [&](uint32_t area, int step, int c, u32x4 (&x)[3]) {
+#pragma unroll
+        for (int m = 0; m < 3; m++)
+            x[m] = *reinterpret_cast<const u32x4 *>(lds + area + ((step * CT + c) * 3 + m) * 1024 + lane * 16);
+    };
+    auto store_half = [&](uint32_t area, int tile, int c, f32x4 x) {
+        u32x2 part[3];
+        split(x, part);
+#pragma unroll
+        for (int m = 0; m < 3; m++)
+            *reinterpret_cast<u32x2 *>(lds + area + (((tile >> 1) * CT + c) * 3 + m) * 1024 + lane * 16 + 8 * (tile & 1)) = part[m];
+    };
+    auto load_step = [&](int i, int what, int s, u32x4 (&x)[2][3]) {
+        if (s > wave / 2) return;
+#pragma unroll
+        for (int m = 0; m < 3; m++)
+            x[s][m] = *reinterpret_cast<const u32x4 *>(chunk_at(i) + what + ((left::step(wave, s) * 3 + m) * 64 + lane) * 4);
+    };
+
+    if (role >= 4) {  // ---- keys and outputs
+        T4 k[KT], q[KT];
+        u32x4 p[2][3];
+        f32x4 front;
+        auto load_rows = [&](int i, int head, T4 (&x)[KT]) {
+            const int row = min(r.begin + i * kC + 16 * wave + r16, r.end - 1);
+            const T *const from = qkv + (int64_t)row * a.stride + head * D + 4 * g4;
+#pragma unroll
+            for (int t = 0; t < KT; t++) x[t] = *reinterpret_cast<const T4 *>(from + 16 * t);
+        };
+        auto parts = [&](const T4 &x, const T4 &y, u32x4 (&o)[NP]) {
+            if constexpr (NP == 1) {
+                const T4 both[2] = {x, y};
+                __builtin_memcpy(&o[0], both, 16);
+            } else {
+                split(f32x4{(float)x[0], (float)x[1], (float)x[2], (float)x[3]},
+                      f32x4{(float)y[0], (float)y[1], (float)y[2], (float)y[3]}, o);
+            }
+        };
+        auto keys_to_lds = [&](int i) {
+            uint8_t *const to = lds + L::keys + (i & 1) * L::key_buffer + (16 * wave + r16) * kKeyPitch<D> + 8 * g4;
+            const bool there = r.begin + i * kC + 16 * wave + r16 < r.end;
+#pragma unroll
+            for (int s = 0; s < KS; s++) {
+                u32x4 x[NP];
+                parts(k[2 * s], k[2 * s + 1], x);
+#pragma unroll
+                for (int m = 0; m < NP; m++) {  // (rows behind the end are zeros: they meet zeros of V')
+                    *reinterpret_cast<u32x2 *>(to + m * L::key_part + 64 * s) = there ? u32x2{x[m][0], x[m][1]} : u32x2{0, 0};
+                    *reinterpret_cast<u32x2 *>(to + m * L::key_part + 64 * s + 32) = there ? u32x2{x[m][2], x[m][3]} : u32x2{0, 0};
+                }
+            }
+        };
+        if (last >= 0) {
+            load_rows(0, a.groups + group, k);
+            keys_to_lds(0);
+            load_rows(1, a.groups + group, k);
+            load_rows(0, group, q);
+            front = factors_at(0, 2);
+            load_step(0, left::p, 0, p);
+            load_step(0, left::p, 1, p);
+        }
+        for (int i = 0; i <= last; i++) {
+            const int row0 = r.begin + i * kC, n = min(kC, r.end - row0);
+            lds_barrier();
+            Sum o[CT];
+#pragma unroll
+            for (int c = 0; c < CT; c++) o[c] = Sum{kZero, kZero};
+#pragma unroll
+            for (int s = 0; s < KS; s++) {
+                u32x4 x[NP];
+                parts(q[2 * s], q[2 * s + 1], x);
+#pragma unroll
+                for (int c = 0; c < CT; c++) {
+                    u32x4 y[3];
+                    operand(L::state, s, c, y);
+                    mma32(x, y, o[c]);
+                }
+            }
+            load_rows(i + 1, group, q);
+#pragma unroll
+            for (int c = 0; c < CT; c++) {
+                o[c].big *= front;
+                o[c].small *= front;
+            }
+            front = factors_at(i + 1, 2);
+            lds_barrier();
+            keys_to_lds(i + 1);
+            load_rows(i + 2, a.groups + group, k);
+            lds_barrier();
+#pragma unroll
+            for (int s = 0; s < 2; s++) {
+                if (s > wave / 2) break;
+#pragma unroll
+                for (int c = 0; c < CT; c++) {
+                    u32x4 y[3];
+                    operand(L::v, s, c, y);
+                    mma32(p[s], y, o[c]);
+                }
+                load_step(i + 1, left::p, s, p);
+            }
+            T *const out = static_cast<T *>(b.out) + ((int64_t)(row0 + 16 * wave + 4 * g4) * a.heads + h) * D + col0 + r16;
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (16 * wave + 4 * g4 + e < n) {
+#pragma unroll
+                    for (int c = 0; c < CT; c++) out[(int64_t)e * a.heads * D + 16 * c] = (T)(o[c].big[e] + o[c].small[e]);
+                }
+        }
+        return;
+    }
+
+    // ---- the state
     const int2 slot = b.slots[j];
     const int64_t size = (int64_t)a.heads * D * D, at0 = (int64_t)h * D * D + col0 + r16;
-    const int group = h % a.groups;
     f32x4 s[ST][CT];
 #pragma unroll
     for (int t = 0; t < ST; t++)
@@ -277,102 +463,130 @@ __global__ __launch_bounds__(256, 1) void chunk_scan_kernel(GdnRows b, RaggedArg
                 s[t][c][e] = (uint32_t)slot.x < (uint32_t)a.states
                                  ? b.state[slot.x * size + at0 + (int64_t)(16 * (wave * ST + t) + 4 * g4 + e) * D + 16 * c]
                                  : 0.0f;
-    // A chunk's operands are loaded while the one before it is worked on, each as soon as its registers are free.
-    typedef T T4 __attribute__((ext_vector_type(4)));
-    f32x4 w[KT], u[CT], p[4], k[ST][4], front, tail;
-    T4 q[KT];
+    u32x4 t[2][3];
+    T v[CT][4];
+    f32x4 beta, grown, tail;
     float fall;
-    const int number0 = first_chunk<kC>(r.begin, j), last = (r.end - r.begin + kC - 1) / kC - 1;
-    auto chunk_at = [&](int i) { return left + ((int64_t)(number0 + min(i, last)) * a.heads + h) * L::floats; };
-    auto load_row = [&](int i, int t) {
-        const int row = r.begin + i * kC + 16 * wave + r16;
-        q[t] = T4{0, 0, 0, 0};
-        if (row < r.end)
-            q[t] = *reinterpret_cast<const T4 *>(static_cast<const T *>(b.qkv) + (int64_t)row * a.stride + group * D + 16 * t + 4 * g4);
-        w[t] = *reinterpret_cast<const f32x4 *>(chunk_at(i) + L::w + ((wave * KT + t) * 64 + lane) * 4);
-    };
-    auto load_rest = [&](int i) {
-        const float *const mine = chunk_at(i);
+    auto load_values = [&](int i) {
 #pragma unroll
-        for (int c = 0; c < CT; c++)
-            u[c] = *reinterpret_cast<const f32x4 *>(mine + L::u + ((wave * KT + col0 / 16 + c) * 64 + lane) * 4);
-        front = *reinterpret_cast<const f32x4 *>(mine + L::v + 16 * wave + 4 * g4);
-        tail = *reinterpret_cast<const f32x4 *>(mine + L::v + kC + 16 * wave + 4 * g4);
-        fall = mine[L::v + 2 * kC];
+        for (int e = 0; e < 4; e++) {
+            const int row = min(r.begin + i * kC + 16 * wave + 4 * g4 + e, r.end - 1);
+#pragma unroll
+            for (int c = 0; c < CT; c++)
+                v[c][e] = qkv[(int64_t)row * a.stride + (2 * a.groups + h) * D + col0 + 16 * c + r16];
+        }
+        beta = factors_at(i, 0);
+        grown = factors_at(i, 1);
     };
-    auto load_p = [&](int i, int t) {
-        if (t <= wave) p[t] = *reinterpret_cast<const f32x4 *>(chunk_at(i) + L::p + (p_tile(wave, t) * 64 + lane) * 4);
-    };
-    auto load_k = [&](int i, int x, int t) {
-        k[x][t] = *reinterpret_cast<const f32x4 *>(keys + ((int64_t)(number0 + min(i, last)) * a.groups + group) * L::keys +
-                                                   ((t * KT + wave * ST + x) * 64 + lane) * 4);
+    auto load_tail = [&](int i) {
+        tail = factors_at(i, 3);
+        // (a scalar load would make every wait for LDS one for memory)
+        fall = *reinterpret_cast<const float *>(chunk_at(i) + left::v + 4 * kC + lane);
     };
     if (last >= 0) {
-#pragma unroll
-        for (int t = 0; t < KT; t++) load_row(0, t);
-        load_rest(0);
-#pragma unroll
-        for (int t = 0; t < 4; t++) {
-            load_p(0, t);
-#pragma unroll
-            for (int x = 0; x < ST; x++) load_k(0, x, t);
-        }
+        load_values(0);
+        load_step(0, left::t, 0, t);
+        load_step(0, left::t, 1, t);
+        load_tail(0);
     }
     for (int i = 0; i <= last; i++) {
-        const int row0 = r.begin + i * kC, n = min(kC, r.end - row0);
-#pragma unroll
-        for (int t = 0; t < ST; t++)
-#pragma unroll
-            for (int c = 0; c < CT; c++) ls[wave * ST + t][c][lane] = s[t][c];
-        lds_barrier();
-        f32x4 ws[CT], o[CT];
-#pragma unroll
-        for (int c = 0; c < CT; c++) ws[c] = o[c] = kZero;
-#pragma unroll
-        for (int t = 0; t < KT; t++) {
-            const f32x4 x = {(float)q[t][0], (float)q[t][1], (float)q[t][2], (float)q[t][3]};
-#pragma unroll
-            for (int c = 0; c < CT; c++) {
-                const f32x4 y = ls[t][c][lane];
-                ws[c] = mma(w[t], y, ws[c]);
-                o[c] = mma(x, y, o[c]);
-            }
-            load_row(i + 1, t);
-        }
-        const float before = fall;
+        const uint32_t keys = L::keys + (i & 1) * L::key_buffer;
 #pragma unroll
         for (int c = 0; c < CT; c++) {
-            const f32x4 x = u[c] - ws[c];
-            lv[wave][c][lane] = x;
-            lt[wave][c][lane] = x * tail;
-            o[c] *= front;
+            if constexpr (ST == 2) {
+                u32x4 part[3];
+                split(s[0][c], s[1][c], part);
+#pragma unroll
+                for (int m = 0; m < 3; m++)
+                    *reinterpret_cast<u32x4 *>(lds + L::state + ((wave * CT + c) * 3 + m) * 1024 + lane * 16) = part[m];
+            } else {
+                store_half(L::state, wave, c, s[0][c]);
+            }
         }
-        load_rest(i + 1);
         lds_barrier();
+        Sum x[CT];
 #pragma unroll
-        for (int x = 0; x < ST; x++)
+        for (int c = 0; c < CT; c++) x[c] = Sum{kZero, kZero};
 #pragma unroll
-            for (int c = 0; c < CT; c++) s[x][c] *= before;
+        for (int d = 0; d < KS; d++) {
+            const uint8_t *const from = lds + keys + (16 * wave + r16) * kKeyPitch<D> + 8 * g4 + 64 * d;
+            u32x4 k[NP];
 #pragma unroll
-        for (int t = 0; t < 4; t++) {
+            for (int m = 0; m < NP; m++) {
+                const u32x2 lo = *reinterpret_cast<const u32x2 *>(from + m * L::key_part);
+                const u32x2 hi = *reinterpret_cast<const u32x2 *>(from + m * L::key_part + 32);
+                k[m] = u32x4{lo[0], lo[1], hi[0], hi[1]};
+            }
 #pragma unroll
             for (int c = 0; c < CT; c++) {
-                const f32x4 y = lt[t][c][lane];
-#pragma unroll
-                for (int x = 0; x < ST; x++) s[x][c] = mma(k[x][t], y, s[x][c]);
-                if (t <= wave) o[c] = mma(p[t], lv[t][c][lane], o[c]);
+                u32x4 y[3];
+                operand(L::state, d, c, y);
+                mma32(k, y, x[c]);
             }
-#pragma unroll
-            for (int x = 0; x < ST; x++) load_k(i + 1, x, t);
-            load_p(i + 1, t);
         }
-        T *const out = static_cast<T *>(b.out) + ((int64_t)(row0 + 16 * wave + 4 * g4) * a.heads + h) * D + col0 + r16;
+        const int n = r.end - (r.begin + i * kC) - 16 * wave - 4 * g4;  // rows from the lane's first on
 #pragma unroll
-        for (int e = 0; e < 4; e++)
-            if (16 * wave + 4 * g4 + e < n) {
+        for (int c = 0; c < CT; c++) {
+            const f32x4 ks = x[c].all();
+            f32x4 y;
 #pragma unroll
-                for (int c = 0; c < CT; c++) out[(int64_t)e * a.heads * D + 16 * c] = (T)o[c][e];
+            for (int e = 0; e < 4; e++) y[e] = e < n ? beta[e] * (float)v[c][e] - grown[e] * ks[e] : 0.0f;
+            store_half(L::r, wave, c, y);
+        }
+        load_values(i + 1);
+        lds_barrier();
+        Sum w[CT];
+#pragma unroll
+        for (int c = 0; c < CT; c++) w[c] = Sum{kZero, kZero};
+#pragma unroll
+        for (int d = 0; d < 2; d++) {
+            if (d > wave / 2) break;
+#pragma unroll
+            for (int c = 0; c < CT; c++) {
+                u32x4 y[3];
+                operand(L::r, d, c, y);
+                mma32(t[d], y, w[c]);
             }
+            load_step(i + 1, left::t, d, t);
+        }
+#pragma unroll
+        for (int c = 0; c < CT; c++) {
+            const f32x4 y = w[c].all();
+            store_half(L::tail, wave, c, y * tail);
+            store_half(L::v, wave, c, y);
+        }
+        lds_barrier();
+        Sum next[ST][CT];
+#pragma unroll
+        for (int u = 0; u < ST; u++)
+#pragma unroll
+            for (int c = 0; c < CT; c++) next[u][c] = Sum{s[u][c] * fall, kZero};
+        load_tail(i + 1);
+#pragma unroll
+        for (int d = 0; d < 2; d++) {
+            // K^T: a lane's eight rows of one column, four rows of 16 columns turned over at a time
+            u32x4 k[ST][NP];
+#pragma unroll
+            for (int u = 0; u < ST; u++)
+#pragma unroll
+                for (int m = 0; m < NP; m++) {
+                    const uint32_t from = keys + m * L::key_part + (32 * d + 4 * g4 + (r16 >> 2)) * kKeyPitch<D> +
+                                          32 * (wave * ST + u) + 8 * (r16 & 3);
+                    const u32x2 lo = columns_of(lds + from), hi = columns_of(lds + from + 16 * kKeyPitch<D>);
+                    k[u][m] = u32x4{lo[0], lo[1], hi[0], hi[1]};
+                }
+#pragma unroll
+            for (int c = 0; c < CT; c++) {
+                u32x4 y[3];
+                operand(L::tail, d, c, y);
+#pragma unroll
+                for (int u = 0; u < ST; u++) mma32(k[u], y, next[u][c]);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < ST; u++)
+#pragma unroll
+            for (int c = 0; c < CT; c++) s[u][c] = next[u][c].all();
     }
     if ((uint32_t)slot.y < (uint32_t)a.states) {
 #pragma unroll
@@ -385,37 +599,43 @@ __global__ __launch_bounds__(256, 1) void chunk_scan_kernel(GdnRows b, RaggedArg
     }
 }
 
-uint64_t left_floats(const RaggedArgs &a) { return a.head_dim == 128 ? Left<128>::floats : Left<64>::floats; }
-uint64_t keys_floats(const RaggedArgs &a) { return a.head_dim == 128 ? Left<128>::keys : Left<64>::keys; }
+template <typename F> hipError_t by_kind(uint32_t dtype, int head_dim, F &&f) {
+    auto by_dim = [&](auto e) {
+        return head_dim == 128 ? f(e, std::integral_constant<int, 128>{}) : f(e, std::integral_constant<int, 64>{});
+    };
+    return dtype == YUUKA_DTYPE_F32 ? by_dim(RowF32{}) : dtype == YUUKA_DTYPE_F16 ? by_dim(RowF16{}) : by_dim(RowBF16{});
+}
 
 }  // namespace
 
 uint64_t gdn_prompt_scratch_bytes(const RaggedArgs &a) {
-    const uint64_t numbers = chunk_numbers<kC>(a.rows, a.requests);
-    return numbers * (a.heads * left_floats(a) + a.groups * keys_floats(a)) * 4;
+    return (uint64_t)chunk_numbers<kC>(a.rows, a.requests) * a.heads * left::dwords * 4;
 }
 
 hipError_t launch_gdn_prompt(const GdnRows &b, uint32_t dtype, const RaggedArgs &a, void *scratch, hipStream_t s) {
     const uint32_t numbers = chunk_numbers<kC>(a.rows, a.requests);
-    float *const left = static_cast<float *>(scratch), *const keys = left + (uint64_t)numbers * a.heads * left_floats(a);
-    hipError_t err = hipSuccess;
-    auto go = [&](auto e, auto d) {
+    return by_kind(dtype, a.head_dim, [&](auto e, auto d) {
         using E = decltype(e);
-        constexpr int D = d();
-        chunk_prepare_kernel<E, D><<<dim3(numbers, a.heads), 256, 0, s>>>(b, a, left, keys);
-        err = hipGetLastError();
-        if (err != hipSuccess) return;
-        chunk_scan_kernel<E, D, 1><<<dim3(a.heads, D / 16, a.requests), 256, 0, s>>>(b, a, left, keys);
-        err = hipGetLastError();
-    };
-    auto by_dim = [&](auto e) {
-        if (a.head_dim == 128) go(e, std::integral_constant<int, 128>{});
-        else go(e, std::integral_constant<int, 64>{});
-    };
-    if (dtype == YUUKA_DTYPE_F32) by_dim(RowF32{});
-    else if (dtype == YUUKA_DTYPE_F16) by_dim(RowF16{});
-    else by_dim(RowBF16{});
-    return err;
+        constexpr int D = d(), CT = 1;
+        uint32_t *const left_all = static_cast<uint32_t *>(scratch);
+        chunk_prepare_kernel<E, D><<<dim3(numbers, a.heads), 512, 0, s>>>(b, a, left_all);
+        hipError_t err = hipGetLastError();
+        if (err != hipSuccess) return err;
+        constexpr auto scan = chunk_scan_kernel<E, D, CT>;
+        constexpr uint32_t bytes = ScanLds<E, D, CT>::total;
+        static_assert(bytes <= 160 * 1024, "LDS of a CU");
+        if constexpr (bytes > 64 * 1024) {  // (a device's own setting)
+            static std::once_flag once[64];
+            int device = 0;
+            (void)hipGetDevice(&device);
+            std::call_once(once[device & 63], [] {
+                (void)hipFuncSetAttribute(reinterpret_cast<const void *>(scan), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                          (int)bytes);
+            });
+        }
+        scan<<<dim3(a.heads, D / 16 / CT, a.requests), 512, bytes, s>>>(b, a, left_all);
+        return hipGetLastError();
+    });
 }
 
 }  // namespace yk
