@@ -301,6 +301,21 @@ __global__ __launch_bounds__(512) void chunk_prepare_kernel(GdnRows b, RaggedArg
     }
 }
 
+// The longest requests go first, so that none of them is left alone at the end: request number `rank` by its
+// rows. (More than 64 are taken as they come.)
+__device__ __forceinline__ int by_length(const int32_t *offsets, const RaggedArgs &a, int rank) {
+    if (a.requests == 1 || a.requests > 64) return rank;
+    const int lane = threadIdx.x & 63;
+    const RowRange r = row_range(offsets, a.rows, min(lane, a.requests - 1));
+    const int mine = lane < a.requests ? r.end - r.begin : -1;
+    int before = 0;
+    for (int i = 0; i < a.requests; i++) {
+        const int other = __builtin_amdgcn_readlane(mine, i);
+        before += other > mine || (other == mine && i < lane);
+    }
+    return __ffsll((unsigned long long)__builtin_amdgcn_ballot_w64(before == rank)) - 1;
+}
+
 // Rows of K in LDS, a plane a part: 16 bytes more than its elements, so that 16 rows of 8 bytes
 // spread over all banks.
 template <int D> constexpr int kKeyPitch = 2 * D + 16;
@@ -316,18 +331,20 @@ template <typename E, int D, int CT> struct ScanLds {
     static constexpr uint32_t total = keys + 2 * key_buffer;
 };
 
-// A workgroup has CT tiles of 16 columns of one head's state, and eight waves: the first four walk the state, wave w
-// with the rows D / 4 w .. of it and the chunk's rows 16 w .. + 15; the others bring the keys to LDS, a chunk
-// ahead, and make the outputs of 16 rows each. Three barriers a chunk:
+// A workgroup has CT tiles of 16 columns of one head's state. Four waves walk the state, wave w with the rows
+// D / 4 w .. of it and the chunk's rows 16 w .. + 15; four make the outputs of 16 rows each, and those, or four
+// more where a key has several parts, bring the keys to LDS, a chunk ahead. Three barriers a chunk:
 //   S and K there | K S -> R; Q S | T R -> V' | S; P V'
+template <typename E> constexpr int kScanWaves = kParts<E> == 3 ? 12 : 8;
 template <typename E, int D, int CT>
-__global__ __launch_bounds__(512) void chunk_scan_kernel(GdnRows b, RaggedArgs a, const uint32_t *__restrict__ left_all) {
+__global__ __launch_bounds__(64 * kScanWaves<E>) void chunk_scan_kernel(GdnRows b, RaggedArgs a, const uint32_t *__restrict__ left_all) {
     typedef typename E::T T;
     typedef T T4 __attribute__((ext_vector_type(4)));
     constexpr int KT = D / 16, KS = D / 32, ST = D / 64, NP = kParts<E>;
+    constexpr bool kApart = kScanWaves<E> == 12;
     using L = ScanLds<E, D, CT>;
     extern __shared__ __align__(16) uint8_t lds[];
-    const int h = blockIdx.x, col0 = blockIdx.y * 16 * CT, j = blockIdx.z;
+    const int h = blockIdx.x, col0 = blockIdx.y * 16 * CT, j = by_length(b.offsets, a, blockIdx.z);
     const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g4 = lane >> 4;
     const int role = __builtin_amdgcn_readfirstlane(tid >> 6), wave = role & 3;
     const RowRange r = row_range(b.offsets, a.rows, j);
@@ -359,9 +376,6 @@ __global__ __launch_bounds__(512) void chunk_scan_kernel(GdnRows b, RaggedArgs a
     };
 
     if (role >= 4) {  // ---- keys and outputs
-        T4 k[KT], q[KT];
-        u32x4 p[2][3];
-        f32x4 front;
         auto load_rows = [&](int i, int head, T4 (&x)[KT]) {
             const int row = min(r.begin + i * kC + 16 * wave + r16, r.end - 1);
             const T *const from = qkv + (int64_t)row * a.stride + head * D + 4 * g4;
@@ -377,6 +391,7 @@ __global__ __launch_bounds__(512) void chunk_scan_kernel(GdnRows b, RaggedArgs a
                       f32x4{(float)y[0], (float)y[1], (float)y[2], (float)y[3]}, o);
             }
         };
+        T4 k[KT];
         auto keys_to_lds = [&](int i) {
             uint8_t *const to = lds + L::keys + (i & 1) * L::key_buffer + (16 * wave + r16) * kKeyPitch<D> + 8 * g4;
             const bool there = r.begin + i * kC + 16 * wave + r16 < r.end;
@@ -391,10 +406,25 @@ __global__ __launch_bounds__(512) void chunk_scan_kernel(GdnRows b, RaggedArgs a
                 }
             }
         };
-        if (last >= 0) {
+        if (last >= 0 && (!kApart || role >= 8)) {
             load_rows(0, a.groups + group, k);
             keys_to_lds(0);
             load_rows(1, a.groups + group, k);
+        }
+        if (kApart && role >= 8) {
+            for (int i = 0; i <= last; i++) {
+                lds_barrier();
+                keys_to_lds(i + 1);
+                load_rows(i + 2, a.groups + group, k);
+                lds_barrier();
+                lds_barrier();
+            }
+            return;
+        }
+        T4 q[KT];
+        u32x4 p[2][3];
+        f32x4 front;
+        if (last >= 0) {
             load_rows(0, group, q);
             front = factors_at(0, 2);
             load_step(0, left::p, 0, p);
@@ -425,8 +455,10 @@ __global__ __launch_bounds__(512) void chunk_scan_kernel(GdnRows b, RaggedArgs a
             }
             front = factors_at(i + 1, 2);
             lds_barrier();
-            keys_to_lds(i + 1);
-            load_rows(i + 2, a.groups + group, k);
+            if constexpr (!kApart) {
+                keys_to_lds(i + 1);
+                load_rows(i + 2, a.groups + group, k);
+            }
             lds_barrier();
 #pragma unroll
             for (int s = 0; s < 2; s++) {
@@ -616,25 +648,38 @@ hipError_t launch_gdn_prompt(const GdnRows &b, uint32_t dtype, const RaggedArgs 
     const uint32_t numbers = chunk_numbers<kC>(a.rows, a.requests);
     return by_kind(dtype, a.head_dim, [&](auto e, auto d) {
         using E = decltype(e);
-        constexpr int D = d(), CT = 1;
+        constexpr int D = d();
         uint32_t *const left_all = static_cast<uint32_t *>(scratch);
         chunk_prepare_kernel<E, D><<<dim3(numbers, a.heads), 512, 0, s>>>(b, a, left_all);
         hipError_t err = hipGetLastError();
         if (err != hipSuccess) return err;
-        constexpr auto scan = chunk_scan_kernel<E, D, CT>;
-        constexpr uint32_t bytes = ScanLds<E, D, CT>::total;
-        static_assert(bytes <= 160 * 1024, "LDS of a CU");
-        if constexpr (bytes > 64 * 1024) {  // (a device's own setting)
-            static std::once_flag once[64];
-            int device = 0;
-            (void)hipGetDevice(&device);
-            std::call_once(once[device & 63], [] {
-                (void)hipFuncSetAttribute(reinterpret_cast<const void *>(scan), hipFuncAttributeMaxDynamicSharedMemorySize,
-                                          (int)bytes);
-            });
-        }
-        scan<<<dim3(a.heads, D / 16 / CT, a.requests), 512, bytes, s>>>(b, a, left_all);
-        return hipGetLastError();
+        auto go = [&](auto tiles) {
+            constexpr int CT = tiles();
+            constexpr uint32_t bytes = ScanLds<E, D, CT>::total;
+            if constexpr (bytes <= 160 * 1024) {  // (more are not asked for)
+                constexpr auto scan = chunk_scan_kernel<E, D, CT>;
+                if constexpr (bytes > 64 * 1024) {  // (a device's own setting)
+                    static std::once_flag once[64];
+                    int device = 0;
+                    (void)hipGetDevice(&device);
+                    std::call_once(once[device & 63], [] {
+                        (void)hipFuncSetAttribute(reinterpret_cast<const void *>(scan),
+                                                  hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+                    });
+                }
+                scan<<<dim3(a.heads, D / 16 / CT, a.requests), 64 * kScanWaves<E>, bytes, s>>>(b, a, left_all);
+                err = hipGetLastError();
+            }
+        };
+        // The most columns that LDS holds and that leave every CU a workgroup: what is loaded for a chunk serves more of
+        // them. us with 1, 2 and 4 tiles, BF16: 1 prompt of 2000 rows, 16 heads of 128 (128 workgroups at one tile) 99, 122,
+        // 174; 4 of 1000 (512) 103, 85, 110; 4 of 1000, 32 heads (1024) 196, 151, 129; 16 of 8192 rows in all (4096)
+        // 433, 347, 278.
+        const int64_t columns = (int64_t)a.requests * a.heads * (D / 16);
+        if (columns >= 4 * 256 && ScanLds<E, D, 4>::total <= 160 * 1024) go(std::integral_constant<int, 4>{});
+        else if (columns >= 2 * 256 && ScanLds<E, D, 2>::total <= 160 * 1024) go(std::integral_constant<int, 2>{});
+        else go(std::integral_constant<int, 1>{});
+        return err;
     });
 }
 
