@@ -65,20 +65,31 @@ __global__ __launch_bounds__(256) void ragged_conv_kernel(typename E::T *__restr
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int c = (blockIdx.y * 64 + lane) * V;
     const bool live = c < a.channels;
-    const int K1 = a.kernel - 1;
+    const int K1 = KT == 4 ? 3 : a.kernel - 1;  // (four taps are four; other numbers are the last of eight)
     const int64_t window = (int64_t)a.channels * K1;
     // the request's window before its rows, oldest first, zeros in front where K < KT
     float past[KT - 1][V] = {};
     auto load_window = [&](int j) {
         const int from = slots[j].x;
+        const bool there = live && (uint32_t)from < (uint32_t)a.states;
+        const float *const at = state + (there ? from * window + (int64_t)c * K1 : 0);
+        if constexpr (KT == 4) {  // V channels of three inputs, side by side
+            float4 y[3 * V / 4];
 #pragma unroll
-        for (int t = 0; t < KT - 1; t++)
+            for (int i = 0; i < 3 * V / 4; i++)
+                y[i] = there ? reinterpret_cast<const float4 *>(at)[i] : make_float4(0.f, 0.f, 0.f, 0.f);
+            const float *const flat = reinterpret_cast<const float *>(y);
 #pragma unroll
-            for (int i = 0; i < V; i++) {
-                const int at = t - (KT - 1 - K1);
-                past[t][i] = live && at >= 0 && (uint32_t)from < (uint32_t)a.states
-                                 ? state[from * window + (int64_t)(c + i) * K1 + at] : 0.0f;
-            }
+            for (int i = 0; i < V; i++)
+#pragma unroll
+                for (int t = 0; t < 3; t++) past[t][i] = flat[3 * i + t];
+        } else {
+#pragma unroll
+            for (int t = 0; t < KT - 1; t++)
+#pragma unroll
+                for (int i = 0; i < V; i++)
+                    past[t][i] = there && t >= KT - 1 - K1 ? at[i * K1 + t - (KT - 1 - K1)] : 0.0f;
+        }
     };
     auto load_row = [&](int row, float (&y)[V]) {
         const Bytes16 none = {0, 0, 0, 0};
@@ -104,13 +115,24 @@ __global__ __launch_bounds__(256) void ragged_conv_kernel(typename E::T *__restr
                         for (int i = 0; i < V; i++) next[t][i] = past[u][i];
             }
         }
+        float *const at = state + to * window + (int64_t)c * K1;
+        if (!live) return;
+        if constexpr (KT == 4) {
+            float4 y[3 * V / 4];
+            float *const flat = reinterpret_cast<float *>(y);
 #pragma unroll
-        for (int t = 0; t < KT - 1; t++)
+            for (int i = 0; i < V; i++)
 #pragma unroll
-            for (int i = 0; i < V; i++) {
-                const int at = t - (KT - 1 - K1);
-                if (live && at >= 0) state[to * window + (int64_t)(c + i) * K1 + at] = next[t][i];
-            }
+                for (int t = 0; t < 3; t++) flat[3 * i + t] = next[t][i];
+#pragma unroll
+            for (int i = 0; i < 3 * V / 4; i++) reinterpret_cast<float4 *>(at)[i] = y[i];
+        } else {
+#pragma unroll
+            for (int t = 0; t < KT - 1; t++)
+#pragma unroll
+                for (int i = 0; i < V; i++)
+                    if (t >= KT - 1 - K1) at[i * K1 + t - (KT - 1 - K1)] = next[t][i];
+        }
     };
     if ((int)blockIdx.x >= row_blocks) {  // requests without rows
         const int j = ((int)blockIdx.x - row_blocks) * 4 + wave;
@@ -132,61 +154,55 @@ __global__ __launch_bounds__(256) void ragged_conv_kernel(typename E::T *__restr
     for (int t = 0; t < KT; t++)
 #pragma unroll
         for (int i = 0; i < V; i++) {
-            const int at = t - (KT - a.kernel);
-            w[t][i] = live && at >= 0 ? weight[(int64_t)(c + i) * a.kernel + at] : 0.0f;
+            const int at = t - (KT - 1 - K1);
+            w[t][i] = live && at >= 0 ? weight[(int64_t)(c + i) * (K1 + 1) + at] : 0.0f;
         }
     const int keys = a.groups * D;
     RowRange r = row_range(offsets, a.rows, j);
     bool fresh = true;  // the window is not in the registers
+    // four rows of the run are on their way while one is worked on
+    Bytes16 ahead[4];
+    auto load_raw = [&](int at) {
+        const Bytes16 none = {0, 0, 0, 0};
+        return live ? *reinterpret_cast<const Bytes16 *>(x + (int64_t)at * a.stride + c) : none;
+    };
+#pragma unroll
+    for (int u = 0; u < 4; u++) ahead[u] = load_raw(min(row + u, last - 1));
     // A request's first K - 1 rows, which need its window, are the wave's that has the first of them: nobody
-    // else reads the slot that it may write.
-    for (;; row++) {
+    // else reads the slot that it may write. False when the wave is done.
+    auto step = [&](Bytes16 &slot) {
         while (row >= r.end) {
-            if (row >= last || ++j >= a.requests) return;
+            if (row >= last || ++j >= a.requests) return false;
             r = row_range(offsets, a.rows, j);
             fresh = true;
         }
         const bool early = row - r.begin < K1, begun = r.begin >= first;
-        if (row >= last && !(early && begun)) return;
-        if (row < r.begin || (early && !begun)) continue;  // (descending offsets leave rows between requests)
+        if (row >= last && !(early && begun)) return false;
+        const Bytes16 raw = row < last ? slot : load_raw(row);
+        slot = load_raw(min(row + 4, last - 1));
+        if (row < r.begin || (early && !begun)) return true;  // (descending offsets leave rows between requests)
         if (fresh) {
             if (row == r.begin) {
                 load_window(j);
                 store_window(j, r);
+            } else {  // K - 1 rows of the request, or more, are before this one
+#pragma unroll
+                for (int t = 0; t < KT - 1; t++)
+                    if (t >= KT - 1 - K1) load_row(max(row - (KT - 1 - t), r.begin), past[t]);
             }
-            // rows of the request before this one
-            const int have = min(row - r.begin, KT - 1);
-            float near[KT - 1][V];
-#pragma unroll
-            for (int t = 0; t < KT - 1; t++) {
-                const int back = KT - 1 - t;
-                if (back <= have) {
-                    load_row(row - back, near[t]);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < V; i++) near[t][i] = 0.0f;
-#pragma unroll
-                    for (int u = 0; u < KT - 1; u++)
-                        if (u == t + have)
-#pragma unroll
-                            for (int i = 0; i < V; i++) near[t][i] = past[u][i];
-                }
-            }
-#pragma unroll
-            for (int t = 0; t < KT - 1; t++)
-#pragma unroll
-                for (int i = 0; i < V; i++) past[t][i] = near[t][i];
             fresh = false;
         }
         float now[V], y[V], squares = 0.0f;
-        load_row(row, now);
+        unpack<E>(raw, now);
 #pragma unroll
         for (int i = 0; i < V; i++) {
             float sum = 0.0f;
 #pragma unroll
             for (int t = 0; t < KT - 1; t++)
                 if (t >= KT - 1 - K1) sum = fmaf(w[t][i], past[t][i], sum);
-            y[i] = silu_f32(fmaf(w[KT - 1][i], now[i], sum));
+            sum = fmaf(w[KT - 1][i], now[i], sum);
+            // SiLU by the hardware's exponential and reciprocal, a unit in the last place each
+            y[i] = sum * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(sum * -1.44269504088896341f));
             squares = fmaf(y[i], y[i], squares);
         }
         if (c < 2 * keys) {  // whole heads: a group of lanes takes one way
@@ -201,6 +217,14 @@ __global__ __launch_bounds__(256) void ragged_conv_kernel(typename E::T *__restr
             for (int i = 0; i < V; i++) past[t][i] = past[t + 1][i];
 #pragma unroll
         for (int i = 0; i < V; i++) past[KT - 2][i] = now[i];
+        return true;
+    };
+    for (;;) {
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            if (!step(ahead[u])) return;
+            row++;
+        }
     }
 }
 
@@ -323,7 +347,11 @@ hipError_t launch_gdn_ragged_conv(void *out, const void *x, uint32_t dtype, cons
     by_type(dtype, [&](auto e) {
         using E = decltype(e);
         typedef typename E::T T;
-        const int run = 16;
+        // A wave's rows: as many as leave the GPU 2048 waves, up to 32, for each wave reads its channels' weights and
+        // K - 1 rows more. us with 512, 1024, 2048 and 4096 waves: 500 rows of 16 heads in F32 19, 14, 13, 20, 2000 of
+        // 32 heads in BF16 43, 43, 35, 39, 8191 (32 rows a wave in each) 82; with 64 rows a wave 105.
+        const int64_t waves = (int64_t)a.rows * ((a.channels + 64 * E::kWide - 1) / (64 * E::kWide));
+        const int run = (int)std::clamp<int64_t>(waves / 2048, 1, 32);
         const int row_blocks = (int)(((int64_t)a.rows + 4 * run - 1) / (4 * run));
         const dim3 grid(row_blocks + (a.requests + 3) / 4, (a.channels + 64 * E::kWide - 1) / (64 * E::kWide));
         auto go = [&](auto taps, auto d) {
@@ -334,7 +362,7 @@ hipError_t launch_gdn_ragged_conv(void *out, const void *x, uint32_t dtype, cons
             if (a.head_dim == 128) go(taps, std::integral_constant<int, 128>{});
             else go(taps, std::integral_constant<int, 64>{});
         };
-        if (a.kernel <= 4) by_dim(std::integral_constant<int, 4>{});
+        if (a.kernel == 4) by_dim(std::integral_constant<int, 4>{});
         else by_dim(std::integral_constant<int, 8>{});
     });
     return hipGetLastError();
