@@ -52,9 +52,10 @@ __device__ __forceinline__ int64_t scan_add(int64_t x, int64_t *sums, int64_t *t
     return before + x;
 }
 
-// One workgroup: sums of the requests' rows and pages.
-__global__ __launch_bounds__(kScan) void batch_scan_kernel(BatchBuffers b, BatchArgs a, int2 *__restrict__ plan) {
-    __shared__ int64_t sums[kScan / 64];
+// The scan by one workgroup: sums of the requests' rows and pages, `put(j, end of its rows, {first, start})` for each;
+// returned, the end of the free list. `write`: this workgroup leaves the outputs.
+template <typename F>
+__device__ __forceinline__ int scan_requests(const BatchBuffers &b, const BatchArgs &a, int64_t *sums, bool write, F &&put) {
     const int tid = threadIdx.x;
     const int64_t next = max(0, b.pool[0]), last = max(next, (int64_t)min(b.pool[1], b.free_entries));
     int64_t rows = 0, pages = 0;  // of the requests before this turn's
@@ -62,33 +63,32 @@ __global__ __launch_bounds__(kScan) void batch_scan_kernel(BatchBuffers b, Batch
         const int j = base + tid;
         const bool live = j < a.requests;
         int64_t n = live ? max(0, b.counts[j]) : 0;
+        const int blocks = live ? b.blocks[j] : 0;
+        const int64_t position = live ? b.positions[2 * j + 1] : 0;
         const int64_t end = scan_add(n, sums, &rows);
         n = max((int64_t)0, min(end, (int64_t)a.rows) - (end - n));  // rows that the arrays hold
-        const int blocks = live ? b.blocks[j] : 0;
-        const PageNeed need = live ? page_need(b.positions[2 * j + 1], n, blocks, a.block_size, a.capacity) : PageNeed{0, 0};
+        const PageNeed need = live ? page_need(position, n, blocks, a.block_size, a.capacity) : PageNeed{0, 0};
         const int64_t start = next + scan_add(need.fresh, sums, &pages) - need.fresh;
         if (!live) continue;
-        b.offsets[j + 1] = (int)min(end, (int64_t)a.rows);
-        plan[j] = make_int2(need.first, (int)min(start, (int64_t)0x7fffffff));
+        put(j, (int)min(end, (int64_t)a.rows), make_int2(need.first, (int)min(start, (int64_t)0x7fffffff)));
         const int64_t taken = clamp64(last - start, 0, need.fresh);
-        b.blocks_out[j] = taken ? need.first + (int)taken : blocks;
+        if (write) b.blocks_out[j] = taken ? need.first + (int)taken : blocks;
     }
-    if (tid) return;
-    b.offsets[0] = 0;
-    plan[a.requests] = make_int2((int)last, 0);
-    const int64_t taken = min(pages, last - next);
-    b.pool_out[0] = (int)(next + taken);
-    if (b.pool_out != b.pool) b.pool_out[1] = (int)min(pages - taken, (int64_t)0x7fffffff);  // else the count stays
+    if (write && tid == 0) {
+        const int64_t taken = min(pages, last - next);
+        b.pool_out[0] = (int)(next + taken);
+        if (b.pool_out != b.pool) b.pool_out[1] = (int)min(pages - taken, (int64_t)0x7fffffff);  // else the count stays
+    }
+    return (int)last;
 }
 
-// A thread a row.
-__global__ __launch_bounds__(256) void batch_rows_kernel(BatchBuffers b, BatchArgs a, const int2 *__restrict__ plan) {
-    const int row = blockIdx.x * 256 + threadIdx.x;
-    if (row >= a.rows) return;
+// One row: `offsets` and `plan` as the scan left them.
+__device__ __forceinline__ void place_row(const BatchBuffers &b, const BatchArgs &a, int row, const int32_t *offsets,
+                                          const int2 *plan, int last) {
     int lo = 0, hi = a.requests;  // the first request that ends behind the row
     while (lo < hi) {
         const int mid = (lo + hi) >> 1;
-        if (b.offsets[mid + 1] > row) hi = mid;
+        if (offsets[mid + 1] > row) hi = mid;
         else lo = mid + 1;
     }
     if (lo == a.requests) {
@@ -96,7 +96,7 @@ __global__ __launch_bounds__(256) void batch_rows_kernel(BatchBuffers b, BatchAr
         b.slots[row] = -1;
         return;
     }
-    const int i = row - b.offsets[lo];
+    const int i = row - offsets[lo];
     const int64_t p = (int64_t)b.positions[2 * lo + 1] + i;
     b.row_info[row] = make_int2(lo, (int)min(p, (int64_t)0x7fffffff));
     int page = -1;
@@ -108,11 +108,48 @@ __global__ __launch_bounds__(256) void batch_rows_kernel(BatchBuffers b, BatchAr
             page = *entry;
         } else {
             const int64_t at = (int64_t)mine.y + (block - mine.x);
-            if (at < plan[a.requests].x) page = b.free_pages[at];
+            if (at < last) page = b.free_pages[at];
             if (i == 0 || (int)p % a.block_size == 0) *entry = page;
         }
     }
     b.slots[row] = page < 0 ? -1 : (int64_t)page * a.block_size + (int)p % a.block_size;
+}
+
+__global__ __launch_bounds__(kScan) void batch_scan_kernel(BatchBuffers b, BatchArgs a, int2 *__restrict__ plan) {
+    __shared__ int64_t sums[kScan / 64];
+    const int last = scan_requests(b, a, sums, true, [&](int j, int end, int2 mine) {
+        b.offsets[j + 1] = end;
+        plan[j] = mine;
+    });
+    if (threadIdx.x == 0) {
+        b.offsets[0] = 0;
+        plan[a.requests] = make_int2(last, 0);
+    }
+}
+
+__global__ __launch_bounds__(256) void batch_rows_kernel(BatchBuffers b, BatchArgs a, const int2 *__restrict__ plan) {
+    const int row = blockIdx.x * 256 + threadIdx.x;
+    if (row < a.rows) place_row(b, a, row, b.offsets, plan, plan[a.requests].x);
+}
+
+// Both for up to kScan requests: every workgroup scans for itself, the first leaves the outputs.
+__global__ __launch_bounds__(kScan) void batch_plan_kernel(BatchBuffers b, BatchArgs a) {
+    __shared__ int64_t sums[kScan / 64];
+    __shared__ int32_t offsets[kScan + 1];
+    __shared__ int2 plan[kScan];
+    const bool write = blockIdx.x == 0;
+    if (threadIdx.x == 0) {
+        offsets[0] = 0;
+        if (write) b.offsets[0] = 0;
+    }
+    const int last = scan_requests(b, a, sums, write, [&](int j, int end, int2 mine) {
+        offsets[j + 1] = end;
+        plan[j] = mine;
+        if (write) b.offsets[j + 1] = end;
+    });
+    __syncthreads();
+    for (int64_t row = (int64_t)blockIdx.x * kScan + threadIdx.x; row < a.rows; row += (int64_t)gridDim.x * kScan)
+        place_row(b, a, (int)row, offsets, plan, last);
 }
 
 }  // namespace
@@ -120,6 +157,13 @@ __global__ __launch_bounds__(256) void batch_rows_kernel(BatchBuffers b, BatchAr
 uint64_t batch_plan_scratch_bytes(const BatchArgs &a) { return ((uint64_t)a.requests + 1) * sizeof(int2); }
 
 hipError_t launch_batch_plan(const BatchBuffers &b, const BatchArgs &a, void *scratch, hipStream_t s) {
+    // One launch where a workgroup scans the requests in one turn and none reads what another overwrites: 16 requests
+    // of one row 10.5 -> 6.8 us, 200 of 16300 rows 10.5 -> 6.9. A workgroup alone takes up to 4096 rows.
+    const bool in_place = b.blocks_out == b.blocks || b.pool_out == b.pool;
+    if (a.requests <= kScan && (!in_place || a.rows <= 4096)) {
+        batch_plan_kernel<<<in_place ? 1 : (uint32_t)((a.rows + kScan - 1) / kScan), kScan, 0, s>>>(b, a);
+        return hipGetLastError();
+    }
     int2 *const plan = static_cast<int2 *>(scratch);
     batch_scan_kernel<<<1, kScan, 0, s>>>(b, a, plan);
     hipError_t err = hipGetLastError();
