@@ -107,6 +107,12 @@ __device__ __forceinline__ u32x2 columns_of(const uint8_t *at) {
         (__attribute__((address_space(3))) s16x4 *)(const_cast<uint8_t *>(at))));
 }
 
+// Loads stay where they stand: the compiler would move those of a next turn down to it.
+__device__ __forceinline__ void pin_loads() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+
 // What the first kernel leaves for a chunk and head: operands as the second loads them, 64 lanes
 // of 16 bytes each (256 dwords).
 namespace left {
@@ -152,11 +158,27 @@ template <int D> struct RowOperand<RowF32, D> {
     }
 };
 
+// Sums of the lanes up to and with each.
+template <int CTRL, int ROWS> __device__ __forceinline__ double add_shifted(double x) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, x);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, ROWS, 0xf, false);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, ROWS, 0xf, false);
+    return x + __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ double lanes_scan(double x) {
+    x = add_shifted<0x111, 0xf>(x);  // by 1, 2, 4 and 8 lanes of a row of 16
+    x = add_shifted<0x112, 0xf>(x);
+    x = add_shifted<0x114, 0xf>(x);
+    x = add_shifted<0x118, 0xf>(x);
+    x = add_shifted<0x142, 0xa>(x);  // the last lane of row 0 to row 1 and of row 2 to row 3
+    return add_shifted<0x143, 0xc>(x);  // lane 31 to rows 2 and 3
+}
+
 // Eight waves: four for k_i . k_j and T, four for q_i . k_j.
 template <typename E, int D>
 __global__ __launch_bounds__(512) void chunk_prepare_kernel(GdnRows b, RaggedArgs a, uint32_t *__restrict__ left_all) {
     typedef typename E::T T;
-    __shared__ double sum[kC];
+    __shared__ double sum[kC];  // of the log decays, base 2
     __shared__ __align__(16) float beta[kC];
     __shared__ __align__(16) float at[kC][kRowPitch];  // A^T, its diagonal blocks later those of T^T
     const int number = blockIdx.x, h = blockIdx.y;
@@ -183,20 +205,18 @@ __global__ __launch_bounds__(512) void chunk_prepare_kernel(GdnRows b, RaggedArg
         const bool there = lane < n;
         const int64_t from = (int64_t)(row0 + (there ? lane : 0)) * a.heads + h;
         const float g = there ? log_decay_of(b, a, from, h) : 0.0f, step = there ? beta_of(b, a, from) : 0.0f;
-        double c = g < kLeast ? kLeast : g;
-        for (int off = 1; off < 64; off <<= 1) {
-            const double x = __shfl_up(c, off);
-            if (lane >= off) c += x;
-        }
-        const double last = __shfl(c, 63);
+        const double c = lanes_scan(1.4426950408889634 * (g < kLeast ? kLeast : g));
+        const double last = __builtin_bit_cast(double, (uint64_t)(uint32_t)__builtin_amdgcn_readlane(
+                                                           (int)(__builtin_bit_cast(uint64_t, c) >> 32), 63) << 32 |
+                                                           (uint32_t)__builtin_amdgcn_readlane((int)__builtin_bit_cast(uint64_t, c), 63));
         sum[lane] = c;
         beta[lane] = step;
-        const float grown = expf((float)c);
+        const float grown = __builtin_amdgcn_exp2f((float)c);
         factors[lane] = step;
         factors[kC + lane] = step * grown;
         factors[2 * kC + lane] = grown * a.scale;
-        factors[3 * kC + lane] = expf((float)(last - c));
-        factors[4 * kC + lane] = expf((float)last);
+        factors[3 * kC + lane] = __builtin_amdgcn_exp2f((float)(last - c));
+        factors[4 * kC + lane] = __builtin_amdgcn_exp2f((float)last);
     }
     // ---- products of rows by tiles of 16 x 16 on and below the diagonal, i the columns of a result:
     // wave 0 has (0,0) (1,0) (1,1), 1 (2,0..2), 2 (3,0) (3,1), 3 (3,2) (3,3)
@@ -210,16 +230,26 @@ __global__ __launch_bounds__(512) void chunk_prepare_kernel(GdnRows b, RaggedArg
         o.load(x + (int64_t)(16 * tile + r16) * a.stride, g4, 16 * tile + r16 < n);
     };
     f32x4 dot[3];
-    {
-        Rows xi, kj;
-#pragma unroll
-        for (int m = 0; m < 3; m++) {
-            if (m >= tiles) break;
-            int i, jt;
-            tile_of(m, &i, &jt);
-            if (m == 0 || (wave == 0 && m == 1)) row_operand(mine, i, xi);
-            row_operand(k, jt, kj);
-            dot[m] = kj.times(xi);
+    {  // every row on its way before the first product
+        Rows x, y, z, u;
+        if (wave == 0) {
+            row_operand(mine, 0, x);
+            row_operand(mine, 1, y);
+            row_operand(k, 0, z);
+            row_operand(k, 1, u);
+            __builtin_amdgcn_sched_barrier(0);
+            dot[0] = z.times(x);
+            dot[1] = z.times(y);
+            dot[2] = u.times(y);
+        } else {
+            row_operand(mine, wave == 1 ? 2 : 3, x);
+            row_operand(k, wave == 3 ? 2 : 0, y);
+            row_operand(k, wave == 3 ? 3 : 1, z);
+            if (wave == 1) row_operand(k, 2, u);
+            __builtin_amdgcn_sched_barrier(0);
+            dot[0] = y.times(x);
+            dot[1] = z.times(x);
+            if (wave == 1) dot[2] = u.times(x);
         }
     }
     // four terms of a row tile's sum over rows: half a step of 32
@@ -240,12 +270,14 @@ __global__ __launch_bounds__(512) void chunk_prepare_kernel(GdnRows b, RaggedArg
         int it, jt;
         tile_of(m, &it, &jt);
         const int i = 16 * it + r16, j0 = 16 * jt + 4 * g4;
+        const double sum_i = sum[i];
+        const float factor = keys ? beta[i] : a.scale;
         f32x4 x;
 #pragma unroll
         for (int e = 0; e < 4; e++) {
             const bool low = keys ? j0 + e < i : j0 + e <= i;
-            const float fall = low ? expf((float)(sum[i] - sum[j0 + e])) : 0.0f;
-            x[e] = low ? dot[m][e] * fall * (keys ? beta[i] : a.scale) : 0.0f;
+            const float fall = low ? __builtin_amdgcn_exp2f((float)(sum_i - sum[j0 + e])) : 0.0f;
+            x[e] = low ? dot[m][e] * fall * factor : 0.0f;
         }
         if (keys) {
 #pragma unroll
@@ -337,7 +369,7 @@ template <typename E, int D, int CT> struct ScanLds {
 //   S and K there | K S -> R; Q S | T R -> V' | S; P V'
 template <typename E> constexpr int kScanWaves = kParts<E> == 3 ? 12 : 8;
 template <typename E, int D, int CT>
-__global__ __launch_bounds__(64 * kScanWaves<E>) void chunk_scan_kernel(GdnRows b, RaggedArgs a, const uint32_t *__restrict__ left_all) {
+__global__ __launch_bounds__(64 * kScanWaves<E>) void chunk_scan_kernel(GdnRows b, RaggedArgs a, const uint32_t *left_all) {
     typedef typename E::T T;
     typedef T T4 __attribute__((ext_vector_type(4)));
     constexpr int KT = D / 16, KS = D / 32, ST = D / 64, NP = kParts<E>;
@@ -368,11 +400,13 @@ __global__ __launch_bounds__(64 * kScanWaves<E>) void chunk_scan_kernel(GdnRows 
         for (int m = 0; m < 3; m++)
             *reinterpret_cast<u32x2 *>(lds + area + (((tile >> 1) * CT + c) * 3 + m) * 1024 + lane * 16 + 8 * (tile & 1)) = part[m];
     };
+    // (No branches among the loads and stores of a turn: a wait counts the least that may have been issued since, and
+    // would be one for what was asked for last.)
     auto load_step = [&](int i, int what, int s, u32x4 (&x)[2][3]) {
-        if (s > wave / 2) return;
+        const int step = left::step(wave, min(s, wave >> 1));
 #pragma unroll
         for (int m = 0; m < 3; m++)
-            x[s][m] = *reinterpret_cast<const u32x4 *>(chunk_at(i) + what + ((left::step(wave, s) * 3 + m) * 64 + lane) * 4);
+            x[s][m] = *reinterpret_cast<const u32x4 *>(chunk_at(i) + what + ((step * 3 + m) * 64 + lane) * 4);
     };
 
     if (role >= 4) {  // ---- keys and outputs
@@ -409,13 +443,14 @@ __global__ __launch_bounds__(64 * kScanWaves<E>) void chunk_scan_kernel(GdnRows 
         if (last >= 0 && (!kApart || role >= 8)) {
             load_rows(0, a.groups + group, k);
             keys_to_lds(0);
-            load_rows(1, a.groups + group, k);
+            if constexpr (kApart) load_rows(1, a.groups + group, k);
         }
         if (kApart && role >= 8) {
             for (int i = 0; i <= last; i++) {
                 lds_barrier();
                 keys_to_lds(i + 1);
                 load_rows(i + 2, a.groups + group, k);
+                pin_loads();
                 lds_barrier();
                 lds_barrier();
             }
@@ -427,6 +462,7 @@ __global__ __launch_bounds__(64 * kScanWaves<E>) void chunk_scan_kernel(GdnRows 
         if (last >= 0) {
             load_rows(0, group, q);
             front = factors_at(0, 2);
+            if constexpr (!kApart) load_rows(1, a.groups + group, k);
             load_step(0, left::p, 0, p);
             load_step(0, left::p, 1, p);
         }
@@ -448,16 +484,19 @@ __global__ __launch_bounds__(64 * kScanWaves<E>) void chunk_scan_kernel(GdnRows 
                 }
             }
             load_rows(i + 1, group, q);
+            pin_loads();
 #pragma unroll
             for (int c = 0; c < CT; c++) {
                 o[c].big *= front;
                 o[c].small *= front;
             }
             front = factors_at(i + 1, 2);
+            pin_loads();
             lds_barrier();
             if constexpr (!kApart) {
                 keys_to_lds(i + 1);
                 load_rows(i + 2, a.groups + group, k);
+                pin_loads();
             }
             lds_barrier();
 #pragma unroll
@@ -469,14 +508,27 @@ __global__ __launch_bounds__(64 * kScanWaves<E>) void chunk_scan_kernel(GdnRows 
                     operand(L::v, s, c, y);
                     mma32(p[s], y, o[c]);
                 }
-                load_step(i + 1, left::p, s, p);
             }
-            T *const out = static_cast<T *>(b.out) + ((int64_t)(row0 + 16 * wave + 4 * g4) * a.heads + h) * D + col0 + r16;
+            load_step(i + 1, left::p, 0, p);
+            load_step(i + 1, left::p, 1, p);
+            pin_loads();
+            // rows behind the end lie behind the buffer, and are not written
+            const uint32_t pitch = a.heads * D * sizeof(T);
+            const uint64_t base = reinterpret_cast<uint64_t>(b.out) + (uint64_t)row0 * pitch;
+            void *const first = reinterpret_cast<void *>((uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)(base >> 32)) << 32 |
+                                                         (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)base));
+            const auto rows = __builtin_amdgcn_make_buffer_rsrc(first, (short)0, __builtin_amdgcn_readfirstlane(n * pitch),
+                                                                0x00020000);
+            const uint32_t at = (16 * wave + 4 * g4) * pitch + (h * D + col0 + r16) * sizeof(T);
 #pragma unroll
             for (int e = 0; e < 4; e++)
-                if (16 * wave + 4 * g4 + e < n) {
 #pragma unroll
-                    for (int c = 0; c < CT; c++) out[(int64_t)e * a.heads * D + 16 * c] = (T)(o[c].big[e] + o[c].small[e]);
+                for (int c = 0; c < CT; c++) {
+                    const T y = (T)(o[c].big[e] + o[c].small[e]);
+                    if constexpr (sizeof(T) == 4)
+                        __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, y), rows, at + e * pitch + 16 * c * sizeof(T), 0, 0);
+                    else
+                        __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, y), rows, at + e * pitch + 16 * c * sizeof(T), 0, 0);
                 }
         }
         return;
@@ -566,6 +618,7 @@ __global__ __launch_bounds__(64 * kScanWaves<E>) void chunk_scan_kernel(GdnRows 
             store_half(L::r, wave, c, y);
         }
         load_values(i + 1);
+        pin_loads();
         lds_barrier();
         Sum w[CT];
 #pragma unroll
@@ -579,8 +632,10 @@ __global__ __launch_bounds__(64 * kScanWaves<E>) void chunk_scan_kernel(GdnRows 
                 operand(L::r, d, c, y);
                 mma32(t[d], y, w[c]);
             }
-            load_step(i + 1, left::t, d, t);
         }
+        load_step(i + 1, left::t, 0, t);
+        load_step(i + 1, left::t, 1, t);
+        pin_loads();
 #pragma unroll
         for (int c = 0; c < CT; c++) {
             const f32x4 y = w[c].all();
@@ -594,6 +649,7 @@ __global__ __launch_bounds__(64 * kScanWaves<E>) void chunk_scan_kernel(GdnRows 
 #pragma unroll
             for (int c = 0; c < CT; c++) next[u][c] = Sum{s[u][c] * fall, kZero};
         load_tail(i + 1);
+        pin_loads();
 #pragma unroll
         for (int d = 0; d < 2; d++) {
             // K^T: a lane's eight rows of one column, four rows of 16 columns turned over at a time
