@@ -253,7 +253,7 @@ __global__ __launch_bounds__(512) void chunk_prepare_kernel(GdnRows b, RaggedArg
             if (i == jt && !(i & 1)) *reinterpret_cast<u32x2 *>(to + u * 256 + 2) = u32x2{0, 0};  // above the diagonal
         }
     };
-    __syncthreads();
+    lds_barrier();
 #pragma unroll
     for (int m = 0; m < 3; m++) {
         if (m >= tiles) break;
@@ -276,7 +276,7 @@ __global__ __launch_bounds__(512) void chunk_prepare_kernel(GdnRows b, RaggedArg
             put(left::p, it, jt, x);
         }
     }
-    __syncthreads();
+    lds_barrier();
     // ---- T: a wave inverts a diagonal block, from T (I + A) = I, a row a lane
     const int diag = 16 * wave;
     if (keys) {
@@ -298,7 +298,7 @@ __global__ __launch_bounds__(512) void chunk_prepare_kernel(GdnRows b, RaggedArg
             for (int c = 0; c < 16; c++) at[diag + c][diag + r16] = t[c];
         }
     }
-    __syncthreads();
+    lds_barrier();
     if (!keys) return;
     // then its row of blocks: T_ij^T = -T_jj^T sum_m A_mj^T T_im^T
     auto block = [&](int jt, int m) { return *reinterpret_cast<const f32x4 *>(&at[16 * jt + r16][16 * m + 4 * g4]); };
