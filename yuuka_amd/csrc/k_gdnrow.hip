@@ -1,6 +1,6 @@
 // k_gdnrow.hip — Gated DeltaNet layers over ragged rows: the causal
 // convolution with SiLU and the q / k norm (forward.go:248-268, 484-493), and the
-// delta rule row by row (recurrent.go:56-105).
+// delta rule for one row of every request (recurrent.go:56-105).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -54,6 +54,8 @@ template <int N> __device__ __forceinline__ float lanes_sum(float x) {
 // rows and keeps the last KT - 1 of them in registers; the wave with a request's first
 // row reads its window and leaves its new one, which may be in the same slot.
 // Requests without rows have their window moved by waves of their own.
+// Bound by memory: 8191 rows of 8192 channels in BF16, 0.27 GB, 78 us, 3.4 TB/s (a copy of 2 GB
+// reaches 4.9).
 template <typename E, int KT, int D>
 __global__ __launch_bounds__(256) void ragged_conv_kernel(typename E::T *__restrict__ out,
                                                           const typename E::T *__restrict__ x,
@@ -230,28 +232,25 @@ __global__ __launch_bounds__(256) void ragged_conv_kernel(typename E::T *__restr
     }
 }
 
-// The delta rule row by row: a workgroup holds COLS columns of one head's state, a
-// thread four of them in every (256 / (COLS / 4))th row.
+// One row of every request:
 //   S = e^g S;  d = beta (v - S^T k);  S += k d^T;  o = S^T q
+// A workgroup holds COLS columns of one head's state, a thread four of them in every
+// (256 / (COLS / 4))th row: the state is read and written once, in registers between, and is all the
+// traffic there is to speak of. The row's own values are asked for before it (after it: 145 us for 141).
+// 200 requests of 32 heads of 128 move 0.84 GB in 141 us, 6.0 TB/s; with 16, 64 and 128 columns a
+// workgroup 154, 146, 146.
 template <typename E, int D, int COLS>
-__global__ __launch_bounds__(256) void ragged_scan_kernel(GdnRows b, RaggedArgs a) {
+__global__ __launch_bounds__(256) void ragged_step_kernel(GdnRows b, RaggedArgs a) {
     constexpr int C4 = COLS / 4, RG = 256 / C4, NR = D / RG, SPAN = C4 < 64 ? C4 : 64;
     static_assert(D % RG == 0, "whole rows");
     __shared__ float qk[2][D], vs[COLS];
     __shared__ float4 part[2][4][C4];
     typedef typename E::T T;
-    const int h = blockIdx.x, col0 = blockIdx.y * COLS, j = blockIdx.z;
+    const int h = blockIdx.x, col0 = blockIdx.y * COLS, j = blockIdx.z;  // (row j is request j's)
     const int t = threadIdx.x, wave = t >> 6, lane = t & 63, c4 = t % C4, rg = t / C4;
-    const RowRange r = b.offsets ? row_range(b.offsets, a.rows, j) : RowRange{j, j + 1};
     const int2 slot = b.slots[j];
     const int64_t size = (int64_t)a.heads * D * D, mine = (int64_t)h * D * D + col0 + 4 * c4;
-    float4 s[NR];
-#pragma unroll
-    for (int m = 0; m < NR; m++)
-        s[m] = (uint32_t)slot.x < (uint32_t)a.states
-                   ? *reinterpret_cast<const float4 *>(b.state + slot.x * size + mine + (int64_t)(rg + RG * m) * D)
-                   : make_float4(0.f, 0.f, 0.f, 0.f);
-    const T *const qkv = static_cast<const T *>(b.qkv);
+    const T *const x = static_cast<const T *>(b.qkv) + (int64_t)j * a.stride;
     const int group = h % a.groups;
     // sum over the row groups of every column, in every thread
     auto total = [&](float4 x, int which) {
@@ -272,50 +271,52 @@ __global__ __launch_bounds__(256) void ragged_scan_kernel(GdnRows b, RaggedArgs 
         }
         return sum;
     };
-    for (int row = r.begin; row < r.end; row++) {
-        const T *const x = qkv + (int64_t)row * a.stride;
-        if (t < D) qk[0][t] = (float)x[group * D + t] * a.scale;
-        else if (t < 2 * D) qk[1][t - D] = (float)x[(a.groups + group) * D + t - D];
-        const float own_v = t < COLS ? (float)x[(2 * a.groups + h) * D + col0 + t] : 0.0f;
-        if (t < COLS) vs[t] = own_v;
-        const float decay = expf(log_decay_of(b, a, (int64_t)row * a.heads + h, h));
-        const float beta = beta_of(b, a, (int64_t)row * a.heads + h);
-        __syncthreads();
-        float4 seen = make_float4(0.f, 0.f, 0.f, 0.f);
+    const float own = t < 2 * D ? (float)x[(t < D ? group : a.groups + group) * D + (t & (D - 1))] : 0.0f;
+    const float own_v = t < COLS ? (float)x[(2 * a.groups + h) * D + col0 + t] : 0.0f;
+    const float decay = expf(log_decay_of(b, a, (int64_t)j * a.heads + h, h));
+    const float beta = beta_of(b, a, (int64_t)j * a.heads + h);
+    float4 s[NR];
 #pragma unroll
-        for (int m = 0; m < NR; m++) {
-            const float k = qk[1][rg + RG * m];
-            s[m].x *= decay; s[m].y *= decay; s[m].z *= decay; s[m].w *= decay;
-            seen.x = fmaf(s[m].x, k, seen.x);
-            seen.y = fmaf(s[m].y, k, seen.y);
-            seen.z = fmaf(s[m].z, k, seen.z);
-            seen.w = fmaf(s[m].w, k, seen.w);
-        }
-        seen = total(seen, 0);
-        const float4 d = make_float4((vs[4 * c4] - seen.x) * beta, (vs[4 * c4 + 1] - seen.y) * beta,
-                                     (vs[4 * c4 + 2] - seen.z) * beta, (vs[4 * c4 + 3] - seen.w) * beta);
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int m = 0; m < NR; m++)
+        s[m] = (uint32_t)slot.x < (uint32_t)a.states
+                   ? *reinterpret_cast<const float4 *>(b.state + slot.x * size + mine + (int64_t)(rg + RG * m) * D)
+                   : make_float4(0.f, 0.f, 0.f, 0.f);
+    if (t < 2 * D) qk[t / D][t & (D - 1)] = t < D ? own * a.scale : own;
+    if (t < COLS) vs[t] = own_v;
+    __syncthreads();
+    float4 seen = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int m = 0; m < NR; m++) {
-            const float k = qk[1][rg + RG * m], q = qk[0][rg + RG * m];
-            s[m].x = fmaf(k, d.x, s[m].x);
-            s[m].y = fmaf(k, d.y, s[m].y);
-            s[m].z = fmaf(k, d.z, s[m].z);
-            s[m].w = fmaf(k, d.w, s[m].w);
-            o.x = fmaf(s[m].x, q, o.x);
-            o.y = fmaf(s[m].y, q, o.y);
-            o.z = fmaf(s[m].z, q, o.z);
-            o.w = fmaf(s[m].w, q, o.w);
-        }
-        o = total(o, 1);
-        if (t < C4) {
-            T *const to = static_cast<T *>(b.out) + ((int64_t)row * a.heads + h) * D + col0 + 4 * t;
-            to[0] = (T)o.x;
-            to[1] = (T)o.y;
-            to[2] = (T)o.z;
-            to[3] = (T)o.w;
-        }
-        __syncthreads();
+    for (int m = 0; m < NR; m++) {
+        const float k = qk[1][rg + RG * m];
+        s[m].x *= decay; s[m].y *= decay; s[m].z *= decay; s[m].w *= decay;
+        seen.x = fmaf(s[m].x, k, seen.x);
+        seen.y = fmaf(s[m].y, k, seen.y);
+        seen.z = fmaf(s[m].z, k, seen.z);
+        seen.w = fmaf(s[m].w, k, seen.w);
+    }
+    seen = total(seen, 0);
+    const float4 d = make_float4((vs[4 * c4] - seen.x) * beta, (vs[4 * c4 + 1] - seen.y) * beta,
+                                 (vs[4 * c4 + 2] - seen.z) * beta, (vs[4 * c4 + 3] - seen.w) * beta);
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int m = 0; m < NR; m++) {
+        const float k = qk[1][rg + RG * m], q = qk[0][rg + RG * m];
+        s[m].x = fmaf(k, d.x, s[m].x);
+        s[m].y = fmaf(k, d.y, s[m].y);
+        s[m].z = fmaf(k, d.z, s[m].z);
+        s[m].w = fmaf(k, d.w, s[m].w);
+        o.x = fmaf(s[m].x, q, o.x);
+        o.y = fmaf(s[m].y, q, o.y);
+        o.z = fmaf(s[m].z, q, o.z);
+        o.w = fmaf(s[m].w, q, o.w);
+    }
+    o = total(o, 1);
+    if (t < C4) {
+        T *const to = static_cast<T *>(b.out) + ((int64_t)j * a.heads + h) * D + col0 + 4 * t;
+        to[0] = (T)o.x;
+        to[1] = (T)o.y;
+        to[2] = (T)o.z;
+        to[3] = (T)o.w;
     }
     if ((uint32_t)slot.y < (uint32_t)a.states) {
 #pragma unroll
@@ -328,18 +329,6 @@ template <typename F> void by_type(uint32_t dtype, F &&f) {
     if (dtype == YUUKA_DTYPE_F32) f(RowF32{});
     else if (dtype == YUUKA_DTYPE_F16) f(RowF16{});
     else f(RowBF16{});
-}
-
-hipError_t launch_scan(const GdnRows &b, uint32_t dtype, const RaggedArgs &a, hipStream_t s) {
-    by_type(dtype, [&](auto e) {
-        using E = decltype(e);
-        auto go = [&](auto d, auto cols) {
-            ragged_scan_kernel<E, d(), cols()><<<dim3(a.heads, d() / cols(), a.requests), 256, 0, s>>>(b, a);
-        };
-        if (a.head_dim == 128) go(std::integral_constant<int, 128>{}, std::integral_constant<int, 32>{});
-        else go(std::integral_constant<int, 64>{}, std::integral_constant<int, 32>{});
-    });
-    return hipGetLastError();
 }
 
 }  // namespace
@@ -371,7 +360,13 @@ hipError_t launch_gdn_ragged_conv(void *out, const void *x, uint32_t dtype, cons
 }
 
 hipError_t launch_gdn_step(const GdnRows &b, uint32_t dtype, const RaggedArgs &a, hipStream_t s) {
-    return launch_scan(b, dtype, a, s);
+    by_type(dtype, [&](auto e) {
+        using E = decltype(e);
+        const dim3 grid(a.heads, a.head_dim / 32, a.requests);
+        if (a.head_dim == 128) ragged_step_kernel<E, 128, 32><<<grid, 256, 0, s>>>(b, a);
+        else ragged_step_kernel<E, 64, 32><<<grid, 256, 0, s>>>(b, a);
+    });
+    return hipGetLastError();
 }
 
 }  // namespace yk

@@ -56,7 +56,7 @@ struct GdnRows {
     const void *qkv;
     const float *alpha, *beta, *dt, *a;
     float *state;
-    const int32_t *offsets;  // null: one row of every request
+    const int32_t *offsets;  // (not of a step: row j is request j's)
     const int2 *slots;
 };
 hipError_t launch_gdn_step(const GdnRows &b, uint32_t dtype, const RaggedArgs &a, hipStream_t s);
