@@ -656,9 +656,12 @@ YUUKA_API yuuka_status yuuka_attn_decode(yuuka_stream * stream, yuuka_buffer * o
  * Ragged batches (extension): requests with different numbers of new rows,
  * laid one after another without padding. Rows offsets[j] .. offsets[j + 1] - 1
  * (int32) are request j's; rows behind the last are neither read nor written.
- * Offsets outside 0 .. rows are taken as the nearest of those, a request that
- * ends before it starts as empty. Every buffer has to be on the stream's device;
- * an output must not overlap an input or another output, except where said.
+ * Offsets ascend. One outside 0 .. rows is taken as the nearest of those, a request
+ * that ends before it starts as empty; where requests have rows in common, the results of
+ * those requests are undefined (nothing outside the arrays is touched). Every buffer has
+ * to be on the stream's device; an output must not overlap an input or another output,
+ * except where said. Calls on one stream run in order; yuuka_batch_plan and
+ * yuuka_gdn_prompt keep what they work out in the stream's workspace.
  * ---------------------------------------------------------------------- */
 typedef struct yuuka_batch_params {
     int32_t requests;   /* 1..65535 */
@@ -682,7 +685,8 @@ typedef struct yuuka_batch_params {
  *   pool_out   int32 <- {next, pages that were missing}; with pool itself only next
  *              moves, and the next call goes on from there
  * Blocks from max(blocks_j, p_j / block_size) to that of the last new row get a page
- * each, in the order of the requests; other entries stay. Once the list is
+ * each, in the order of the requests; other entries stay, among them those that a
+ * position past the blocks in use leaves between. Once the list is
  * empty they get -1, as do the slots of their rows, and blocks_out ends before
  * them. A row whose position is below 0 or from `capacity` on, or whose entry is
  * below 0, has the slot -1. Rows that the arrays have no room for take no page.
@@ -744,7 +748,14 @@ YUUKA_API yuuka_status yuuka_gdn_conv(yuuka_stream * stream, yuuka_buffer * out,
  * [rows][heads][head_dim], rounded once to the nearest.
  * Keys of norm 1 (as the convolution leaves them), beta in 0..1 and g <= 0 are what the
  * rule is stable for. yuuka_gdn_step takes one row of every request, row j
- * of request j (`rows` is not less than `requests`). */
+ * of request j (`rows` is not less than `requests`).
+ * Precision: FP32 sums and states. yuuka_gdn_prompt solves 64 rows of a request at a
+ * time, its float32 factors as three bf16 parts whose products below 2^-23 of the whole are
+ * left out; factors below 2^-102 lose parts, and a decay below e^-200 is zero. A
+ * key, query, alpha or beta that is not finite makes NaN of its head's rows among the
+ * same 64 (earlier ones too) and of those after, a value that is not finite of its
+ * column there; other requests and heads stay clean. Its workspace holds 37.9 KB a
+ * head for every 64 rows of `rows`, and as much for every request. */
 YUUKA_API yuuka_status yuuka_gdn_prompt(yuuka_stream * stream, yuuka_buffer * out, const yuuka_buffer * qkv,
                         const yuuka_buffer * alpha, const yuuka_buffer * beta, const yuuka_buffer * dt,
                         const yuuka_buffer * a, yuuka_buffer * states, const yuuka_buffer * offsets,

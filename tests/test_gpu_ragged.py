@@ -384,6 +384,23 @@ def test_prompt(dev, stream, dtype, counts, groups, heads, D, raw):
     check_delta(got, (*pad, *want[2:]), dtype, live)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,groups,heads,D", [(40, 1, 2, 128), (60, 2, 4, 128), (80, 1, 2, 64), (70, 2, 4, 64)])
+def test_prompts_of_many_requests(dev, stream, dtype, n, groups, heads, D):
+    """Workgroups of two and four tiles of columns, and more requests than are put in order."""
+    rng = np.random.default_rng(n + D)
+    counts = [int(x) for x in rng.permutation([0, 1, 64, 65, 130, 200] + [int(x) for x in rng.integers(0, 20, n - 6)])]
+    rows = sum(counts)
+    qkv = unit_rows(rng, rows, groups, heads, D, dtype)
+    alpha, beta, _, _, g, b = gates(rng, rows, heads, False)
+    states = rng.normal(0, 0.3, (n, heads, D, D)).astype(np.float32)
+    slots = np.stack([rng.permutation(n)] * 2, 1)
+    got = run_delta(dev, stream, dtype, qkv, alpha, beta, None, None, states, counts, slots, groups, heads, D)
+    want = delta_reference(from_bits(qkv, dtype), g, b, states.astype(np.float64), offsets_of(counts), slots, groups, heads,
+                           D, 1.0)
+    check_delta(got, want, dtype, rows)
+
+
 @pytest.mark.parametrize("raw", [True, False])
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("n,groups,heads,D", [(1, 1, 1, 64), (1, 16, 16, 128), (5, 2, 4, 128), (9, 1, 3, 64), (70, 1, 2, 128)])
@@ -634,6 +651,59 @@ def test_a_ragged_batch_captured(dev, stream):
     for g in graphs:
         g.destroy()
     s2.destroy()
+
+
+def test_tokens_captured(dev, stream):
+    """A token of every request, pages and all, as one graph replayed: 1100 requests of which some take none."""
+    rng = np.random.default_rng(21)
+    n, groups, heads, D, block, capacity = 1100, 1, 1, 64, 16, 64
+    channels, entries = 3 * D, capacity // block
+    weight = rng.normal(0, 0.5, (channels, 4)).astype(np.float32)
+    windows, states = np.zeros((n, channels, 3)), np.zeros((n, heads, D, D))
+    where = np.stack([np.arange(n)] * 2, 1).astype(np.int32)
+    up, alloc = dev.upload, dev.alloc
+    b = dict(positions=alloc(8 * n), counts=alloc(4 * n), blocks=up(np.zeros(n, np.int32)),
+             table=up(np.full((n, entries), -1, np.int32)), free=up(rng.permutation(n * entries).astype(np.int32)),
+             pool=up(i32(0, n * entries)), offsets=alloc(4 * (n + 1)), info=alloc(8 * n), slots=alloc(8 * n),
+             x=alloc(4 * n * channels), y=alloc(4 * n * channels), weight=up(weight), where=up(where),
+             windows=up(windows.astype(np.float32)), states=up(states.astype(np.float32)), alpha=alloc(4 * n), beta=alloc(4 * n),
+             out=alloc(4 * n * D))
+    plan = hip.Plan(dev)
+    plan.add(hip.OP["BATCH_PLAN"], [b[k] for k in ("positions", "counts", "blocks", "table", "free", "pool", "offsets", "info",
+                                                   "slots", "blocks", "pool")], n=[n, n], u=[block, capacity])
+    plan.add(hip.OP["GDN_CONV"], [b[k] for k in ("y", "x", "weight", "windows", "offsets", "where")],
+             n=[n, n, groups, heads, D, 0], u=[hip.F32, 4], f=[1.0, 1e-6])
+    plan.add(hip.OP["GDN_STEP"], [b[k] for k in ("out", "y", "alpha", "beta", "states")] + [None, b["where"]],
+             n=[n, n, groups, heads, D, 0], u=[hip.F32, 0, 1], f=[1.0])
+    graph = hip.Graph(plan, stream, None)
+    position, used, blocks = np.zeros(n, np.int64), 0, np.zeros(n, np.int64)
+    free = b["free"].read(np.int32)
+    for turn in range(4):
+        x = rng.normal(0, 1, (n, channels)).astype(np.float32)
+        alpha = -rng.uniform(0, 1, (n, 1)).astype(np.float32)
+        beta = rng.uniform(0, 1, (n, 1)).astype(np.float32)
+        for name, v in (("x", x), ("alpha", alpha), ("beta", beta), ("counts", np.ones(n, np.int32)),
+                        ("positions", np.stack([np.zeros(n), position], 1).astype(np.int32))):
+            b[name].write(v)
+        graph.replay(stream)
+        stream.sync()
+        offsets = np.arange(n + 1)
+        assert np.array_equal(b["offsets"].read(np.int32), offsets)
+        fresh = position // block >= blocks
+        slots = b["slots"].read(np.int64)
+        assert np.array_equal(slots[fresh] // block, free[used:used + fresh.sum()])
+        used += int(fresh.sum())
+        blocks = np.maximum(blocks, position // block + 1)
+        assert np.array_equal(slots % block, position % block) and len(set(slots.tolist())) == n
+        y, y_off, windows = conv_reference(x.astype(np.float64), weight.astype(np.float64), windows, offsets, where, groups, D,
+                                           1.0, 1e-6)
+        out, off, states, _ = delta_reference(y, alpha.astype(np.float64), beta.astype(np.float64), states, offsets, where,
+                                              groups, heads, D, 1.0)
+        tol = off + 64 * np.max(y_off) * max(1, np.max(np.abs(out))) + U * np.abs(out)
+        assert np.all(np.abs(b["out"].read(np.float32).reshape(out.shape) - out) <= tol)
+        position += np.where(np.arange(n) % 3 == turn % 3, 15, 1)
+    graph.destroy()
+    plan.destroy()
 
 
 def test_attention_over_planned_pages(dev, stream):
