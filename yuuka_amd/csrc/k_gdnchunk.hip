@@ -338,10 +338,6 @@ __device__ __forceinline__ int by_length(const int32_t *offsets, const RaggedArg
     return __ffsll((unsigned long long)__builtin_amdgcn_ballot_w64(before == rank)) - 1;
 }
 
-// Rows of K in LDS, a plane a part: 16 bytes more than its elements, so that 16 rows of 8 bytes
-// spread over all banks.
-template <int D> constexpr int kKeyPitch = 2 * D + 16;
-
 template <typename E, int D, int CT> struct ScanLds {
     static constexpr int KS = D / 32, NP = kParts<E>;
     static constexpr uint32_t state = 0;                             // S, [32 dims of k][tile][part]
@@ -349,8 +345,15 @@ template <typename E, int D, int CT> struct ScanLds {
     static constexpr uint32_t v = r + 2 * CT * 3 * 1024;             // V'
     static constexpr uint32_t tail = v + 2 * CT * 3 * 1024;          // e^(c_last - c) V'
     static constexpr uint32_t keys = tail + 2 * CT * 3 * 1024;       // [chunk & 1][part][row]
-    static constexpr uint32_t key_part = kC * kKeyPitch<D>, key_buffer = NP * key_part;
+    // Rows of K, a plane a part, 16 bytes apart where LDS holds that. Without them, piece x of 8 bytes of a row is
+    // at x ^ turn(row), so that 16 rows of a piece and four rows of four lie in different banks: 64 prompts of 300 rows
+    // in all, 16 heads in F32, 245 -> 160 us with two tiles for one, 1 of 8191 rows (one tile) 352 -> 362.
+    static constexpr bool turned = keys + 2 * NP * kC * (2 * D + 16) > 160 * 1024;
+    static constexpr uint32_t pitch = 2 * D + (turned ? 0 : 16), key_part = kC * pitch, key_buffer = NP * key_part;
     static constexpr uint32_t total = keys + 2 * key_buffer;
+    static __device__ __forceinline__ int at(int row, int piece) {
+        return row * pitch + 8 * (turned ? piece ^ ((row & 3) << 2 | (row >> 2 & 3)) : piece);
+    }
 };
 
 // A workgroup has CT tiles of 16 columns of one head's state. Four waves walk the state, wave w with the rows
@@ -390,6 +393,8 @@ __global__ __launch_bounds__(64 * kScanWaves<E>) void chunk_scan_kernel(GdnRows 
         for (int m = 0; m < 3; m++)
             *reinterpret_cast<u32x2 *>(lds + area + (((tile >> 1) * CT + c) * 3 + m) * 1024 + lane * 16 + 8 * (tile & 1)) = part[m];
     };
+    // the lane's four terms of tile t of its key, of 16
+    auto key_at = [&](int t) { return L::at(r16, 4 * t + g4); };
     // (No branches among the loads and stores of a turn: a wait counts the least that may have been issued since, and
     // would be one for what was asked for last.)
     auto load_step = [&](int i, int what, int s, u32x4 (&x)[2][3]) {
@@ -417,7 +422,7 @@ __global__ __launch_bounds__(64 * kScanWaves<E>) void chunk_scan_kernel(GdnRows 
         };
         T4 k[KT];
         auto keys_to_lds = [&](int i) {
-            uint8_t *const to = lds + L::keys + (i & 1) * L::key_buffer + (16 * wave + r16) * kKeyPitch<D> + 8 * g4;
+            uint8_t *const to = lds + L::keys + (i & 1) * L::key_buffer + 16 * wave * L::pitch;
             const bool there = r.begin + i * kC + 16 * wave + r16 < r.end;
 #pragma unroll
             for (int s = 0; s < KS; s++) {
@@ -425,8 +430,8 @@ __global__ __launch_bounds__(64 * kScanWaves<E>) void chunk_scan_kernel(GdnRows 
                 parts(k[2 * s], k[2 * s + 1], x);
 #pragma unroll
                 for (int m = 0; m < NP; m++) {  // (rows behind the end are zeros: they meet zeros of V')
-                    *reinterpret_cast<u32x2 *>(to + m * L::key_part + 64 * s) = there ? u32x2{x[m][0], x[m][1]} : u32x2{0, 0};
-                    *reinterpret_cast<u32x2 *>(to + m * L::key_part + 64 * s + 32) = there ? u32x2{x[m][2], x[m][3]} : u32x2{0, 0};
+                    *reinterpret_cast<u32x2 *>(to + m * L::key_part + key_at(2 * s)) = there ? u32x2{x[m][0], x[m][1]} : u32x2{0, 0};
+                    *reinterpret_cast<u32x2 *>(to + m * L::key_part + key_at(2 * s + 1)) = there ? u32x2{x[m][2], x[m][3]} : u32x2{0, 0};
                 }
             }
         };
@@ -583,12 +588,12 @@ __global__ __launch_bounds__(64 * kScanWaves<E>) void chunk_scan_kernel(GdnRows 
         for (int c = 0; c < CT; c++) x[c] = Sum{kZero, kZero};
 #pragma unroll
         for (int d = 0; d < KS; d++) {
-            const uint8_t *const from = lds + keys + (16 * wave + r16) * kKeyPitch<D> + 8 * g4 + 64 * d;
+            const uint8_t *const from = lds + keys + 16 * wave * L::pitch;
             u32x4 k[NP];
 #pragma unroll
             for (int m = 0; m < NP; m++) {
-                const u32x2 lo = *reinterpret_cast<const u32x2 *>(from + m * L::key_part);
-                const u32x2 hi = *reinterpret_cast<const u32x2 *>(from + m * L::key_part + 32);
+                const u32x2 lo = *reinterpret_cast<const u32x2 *>(from + m * L::key_part + key_at(2 * d));
+                const u32x2 hi = *reinterpret_cast<const u32x2 *>(from + m * L::key_part + key_at(2 * d + 1));
                 k[m] = u32x4{lo[0], lo[1], hi[0], hi[1]};
             }
 #pragma unroll
@@ -648,9 +653,9 @@ __global__ __launch_bounds__(64 * kScanWaves<E>) void chunk_scan_kernel(GdnRows 
             for (int u = 0; u < ST; u++)
 #pragma unroll
                 for (int m = 0; m < NP; m++) {
-                    const uint32_t from = keys + m * L::key_part + (32 * d + 4 * g4 + (r16 >> 2)) * kKeyPitch<D> +
-                                          32 * (wave * ST + u) + 8 * (r16 & 3);
-                    const u32x2 lo = columns_of(lds + from), hi = columns_of(lds + from + 16 * kKeyPitch<D>);
+                    const uint32_t from = keys + m * L::key_part + 32 * d * L::pitch +
+                                          L::at(4 * g4 + (r16 >> 2), 4 * (wave * ST + u) + (r16 & 3));
+                    const u32x2 lo = columns_of(lds + from), hi = columns_of(lds + from + 16 * L::pitch);
                     k[u][m] = u32x4{lo[0], lo[1], hi[0], hi[1]};
                 }
 #pragma unroll
