@@ -385,9 +385,10 @@ def test_prompt(dev, stream, dtype, counts, groups, heads, D, raw):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("n,groups,heads,D", [(40, 1, 2, 128), (60, 2, 4, 128), (80, 1, 2, 64), (70, 2, 4, 64)])
+@pytest.mark.parametrize("n,groups,heads,D", [(40, 1, 2, 128), (60, 2, 4, 128), (80, 1, 2, 64), (70, 2, 4, 64), (60, 2, 8, 128),
+                                              (70, 1, 8, 64), (90, 2, 6, 64)])
 def test_prompts_of_many_requests(dev, stream, dtype, n, groups, heads, D):
-    """Workgroups of two and four tiles of columns, and more requests than are put in order."""
+    """Workgroups of two and four tiles of columns and of two heads, and more requests than are put in order."""
     rng = np.random.default_rng(n + D)
     counts = [int(x) for x in rng.permutation([0, 1, 64, 65, 130, 200] + [int(x) for x in rng.integers(0, 20, n - 6)])]
     rows = sum(counts)

@@ -174,14 +174,16 @@ __device__ __forceinline__ double lanes_scan(double x) {
     return add_shifted<0x143, 0xc>(x);  // lane 31 to rows 2 and 3
 }
 
-// Eight waves: four for k_i . k_j and T, four for q_i . k_j.
-template <typename E, int D>
+// Eight waves: four for k_i . k_j, four for q_i . k_j, then four for the T of every head. HH heads of a group share
+// the products.
+template <typename E, int D, int HH>
 __global__ __launch_bounds__(512) void chunk_prepare_kernel(GdnRows b, RaggedArgs a, uint32_t *__restrict__ left_all) {
     typedef typename E::T T;
-    __shared__ double sum[kC];  // of the log decays, base 2
-    __shared__ __align__(16) float beta[kC];
-    __shared__ __align__(16) float at[kC][kRowPitch];  // A^T, its diagonal blocks later those of T^T
-    const int number = blockIdx.x, h = blockIdx.y;
+    __shared__ double sum[HH][kC];  // of the log decays, base 2
+    __shared__ __align__(16) float beta[HH][kC];
+    __shared__ __align__(16) float at_all[HH][kC][kRowPitch];  // A^T, its diagonal blocks later those of T^T
+    const int number = blockIdx.x, group = blockIdx.y % a.groups;
+    auto head = [&](int u) { return group + a.groups * (HH * (int)(blockIdx.y / a.groups) + u); };
     // the request whose chunk this is
     const int after = wave_first(a.requests, [&](int j) {
         return first_chunk<kC>(row_range(b.offsets, a.rows, j).begin, j) > number;
@@ -193,15 +195,15 @@ __global__ __launch_bounds__(512) void chunk_prepare_kernel(GdnRows b, RaggedArg
     if (n <= 0) return;
     const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g4 = lane >> 4;
     // the waves' parts differ in length: turned from chunk to chunk, so that no SIMD has the longest each time
-    const int role = (__builtin_amdgcn_readfirstlane(tid >> 6) + number + h) & 7, wave = role & 3;
+    const int role = (__builtin_amdgcn_readfirstlane(tid >> 6) + number + blockIdx.y) & 7, wave = role & 3;
     const bool keys = role < 4;
     const T *const rows = static_cast<const T *>(b.qkv) + (int64_t)row0 * a.stride;
-    const int group = h % a.groups;
     const T *const k = rows + (a.groups + group) * D, *const mine = keys ? k : rows + group * D;
-    uint32_t *const left_here = left_all + ((int64_t)number * a.heads + h) * left::dwords;
+    auto left_here = [&](int u) { return left_all + ((int64_t)number * a.heads + head(u)) * left::dwords; };
 
-    if (role == 7) {  // a row a lane
-        float *const factors = reinterpret_cast<float *>(left_here + left::v);
+    if (role >= 8 - HH) {  // a row a lane
+        const int u = 7 - role, h = head(u);
+        float *const factors = reinterpret_cast<float *>(left_here(u) + left::v);
         const bool there = lane < n;
         const int64_t from = (int64_t)(row0 + (there ? lane : 0)) * a.heads + h;
         const float g = there ? log_decay_of(b, a, from, h) : 0.0f, step = there ? beta_of(b, a, from) : 0.0f;
@@ -209,8 +211,8 @@ __global__ __launch_bounds__(512) void chunk_prepare_kernel(GdnRows b, RaggedArg
         const double last = __builtin_bit_cast(double, (uint64_t)(uint32_t)__builtin_amdgcn_readlane(
                                                            (int)(__builtin_bit_cast(uint64_t, c) >> 32), 63) << 32 |
                                                            (uint32_t)__builtin_amdgcn_readlane((int)__builtin_bit_cast(uint64_t, c), 63));
-        sum[lane] = c;
-        beta[lane] = step;
+        sum[u][lane] = c;
+        beta[u][lane] = step;
         const float grown = __builtin_amdgcn_exp2f((float)c);
         factors[lane] = step;
         factors[kC + lane] = step * grown;
@@ -243,10 +245,10 @@ __global__ __launch_bounds__(512) void chunk_prepare_kernel(GdnRows b, RaggedArg
         }
     }
     // four terms of a row tile's sum over rows: half a step of 32
-    auto put = [&](int what, int i, int jt, f32x4 x) {
+    auto put = [&](uint32_t *area, int i, int jt, f32x4 x) {
         u32x2 part[3];
         split(x, part);
-        uint32_t *const to = left_here + what + (left::step(i, jt >> 1) * 3 * 64 + lane) * 4;
+        uint32_t *const to = area + (left::step(i, jt >> 1) * 3 * 64 + lane) * 4;
 #pragma unroll
         for (int u = 0; u < 3; u++) {
             *reinterpret_cast<u32x2 *>(to + u * 256 + 2 * (jt & 1)) = part[u];
@@ -260,26 +262,31 @@ __global__ __launch_bounds__(512) void chunk_prepare_kernel(GdnRows b, RaggedArg
         int it, jt;
         tile_of(m, &it, &jt);
         const int i = 16 * it + r16, j0 = 16 * jt + 4 * g4;
-        const double sum_i = sum[i];
-        const float factor = keys ? beta[i] : a.scale;
-        f32x4 x;
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            const bool low = keys ? j0 + e < i : j0 + e <= i;
-            const float fall = low ? __builtin_amdgcn_exp2f((float)(sum_i - sum[j0 + e])) : 0.0f;
-            x[e] = low ? dot[m][e] * fall * factor : 0.0f;
-        }
-        if (keys) {
+        for (int u = 0; u < HH; u++) {
+            const double sum_i = sum[u][i];
+            const float factor = keys ? beta[u][i] : a.scale;
+            f32x4 x;
 #pragma unroll
-            for (int e = 0; e < 4; e++) at[j0 + e][i] = x[e];
-        } else {
-            put(left::p, it, jt, x);
+            for (int e = 0; e < 4; e++) {
+                const bool low = keys ? j0 + e < i : j0 + e <= i;
+                const float fall = low ? __builtin_amdgcn_exp2f((float)(sum_i - sum[u][j0 + e])) : 0.0f;
+                x[e] = low ? dot[m][e] * fall * factor : 0.0f;
+            }
+            if (keys) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) at_all[u][j0 + e][i] = x[e];
+            } else {
+                put(left_here(u) + left::p, it, jt, x);
+            }
         }
     }
     lds_barrier();
     // ---- T: a wave inverts a diagonal block, from T (I + A) = I, a row a lane
-    const int diag = 16 * wave;
-    if (keys) {
+    const int diag = 16 * wave, which = HH == 2 ? role >> 2 : 0;
+    const bool inverts = HH == 2 || keys;
+    auto &at = at_all[which];
+    if (inverts) {
         float t[16];
 #pragma unroll
         for (int c = 15; c >= 0; c--) {
@@ -299,7 +306,7 @@ __global__ __launch_bounds__(512) void chunk_prepare_kernel(GdnRows b, RaggedArg
         }
     }
     lds_barrier();
-    if (!keys) return;
+    if (!inverts) return;
     // then its row of blocks: T_ij^T = -T_jj^T sum_m A_mj^T T_im^T
     auto block = [&](int jt, int m) { return *reinterpret_cast<const f32x4 *>(&at[16 * jt + r16][16 * m + 4 * g4]); };
     f32x4 t[4];
@@ -319,7 +326,7 @@ __global__ __launch_bounds__(512) void chunk_prepare_kernel(GdnRows b, RaggedArg
                 if (m <= wave) x = mma(block(jt, m), t[m], x);
             t[jt] = mma(block(jt, jt), -x, kZero);
         }
-        put(left::t, wave, jt, t[jt]);
+        put(left_here(which) + left::t, wave, jt, t[jt]);
     }
 }
 
@@ -701,7 +708,11 @@ hipError_t launch_gdn_prompt(const GdnRows &b, uint32_t dtype, const RaggedArgs 
         using E = decltype(e);
         constexpr int D = d();
         uint32_t *const left_all = static_cast<uint32_t *>(scratch);
-        chunk_prepare_kernel<E, D><<<dim3(numbers, a.heads), 512, 0, s>>>(b, a, left_all);
+        // Two heads a workgroup where that leaves every CU one. us of the whole call: 32 heads of 16 groups, 2000 rows in
+        // F32 142 -> 126, 16 x 8192 rows in BF16 266 -> 260; 500 rows in BF16 38 -> 40, which stay at one.
+        if (a.heads / a.groups % 2 == 0 && (int64_t)numbers * a.heads >= 2 * 256)
+            chunk_prepare_kernel<E, D, 2><<<dim3(numbers, a.heads / 2), 512, 0, s>>>(b, a, left_all);
+        else chunk_prepare_kernel<E, D, 1><<<dim3(numbers, a.heads), 512, 0, s>>>(b, a, left_all);
         hipError_t err = hipGetLastError();
         if (err != hipSuccess) return err;
         auto go = [&](auto tiles) {
