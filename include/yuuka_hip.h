@@ -754,7 +754,7 @@ YUUKA_API yuuka_status yuuka_gdn_conv(yuuka_stream * stream, yuuka_buffer * out,
  * left out; factors below 2^-102 lose parts, and a decay below e^-200 is zero. A
  * key, query, alpha or beta that is not finite makes NaN of its head's rows among the
  * same 64 (earlier ones too) and of those after, a value that is not finite of its
- * column there; other requests and heads stay clean. Its workspace holds 37.9 KB a
+ * column there; other requests and heads stay clean. Its workspace holds 25.9 KB a
  * head for every 64 rows of `rows`, and as much for every request. */
 YUUKA_API yuuka_status yuuka_gdn_prompt(yuuka_stream * stream, yuuka_buffer * out, const yuuka_buffer * qkv,
                         const yuuka_buffer * alpha, const yuuka_buffer * beta, const yuuka_buffer * dt,

@@ -116,8 +116,8 @@ __device__ __forceinline__ void pin_loads() {
 // What the first kernel leaves for a chunk and head: operands as the second loads them, 64 lanes
 // of 16 bytes each (256 dwords).
 namespace left {
-constexpr int t = 0;              // [step][part] of T
-constexpr int p = 6 * 3 * 256;    // [step][part] of P
+constexpr int t = 0;              // [step][tile] of T, float32
+constexpr int p = 6 * 2 * 256;    // [step][tile] of P
 constexpr int v = 2 * p;          // float32: beta, beta e^c, scale e^c, e^(c_last - c) of every row, e^c_last 64 times
 constexpr int dwords = v + 5 * kC;
 // Row tile i against rows 32 s .. (those up to its own are there).
@@ -246,14 +246,9 @@ __global__ __launch_bounds__(512) void chunk_prepare_kernel(GdnRows b, RaggedArg
     }
     // four terms of a row tile's sum over rows: half a step of 32
     auto put = [&](uint32_t *area, int i, int jt, f32x4 x) {
-        u32x2 part[3];
-        split(x, part);
-        uint32_t *const to = area + (left::step(i, jt >> 1) * 3 * 64 + lane) * 4;
-#pragma unroll
-        for (int u = 0; u < 3; u++) {
-            *reinterpret_cast<u32x2 *>(to + u * 256 + 2 * (jt & 1)) = part[u];
-            if (i == jt && !(i & 1)) *reinterpret_cast<u32x2 *>(to + u * 256 + 2) = u32x2{0, 0};  // above the diagonal
-        }
+        uint32_t *const to = area + (left::step(i, jt >> 1) * 2 * 64 + lane) * 4;
+        *reinterpret_cast<f32x4 *>(to + 256 * (jt & 1)) = x;
+        if (i == jt && !(i & 1)) *reinterpret_cast<f32x4 *>(to + 256) = kZero;  // above the diagonal
     };
     lds_barrier();
 #pragma unroll
@@ -404,11 +399,11 @@ __global__ __launch_bounds__(64 * kScanWaves<E>) void chunk_scan_kernel(GdnRows 
     auto key_at = [&](int t) { return L::at(r16, 4 * t + g4); };
     // (No branches among the loads and stores of a turn: a wait counts the least that may have been issued since, and
     // would be one for what was asked for last.)
-    auto load_step = [&](int i, int what, int s, u32x4 (&x)[2][3]) {
+    auto load_step = [&](int i, int what, int s, f32x4 (&x)[2][2]) {
         const int step = left::step(wave, min(s, wave >> 1));
 #pragma unroll
-        for (int m = 0; m < 3; m++)
-            x[s][m] = *reinterpret_cast<const u32x4 *>(chunk_at(i) + what + ((step * 3 + m) * 64 + lane) * 4);
+        for (int m = 0; m < 2; m++)
+            x[s][m] = *reinterpret_cast<const f32x4 *>(chunk_at(i) + what + ((step * 2 + m) * 64 + lane) * 4);
     };
 
     if (role >= 4) {  // ---- keys and outputs
@@ -459,7 +454,7 @@ __global__ __launch_bounds__(64 * kScanWaves<E>) void chunk_scan_kernel(GdnRows 
             return;
         }
         T4 q[KT];
-        u32x4 p[2][3];
+        f32x4 p[2][2];
         f32x4 front;
         if (last >= 0) {
             load_rows(0, group, q);
@@ -504,11 +499,13 @@ __global__ __launch_bounds__(64 * kScanWaves<E>) void chunk_scan_kernel(GdnRows 
 #pragma unroll
             for (int s = 0; s < 2; s++) {
                 if (s > wave / 2) break;
+                u32x4 x[3];
+                split(p[s][0], p[s][1], x);
 #pragma unroll
                 for (int c = 0; c < CT; c++) {
                     u32x4 y[3];
                     operand(L::v, s, c, y);
-                    mma32(p[s], y, o[c]);
+                    mma32(x, y, o[c]);
                 }
             }
             load_step(i + 1, left::p, 0, p);
@@ -549,7 +546,7 @@ __global__ __launch_bounds__(64 * kScanWaves<E>) void chunk_scan_kernel(GdnRows 
                 s[t][c][e] = (uint32_t)slot.x < (uint32_t)a.states
                                  ? b.state[slot.x * size + at0 + (int64_t)(16 * (wave * ST + t) + 4 * g4 + e) * D + 16 * c]
                                  : 0.0f;
-    u32x4 t[2][3];
+    f32x4 t[2][2];
     T v[CT][4];
     f32x4 beta, grown, tail;
     float fall;
@@ -628,11 +625,13 @@ __global__ __launch_bounds__(64 * kScanWaves<E>) void chunk_scan_kernel(GdnRows 
 #pragma unroll
         for (int d = 0; d < 2; d++) {
             if (d > wave / 2) break;
+            u32x4 z[3];
+            split(t[d][0], t[d][1], z);
 #pragma unroll
             for (int c = 0; c < CT; c++) {
                 u32x4 y[3];
                 operand(L::r, d, c, y);
-                mma32(t[d], y, w[c]);
+                mma32(z, y, w[c]);
             }
         }
         load_step(i + 1, left::t, 0, t);
