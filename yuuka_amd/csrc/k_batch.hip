@@ -10,6 +10,9 @@
 //   slot of position p = page * block + p % block
 // Every block that gets a page holds a new row, so that the rows alone write the
 // tables: the first of a block does.
+//
+// Bound by the launch: 16 requests of one row 6.7 us, 200 of 16300 rows (0.3 MB) 6.8. The sums are in 64 bits, so that no
+// counts overflow them.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

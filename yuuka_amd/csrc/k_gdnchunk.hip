@@ -7,7 +7,13 @@
 //   out = e^c (Q S) + P V',     P_ij = (q_i . k_j) e^(c_i - c_j)  for i >= j
 //   S <- e^(c_last) S + K^T diag(e^(c_last - c)) V'
 // The first kernel makes T and P of every chunk and head, all chunks at once; the second
-// walks the chunks of a request with S in registers.
+// walks the chunks of a request with S in registers. Row after row, with two sums over the workgroup each, 8191 rows
+// of 16 heads of 128 in F32 take 17.7 ms; 64 at a time 0.42.
+//
+// The bytes that cannot be done without are 0.27 GB there, 56 us at the rate of a large copy, and the products 0.1 TFLOP of
+// bf16. Neither binds: the second kernel's chain does, 2.7 us a chunk (2.0 with nothing loaded from memory), of three
+// phases that each write LDS, wait for a barrier, read LDS and run a chain of matrix instructions. Matrix
+// instructions are busy 24 % of the cycles of the 128 CUs that have a workgroup, vector ones issue in 47 %.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -175,7 +181,9 @@ __device__ __forceinline__ double lanes_scan(double x) {
 }
 
 // Eight waves: four for k_i . k_j, four for q_i . k_j, then four for the T of every head. HH heads of a group share
-// the products.
+// the products. Small dependent phases: waves wait in 61 % of their cycles, vector instructions issue in 36 %, and
+// neither fewer registers nor less traffic alone made it faster. 81 us for 8191 rows of 16 heads of 128 in F32 (0.22 GB
+// moved, 2.7 TB/s), 62 for 16 x 8192 rows of 32 heads in BF16.
 template <typename E, int D, int HH>
 __global__ __launch_bounds__(512) void chunk_prepare_kernel(GdnRows b, RaggedArgs a, uint32_t *__restrict__ left_all) {
     typedef typename E::T T;
@@ -232,7 +240,7 @@ __global__ __launch_bounds__(512) void chunk_prepare_kernel(GdnRows b, RaggedArg
         o.load(x + (int64_t)(16 * tile + r16) * a.stride, g4, 16 * tile + r16 < n);
     };
     f32x4 dot[3];
-    {  // (all rows asked for before the first product: 148 registers for 84, 8191 rows 88 -> 105 us)
+    {  // (all rows asked for before the first product take 148 registers for 84, and a fifth longer)
         Rows xi, kj;
 #pragma unroll
         for (int m = 0; m < 3; m++) {
@@ -348,8 +356,9 @@ template <typename E, int D, int CT> struct ScanLds {
     static constexpr uint32_t tail = v + 2 * CT * 3 * 1024;          // e^(c_last - c) V'
     static constexpr uint32_t keys = tail + 2 * CT * 3 * 1024;       // [chunk & 1][part][row]
     // Rows of K, a plane a part, 16 bytes apart where LDS holds that. Without them, piece x of 8 bytes of a row is
-    // at x ^ turn(row), so that 16 rows of a piece and four rows of four lie in different banks: 64 prompts of 300 rows
-    // in all, 16 heads in F32, 245 -> 160 us with two tiles for one, 1 of 8191 rows (one tile) 352 -> 362.
+    // at x ^ turn(row), so that 16 rows of a piece and four rows of four lie in different banks: float32 keys of 128
+    // dims then leave room for two tiles (16 prompts of 8000 rows in all, 32 heads, 526 -> 410 us); with one tile the turn
+    // takes longer than the space (1 prompt of 8191 rows, the second kernel, 352 -> 362).
     static constexpr bool turned = keys + 2 * NP * kC * (2 * D + 16) > 160 * 1024;
     static constexpr uint32_t pitch = 2 * D + (turned ? 0 : 16), key_part = kC * pitch, key_buffer = NP * key_part;
     static constexpr uint32_t total = keys + 2 * key_buffer;
@@ -360,8 +369,11 @@ template <typename E, int D, int CT> struct ScanLds {
 
 // A workgroup has CT tiles of 16 columns of one head's state. Four waves walk the state, wave w with the rows
 // D / 4 w .. of it and the chunk's rows 16 w .. + 15; four make the outputs of 16 rows each, and those, or four
-// more where a key has several parts, bring the keys to LDS, a chunk ahead. Three barriers a chunk:
+// more where a key has several parts (float32 keys split by the waves of the outputs: a fifth longer), bring the keys to
+// LDS, a chunk ahead. Three barriers a chunk:
 //   S and K there | K S -> R; Q S | T R -> V' | S; P V'
+// What a chunk needs from memory is asked for one chunk ahead; two ahead, or W = T (beta e^c K) from the
+// first kernel for one phase less, took more registers than there are and were slower.
 template <typename E> constexpr int kScanWaves = kParts<E> == 3 ? 12 : 8;
 template <typename E, int D, int CT>
 __global__ __launch_bounds__(64 * kScanWaves<E>) void chunk_scan_kernel(GdnRows b, RaggedArgs a, const uint32_t *left_all) {
@@ -733,9 +745,9 @@ hipError_t launch_gdn_prompt(const GdnRows &b, uint32_t dtype, const RaggedArgs 
             }
         };
         // The most columns that LDS holds and that leave every CU a workgroup: what is loaded for a chunk serves more of
-        // them. us with 1, 2 and 4 tiles, BF16: 1 prompt of 2000 rows, 16 heads of 128 (128 workgroups at one tile) 99, 122,
-        // 174; 4 of 1000 (512) 103, 85, 110; 4 of 1000, 32 heads (1024) 196, 151, 129; 16 of 8192 rows in all (4096)
-        // 433, 347, 278.
+        // them. us with 1, 2 and 4 tiles, BF16: 1 prompt of 2000 rows, 16 heads of 128 (128 workgroups at one tile) 90, 119,
+        // 178; 4 of 1000 (512) 104, 83, 109; 4 of 1000, 32 heads (1024) 184, 142, 128; 16 of 8192 rows in all (4096)
+        // 388, 302, 260. F32, 16 heads: 4 of 1000 rows 138, 113, 64 of 300 in all 241, 157.
         const int64_t columns = (int64_t)a.requests * a.heads * (D / 16);
         if (columns >= 4 * 256 && ScanLds<E, D, 4>::total <= 160 * 1024) go(std::integral_constant<int, 4>{});
         else if (columns >= 2 * 256 && ScanLds<E, D, 2>::total <= 160 * 1024) go(std::integral_constant<int, 2>{});
