@@ -227,6 +227,9 @@ CONVS = [  # counts, groups, heads, D, taps
     ([1], 1, 1, 64, 4), ([7, 0, 1, 2, 3, 5, 0, 0, 100, 4], 2, 4, 64, 4), ([130, 1, 1, 1, 65], 1, 2, 128, 4),
     ([9, 2, 1, 30], 1, 3, 128, 2), ([1, 1, 2, 50, 3, 8, 7, 6, 0], 2, 2, 64, 8), ([1] * 70, 1, 1, 128, 3),
     ([5, 0, 33], 3, 3, 128, 5), ([0, 0], 1, 1, 64, 4),
+    # several rows a wave, with requests that start, end and lie within
+    ([1] * 9 + [0, 2, 3, 0, 5, 40, 1, 900, 0, 0, 1500, 33, 2, 2, 2], 4, 12, 128, 4),
+    ([1] * 9 + [0, 2, 3, 0, 5, 40, 1, 1900, 0, 0, 2500, 33, 2, 2, 2], 4, 8, 64, 3),
 ]
 
 

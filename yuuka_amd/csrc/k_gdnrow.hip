@@ -54,19 +54,36 @@ template <int N> __device__ __forceinline__ float lanes_sum(float x) {
 // rows and keeps the last KT - 1 of them in registers; the wave with a request's first
 // row reads its window and leaves its new one, which may be in the same slot.
 // Requests without rows have their window moved by waves of their own.
-// Bound by memory: 8191 rows of 8192 channels in BF16, 0.27 GB, 78 us, 3.4 TB/s (a copy of 2 GB
-// reaches 4.9).
+// 8191 rows of 8192 channels in BF16, 0.27 GB, 71 us, 3.8 TB/s (a large copy reaches 4.7 to 5.1): half vector
+// issue, half the latency of a row's chain, with four waves a SIMD.
 template <typename E, int KT, int D>
 __global__ __launch_bounds__(256) void ragged_conv_kernel(typename E::T *__restrict__ out,
                                                           const typename E::T *__restrict__ x,
                                                           const float *__restrict__ weight, float *__restrict__ state,
                                                           const int32_t *__restrict__ offsets,
                                                           const int2 *__restrict__ slots, RaggedArgs a, int run,
-                                                          int row_blocks) {
+                                                          int row_blocks, int columns) {
     constexpr int V = E::kWide;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const int c = (blockIdx.y * 64 + lane) * V;
+    const bool moves = (int)blockIdx.y >= columns;  // windows of requests without rows
+    const int item = moves ? ((int)blockIdx.y - columns) * (int)gridDim.x + (int)blockIdx.x : 0;
+    const int column = moves ? item % columns : (int)blockIdx.y;
+    if (!moves && (int)blockIdx.x >= row_blocks) return;
+    const int c = (column * 64 + lane) * V;
     const bool live = c < a.channels;
+    // The taps of the workgroup's channels, a channel's four in a place whose low bits are turned by the reading lane's,
+    // so that lanes, whose channels are V apart, meet few banks. Read from memory by every lane for itself, 128 bytes
+    // apart, they took 9 of 80 us.
+    __shared__ float4 taps[KT == 4 ? 64 * V : 1];
+    if constexpr (KT == 4) {
+        const int c0 = column * 64 * V;
+#pragma unroll
+        for (int u = 0; u < V / 4; u++) {
+            const int n = u * 256 + threadIdx.x;
+            taps[n ^ (V == 8 ? n >> 3 & 7 : n >> 2 & 3)] = reinterpret_cast<const float4 *>(weight)[min(c0 + n, a.channels - 1)];
+        }
+        __syncthreads();
+    }
     const int K1 = KT == 4 ? 3 : a.kernel - 1;  // (four taps are four; other numbers are the last of eight)
     const int64_t window = (int64_t)a.channels * K1;
     // the request's window before its rows, oldest first, zeros in front where K < KT
@@ -136,8 +153,8 @@ __global__ __launch_bounds__(256) void ragged_conv_kernel(typename E::T *__restr
                     if (t >= KT - 1 - K1) at[i * K1 + t - (KT - 1 - K1)] = next[t][i];
         }
     };
-    if ((int)blockIdx.x >= row_blocks) {  // requests without rows
-        const int j = ((int)blockIdx.x - row_blocks) * 4 + wave;
+    if (moves) {
+        const int j = item / columns * 4 + wave;
         if (j >= a.requests) return;
         const RowRange r = row_range(offsets, a.rows, j);
         if (r.end > r.begin) return;
@@ -153,12 +170,19 @@ __global__ __launch_bounds__(256) void ragged_conv_kernel(typename E::T *__restr
     if (j >= a.requests) return;
     float w[KT][V];
 #pragma unroll
-    for (int t = 0; t < KT; t++)
+    for (int i = 0; i < V; i++) {
+        if constexpr (KT == 4) {
+            const int n = lane * V + i;
+            const float4 y = taps[n ^ (V == 8 ? n >> 3 & 7 : n >> 2 & 3)];
+            w[0][i] = y.x, w[1][i] = y.y, w[2][i] = y.z, w[3][i] = y.w;
+        } else {
 #pragma unroll
-        for (int i = 0; i < V; i++) {
-            const int at = t - (KT - 1 - K1);
-            w[t][i] = live && at >= 0 ? weight[(int64_t)(c + i) * (K1 + 1) + at] : 0.0f;
+            for (int t = 0; t < KT; t++) {
+                const int at = t - (KT - 1 - K1);
+                w[t][i] = live && at >= 0 ? weight[(int64_t)(c + i) * (K1 + 1) + at] : 0.0f;
+            }
         }
+    }
     const int keys = a.groups * D;
     RowRange r = row_range(offsets, a.rows, j);
     bool fresh = true;  // the window is not in the registers
@@ -338,16 +362,23 @@ hipError_t launch_gdn_ragged_conv(void *out, const void *x, uint32_t dtype, cons
     by_type(dtype, [&](auto e) {
         using E = decltype(e);
         typedef typename E::T T;
-        // A wave's rows: as many as leave the GPU 2048 waves, up to 32, for each wave reads its channels' weights and
-        // K - 1 rows more. us with 512, 1024, 2048 and 4096 waves: 500 rows of 16 heads in F32 19, 14, 13, 20, 2000 of
-        // 32 heads in BF16 43, 43, 35, 39, 8191 (32 rows a wave in each) 82; with 64 rows a wave 105.
-        const int64_t waves = (int64_t)a.rows * ((a.channels + 64 * E::kWide - 1) / (64 * E::kWide));
-        const int run = (int)std::clamp<int64_t>(waves / 2048, 1, 32);
+        // A wave's rows: as few as leave every CU the same number of workgroups, four or a multiple, and up to 32 (16 in
+        // F32, of half the channels). A wave's start, with request, taps and K - 1 rows more, is what fewer cost: 7 prompts of
+        // 8191 rows, 32 heads in BF16, 8, 16 and 32 rows a wave 84, 77 and 71 us, 31 (a fifth workgroup on some CUs) 91;
+        // 16 of 8000 rows, 32 heads in F32, 120, 115 and 127.
+        constexpr int kRows = 4 * E::kWide;
+        const int columns = (a.channels + 64 * E::kWide - 1) / (64 * E::kWide);
+        const int64_t turns = ((int64_t)a.rows * columns + kRows * 4096 - 1) / (kRows * 4096);
+        const int64_t runs = 4 * std::max<int64_t>(1024 * turns / columns, 1);
+        const int run = (int)((a.rows + runs - 1) / runs);
         const int row_blocks = (int)(((int64_t)a.rows + 4 * run - 1) / (4 * run));
-        const dim3 grid(row_blocks + (a.requests + 3) / 4, (a.channels + 64 * E::kWide - 1) / (64 * E::kWide));
+        // Windows that only move come after the rows, which are thus spread evenly: 16 prompts of 8000 rows, 16 heads in
+        // F16, 74 -> 57 us.
+        const int fours = (a.requests + 3) / 4, width = std::max(row_blocks, (fours + 7) / 8);
+        const dim3 grid(width, columns + (int)(((int64_t)fours * columns + width - 1) / width));
         auto go = [&](auto taps, auto d) {
             ragged_conv_kernel<E, taps(), d()><<<grid, 256, 0, s>>>(static_cast<T *>(out), static_cast<const T *>(x), weight,
-                                                                    state, offsets, slots, a, run, row_blocks);
+                                                                    state, offsets, slots, a, run, row_blocks, columns);
         };
         auto by_dim = [&](auto taps) {
             if (a.head_dim == 128) go(taps, std::integral_constant<int, 128>{});
