@@ -13,7 +13,7 @@
 // The bytes that cannot be done without are 0.27 GB there, 56 us at the rate of a large copy, and the products 0.1 TFLOP of
 // bf16. Neither binds: the second kernel's chain does, 2.7 us a chunk (2.0 with nothing loaded from memory), of three
 // phases that each write LDS, wait for a barrier, read LDS and run a chain of matrix instructions. Matrix
-// instructions are busy 24 % of the cycles of the 128 CUs that have a workgroup, vector ones issue in 47 %.
+// instructions are busy 24 % of the cycles of the 128 CUs that have a workgroup, vector ones issue in 56 %.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -181,9 +181,9 @@ __device__ __forceinline__ double lanes_scan(double x) {
 }
 
 // Eight waves: four for k_i . k_j, four for q_i . k_j, then four for the T of every head. HH heads of a group share
-// the products. Small dependent phases: waves wait in 61 % of their cycles, vector instructions issue in 36 %, and
-// neither fewer registers nor less traffic alone made it faster. 81 us for 8191 rows of 16 heads of 128 in F32 (0.22 GB
-// moved, 2.7 TB/s), 62 for 16 x 8192 rows of 32 heads in BF16.
+// the products. Small dependent phases: waves wait in 58 % of their cycles, vector instructions issue in 40 % (BF16;
+// in F32 21 %, the matrix units busy in 26 %). 81 us for 8191 rows of 16 heads of 128 in F32 (0.12 GB moved), 61 for 8192
+// rows of 16 prompts and 32 heads in BF16 (0.15 GB).
 template <typename E, int D, int HH>
 __global__ __launch_bounds__(512) void chunk_prepare_kernel(GdnRows b, RaggedArgs a, uint32_t *__restrict__ left_all) {
     typedef typename E::T T;
