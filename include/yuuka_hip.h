@@ -749,8 +749,8 @@ YUUKA_API yuuka_status yuuka_gdn_conv(yuuka_stream * stream, yuuka_buffer * out,
  * Keys of norm 1 (as the convolution leaves them), beta in 0..1 and g <= 0 are what the
  * rule is stable for. yuuka_gdn_step takes one row of every request, row j
  * of request j (`rows` is not less than `requests`).
- * Precision: FP32 sums and states. yuuka_gdn_prompt solves 64 rows of a request at a
- * time, its float32 factors as three bf16 parts whose products below 2^-23 of the whole are
+ * Precision: FP32 sums and states. yuuka_gdn_prompt takes requests of one or two rows row
+ * by row, and solves 64 rows of a longer one at a time, its float32 factors as three bf16 parts whose products below 2^-23 of the whole are
  * left out; factors below 2^-102 lose parts, and a decay below e^-200 is zero. A
  * key, query, alpha or beta that is not finite makes NaN of its head's rows among the
  * same 64 (earlier ones too) and of those after, a value that is not finite of its

@@ -356,7 +356,8 @@ def check_delta(got, want, dtype, live):
 DELTAS = [  # counts, groups, heads, D
     ([1], 1, 1, 64), ([1], 1, 2, 128), ([3, 0, 1, 2], 2, 4, 64), ([15, 16, 17, 31, 32, 33], 1, 2, 128),
     ([63, 64, 65], 1, 1, 64), ([63, 64, 65, 0], 2, 2, 128), ([130, 1, 0, 0, 200, 7], 1, 3, 128), ([300], 2, 4, 64),
-    ([127, 128, 129], 1, 1, 128), ([5] * 40, 1, 2, 64), ([0], 1, 1, 128),
+    ([127, 128, 129], 1, 1, 128), ([5] * 40, 1, 2, 64), ([0], 1, 1, 128), ([1, 2, 0] * 25, 2, 8, 64), ([2, 1] * 40, 1, 8, 128),
+    ([1] * 70, 1, 1, 128),
 ]
 
 

@@ -180,12 +180,104 @@ __device__ __forceinline__ double lanes_scan(double x) {
     return add_shifted<0x143, 0xc>(x);  // lane 31 to rows 2 and 3
 }
 
+// A request of one or two rows, row after row by the first kernel: S = e^g S;  d = beta (v - S^T k);  S += k d^T;
+// o = S^T q. A workgroup has a head's state, a thread four columns of every (2048 / D)th row. 200 requests of 16
+// heads of 128 in BF16 of one, two and four rows each 236, 237 and 238 us in chunks, 89, 98 and 117 (then by four
+// rows) this way; with four, a batch of 96 requests of unequal lengths, 6000 rows of 16 heads of 64 in F16, takes 102 us for 97.
+constexpr int kFew = 2;
+template <typename E, int D>
+__device__ __forceinline__ void few_rows(const GdnRows &b, const RaggedArgs &a, RowRange r, int j, int h, float *lds) {
+    typedef typename E::T T;
+    constexpr int C4 = D / 4, RG = 512 / C4, NR = D / RG;
+    float *const qkv = lds;  // q, k and v of the row
+    float4 *const part = reinterpret_cast<float4 *>(lds + 3 * D);  // [2][8][C4]
+    const int t = threadIdx.x, wave = t >> 6, lane = t & 63, c4 = t % C4, rg = t / C4, group = h % a.groups;
+    const int64_t size = (int64_t)a.heads * D * D, mine = (int64_t)h * D * D + 4 * c4;
+    const int2 slot = b.slots[j];
+    float4 s[NR];
+#pragma unroll
+    for (int m = 0; m < NR; m++)
+        s[m] = (uint32_t)slot.x < (uint32_t)a.states
+                   ? *reinterpret_cast<const float4 *>(b.state + slot.x * size + mine + (int64_t)(rg + RG * m) * D)
+                   : make_float4(0.f, 0.f, 0.f, 0.f);
+    // sum over the row groups of every column, in every thread
+    auto total = [&](float4 x, int which) {
+#pragma unroll
+        for (int off = C4; off < 64; off <<= 1) {
+            x.x += __shfl_xor(x.x, off);
+            x.y += __shfl_xor(x.y, off);
+            x.z += __shfl_xor(x.z, off);
+            x.w += __shfl_xor(x.w, off);
+        }
+        if (lane < C4) part[(which * 8 + wave) * C4 + c4] = x;
+        lds_barrier();
+        float4 sum = part[which * 8 * C4 + c4];
+#pragma unroll
+        for (int w = 1; w < 8; w++) {
+            const float4 y = part[(which * 8 + w) * C4 + c4];
+            sum.x += y.x; sum.y += y.y; sum.z += y.z; sum.w += y.w;
+        }
+        return sum;
+    };
+    for (int row = r.begin; row < r.end; row++) {
+        const T *const x = static_cast<const T *>(b.qkv) + (int64_t)row * a.stride;
+        if (t < 3 * D) {
+            const int part_of = t / D;
+            const float y = (float)x[(part_of == 0 ? group : part_of == 1 ? a.groups + group : 2 * a.groups + h) * D + t % D];
+            qkv[t] = part_of == 0 ? y * a.scale : y;
+        }
+        const float decay = expf(log_decay_of(b, a, (int64_t)row * a.heads + h, h));
+        const float beta = beta_of(b, a, (int64_t)row * a.heads + h);
+        lds_barrier();
+        float4 seen = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int m = 0; m < NR; m++) {
+            const float k = qkv[D + rg + RG * m];
+            s[m].x *= decay; s[m].y *= decay; s[m].z *= decay; s[m].w *= decay;
+            seen.x = fmaf(s[m].x, k, seen.x);
+            seen.y = fmaf(s[m].y, k, seen.y);
+            seen.z = fmaf(s[m].z, k, seen.z);
+            seen.w = fmaf(s[m].w, k, seen.w);
+        }
+        seen = total(seen, 0);
+        const float4 v = *reinterpret_cast<const float4 *>(qkv + 2 * D + 4 * c4);
+        const float4 d = make_float4((v.x - seen.x) * beta, (v.y - seen.y) * beta, (v.z - seen.z) * beta, (v.w - seen.w) * beta);
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int m = 0; m < NR; m++) {
+            const float q = qkv[rg + RG * m], k = qkv[D + rg + RG * m];
+            s[m].x = fmaf(k, d.x, s[m].x);
+            s[m].y = fmaf(k, d.y, s[m].y);
+            s[m].z = fmaf(k, d.z, s[m].z);
+            s[m].w = fmaf(k, d.w, s[m].w);
+            o.x = fmaf(s[m].x, q, o.x);
+            o.y = fmaf(s[m].y, q, o.y);
+            o.z = fmaf(s[m].z, q, o.z);
+            o.w = fmaf(s[m].w, q, o.w);
+        }
+        o = total(o, 1);
+        if (t < C4) {
+            T *const to = static_cast<T *>(b.out) + ((int64_t)row * a.heads + h) * D + 4 * t;
+            to[0] = (T)o.x;
+            to[1] = (T)o.y;
+            to[2] = (T)o.z;
+            to[3] = (T)o.w;
+        }
+    }
+    if ((uint32_t)slot.y < (uint32_t)a.states) {
+#pragma unroll
+        for (int m = 0; m < NR; m++)
+            *reinterpret_cast<float4 *>(b.state + slot.y * size + mine + (int64_t)(rg + RG * m) * D) = s[m];
+    }
+}
+
 // Eight waves: four for k_i . k_j, four for q_i . k_j, then four for the T of every head. HH heads of a group share
 // the products. Small dependent phases: waves wait in 58 % of their cycles, vector instructions issue in 40 % (BF16;
 // in F32 21 %, the matrix units busy in 26 %). 81 us for 8191 rows of 16 heads of 128 in F32 (0.12 GB moved), 61 for 8192
 // rows of 16 prompts and 32 heads in BF16 (0.15 GB).
+// (Six waves a SIMD for 16-bit rows: the registers of few_rows would leave five, 62 -> 70 us.)
 template <typename E, int D, int HH>
-__global__ __launch_bounds__(512) void chunk_prepare_kernel(GdnRows b, RaggedArgs a, uint32_t *__restrict__ left_all) {
+__global__ __launch_bounds__(512, (kParts<E> == 3 ? 1 : 6)) void chunk_prepare_kernel(GdnRows b, RaggedArgs a, uint32_t *__restrict__ left_all) {
     typedef typename E::T T;
     __shared__ double sum[HH][kC];  // of the log decays, base 2
     __shared__ __align__(16) float beta[HH][kC];
@@ -201,6 +293,10 @@ __global__ __launch_bounds__(512) void chunk_prepare_kernel(GdnRows b, RaggedArg
     const RowRange r = row_range(b.offsets, a.rows, j);
     const int row0 = r.begin + (number - first_chunk<kC>(r.begin, j)) * kC, n = min(kC, r.end - row0);
     if (n <= 0) return;
+    if (r.end - r.begin <= kFew) {  // (the second kernel leaves them out)
+        for (int u = 0; u < HH; u++) few_rows<E, D>(b, a, r, j, head(u), &at_all[0][0][0]);
+        return;
+    }
     const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g4 = lane >> 4;
     // the waves' parts differ in length: turned from chunk to chunk, so that no SIMD has the longest each time
     const int role = (__builtin_amdgcn_readfirstlane(tid >> 6) + number + blockIdx.y) & 7, wave = role & 3;
@@ -387,6 +483,7 @@ __global__ __launch_bounds__(64 * kScanWaves<E>) void chunk_scan_kernel(GdnRows 
     const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g4 = lane >> 4;
     const int role = __builtin_amdgcn_readfirstlane(tid >> 6), wave = role & 3;
     const RowRange r = row_range(b.offsets, a.rows, j);
+    if (r.end > r.begin && r.end - r.begin <= kFew) return;  // done by the first kernel
     const int group = h % a.groups;
     const int number0 = first_chunk<kC>(r.begin, j), last = (r.end - r.begin + kC - 1) / kC - 1;
     const T *const qkv = static_cast<const T *>(b.qkv);
