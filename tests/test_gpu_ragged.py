@@ -268,6 +268,40 @@ def test_conv(dev, stream, dtype, counts, groups, heads, D, K, in_place):
     assert np.array_equal(wb.read(np.float32).reshape(windows.shape), new.astype(np.float32))
 
 
+PARTS = [  # rows in front of the first request, counts, groups, heads, D, taps
+    (1, [1], 1, 1, 64, 4), (8, [8], 1, 1, 128, 4), (70, [1, 2, 3, 0, 40, 1], 2, 4, 64, 4),
+    (900, [2, 1, 0, 3, 1, 1, 1500, 5], 4, 8, 128, 4), (2000, [1] * 20 + [0, 700, 2], 4, 12, 128, 4),
+    (130, [3, 9, 1, 0, 2], 1, 2, 128, 8), (33, [1, 50], 2, 2, 64, 2),
+]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("front,counts,groups,heads,D,K", PARTS)
+def test_conv_of_a_part_of_a_batch(dev, stream, dtype, front, counts, groups, heads, D, K):
+    """A batch whose first request does not start with the first row, every window left where it was read."""
+    rng = np.random.default_rng(front + D + K)
+    n, behind, channels = len(counts), 3, (2 * groups + heads) * D
+    live = sum(counts)
+    rows, offsets = front + live + behind, offsets_of(counts) + front
+    x = to_bits(rng.normal(0, 1, (rows, channels)), dtype)
+    x[:front] = x[front + live:] = to_bits(np.full(channels, np.nan), dtype)
+    w = rng.normal(0, 0.5, (channels, K)).astype(np.float32)
+    windows = rng.normal(0, 1, (n, channels, K - 1)).astype(np.float32)
+    slots = np.stack([rng.permutation(n)] * 2, 1).astype(np.int32)
+    ob, wb = dev.upload(to_bits(np.full((rows, channels), 7.0), dtype)), dev.upload(windows)
+    scale = D ** -0.5
+    p = hip.gdn_params(dtype, n, rows, groups, heads, D, kernel=K, scale=scale, eps=1e-6)
+    hip.gdn_conv(stream, ob, dev.upload(x), dev.upload(w), wb, dev.upload(offsets), dev.upload(slots), p)
+    stream.sync()
+    own = slice(front, front + live)
+    want, error, new = conv_reference(from_bits(x[own], dtype), w.astype(np.float64), windows.astype(np.float64),
+                                      offsets - front, slots, groups, D, scale, 1e-6)
+    got = from_bits(ob.read(np_type(dtype)).reshape(rows, channels), dtype)
+    assert np.all(got[:front] == 7.0) and np.all(got[front + live:] == 7.0)
+    assert np.all(np.abs(got[own] - want) <= error + HALF[dtype] * np.abs(want) + (2.0 ** -25 if dtype == hip.F16 else 0))
+    assert np.array_equal(wb.read(np.float32).reshape(windows.shape), new.astype(np.float32))
+
+
 # ------------------------------------------------------------- the delta rule
 
 def delta_reference(qkv, g, beta, states, offsets, slots, groups, heads, D, scale):

@@ -105,6 +105,74 @@ def test_no_offset_or_slot_leads_outside(tmp_path):
     assert out.split() == ["1", "0"]
 
 
+WALK = r"""
+#include "ragged_addr.h"
+#include <cstdio>
+#include <random>
+#include <vector>
+
+using namespace yk;
+
+// The convolution's walk over the rows, wave by wave, as k_gdnrow.hip has it.
+int main() {
+    std::mt19937 rng(11);
+    auto pick = [&](int lo, int hi) { return lo + (int)(rng() % (unsigned)(hi - lo + 1)); };
+    long bad = 0, front = 0;
+    for (int trial = 0; trial < 20000; trial++) {
+        const int n = pick(1, 8), early = pick(1, 7), run = pick(1, 33);
+        std::vector<int32_t> off(n + 1);
+        off[0] = pick(0, 1) ? 0 : pick(1, 120);  // a part of a batch: rows in front of it are nobody's
+        for (int j = 0; j < n; j++) off[j + 1] = off[j] + (pick(0, 3) ? pick(0, 1) ? pick(0, 4) : pick(0, 90) : 0);
+        const int rows = off[n] + pick(0, 40) + 1;
+        std::vector<int> outs(rows, 0), windows(n, 0);
+        for (int first = 0; first < rows; first += run) {
+            const int last = first + run < rows ? first + run : rows;
+            int row = first, j = 0, steps = 0;
+            while (j < n && off[j + 1] <= row) j++;
+            if (j == n) continue;
+            RowRange r = row_range(off.data(), rows, j);
+            bool fresh = true;
+            for (;; row++) {
+                if (++steps > run + early + 1) { bad++; break; }  // no further than the rows that it has
+                bool end = false;
+                while (row >= r.end) {
+                    if (row >= last || ++j >= n) { end = true; break; }
+                    r = row_range(off.data(), rows, j);
+                    fresh = true;
+                }
+                if (end) break;
+                const RowTurn turn = row_turn(r, row, first, last, early);
+                if (turn == kRowDone) break;
+                if (turn == kRowSkipped) continue;
+                if (row < r.begin || row >= rows) { bad++; break; }
+                if (fresh && row == r.begin) windows[j]++;
+                else if (fresh && row - r.begin < early) bad++;  // needs inputs of the window
+                fresh = false;
+                outs[row]++;
+            }
+        }
+        for (int row = 0; row < rows; row++) bad += outs[row] != (row >= off[0] && row < off[n]);
+        for (int j = 0; j < n; j++) bad += windows[j] != (off[j + 1] > off[j]);
+        front += off[0] > run;
+    }
+    printf("%d %ld\n", front > 5000, bad);
+}
+"""
+
+
+def test_every_row_and_window_of_a_convolution_is_one_waves(tmp_path):
+    """Whatever row a batch starts with: each of its rows is computed once, and each window read and written by one wave."""
+    cxx = shutil.which("g++") or shutil.which("clang++")
+    if not cxx:
+        pytest.skip("no host C++ compiler")
+    src = tmp_path / "walk.cpp"
+    src.write_text(WALK)
+    subprocess.run([cxx, "-O1", "-std=c++17", "-Wall", "-fsanitize=undefined", "-fno-sanitize-recover", f"-I{CSRC}",
+                    str(src), "-o", str(tmp_path / "walk")], check=True)
+    out = subprocess.run([str(tmp_path / "walk")], check=True, capture_output=True, text=True).stdout
+    assert out.split() == ["1", "0"]
+
+
 # ------------------------------------------------------------- refusals
 # Handles as internal.h lays them out, over memory that nothing reads: a refused call
 # launches nothing.

@@ -196,19 +196,19 @@ __global__ __launch_bounds__(256) void ragged_conv_kernel(typename E::T *__restr
     };
 #pragma unroll
     for (int u = 0; u < kAhead; u++) ahead[u] = load_raw(min(row + u, last - 1));
-    // A request's first K - 1 rows, which need its window, are the wave's that has the first of them: nobody
-    // else reads the slot that it may write. False when the wave is done.
+    // A request's window is the wave's that has its first row: nobody else reads the slot that it may write. False when
+    // the wave is done.
     auto step = [&](Bytes16 &slot) {
         while (row >= r.end) {
             if (row >= last || ++j >= a.requests) return false;
             r = row_range(offsets, a.rows, j);
             fresh = true;
         }
-        const bool early = row - r.begin < K1, begun = r.begin >= first;
-        if (row >= last && !(early && begun)) return false;
+        const RowTurn turn = row_turn(r, row, (int)first, last, K1);
+        if (turn == kRowDone) return false;
         const Bytes16 raw = row < last ? slot : load_raw(row);
         slot = load_raw(min(row + kAhead, last - 1));
-        if (row < r.begin || (early && !begun)) return true;  // (descending offsets leave rows between requests)
+        if (turn == kRowSkipped) return true;
         if (fresh) {
             if (row == r.begin) {
                 load_window(j);

@@ -25,6 +25,16 @@ YK_HD RowRange row_range(const int32_t *offsets, int rows, int j) {
     return {begin, end > begin ? end : begin};
 }
 
+// What the convolution's wave with rows first .. last - 1 does with `row`, `r` being the first request that ends
+// behind it. A request's first `early` rows need its window: they are the wave's that has the first of them, which goes
+// past its own last row for these and for no others. Rows before a request are nobody's.
+enum RowTurn { kRowDone, kRowSkipped, kRowTaken };
+YK_HD RowTurn row_turn(RowRange r, int row, int first, int last, int early) {
+    const bool begun = r.begin >= first && r.begin < last, needs_window = row - r.begin < early;
+    if (row >= last && !(begun && needs_window)) return kRowDone;
+    return row < r.begin || (needs_window && !begun) ? kRowSkipped : kRowTaken;
+}
+
 // The pages of a request at `position` that takes `count` rows, with `blocks`
 // entries of its table in use: new ones are table entries first .. first + fresh - 1.
 struct PageNeed {
