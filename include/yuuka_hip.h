@@ -655,11 +655,11 @@ YUUKA_API yuuka_status yuuka_attn_decode(yuuka_stream * stream, yuuka_buffer * o
 /* ----------------------------------------------------------------------
  * Ragged batches (extension): requests with different numbers of new rows,
  * laid one after another without padding. Rows offsets[j] .. offsets[j + 1] - 1
- * (int32) are request j's; rows behind the last are neither read nor written.
- * Offsets ascend. One outside 0 .. rows is taken as the nearest of those, a request
- * that ends before it starts as empty; where requests have rows in common, the results of
- * those requests are undefined (nothing outside the arrays is touched). Every buffer has
- * to be on the stream's device; an output must not overlap an input or another output,
+ * (int32) are request j's; rows in front of the first and behind the last are neither
+ * read nor written. One outside 0 .. rows is taken as the nearest of those. Offsets
+ * have to ascend (two alike: a request without rows): where they do not, the results of
+ * all requests are undefined, outputs, states and windows alike (nothing outside the
+ * arrays is touched). Every buffer has to be on the stream's device; an output must not overlap an input or another output,
  * except where said. Calls on one stream run in order; yuuka_batch_plan and
  * yuuka_gdn_prompt keep what they work out in the stream's workspace.
  * ---------------------------------------------------------------------- */

@@ -550,6 +550,54 @@ def test_offsets_that_lie(dev, stream):
     assert np.array_equal(got[1][1], states[1])
 
 
+@pytest.mark.parametrize("offsets", [(200, 0, 100), (50, 20, 60), (150, -5, 120, 7, 7, 200), (2 ** 31 - 1, 0, 64, -2 ** 31, 130)])
+def test_offsets_out_of_order(dev, stream, offsets):
+    """Results are undefined there, but nothing outside the rows and the slots is touched, and the next call is sound."""
+    rng = np.random.default_rng(len(offsets))
+    groups, heads, D, rows, n = 1, 2, 64, 200, len(offsets) - 1
+    qkv = unit_rows(rng, rows, groups, heads, D, hip.F32)
+    alpha, beta, _, _, g, b = gates(rng, rows, heads, False)
+    states = rng.normal(0, 0.3, (n + 1, heads, D, D)).astype(np.float32)
+    windows = rng.normal(0, 1, (n + 1, qkv.shape[1], 3)).astype(np.float32)
+    slots = np.stack([np.arange(n)] * 2, 1).astype(np.int32)
+    p = hip.gdn_params(hip.F32, n, rows, groups, heads, D, log_decay=True)
+    ends = dev.upload(i32(*offsets))
+    y, o = dev.upload(np.full((rows + 70, qkv.shape[1]), 7, np.float32)), dev.upload(np.full((rows + 70, heads, D), 7, np.float32))
+    wb, sb = dev.upload(windows), dev.upload(states)
+    where, weight = dev.upload(slots), dev.upload(rng.normal(0, 0.5, (qkv.shape[1], 4)).astype(np.float32))
+    hip.gdn_conv(stream, y, dev.upload(qkv), weight, wb, ends, where, p)
+    hip.gdn_prompt(stream, o, dev.upload(qkv), dev.upload(alpha), dev.upload(beta), sb, ends, where, p)
+    stream.sync()
+    for buf in (y, o):
+        assert np.all(buf.read(np.float32).reshape(rows + 70, -1)[rows:] == 7)
+    assert np.array_equal(wb.read(np.float32).reshape(windows.shape)[n], windows[n])
+    assert np.array_equal(sb.read(np.float32).reshape(states.shape)[n], states[n])
+    got = run_delta(dev, stream, hip.F32, qkv, alpha, beta, None, None, states, [rows - 90, 90], [[0, 0], [1, 1]], groups, heads, D)
+    want = delta_reference(qkv.astype(np.float64), g, b, states.astype(np.float64), i32(0, rows - 90, rows),
+                           np.array([[0, 0], [1, 1]]), groups, heads, D, 1.0)
+    check_delta(got, want, hip.F32, rows)
+
+
+@pytest.mark.parametrize("front", [1, 70, 200])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_prompt_of_a_part_of_a_batch(dev, stream, dtype, front):
+    """Requests that start behind the first row, with as many of one and two rows: the rows in front are left alone."""
+    rng = np.random.default_rng(front)
+    groups, heads, D, counts = 1, 2, 64, [1, 90, 0, 2, 3, 130]
+    n, live = len(counts), sum(counts)
+    qkv = unit_rows(rng, front + live, groups, heads, D, dtype)
+    qkv[:front] = to_bits(np.full(qkv.shape[1], np.nan), dtype)
+    alpha, beta, _, _, g, b = gates(rng, front + live, heads, False)
+    states = rng.normal(0, 0.3, (n, heads, D, D)).astype(np.float32)
+    slots = np.stack([rng.permutation(n)] * 2, 1)
+    out, new = run_delta(dev, stream, dtype, qkv, alpha, beta, None, None, states, None, slots, groups, heads, D,
+                         offsets=offsets_of(counts) + i32(front))
+    want = delta_reference(from_bits(qkv[front:], dtype), g[front:], b[front:], states.astype(np.float64), offsets_of(counts),
+                           slots, groups, heads, D, 1.0)
+    assert np.all(out[:front] == 7.0)
+    check_delta((out[front:], new), want, dtype, live)
+
+
 @pytest.mark.parametrize("D", [64, 128])
 def test_a_prompt_in_pieces(dev, stream, D):
     """A prompt in one call, in three, and token by token."""

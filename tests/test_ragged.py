@@ -173,6 +173,94 @@ def test_every_row_and_window_of_a_convolution_is_one_waves(tmp_path):
     assert out.split() == ["1", "0"]
 
 
+DISORDER = r"""
+#include "ragged_addr.h"
+#include <algorithm>
+#include <cstdio>
+#include <random>
+#include <vector>
+
+using namespace yk;
+
+// The 64-fold search of ragged_dev.h, all lanes at once.
+template <typename F> int wave_first(int n, F &&after) {
+    int lo = 0, hi = n;
+    while (lo < hi) {
+        const int step = (hi - lo + 63) / 64;
+        int k = 0;
+        while (k < 64 && !after((int)std::min<int64_t>(lo + (int64_t)step * (k + 1) - 1, hi - 1))) k++;
+        if (k == 64) return hi;
+        const int first = (int)std::min<int64_t>(lo + (int64_t)step * (k + 1) - 1, hi - 1);
+        if (step == 1) return first;
+        lo += step * k;
+        hi = first;
+    }
+    return lo;
+}
+
+int main() {
+    std::mt19937 rng(5);
+    auto pick = [&](int lo, int hi) { return lo + (int)(rng() % (unsigned)(hi - lo + 1)); };
+    const int32_t edge[] = {INT32_MIN, -1, 0, 1, INT32_MAX, 1000000};
+    long bad = 0, taken = 0;
+    for (int trial = 0; trial < 20000; trial++) {
+        const int n = pick(0, 9) ? pick(1, 9) : pick(60, 300), rows = pick(1, 300), early = pick(1, 7), run = pick(1, 33);
+        std::vector<int32_t> off(n + 1);
+        for (auto &o : off) o = pick(0, 5) ? pick(0, rows) : edge[pick(0, 5)];
+        // the convolution: every wave ends, and takes rows of the arrays alone
+        for (int first = 0; first < rows; first += run) {
+            const int last = std::min(first + run, rows);
+            int row = first, j = wave_first(n, [&](int i) { return off[i + 1] > row; });
+            if (j >= n) continue;
+            RowRange r = row_range(off.data(), rows, j);
+            for (int steps = 0;; row++) {
+                if (++steps > run + early + 1) { bad++; break; }
+                bool end = false;
+                while (row >= r.end) {
+                    if (row >= last || ++j >= n) { end = true; break; }
+                    r = row_range(off.data(), rows, j);
+                }
+                if (end) break;
+                const RowTurn turn = row_turn(r, row, first, last, early);
+                if (turn == kRowDone) break;
+                if (turn == kRowSkipped) continue;
+                if (row < 0 || row >= rows || row < r.begin) bad++;
+                taken++;
+            }
+        }
+        // the delta rule: chunks of rows of the arrays, whose places in the workspace are there
+        const int numbers = chunk_numbers<64>(rows, n);
+        for (int number = 0; number < numbers; number++) {
+            const int j = wave_first(n, [&](int i) { return first_chunk<64>(row_range(off.data(), rows, i).begin, i) > number; }) - 1;
+            if (j < 0) continue;
+            const RowRange r = row_range(off.data(), rows, j);
+            const int row0 = r.begin + (number - first_chunk<64>(r.begin, j)) * 64, some = std::min(64, r.end - row0);
+            if (j >= n || row0 < 0 || (some > 0 && row0 + some > rows)) bad++;
+        }
+        for (int j = 0; j < n; j++) {
+            const RowRange r = row_range(off.data(), rows, j);
+            const int last = (r.end - r.begin + 63) / 64 - 1;
+            if (last >= 0 && first_chunk<64>(r.begin, j) + last >= numbers) bad++;
+        }
+    }
+    printf("%d %ld\n", taken > 100000, bad);
+}
+"""
+
+
+def test_offsets_out_of_order_stay_inside(tmp_path):
+    """Where offsets do not ascend results are undefined; every wave ends, and nothing outside the arrays is touched."""
+    cxx = shutil.which("g++") or shutil.which("clang++")
+    if not cxx:
+        pytest.skip("no host C++ compiler")
+    src = tmp_path / "disorder.cpp"
+    src.write_text(DISORDER)
+    subprocess.run([cxx, "-O1", "-std=c++17", "-Wall", "-fsanitize=undefined", "-fno-sanitize-recover", f"-I{CSRC}",
+                    str(src), "-o", str(tmp_path / "disorder")], check=True)
+    out = subprocess.run([str(tmp_path / "disorder")], check=True, capture_output=True, text=True).stdout
+    assert out.split() == ["1", "0"]
+
+
 # ------------------------------------------------------------- refusals
 # Handles as internal.h lays them out, over memory that nothing reads: a refused call
 # launches nothing.

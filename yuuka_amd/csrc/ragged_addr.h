@@ -15,7 +15,7 @@ namespace yk {
 
 YK_HD int64_t clamp64(int64_t x, int64_t lo, int64_t hi) { return x < lo ? lo : x > hi ? hi : x; }
 
-// Rows of request j: offsets are taken to be within the row arrays, and a
+// Rows of request j, inside the row arrays whatever the offsets are: each is taken to be within them, and a
 // request whose end lies before its start to be empty.
 struct RowRange {
     int begin, end;
@@ -50,7 +50,7 @@ YK_HD PageNeed page_need(int64_t position, int64_t count, int64_t blocks, int bl
 }
 
 // Rows are worked on in chunks; those of request j, whose rows start at
-// `begin`, are numbered from here on, and the numbers of two requests never meet:
+// `begin`, are numbered from here on, and the numbers of two requests never meet where offsets ascend:
 // (begin + n) / C - begin / C + 1 is n / C, rounded up, at the least.
 template <int C> YK_HD int first_chunk(int begin, int j) { return begin / C + j; }
 template <int C> YK_HD int chunk_numbers(int rows, int requests) { return rows / C + requests; }
