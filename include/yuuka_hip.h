@@ -749,13 +749,16 @@ YUUKA_API yuuka_status yuuka_gdn_conv(yuuka_stream * stream, yuuka_buffer * out,
  * Keys of norm 1 (as the convolution leaves them), beta in 0..1 and g <= 0 are what the
  * rule is stable for. yuuka_gdn_step takes one row of every request, row j
  * of request j (`rows` is not less than `requests`).
- * Precision: FP32 sums and states. yuuka_gdn_prompt takes requests of one or two rows row
- * by row, and solves 64 rows of a longer one at a time, its float32 factors as three bf16 parts whose products below 2^-23 of the whole are
- * left out; factors below 2^-102 lose parts, and a decay below e^-200 is zero. A
- * key, query, alpha or beta that is not finite makes NaN of its head's rows among the
- * same 64 (earlier ones too) and of those after, a value that is not finite of its
- * column there; other requests and heads stay clean. Its workspace holds 25.9 KB a
- * head for every 64 rows of `rows`, and as much for every request. */
+ * Precision: FP32 sums and states. yuuka_gdn_prompt takes requests of one or two rows
+ * row by row, and solves 64 rows of a longer one at a time, its float32 factors as three
+ * bf16 parts whose products below 2^-23 of the whole are left out; factors below 2^-102
+ * lose parts, and a decay below e^-200 is zero.
+ * What is not finite goes as the rule does, row by row: a key, a log decay (NaN or +inf;
+ * -inf is a decay of zero) or a step size leaves its head's rows from its own on and its
+ * new state not finite, a value those of its column, a query its own row. Rows before it,
+ * other heads and other requests stay clean.
+ * The workspace of yuuka_gdn_prompt holds 25.9 KB a head for every 64 rows of `rows`, and
+ * as much for every request. */
 YUUKA_API yuuka_status yuuka_gdn_prompt(yuuka_stream * stream, yuuka_buffer * out, const yuuka_buffer * qkv,
                         const yuuka_buffer * alpha, const yuuka_buffer * beta, const yuuka_buffer * dt,
                         const yuuka_buffer * a, yuuka_buffer * states, const yuuka_buffer * offsets,

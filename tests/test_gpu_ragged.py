@@ -530,6 +530,61 @@ def test_a_nan_stays_with_its_request(dev, stream):
     assert np.isfinite(new[[0, 2]]).all() and np.isfinite(new[1, [0, 3]]).all()
 
 
+@pytest.mark.parametrize("what", ["key", "query", "value", "infinite value", "decay", "growth", "step", "state", "huge keys"])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,groups,heads,D", [(7, 1, 3, 64), (20, 2, 4, 128), (70, 1, 2, 128), (70, 2, 4, 64)])
+def test_rows_before_one_that_is_not_finite(dev, stream, dtype, n, groups, heads, D, what):
+    """As the rule goes row by row: what is not finite reaches its own row and those after it, and of another head or column none."""
+    rng = np.random.default_rng(n + D + len(what))
+    counts = ([130, 3, 64, 65, 1, 17, 2] * n)[:n] if n < 40 else [int(x) for x in rng.permutation([130, 64, 65, 1, 2, 0] + [
+        int(x) for x in rng.integers(1, 40, n - 6)])]
+    rows, off = sum(counts), offsets_of(counts)
+    qkv = unit_rows(rng, rows, groups, heads, D, dtype).reshape(rows, -1, D)
+    alpha, beta, _, _, _, _ = gates(rng, rows, heads, False)
+    states = rng.normal(0, 0.3, (n, heads, D, D)).astype(np.float32)
+    slots = np.stack([rng.permutation(n)] * 2, 1)
+    bad = to_bits(np.array([np.nan, np.inf]), dtype)
+    at = np.array([off[j] + rng.integers(0, c) if c else -1 for j, c in enumerate(counts)])
+    for j in range(0, n, 2):
+        if at[j] < 0:
+            continue
+        if counts[j] == 130:
+            at[j] = off[j] + 64 + 20
+        if what == "key":
+            qkv[at[j], groups + groups - 1, 7] = bad[j // 2 % 2]
+        elif what == "query":
+            qkv[at[j], 0, D - 1] = bad[j // 2 % 2]
+        elif what in ("value", "infinite value"):
+            qkv[at[j], 2 * groups + heads - 1, 21] = bad[int(what == "infinite value")]
+        elif what in ("decay", "growth"):
+            alpha[at[j], heads - 1] = np.nan if what == "decay" else np.inf
+        elif what == "step":
+            beta[at[j], 0] = (np.nan, np.inf)[j // 2 % 2]
+        elif what == "state":
+            states[slots[j, 0], 0, 3, D - 2] = (np.nan, np.inf)[j // 2 % 2]
+        else:  # their products with one another pass the type's largest value (F16: their sum of squares does not)
+            big = 6e4 if dtype == hip.F16 else 1e20
+            qkv[at[j]:off[j + 1], groups] = to_bits(np.full(D, big), dtype)
+    qkv = qkv.reshape(rows, -1)
+    got = run_delta(dev, stream, dtype, qkv, alpha, beta, None, None, states, counts, slots, groups, heads, D)
+    with np.errstate(all="ignore"):
+        want = delta_reference(from_bits(qkv, dtype), alpha.astype(np.float64), beta.astype(np.float64),
+                               states.astype(np.float64), off, slots, groups, heads, D, 1.0)
+    (o, s), (wo, o_off, ws, s_off) = got, want
+    fine, fine_s = np.isfinite(wo), np.isfinite(ws)
+    if what == "huge keys":  # (64 bits hold what float32 does not; keys beyond norm 1 have no bound)
+        for j in range(0, n, 2):
+            fine[at[j]:off[j + 1]] = False
+            fine_s[slots[j, 1]] = False
+    else:
+        assert not np.isfinite(o[~fine]).any() and not np.isfinite(s[~fine_s]).any()
+        assert not fine.all()
+    with np.errstate(all="ignore"):
+        tol = o_off + HALF[dtype] * np.abs(wo) + (2.0 ** -25 if dtype == hip.F16 else 0)
+        assert np.all((np.abs(o - wo) <= tol)[fine])
+        assert np.all((np.abs(s - ws) <= s_off + U * np.abs(ws))[fine_s])
+
+
 def test_offsets_that_lie(dev, stream):
     """Offsets outside the arrays are taken as their ends; a request that ends before it starts is empty."""
     rng = np.random.default_rng(8)

@@ -99,6 +99,21 @@ template <int N> __device__ __forceinline__ void split(f32x4 x, f32x4 y, u32x4 (
 // bf16 parts that hold a row's element exactly.
 template <typename E> constexpr int kParts = std::is_same<E, RowF32>::value ? 3 : std::is_same<E, RowF16>::value ? 2 : 1;
 
+__device__ __forceinline__ bool finite(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
+// Whether any value of a wave is not finite: zero times such a value is NaN, and so is a sum with it.
+template <int N> __device__ __forceinline__ bool any_not_finite(const f32x4 (&x)[N]) {
+    float zero = 0.0f;
+#pragma unroll
+    for (int c = 0; c < N; c++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) zero = fmaf(x[c][e], 0.0f, zero);
+    return __builtin_amdgcn_ballot_w64(zero != 0.0f) != 0;
+}
+// Of two bf16 first parts, all bits of those that are finite (a part has the value's exponent).
+__device__ __forceinline__ uint32_t finite_halves(uint32_t u) {
+    return ((u & 0x7f80u) == 0x7f80u ? 0u : 0xffffu) | ((u & 0x7f800000u) == 0x7f800000u ? 0u : 0xffff0000u);
+}
+
 // A barrier for what is in LDS: loads from memory stay under way.
 __device__ __forceinline__ void lds_barrier() {
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
@@ -282,6 +297,7 @@ __global__ __launch_bounds__(512, (kParts<E> == 3 ? 1 : 6)) void chunk_prepare_k
     __shared__ double sum[HH][kC];  // of the log decays, base 2
     __shared__ __align__(16) float beta[HH][kC];
     __shared__ __align__(16) float at_all[HH][kC][kRowPitch];  // A^T, its diagonal blocks later those of T^T
+    __shared__ int lost[HH][kC];  // rows of A with a value that is not finite
     const int number = blockIdx.x, group = blockIdx.y % a.groups;
     auto head = [&](int u) { return group + a.groups * (HH * (int)(blockIdx.y / a.groups) + u); };
     // the request whose chunk this is
@@ -317,6 +333,7 @@ __global__ __launch_bounds__(512, (kParts<E> == 3 ? 1 : 6)) void chunk_prepare_k
                                                            (uint32_t)__builtin_amdgcn_readlane((int)__builtin_bit_cast(uint64_t, c), 63));
         sum[u][lane] = c;
         beta[u][lane] = step;
+        lost[u][lane] = 0;
         const float grown = __builtin_amdgcn_exp2f((float)c);
         factors[lane] = step;
         factors[kC + lane] = step * grown;
@@ -373,6 +390,17 @@ __global__ __launch_bounds__(512, (kParts<E> == 3 ? 1 : 6)) void chunk_prepare_k
                 x[e] = low ? dot[m][e] * fall * factor : 0.0f;
             }
             if (keys) {
+                // What is not finite in A would make NaN of rows of T before its own, where it meets their zeros: it is
+                // taken as zero, and its row's T_ii becomes NaN below.
+                const f32x4 all[1] = {x};
+                if (__builtin_expect(any_not_finite(all), false)) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        if (finite(x[e])) continue;
+                        x[e] = 0.0f;
+                        lost[u][i] = 1;
+                    }
+                }
 #pragma unroll
                 for (int e = 0; e < 4; e++) at_all[u][j0 + e][i] = x[e];
             } else {
@@ -418,6 +446,11 @@ __global__ __launch_bounds__(512, (kParts<E> == 3 ? 1 : 6)) void chunk_prepare_k
         if (jt == wave) {
 #pragma unroll
             for (int e = 0; e < 4; e++) t[jt][e] = at[diag + 4 * g4 + e][diag + r16];
+            if (lost[which][diag + r16]) {
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    if (4 * g4 + e == r16) t[jt][e] = __builtin_nanf("");
+            }
         } else {
             f32x4 x = kZero;
 #pragma unroll
@@ -457,7 +490,8 @@ template <typename E, int D, int CT> struct ScanLds {
     // takes longer than the space (1 prompt of 8191 rows, the second kernel, 352 -> 362).
     static constexpr bool turned = keys + 2 * NP * kC * (2 * D + 16) > 160 * 1024;
     static constexpr uint32_t pitch = 2 * D + (turned ? 0 : 16), key_part = kC * pitch, key_buffer = NP * key_part;
-    static constexpr uint32_t total = keys + 2 * key_buffer;
+    static constexpr uint32_t lost = keys + 2 * key_buffer;  // the first row of every column that is not finite
+    static constexpr uint32_t total = lost + 64 * CT;
     static __device__ __forceinline__ int at(int row, int piece) {
         return row * pitch + 8 * (turned ? piece ^ ((row & 3) << 2 | (row >> 2 & 3)) : piece);
     }
@@ -468,6 +502,11 @@ template <typename E, int D, int CT> struct ScanLds {
 // more where a key has several parts (float32 keys split by the waves of the outputs: a fifth longer), bring the keys to
 // LDS, a chunk ahead. Three barriers a chunk:
 //   S and K there | K S -> R; Q S | T R -> V' | S; P V'
+// What is not finite in R or V' would make NaN of rows before its own, where it meets the zeros of T and P. A wave whose
+// V' has such a value works it out again with zeros for those of R, and leaves zeros for its own; the column's outputs
+// from that row on and its state are replaced by NaN behind the loop. us of this kernel without any of it and so: 8191
+// rows of 16 heads of 128 in F32 340, 342; 16 prompts of 8192 rows, 32 heads in BF16 217, 210; 96 of 6000 rows, 16 heads
+// of 64 in F16 65, 66. (With R looked at as well, before it is stored, and the outputs replaced in their turn: 366, 217, 68.)
 // What a chunk needs from memory is asked for one chunk ahead; two ahead, or W = T (beta e^c K) from the
 // first kernel for one phase less, took more registers than there are and were slower.
 template <typename E> constexpr int kScanWaves = kParts<E> == 3 ? 12 : 8;
@@ -486,6 +525,14 @@ __global__ __launch_bounds__(64 * kScanWaves<E>) void chunk_scan_kernel(GdnRows 
     if (r.end > r.begin && r.end - r.begin <= kFew) return;  // done by the first kernel
     const int group = h % a.groups;
     const int number0 = first_chunk<kC>(r.begin, j), last = (r.end - r.begin + kC - 1) / kC - 1;
+    int *const lost = reinterpret_cast<int *>(lds + L::lost);  // (rows are counted from the request's first)
+    if (tid < 16 * CT) lost[tid] = 0x7fffffff;
+    auto any_lost = [&]() -> bool {  // behind the last chunk
+        if (last < 0) return false;
+        int from = 0x7fffffff;
+        if (lane < 16 * CT) from = lost[lane];
+        return __builtin_expect(__builtin_amdgcn_ballot_w64(from < r.end - r.begin) != 0, false);
+    };
     const T *const qkv = static_cast<const T *>(b.qkv);
     auto chunk_at = [&](int i) { return left_all + ((int64_t)(number0 + min(i, last)) * a.heads + h) * left::dwords; };
     auto factors_at = [&](int i, int which) {  // of the lane's four rows
@@ -639,6 +686,19 @@ __global__ __launch_bounds__(64 * kScanWaves<E>) void chunk_scan_kernel(GdnRows 
                         __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, y), rows, at + e * pitch + 16 * c * sizeof(T), 0, 0);
                 }
         }
+        if (!any_lost()) return;
+#pragma unroll 1
+        for (int c = 0; c < CT; c++) {  // (each wave the rows that it has stored, so that its stores are in order)
+            T *const column = static_cast<T *>(b.out) + ((int64_t)r.begin * a.heads + h) * D + col0 + 16 * c + r16;
+            const int from = lost[16 * c + r16];
+            if (from >= r.end - r.begin) continue;
+            for (int row = from / kC * kC + 16 * wave; row < r.end - r.begin; row += kC)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int mine = row + 4 * g4 + e;
+                    if (mine >= from && mine < r.end - r.begin) column[(int64_t)mine * a.heads * D] = (T)__builtin_nanf("");
+                }
+        }
         return;
     }
 
@@ -681,6 +741,41 @@ __global__ __launch_bounds__(64 * kScanWaves<E>) void chunk_scan_kernel(GdnRows 
         load_step(0, left::t, 1, t);
         load_tail(0);
     }
+    // V' again without what is not finite, whose columns are lost from there on
+    auto again = [&](int i) {
+        f32x4 tt[2][2];
+        load_step(i, left::t, 0, tt);
+        load_step(i, left::t, 1, tt);
+#pragma unroll 1
+        for (int c = 0; c < CT; c++) {
+            Sum w = {kZero, kZero};
+#pragma unroll
+            for (int d = 0; d < 2; d++) {
+                if (d > wave / 2) break;
+                u32x4 z[3], x[3];
+                split(tt[d][0], tt[d][1], z);
+                operand(L::r, d, c, x);
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const uint32_t keep = finite_halves(x[0][k]);
+#pragma unroll
+                    for (int m = 0; m < 3; m++) x[m][k] &= keep;
+                }
+                mma32(z, x, w);
+            }
+            f32x4 y = w.all();
+            const u32x2 own = *reinterpret_cast<const u32x2 *>(lds + L::r + ((wave >> 1) * CT + c) * 3 * 1024 + lane * 16 +
+                                                               8 * (wave & 1));  // R as `store_half` left it
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                if ((finite_halves(own[e >> 1]) >> 16 * (e & 1) & 1) && finite(y[e])) continue;
+                y[e] = 0.0f;
+                atomicMin(lost + 16 * c + r16, i * kC + 16 * wave + 4 * g4 + e);
+            }
+            store_half(L::tail, wave, c, y * tail);
+            store_half(L::v, wave, c, y);
+        }
+    };
     for (int i = 0; i <= last; i++) {
         const uint32_t keys = L::keys + (i & 1) * L::key_buffer;
 #pragma unroll
@@ -746,12 +841,15 @@ __global__ __launch_bounds__(64 * kScanWaves<E>) void chunk_scan_kernel(GdnRows 
         load_step(i + 1, left::t, 0, t);
         load_step(i + 1, left::t, 1, t);
         pin_loads();
+        f32x4 y[CT];
+#pragma unroll
+        for (int c = 0; c < CT; c++) y[c] = w[c].all();
 #pragma unroll
         for (int c = 0; c < CT; c++) {
-            const f32x4 y = w[c].all();
-            store_half(L::tail, wave, c, y * tail);
-            store_half(L::v, wave, c, y);
+            store_half(L::tail, wave, c, y[c] * tail);
+            store_half(L::v, wave, c, y[c]);
         }
+        if (__builtin_expect(any_not_finite(y), false)) again(i);
         lds_barrier();
         Sum next[ST][CT];
 #pragma unroll
@@ -787,6 +885,16 @@ __global__ __launch_bounds__(64 * kScanWaves<E>) void chunk_scan_kernel(GdnRows 
             for (int c = 0; c < CT; c++) s[u][c] = next[u][c].all();
     }
     if ((uint32_t)slot.y < (uint32_t)a.states) {
+        if (any_lost()) {
+#pragma unroll
+            for (int c = 0; c < CT; c++) {
+                const bool mine = lost[16 * c + r16] < r.end - r.begin;
+#pragma unroll
+                for (int t = 0; t < ST; t++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) s[t][c][e] = mine ? __builtin_nanf("") : s[t][c][e];
+            }
+        }
 #pragma unroll
         for (int t = 0; t < ST; t++)
 #pragma unroll
