@@ -928,3 +928,50 @@ def test_states_past_four_gigabytes(dev, stream):
     got = pool.read(np.float32, heads * D * D, (far + 1) * size).reshape(1, heads, D, D)
     check_delta((out, got), want, hip.F32, rows)
     pool.free()
+
+
+def test_windows_and_rows_past_four_gigabytes(dev, stream):
+    """Windows in slots and rows that lie behind 2^32 bytes: the convolution, and the delta rule over the same rows."""
+    rng = np.random.default_rng(14)
+    groups, heads, D, rows, far = 16, 16, 128, 180000, 59000
+    channels, counts = (2 * groups + heads) * D, [2, 70]
+    front, live = rows - sum(counts), sum(counts)
+    x, y, pool = dev.alloc(rows * channels * 4), dev.alloc(rows * channels * 4), dev.alloc((far + 4) * channels * 3 * 4)
+    copy = hip.lib().yuuka_buffer_copy
+
+    def put(buf, at, data):
+        src = dev.upload(data)
+        hip.check(copy(stream.ptr, buf.ptr, at, src.ptr, 0, data.nbytes, None), "copy")
+        stream.sync()
+
+    data = rng.normal(0, 1, (live, channels)).astype(np.float32)
+    windows = rng.normal(0, 1, (4, channels, 3)).astype(np.float32)
+    w = rng.normal(0, 0.5, (channels, 4)).astype(np.float32)
+    put(x, front * channels * 4, data)
+    put(pool, far * channels * 12, windows)
+    offsets, slots = offsets_of(counts), np.array([[0, 2], [1, 1]])
+    ends, where = dev.upload(offsets + i32(front)), dev.upload((slots + far).astype(np.int32))
+    p = hip.gdn_params(hip.F32, 2, rows, groups, heads, D, scale=D ** -0.5, eps=1e-6)
+    hip.gdn_conv(stream, y, x, dev.upload(w), pool, ends, where, p)
+    stream.sync()
+    want, error, new = conv_reference(data.astype(np.float64), w.astype(np.float64), windows.astype(np.float64), offsets, slots,
+                                      groups, D, D ** -0.5, 1e-6)
+    got = y.read(np.float32, live * channels, front * channels * 4).reshape(live, channels)
+    assert np.all(np.abs(got - want) <= error + U * np.abs(want))
+    assert np.array_equal(pool.read(np.float32, 4 * channels * 3, far * channels * 12).reshape(windows.shape), new.astype(np.float32))
+    qkv = unit_rows(rng, live, groups, heads, D, hip.F32)
+    put(x, front * channels * 4, qkv)
+    alpha, beta, _, _, g, b = gates(rng, live, heads, False)
+    states = rng.normal(0, 0.3, (3, heads, D, D)).astype(np.float32)
+    gap = np.zeros((front, heads), np.float32)
+    ob, sb = dev.alloc(rows * heads * D * 4), dev.upload(states)
+    p.log_decay = 1
+    p.scale = 1.0
+    hip.gdn_prompt(stream, ob, x, dev.upload(np.concatenate([gap, alpha])), dev.upload(np.concatenate([gap, beta])), sb, ends,
+                   dev.upload(slots.astype(np.int32)), p)
+    stream.sync()
+    got = ob.read(np.float32, live * heads * D, front * heads * D * 4).reshape(live, heads, D), sb.read(np.float32).reshape(states.shape)
+    want = delta_reference(qkv.astype(np.float64), g, b, states.astype(np.float64), offsets, slots, groups, heads, D, 1.0)
+    check_delta(got, want, hip.F32, live)
+    for buf in (x, y, pool, ob):
+        buf.free()
