@@ -134,6 +134,12 @@ def test_batch_plan(dev, stream, n, rows, block, capacity, most, frees, first, i
         assert np.array_equal(w, g), name
 
 
+@pytest.mark.parametrize("n,rows", [(200, 1024), (200, 1025), (90, 2047), (1024, 2048), (200, 2049), (1025, 2048), (7, 5000)])
+def test_batch_plan_in_place(dev, stream, n, rows):
+    """By one workgroup in a few turns, and by two launches."""
+    test_batch_plan(dev, stream, n, rows, 16, 4000, max(2, 2 * rows // n), n + rows // 16 + 100, 3, True)
+
+
 @pytest.mark.parametrize("pool", [(-5, 3), (0, 1000), (7, 5), (2 ** 31 - 1, 2 ** 31 - 1), (2, -8)])
 def test_free_lists_that_lie(dev, stream, pool):
     """Bounds of the list that lie outside of it: no page from there."""

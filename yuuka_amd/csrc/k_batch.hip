@@ -11,8 +11,8 @@
 // Every block that gets a page holds a new row, so that the rows alone write the
 // tables: the first of a block does.
 //
-// Bound by the launch: 16 requests of one row 6.7 us, 200 of 16300 rows (0.3 MB) 6.8. The sums are in 64 bits, so that no
-// counts overflow them.
+// Bound by the launch: 16 requests of one row 6.4 us, 200 of 16300 rows (0.3 MB) 6.5; 4.8 to 7.9 in place, as a serving
+// loop calls it. The sums are in 64 bits, so that no counts overflow them.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -161,9 +161,10 @@ uint64_t batch_plan_scratch_bytes(const BatchArgs &a) { return ((uint64_t)a.requ
 
 hipError_t launch_batch_plan(const BatchBuffers &b, const BatchArgs &a, void *scratch, hipStream_t s) {
     // One launch where a workgroup scans the requests in one turn and none reads what another overwrites: 16 requests
-    // of one row 10.5 -> 6.8 us, 200 of 16300 rows 10.5 -> 6.9. A workgroup alone takes up to 4096 rows.
+    // of one row 10.5 -> 6.8 us, 200 of 16300 rows 10.5 -> 6.9. In place a workgroup alone takes 1024, 2048 and 4096 rows of
+    // 200 requests in 5.6, 6.7 and 9.0 us (host loop), two launches take 7.9, also for 16300.
     const bool in_place = b.blocks_out == b.blocks || b.pool_out == b.pool;
-    if (a.requests <= kScan && (!in_place || a.rows <= 4096)) {
+    if (a.requests <= kScan && (!in_place || a.rows <= 2048)) {
         batch_plan_kernel<<<in_place ? 1 : (uint32_t)((a.rows + kScan - 1) / kScan), kScan, 0, s>>>(b, a);
         return hipGetLastError();
     }
