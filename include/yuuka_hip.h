@@ -699,9 +699,11 @@ YUUKA_API yuuka_status yuuka_batch_plan(yuuka_stream * stream, const yuuka_buffe
 
 /* yuuka_kv_append of `rows` rows that each go to a slot of their own: slots int64
  * [rows] as yuuka_batch_plan writes them; a slot outside the pool drops its
- * row, and of two rows with one slot the pool holds either's bytes. `rope` has a
- * row's {cos, sin} each row. Of the parameters capacity, requests, request_rows and
- * displacement are not used. */
+ * row. Where two rows have one slot its content is undefined: each byte is the one's or
+ * the other's. `rope` has a row's {cos, sin} each row: ROPE_TABLE writes them with row_info
+ * as its own positions, each row a request of one (OWN_POS, n = {1, rot_dim, 0, rows}; 4096
+ * rows an op). Of the parameters capacity, requests, request_rows and displacement are not
+ * used. */
 YUUKA_API yuuka_status yuuka_kv_append_slots(yuuka_stream * stream, const yuuka_buffer * k, const yuuka_buffer * v,
                         yuuka_buffer * kpool, yuuka_buffer * vpool, const yuuka_buffer * slots,
                         const yuuka_buffer * k_norm, const yuuka_buffer * rope, const yuuka_kv_params * params,

@@ -197,6 +197,62 @@ def test_append_by_slot(dev, stream, dtype, nk, D, bs, rows, norm, rot):
     assert not changed[~np.isin(page, table)].any()
 
 
+@pytest.mark.parametrize("dtype", [hip.F32, hip.Q8_0])
+def test_append_by_slot_rotated_by_the_plans_positions(dev, stream, dtype):
+    """Rotations of rows at the positions that the plan works out, more rows than one op takes, captured and replayed."""
+    rng = np.random.default_rng(31)
+    n, rows, nk, D, rot, block, capacity, base = 5, 5000, 2, 64, 32, 16, 4096, 1e4
+    entries = capacity // block
+    up, alloc = dev.upload, dev.alloc
+    b = dict(positions=alloc(8 * n), counts=alloc(4 * n), blocks=up(np.zeros(n, np.int32)),
+             table=up(np.full((n, entries), -1, np.int32)), free=up(rng.permutation(n * entries).astype(np.int32)),
+             pool=up(i32(0, n * entries)), offsets=alloc(4 * (n + 1)), info=alloc(8 * rows), slots=alloc(8 * rows),
+             k=alloc(4 * rows * nk * D), v=alloc(4 * rows * nk * D), rope=alloc(4 * rows * rot))
+    p = hip.kv_params(dtype, block, capacity, nk, D, rows, rope_dim=rot)
+    pools = [alloc(n * entries * hip.kv_page_bytes(p)) for _ in range(2)]
+    plan = hip.Plan(dev)
+    plan.add(hip.OP["BATCH_PLAN"], [b[k] for k in ("positions", "counts", "blocks", "table", "free", "pool", "offsets", "info",
+                                                   "slots", "blocks", "pool")], n=[n, rows], u=[block, capacity])
+    for first in range(0, rows, 4096):
+        offs = [first * rot * 4] + [0] * 14 + [first * 8]
+        plan.add(hip.OP["ROPE_TABLE"], [b["rope"]] + [None] * 14 + [b["info"]], offs=offs,
+                 n=[1, rot, 0, min(4096, rows - first)], f=[base], flags=hip.FLAG_OWN_POS)
+    plan.add(hip.OP["KV_APPEND_SLOTS"], [b["k"], b["v"], *pools, b["slots"], None, b["rope"]], n=[nk, 0, D, nk * D, rows],
+             u=[block, 0, dtype, rot], f=[0, 1e-6])
+    graph = hip.Graph(plan, stream, None)
+    position, cached = np.zeros(n, np.int64), [np.zeros((0, nk, D)) for _ in range(n)]
+    for counts in ([700, 0, 1, 2900, 30], [1, 1, 1, 1, 1], [0, 3000, 90, 2, 1]):
+        k, v = rng.normal(0, 1, (2, rows, nk, D)).astype(np.float32)
+        for name, x in (("k", k), ("v", v), ("counts", i32(*counts)),
+                        ("positions", np.stack([np.full(n, 9), position], 1).astype(np.int32))):
+            b[name].write(x)
+        graph.replay(stream)
+        stream.sync()
+        off = offsets_of(counts)
+        for j, c in enumerate(counts):
+            own = k[off[j]:off[j + 1]].astype(np.float64)
+            angle = (position[j] + np.arange(c))[:, None] * base ** (-np.arange(0, rot, 2) / rot)
+            x, y, cos, sin = own[..., :rot // 2], own[..., rot // 2:rot], np.cos(angle)[:, None], np.sin(angle)[:, None]
+            turned = np.concatenate([x * cos - y * sin, x * sin + y * cos, own[..., rot:]], 2)
+            cached[j] = np.concatenate([cached[j], turned])
+        position += np.array(counts)
+    most = int(position.max())
+    out = [alloc(n * most * nk * D * 4) for _ in range(2)]
+    hip.kv_read(stream, *out, *pools, b["table"], hip.kv_params(dtype, block, capacity, nk, D, most, n))
+    stream.sync()
+    got = out[0].read(np.float32).reshape(n, most, nk, D)
+    for j in range(n):
+        want = cached[j]
+        # u each for the table, the product and the sum, of |x| + |y| <= 2 sqrt(2) times the larger of the turned two
+        tol = 9 * U * np.abs(want).max(2, initial=1, keepdims=True)
+        if dtype == hip.Q8_0:  # half a step of the 32 values' largest by 127, and the scale's own rounding to half
+            most_of = np.repeat(np.abs(want).reshape(len(want), nk, D // 32, 32).max(3), 32, 2)
+            tol = tol + most_of * (0.5 / 127 + 2.0 ** -11 + 2.0 ** -12)
+        assert np.all(np.abs(got[j, :len(want)] - want) <= tol)
+    graph.destroy()
+    plan.destroy()
+
+
 # ----------------------------------------------------------------- convolution
 
 def conv_reference(x, w, windows, offsets, slots, groups, D, scale, eps):

@@ -8,12 +8,12 @@
 //   S <- e^(c_last) S + K^T diag(e^(c_last - c)) V'
 // The first kernel makes T and P of every chunk and head, all chunks at once; the second
 // walks the chunks of a request with S in registers. Row after row, with two sums over the workgroup each, 8191 rows
-// of 16 heads of 128 in F32 take 17.7 ms; 64 at a time 0.42.
+// of 16 heads of 128 in F32 take 17.7 ms; 64 at a time 0.43.
 //
 // The bytes that cannot be done without are 0.27 GB there, 56 us at the rate of a large copy, and the products 0.1 TFLOP of
 // bf16. Neither binds: the second kernel's chain does, 2.7 us a chunk (2.0 with nothing loaded from memory), of three
 // phases that each write LDS, wait for a barrier, read LDS and run a chain of matrix instructions. Matrix
-// instructions are busy 24 % of the cycles of the 128 CUs that have a workgroup, vector ones issue in 56 %.
+// instructions are busy 24 % of the cycles of the 128 CUs that have a workgroup, vector ones issue in 57 %.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -158,9 +158,11 @@ template <typename E, int D> struct RowOperand {  // 16-bit: products are exact
 #pragma unroll
         for (int s = 0; s < D / 32; s++) {
             if constexpr (std::is_same<E, RowF16>::value)
-                c = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, x[s]), __builtin_bit_cast(f16x8, o.x[s]), c, 0, 0, 0);
+                c = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, x[s]),
+                                                           __builtin_bit_cast(f16x8, o.x[s]), c, 0, 0, 0);
             else
-                c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x[s]), __builtin_bit_cast(bf16x8, o.x[s]), c, 0, 0, 0);
+                c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x[s]),
+                                                            __builtin_bit_cast(bf16x8, o.x[s]), c, 0, 0, 0);
         }
         return c;
     }
@@ -197,8 +199,9 @@ __device__ __forceinline__ double lanes_scan(double x) {
 
 // A request of one or two rows, row after row by the first kernel: S = e^g S;  d = beta (v - S^T k);  S += k d^T;
 // o = S^T q. A workgroup has a head's state, a thread four columns of every (2048 / D)th row. 200 requests of 16
-// heads of 128 in BF16 of one, two and four rows each 236, 237 and 238 us in chunks, 89, 98 and 117 (then by four
-// rows) this way; with four, a batch of 96 requests of unequal lengths, 6000 rows of 16 heads of 64 in F16, takes 102 us for 97.
+// heads of 128 in BF16 of one, two and four rows each 236, 237 and 238 us in chunks, 88, 96 and 117 (then by four
+// rows) this way; with four, a batch of 96 requests of unequal lengths, 6000 rows of 16 heads of 64 in F16, took 102 us
+// for 97.
 constexpr int kFew = 2;
 template <typename E, int D>
 __device__ __forceinline__ void few_rows(const GdnRows &b, const RaggedArgs &a, RowRange r, int j, int h, float *lds) {
@@ -287,12 +290,13 @@ __device__ __forceinline__ void few_rows(const GdnRows &b, const RaggedArgs &a, 
 }
 
 // Eight waves: four for k_i . k_j, four for q_i . k_j, then four for the T of every head. HH heads of a group share
-// the products. Small dependent phases: waves wait in 58 % of their cycles, vector instructions issue in 40 % (BF16;
-// in F32 21 %, the matrix units busy in 26 %). 81 us for 8191 rows of 16 heads of 128 in F32 (0.12 GB moved), 61 for 8192
-// rows of 16 prompts and 32 heads in BF16 (0.15 GB).
+// the products. Small dependent phases: waves wait in 63 % of their cycles, vector instructions issue in 39 % (BF16;
+// in F32 57 and 21 %, the matrix units busy in 26 %). 81 us for 8191 rows of 16 heads of 128 in F32 (0.12 GB moved), 62
+// for 8192 rows of 16 prompts and 32 heads in BF16 (0.15 GB).
 // (Six waves a SIMD for 16-bit rows: the registers of few_rows would leave five, 62 -> 70 us.)
 template <typename E, int D, int HH>
-__global__ __launch_bounds__(512, (kParts<E> == 3 ? 1 : 6)) void chunk_prepare_kernel(GdnRows b, RaggedArgs a, uint32_t *__restrict__ left_all) {
+__global__ __launch_bounds__(512, (kParts<E> == 3 ? 1 : 6)) void chunk_prepare_kernel(GdnRows b, RaggedArgs a,
+                                                                                     uint32_t *__restrict__ left_all) {
     typedef typename E::T T;
     __shared__ double sum[HH][kC];  // of the log decays, base 2
     __shared__ __align__(16) float beta[HH][kC];
@@ -328,9 +332,10 @@ __global__ __launch_bounds__(512, (kParts<E> == 3 ? 1 : 6)) void chunk_prepare_k
         const int64_t from = (int64_t)(row0 + (there ? lane : 0)) * a.heads + h;
         const float g = there ? log_decay_of(b, a, from, h) : 0.0f, step = there ? beta_of(b, a, from) : 0.0f;
         const double c = lanes_scan(1.4426950408889634 * (g < kLeast ? kLeast : g));
-        const double last = __builtin_bit_cast(double, (uint64_t)(uint32_t)__builtin_amdgcn_readlane(
-                                                           (int)(__builtin_bit_cast(uint64_t, c) >> 32), 63) << 32 |
-                                                           (uint32_t)__builtin_amdgcn_readlane((int)__builtin_bit_cast(uint64_t, c), 63));
+        const uint64_t bits = __builtin_bit_cast(uint64_t, c);
+        const double last = __builtin_bit_cast(
+            double, (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(bits >> 32), 63) << 32 |
+                        (uint32_t)__builtin_amdgcn_readlane((int)bits, 63));
         sum[u][lane] = c;
         beta[u][lane] = step;
         lost[u][lane] = 0;
@@ -588,8 +593,10 @@ __global__ __launch_bounds__(64 * kScanWaves<E>) void chunk_scan_kernel(GdnRows 
                 parts(k[2 * s], k[2 * s + 1], x);
 #pragma unroll
                 for (int m = 0; m < NP; m++) {  // (rows behind the end are zeros: they meet zeros of V')
-                    *reinterpret_cast<u32x2 *>(to + m * L::key_part + key_at(2 * s)) = there ? u32x2{x[m][0], x[m][1]} : u32x2{0, 0};
-                    *reinterpret_cast<u32x2 *>(to + m * L::key_part + key_at(2 * s + 1)) = there ? u32x2{x[m][2], x[m][3]} : u32x2{0, 0};
+                    *reinterpret_cast<u32x2 *>(to + m * L::key_part + key_at(2 * s)) =
+                        there ? u32x2{x[m][0], x[m][1]} : u32x2{0, 0};
+                    *reinterpret_cast<u32x2 *>(to + m * L::key_part + key_at(2 * s + 1)) =
+                        there ? u32x2{x[m][2], x[m][3]} : u32x2{0, 0};
                 }
             }
         };
@@ -680,10 +687,11 @@ __global__ __launch_bounds__(64 * kScanWaves<E>) void chunk_scan_kernel(GdnRows 
 #pragma unroll
                 for (int c = 0; c < CT; c++) {
                     const T y = (T)(o[c].big[e] + o[c].small[e]);
+                    const uint32_t to = at + e * pitch + 16 * c * sizeof(T);
                     if constexpr (sizeof(T) == 4)
-                        __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, y), rows, at + e * pitch + 16 * c * sizeof(T), 0, 0);
+                        __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, y), rows, to, 0, 0);
                     else
-                        __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, y), rows, at + e * pitch + 16 * c * sizeof(T), 0, 0);
+                        __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, y), rows, to, 0, 0);
                 }
         }
         if (!any_lost()) return;
@@ -924,8 +932,9 @@ hipError_t launch_gdn_prompt(const GdnRows &b, uint32_t dtype, const RaggedArgs 
         using E = decltype(e);
         constexpr int D = d();
         uint32_t *const left_all = static_cast<uint32_t *>(scratch);
-        // Two heads a workgroup where that leaves every CU one. us of the whole call: 32 heads of 16 groups, 2000 rows in
-        // F32 142 -> 126, 16 x 8192 rows in BF16 266 -> 260; 500 rows in BF16 38 -> 40, which stay at one.
+        // Two heads a workgroup where that leaves every CU one. us of the whole call with one and with two: 32 heads of 16
+        // groups, 2000 rows in F32 126 and 112, 16 prompts of 8192 rows in all in BF16 267 and 245; 500 rows in BF16 33 and
+        // 35, which stay at one.
         if (a.heads / a.groups % 2 == 0 && (int64_t)numbers * a.heads >= 2 * 256)
             chunk_prepare_kernel<E, D, 2><<<dim3(numbers, a.heads / 2), 512, 0, s>>>(b, a, left_all);
         else chunk_prepare_kernel<E, D, 1><<<dim3(numbers, a.heads), 512, 0, s>>>(b, a, left_all);
@@ -950,9 +959,9 @@ hipError_t launch_gdn_prompt(const GdnRows &b, uint32_t dtype, const RaggedArgs 
             }
         };
         // The most columns that LDS holds and that leave every CU a workgroup: what is loaded for a chunk serves more of
-        // them. us with 1, 2 and 4 tiles, BF16: 1 prompt of 2000 rows, 16 heads of 128 (128 workgroups at one tile) 90, 119,
-        // 178; 4 of 1000 (512) 104, 83, 109; 4 of 1000, 32 heads (1024) 184, 142, 128; 16 of 8192 rows in all (4096)
-        // 388, 302, 260. F32, 16 heads: 4 of 1000 rows 138, 113, 64 of 300 in all 241, 157.
+        // them. us with 1, 2 and 4 tiles, BF16: 1 prompt of 2000 rows, 16 heads of 128 (128 workgroups at one tile) 88, 120,
+        // 167; 4 of 1000 (512) 101, 82, 105; 4 of 1000, 32 heads (1024) 182, 138, 114; 16 of 8192 rows in all (4096)
+        // 388, 305, 244. F32, 16 heads: 4 of 1000 rows 137, 110, 64 of 300 in all 282, 184.
         const int64_t columns = (int64_t)a.requests * a.heads * (D / 16);
         if (columns >= 4 * 256 && ScanLds<E, D, 4>::total <= 160 * 1024) go(std::integral_constant<int, 4>{});
         else if (columns >= 2 * 256 && ScanLds<E, D, 2>::total <= 160 * 1024) go(std::integral_constant<int, 2>{});

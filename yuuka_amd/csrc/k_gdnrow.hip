@@ -54,8 +54,8 @@ template <int N> __device__ __forceinline__ float lanes_sum(float x) {
 // rows and keeps the last KT - 1 of them in registers; the wave with a request's first
 // row reads its window and leaves its new one, which may be in the same slot.
 // Requests without rows have their window moved by waves of their own.
-// 8191 rows of 8192 channels in BF16, 0.27 GB, 71 us, 3.8 TB/s (a large copy reaches 4.7 to 5.1): half vector
-// issue, half the latency of a row's chain, with four waves a SIMD.
+// 8191 rows of 8192 channels in BF16, 0.27 GB, 71 us, 3.8 TB/s (a large copy reaches 4.7 to 5.1): vector
+// instructions issue in 74 % of the SIMDs' cycles, and waves, four a SIMD, wait in 53 % of theirs.
 template <typename E, int KT, int D>
 __global__ __launch_bounds__(256) void ragged_conv_kernel(typename E::T *__restrict__ out,
                                                           const typename E::T *__restrict__ x,
@@ -362,8 +362,9 @@ hipError_t launch_gdn_ragged_conv(void *out, const void *x, uint32_t dtype, cons
     by_type(dtype, [&](auto e) {
         using E = decltype(e);
         typedef typename E::T T;
-        // A wave's rows: as few as leave every CU the same number of workgroups, four or a multiple, and up to 32 (16 in
-        // F32, of half the channels). A wave's start, with request, taps and K - 1 rows more, is what fewer cost: 7 prompts of
+        // A wave's rows: as few as leave every CU the same number of workgroups, four or a multiple, and about 32 at most (16
+        // in F32, of half the channels; a row or two more where the columns do not divide the workgroups, and more for
+        // hundreds of columns and few rows). A wave's start, with request, taps and K - 1 rows more, is what fewer cost: 7 prompts of
         // 8191 rows, 32 heads in BF16, 8, 16 and 32 rows a wave 84, 77 and 71 us, 31 (a fifth workgroup on some CUs) 91;
         // 16 of 8000 rows, 32 heads in F32, 120, 115 and 127.
         constexpr int kRows = 4 * E::kWide;
