@@ -937,6 +937,23 @@ def test_attention_over_planned_pages(dev, stream):
     plan.destroy()
 
 
+def test_a_refused_workspace_leaves_no_error(dev, stream):
+    """A call whose workspace no card has (1.7 TB), and a buffer of a petabyte, are refused; the next call is sound."""
+    n, heads, D = 65535, 1024, 64
+    small = [dev.alloc(4 * (2 + heads) * D) for _ in range(2)] + [dev.alloc(4 * heads) for _ in range(2)]
+    for refused in (lambda: hip.gdn_prompt(stream, *small, dev.alloc(4 * heads * D * D), dev.upload(np.zeros(n + 1, np.int32)),
+                                           dev.upload(np.full((n, 2), -1, np.int32)),
+                                           hip.gdn_params(hip.F32, n, 1, 1, heads, D, log_decay=True)),
+                    lambda: dev.alloc(1 << 50)):
+        with pytest.raises(hip.HipError) as e:
+            refused()
+        assert e.value.status == hip.ALLOCATION
+        args = (i32(0, 20), i32(40, 100), i32(0, 2), np.full((2, 20), 9, np.int32), np.arange(60, dtype=np.int32), i32(0, 60), 140, 16, 320)
+        for w, g in zip(plan_reference(*args), run_plan(dev, stream, *args)):
+            assert np.array_equal(w, g)
+        test_a_prompt_in_pieces(dev, stream, 64)
+
+
 def test_two_streams_at_once(dev, stream):
     s2 = hip.Stream(dev)
     rng = np.random.default_rng(2)

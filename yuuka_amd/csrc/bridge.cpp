@@ -36,7 +36,10 @@ yuuka_status fail(yuuka_status status, const char *fmt, ...) {
     return status;
 }
 
-const char *hip_error(hipError_t err) { return hipGetErrorString(err); }
+const char *hip_error(hipError_t err) {
+    (void)hipGetLastError();
+    return hipGetErrorString(err);
+}
 
 yuuka_status ensure_scratch(yuuka_stream *stream, yk_scratch *area, uint64_t bytes) {
     if (area->bytes >= bytes) return YUUKA_OK;

@@ -46,6 +46,8 @@ namespace yk {
 
 // Thread-local error message (reference bridge.cpp:47-57 convention).
 yuuka_status fail(yuuka_status status, const char *fmt, ...) __attribute__((format(printf, 2, 3)));
+// The text of an error that is reported to the caller. The runtime forgets it, so that the check behind the next
+// launch does not take it for its own.
 const char *hip_error(hipError_t err);
 
 // Grows a stream scratch area to at least `bytes`; zero-fills new memory.
