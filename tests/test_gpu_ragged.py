@@ -937,6 +937,39 @@ def test_attention_over_planned_pages(dev, stream):
     plan.destroy()
 
 
+@pytest.mark.parametrize("dtype,groups,heads,D", [(hip.F32, 1024, 1024, 128), (hip.BF16, 1, 1024, 64), (hip.F16, 512, 1024, 64)])
+def test_as_many_heads_as_are_served(dev, stream, dtype, groups, heads, D):
+    """1024 heads: more columns of channels than the convolution has workgroups to spread, and a workgroup's rule for few rows."""
+    rng = np.random.default_rng(groups + D)
+    counts, channels = [1, 0, 70, 2, 6], (2 * groups + heads) * D
+    n, rows = len(counts), sum(counts)
+    offsets, slots = offsets_of(counts), np.stack([rng.permutation(n)] * 2, 1).astype(np.int32)
+    x = to_bits(rng.normal(0, 1, (rows, channels)), dtype)
+    w = rng.normal(0, 0.5, (channels, 4)).astype(np.float32)
+    windows = rng.normal(0, 1, (n, channels, 3)).astype(np.float32)
+    ob, wb = dev.alloc(x.nbytes), dev.upload(windows)
+    p = hip.gdn_params(dtype, n, rows, groups, heads, D, scale=D ** -0.5, eps=1e-6)
+    hip.gdn_conv(stream, ob, dev.upload(x), dev.upload(w), wb, dev.upload(offsets), dev.upload(slots), p)
+    stream.sync()
+    want, error, new = conv_reference(from_bits(x, dtype), w.astype(np.float64), windows.astype(np.float64), offsets, slots,
+                                      groups, D, D ** -0.5, 1e-6)
+    got = from_bits(ob.read(np_type(dtype)).reshape(rows, channels), dtype)
+    assert np.all(np.abs(got - want) <= error + HALF[dtype] * np.abs(want) + (2.0 ** -25 if dtype == hip.F16 else 0))
+    assert np.array_equal(wb.read(np.float32).reshape(windows.shape), new.astype(np.float32))
+    qkv = unit_rows(rng, rows, groups, heads, D, dtype)
+    alpha, beta, dt, a, g, b = gates(rng, rows, heads, True)
+    states = rng.normal(0, 0.3, (n, heads, D, D)).astype(np.float32)
+    got = run_delta(dev, stream, dtype, qkv, alpha, beta, dt, a, states, counts, slots, groups, heads, D)
+    check_delta(got, delta_reference(from_bits(qkv, dtype), g, b, states.astype(np.float64), offsets, slots, groups, heads, D, 1.0),
+                dtype, rows)
+    got = run_delta(dev, stream, dtype, qkv, alpha, beta, dt, a, states, None, slots, groups, heads, D, step=True)
+    first = slice(0, n)
+    (out, new), want = got, delta_reference(from_bits(qkv[first], dtype), g[first], b[first], states.astype(np.float64),
+                                            np.arange(n + 1), slots, groups, heads, D, 1.0)
+    assert np.all(out[n:] == 7.0)
+    check_delta((out[first], new), want, dtype, n)
+
+
 def test_a_refused_workspace_leaves_no_error(dev, stream):
     """A call whose workspace no card has (1.7 TB), and a buffer of a petabyte, are refused; the next call is sound."""
     n, heads, D = 65535, 1024, 64
